@@ -17,7 +17,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libbchip.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "bchip.h")
 
-F32, F16 = 0, 1
+F32, F16, Q4 = 0, 1, 2
+# A 4-bit buffer: units of 256 elements, 128 bytes of codes and eight f16 scales.
+Q4_UNIT, Q4_UNIT_BYTES, Q4_BLOCK = 256, 144, 32
 OK, E_ARG, E_HIP, E_NODEV, E_DISABLED, E_UNSUPPORTED, E_OOM = 0, -1, -2, -3, -4, -5, -6
 CHUNK_MULTI = 192
 # ggml weight types (quant.rs:35-49) and (weights, bytes) per block (quant.rs:69-82).
@@ -116,6 +118,11 @@ def check(code: int) -> None:
 
 def esize(t: int) -> int:
     return 2 if t == F16 else 4
+
+
+def nbytes_of(t: int, n: int) -> int:
+    """Bytes of a buffer of n elements of type t (4-bit codes: whole units)."""
+    return -(-n // Q4_UNIT) * Q4_UNIT_BYTES if t == Q4 else n * esize(t)
 
 
 class Buf:
@@ -321,7 +328,7 @@ def grown_capacity(cap: int, need: int, context: int) -> int:
 class KvCache:
     """A model's KV cache on the device, the reference's Cache (gpu/mod.rs:300-337) with
     Gpu::new_cache and Gpu::reserve (mod.rs:398-423): per layer a K and a V buffer of
-    cap x kvd elements of kv_type (kvd = n_head_kv * head_dim), grown by doubling, the kept
+    cap x kvd elements of kv_type (F32, F16 or Q4; kvd = n_head_kv * head_dim), grown by doubling, the kept
     prefix copied for every layer in one launch (bchip_cache_grow), and Cache::keep in one
     launch (bchip_keep)."""
 
@@ -338,7 +345,7 @@ class KvCache:
         if keep > self.cap:
             raise ValueError(f"keep {keep} past the cache's {self.cap} tokens")
         cap = grown_capacity(self.cap, need, context)
-        nbytes = cap * self.kvd * esize(self.kv_type)
+        nbytes = nbytes_of(self.kv_type, cap * self.kvd)
         k = [Buf(self.ctx, nbytes) for _ in range(self.n_layer)]
         v = [Buf(self.ctx, nbytes) for _ in range(self.n_layer)]
         old = self.k + self.v
@@ -355,7 +362,7 @@ class KvCache:
 
     def bytes(self) -> int:
         """Cache::bytes: device bytes the cache holds."""
-        return len(self.k) * 2 * self.cap * self.kvd * esize(self.kv_type)
+        return len(self.k) * 2 * nbytes_of(self.kv_type, self.cap * self.kvd)
 
     def free(self) -> None:
         for b in self.k + self.v:

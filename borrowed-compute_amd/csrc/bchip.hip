@@ -21,6 +21,7 @@
 
 #include "common.hpp"
 #include "internal.hpp"
+#include "q4.hpp"
 
 using namespace bchip;
 
@@ -144,7 +145,13 @@ int check_span(const bchip_ctx* c, const void* p, uint64_t bytes, const char* wh
     return check_at(c, p, 0, bytes, what);
 }
 
-uint32_t esize(uint32_t type) { return type == BCHIP_F16 ? 2u : 4u; }
+// Bytes of n elements of a type (a 4-bit cache: whole units), and the types that bchip_fill_normal
+// takes, or a cache may have.
+uint64_t bytes_of(uint32_t type, uint64_t n) {
+    if (type == BCHIP_Q4) return n > UINT64_MAX - Q4_UNIT ? UINT64_MAX : sat_mul((n + Q4_UNIT - 1) / Q4_UNIT, Q4_UNIT_BYTES);
+    return sat_mul(n, type == BCHIP_F16 ? 2u : 4u);
+}
+constexpr uint32_t LAST_TYPE = BCHIP_Q4;
 
 // Bytes from p to the end of the bchip_alloc allocation holding it, or UINT64_MAX for
 // memory this library did not allocate.
@@ -155,6 +162,13 @@ uint64_t bytes_left(const bchip_ctx* c, const void* p) {
     --it;
     if (a >= it->first + it->second) return UINT64_MAX;
     return it->first + it->second - a;
+}
+
+// Slots of kvd elements that both caches hold, as far as is known.
+uint64_t slots_held(const bchip_ctx* c, const void* kc, const void* vc, uint32_t type, uint64_t kvd) {
+    const uint64_t bytes = std::min(bytes_left(c, kc), bytes_left(c, vc));
+    if (type == BCHIP_Q4) return sat_mul(bytes / Q4_UNIT_BYTES, Q4_UNIT) / kvd;
+    return bytes / bytes_of(type, kvd);
 }
 
 #define CHECK(expr)                  \
@@ -169,6 +183,13 @@ int check_heads(uint32_t nh, uint32_t nkv, uint32_t hd) {
     if (nh / nkv > 16) return fail(BCHIP_E_UNSUPPORTED, "group of %u query heads per KV head (at most 16)", nh / nkv);
     if (hd == 0 || hd % 8 != 0 || hd > MAX_HD)
         return fail(BCHIP_E_UNSUPPORTED, "head_dim %u (a multiple of 8 up to %u)", hd, MAX_HD);
+    return BCHIP_OK;
+}
+
+// What a 4-bit cache asks beside: heads of whole blocks, and tile offsets within 32 bits.
+int check_q4(uint32_t nkv, uint32_t hd) {
+    if (hd % Q4_BLOCK) return fail(BCHIP_E_UNSUPPORTED, "head_dim %u (a 4-bit cache takes multiples of %u)", hd, Q4_BLOCK);
+    if ((uint64_t)nkv * hd > (1u << 24)) return fail(BCHIP_E_UNSUPPORTED, "%u KV heads of %u (a 4-bit cache's slot holds at most 2^24 elements)", nkv, hd);
     return BCHIP_OK;
 }
 
@@ -196,6 +217,34 @@ void Workspace::set_fixed(void* base, size_t o_bytes, size_t ml_bytes, size_t q_
     gerr_host = owner.gerr_host;
 }
 
+void Workspace::drop(void* p) {
+    if (!p) return;
+    if (captured) retired.push_back(p);
+    else (void)hipFree(p);
+}
+
+bool Workspace::had(hipStream_t s, bool enough) {
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(s, &cap) != hipSuccess) (void)hipGetLastError();
+    if (cap == hipStreamCaptureStatusNone) return true;
+    captured |= enough && !fixed;
+    return enough;
+}
+
+bool Workspace::reserve_if(size_t need_slots, size_t hd_pad, hipStream_t s) {
+    if (!fixed && !had(s, need_slots <= slots && hd_pad <= hdp && o)) return false;
+    if (reserve(need_slots, hd_pad) == hipSuccess) return true;
+    (void)hipGetLastError();
+    return false;
+}
+
+bool Workspace::reserve_vt_if(size_t bytes, hipStream_t s) {
+    if (!fixed && !had(s, bytes <= vt_bytes && vt)) return false;
+    if (reserve_vt(bytes) == hipSuccess) return true;
+    (void)hipGetLastError();
+    return false;
+}
+
 hipError_t Workspace::reserve(size_t need_slots, size_t hd_pad) {
     if (fixed) {
         if (need_slots * hd_pad * sizeof(float) > o_cap || need_slots * 2 * sizeof(float) > ml_cap)
@@ -206,8 +255,8 @@ hipError_t Workspace::reserve(size_t need_slots, size_t hd_pad) {
     }
     if (need_slots <= slots && hd_pad <= hdp && o) return hipSuccess;
     const size_t ns = std::max(need_slots, slots), nh = std::max(hd_pad, hdp);
-    if (o) (void)hipFree(o);
-    if (ml) (void)hipFree(ml);
+    drop(o);
+    drop(ml);
     o = ml = nullptr;
     slots = 0;
     hdp = nh;
@@ -222,7 +271,7 @@ hipError_t Workspace::reserve(size_t need_slots, size_t hd_pad) {
 hipError_t Workspace::reserve_vt(size_t bytes) {
     if (fixed) return hipErrorOutOfMemory;
     if (bytes <= vt_bytes && vt) return hipSuccess;
-    if (vt) (void)hipFree(vt);
+    drop(vt);
     vt = nullptr;
     vt_bytes = 0;
     hipError_t e = hipMalloc(&vt, bytes);
@@ -283,6 +332,8 @@ void Workspace::release() {
     if (ml) (void)hipFree(ml);
     if (vt) (void)hipFree(vt);
     if (qrot) (void)hipFree(qrot);
+    for (void* r : retired) (void)hipFree(r);
+    retired.clear();
     o = ml = nullptr;
     vt = nullptr;
     qrot = nullptr;
@@ -531,10 +582,18 @@ int bchip_copy(bchip_ctx* c, const void* src, uint32_t st, void* dst, uint32_t d
     CHECK(enter(c));
     if (n == 0) return BCHIP_OK;
     if (!src || !dst) return fail(BCHIP_E_ARG, "null pointer");
-    if (st > 1 || dt > 1) return fail(BCHIP_E_ARG, "element types %u, %u", st, dt);
-    CHECK(check_span(c, src, sat_mul(n, esize(st)), "copy source"));
-    CHECK(check_at(c, dst, sat_mul(off, esize(dt)), sat_mul(n, esize(dt)), "copy destination"));
-    HIP_TRY(copy_launch(src, st, dst, dt, off, n, c->stream), "copy");
+    if (st > LAST_TYPE || dt > LAST_TYPE) return fail(BCHIP_E_ARG, "element types %u, %u", st, dt);
+    const bool q4 = st == BCHIP_Q4 || dt == BCHIP_Q4;
+    if (q4 && (n % Q4_BLOCK || (dt == BCHIP_Q4 && off % Q4_BLOCK)))
+        return fail(BCHIP_E_ARG, "%llu elements at %llu: 4-bit codes move in blocks of %u", (unsigned long long)n,
+                    (unsigned long long)off, Q4_BLOCK);
+    if ((st == BCHIP_Q4 && !aligned16(src)) || (dt == BCHIP_Q4 && !aligned16(dst)))
+        return fail(BCHIP_E_ARG, "a 4-bit buffer must be 16-byte aligned");
+    CHECK(check_span(c, src, bytes_of(st, n), "copy source"));
+    if (dt == BCHIP_Q4) CHECK(check_span(c, dst, bytes_of(dt, sat_add(off, n)), "copy destination"));
+    else CHECK(check_at(c, dst, bytes_of(dt, off), bytes_of(dt, n), "copy destination"));
+    HIP_TRY(q4 ? copy_q4_launch(src, st, dst, dt, off, n, c->stream) : copy_launch(src, st, dst, dt, off, n, c->stream),
+            "copy");
     return BCHIP_OK;
 }
 
@@ -542,11 +601,14 @@ int bchip_move(bchip_ctx* c, void* buf, uint32_t type, uint64_t from, uint64_t t
     CHECK(enter(c));
     if (n == 0) return BCHIP_OK;
     if (!buf) return fail(BCHIP_E_ARG, "null pointer");
-    if (type > 1) return fail(BCHIP_E_ARG, "element type %u", type);
+    if (type > LAST_TYPE) return fail(BCHIP_E_ARG, "element type %u", type);
     if (to > from) return fail(BCHIP_E_ARG, "move to %llu after from %llu", (unsigned long long)to,
                                 (unsigned long long)from);
-    CHECK(check_span(c, buf, sat_mul(sat_add(from, n), esize(type)), "move"));
-    HIP_TRY(move_launch(buf, type, from, to, n, c->stream), "move");
+    if (type == BCHIP_Q4 && (from % Q4_BLOCK || to % Q4_BLOCK || n % Q4_BLOCK || !aligned16(buf)))
+        return fail(BCHIP_E_ARG, "4-bit codes move in blocks of %u, in a 16-byte aligned buffer", Q4_BLOCK);
+    CHECK(check_span(c, buf, bytes_of(type, sat_add(from, n)), "move"));
+    HIP_TRY(type == BCHIP_Q4 ? move_q4_launch(buf, from, to, n, c->stream) : move_launch(buf, type, from, to, n, c->stream),
+            "move");
     return BCHIP_OK;
 }
 
@@ -555,10 +617,12 @@ int bchip_cache_grow(bchip_ctx* c, const void* const* src, void* const* dst, uin
     CHECK(enter(c));
     if (nbufs == 0 || total == 0) return BCHIP_OK;
     if (!dst || (keep > 0 && !src)) return fail(BCHIP_E_ARG, "null pointer");
-    if (type > 1) return fail(BCHIP_E_ARG, "element type %u", type);
+    if (type > LAST_TYPE) return fail(BCHIP_E_ARG, "element type %u", type);
+    if (type == BCHIP_Q4 && (keep % Q4_BLOCK || total % Q4_BLOCK))
+        return fail(BCHIP_E_ARG, "4-bit codes move in blocks of %u", Q4_BLOCK);
     if (keep > total) return fail(BCHIP_E_ARG, "keep %llu past total %llu", (unsigned long long)keep,
                                   (unsigned long long)total);
-    const uint64_t kb = sat_mul(keep, esize(type)), tb = sat_mul(total, esize(type));
+    const uint64_t kb = bytes_of(type, keep), tb = bytes_of(type, total);
     for (uint32_t b = 0; b < nbufs; b++) {
         const uint8_t* s = keep > 0 ? (const uint8_t*)src[b] : nullptr;
         const uint8_t* d = (const uint8_t*)dst[b];
@@ -571,7 +635,9 @@ int bchip_cache_grow(bchip_ctx* c, const void* const* src, void* const* dst, uin
     std::vector<const void*> sv(nbufs, nullptr);
     if (keep > 0)
         for (uint32_t b = 0; b < nbufs; b++) sv[b] = src[b];
-    HIP_TRY(grow_launch(sv.data(), dst, nbufs, kb, tb, c->stream), "cache_grow");
+    HIP_TRY(type == BCHIP_Q4 ? grow_q4_launch(sv.data(), dst, nbufs, keep, total, c->stream)
+                             : grow_launch(sv.data(), dst, nbufs, kb, tb, c->stream),
+            "cache_grow");
     return BCHIP_OK;
 }
 
@@ -580,16 +646,20 @@ int bchip_keep(bchip_ctx* c, void* const* bufs, uint32_t nbufs, uint32_t type, u
     CHECK(enter(c));
     if (nbufs == 0 || nrows == 0) return BCHIP_OK;
     if (!bufs || !rows) return fail(BCHIP_E_ARG, "null pointer");
-    if (type > 1) return fail(BCHIP_E_ARG, "element type %u", type);
+    if (type > LAST_TYPE) return fail(BCHIP_E_ARG, "element type %u", type);
+    if (type == BCHIP_Q4 && width % Q4_BLOCK) return fail(BCHIP_E_ARG, "rows of %u: 4-bit codes move in blocks of %u", width, Q4_BLOCK);
     if (nrows > 64) return fail(BCHIP_E_ARG, "%u rows (at most 64)", nrows);
     for (uint32_t i = 0; i + 1 < nrows; i++)
         if (rows[i] >= rows[i + 1]) return fail(BCHIP_E_ARG, "rows are not an ascending path");
-    const uint64_t end = sat_mul(sat_mul(sat_add(base, (uint64_t)rows[nrows - 1] + 1), width), esize(type));
+    const uint64_t end = bytes_of(type, sat_mul(sat_add(base, (uint64_t)rows[nrows - 1] + 1), width));
     for (uint32_t b = 0; b < nbufs; b++) {
         if (!bufs[b]) return fail(BCHIP_E_ARG, "null buffer %u", b);
+        if (type == BCHIP_Q4 && !aligned16(bufs[b])) return fail(BCHIP_E_ARG, "buffer %u: not 16-byte aligned", b);
         CHECK(check_span(c, bufs[b], end, "keep"));
     }
-    HIP_TRY(keep_launch(bufs, nbufs, type, width, base, rows, nrows, c->stream), "keep");
+    HIP_TRY(type == BCHIP_Q4 ? keep_q4_launch(bufs, nbufs, width, base, rows, nrows, c->stream)
+                             : keep_launch(bufs, nbufs, type, width, base, rows, nrows, c->stream),
+            "keep");
     return BCHIP_OK;
 }
 
@@ -599,14 +669,18 @@ int bchip_rope_append(bchip_ctx* c, float* q, const float* k, const float* v, vo
     CHECK(enter(c));
     if (rows == 0) return BCHIP_OK;
     if (!q || !k || !v || !kc || !vc || !inv_freq || !positions) return fail(BCHIP_E_ARG, "null pointer");
-    if (kv_type > 1) return fail(BCHIP_E_ARG, "element type %u", kv_type);
+    if (kv_type > LAST_TYPE) return fail(BCHIP_E_ARG, "element type %u", kv_type);
     if (hd % 2 || rope_dim % 2 || rope_dim > hd) return fail(BCHIP_E_ARG, "rope_dim %u for head_dim %u", rope_dim, hd);
     if (nh == 0 || nkv == 0) return fail(BCHIP_E_ARG, "no heads");
+    if (kv_type == BCHIP_Q4) {
+        CHECK(check_q4(nkv, hd));
+        if (!aligned16(kc) || !aligned16(vc)) return fail(BCHIP_E_ARG, "4-bit caches must be 16-byte aligned");
+    }
     const uint64_t kvd = (uint64_t)nkv * hd;
     CHECK(check_span(c, q, sat_mul(sat_mul(rows, nh), (uint64_t)hd * 4), "q"));
     CHECK(check_span(c, k, sat_mul(rows, kvd * 4), "k"));
     CHECK(check_span(c, v, sat_mul(rows, kvd * 4), "v"));
-    const uint64_t cache_bytes = sat_mul(sat_mul(sat_add(slot0, rows), kvd), esize(kv_type));
+    const uint64_t cache_bytes = bytes_of(kv_type, sat_mul(sat_add(slot0, rows), kvd));
     CHECK(check_span(c, kc, cache_bytes, "kc"));
     CHECK(check_span(c, vc, cache_bytes, "vc"));
     CHECK(check_span(c, positions, (uint64_t)rows * 4, "positions"));
@@ -623,8 +697,9 @@ int bchip_attention(bchip_ctx* c, const float* q, const void* kc, const void* vc
     CHECK(enter(c));
     if (rows == 0) return BCHIP_OK;
     if (!q || !kc || !vc || !out) return fail(BCHIP_E_ARG, "null pointer");
-    if (kv_type > 1) return fail(BCHIP_E_ARG, "element type %u", kv_type);
+    if (kv_type > LAST_TYPE) return fail(BCHIP_E_ARG, "element type %u", kv_type);
     CHECK(check_heads(nh, nkv, hd));
+    if (kv_type == BCHIP_Q4) CHECK(check_q4(nkv, hd));
     if (!aligned16(q) || !aligned16(out) || !aligned16(kc) || !aligned16(vc))
         return fail(BCHIP_E_ARG, "q, out and the caches must be 16-byte aligned");
     if ((uint64_t)pos + rows > 0xffffffffull) return fail(BCHIP_E_ARG, "position past 2^32");
@@ -637,10 +712,9 @@ int bchip_attention(bchip_ctx* c, const float* q, const void* kc, const void* vc
     const uint64_t kvd = (uint64_t)nkv * hd, slots = (uint64_t)pos + rows;
     CHECK(check_span(c, q, sat_mul(sat_mul(rows, nh), (uint64_t)hd * 4), "q"));
     CHECK(check_span(c, out, sat_mul(sat_mul(rows, nh), (uint64_t)hd * 4), "out"));
-    CHECK(check_span(c, kc, sat_mul(slots, kvd * esize(kv_type)), "kc"));
-    CHECK(check_span(c, vc, sat_mul(slots, kvd * esize(kv_type)), "vc"));
-    const uint64_t row_bytes = kvd * esize(kv_type);
-    const uint64_t limit = std::min(bytes_left(c, kc), bytes_left(c, vc)) / row_bytes;
+    CHECK(check_span(c, kc, bytes_of(kv_type, sat_mul(slots, kvd)), "kc"));
+    CHECK(check_span(c, vc, bytes_of(kv_type, sat_mul(slots, kvd)), "vc"));
+    const uint64_t limit = slots_held(c, kc, vc, kv_type, kvd);
     AttnCall a{q, kc, vc, kv_type, out, masks, tree ? 1u : 0u, rows, nh, nkv, hd, pos, scale, limit};
     c->take_marks(a);
     hipError_t e;
@@ -650,8 +724,11 @@ int bchip_attention(bchip_ctx* c, const float* q, const void* kc, const void* vc
     // shared kernels, which read each K/V block once for every row and head of a KV head they
     // hold (split over the list when there are few of them). Every multi-row kernel computes a
     // row with the same arithmetic, so the choice does not change a bit of the result.
+    // 4-bit caches: kernels of their own for every form.
     if (kv_type == BCHIP_F32) {
         e = f32_attention(a, 0, c->ws, c->stream);
+    } else if (kv_type == BCHIP_Q4) {
+        e = q4_attention(a, c->ws, c->stream);
     } else if (rows == 1 && !tree) {
         Item item{};
         item.row = 0;
@@ -690,8 +767,9 @@ int bchip_rope_append_attention_rows(bchip_ctx* c, float* q, const float* k, con
     CHECK(enter(c));
     if (rows == 0) return BCHIP_OK;
     if (!q || !k || !v || !kc || !vc || !inv_freq || !positions || !out) return fail(BCHIP_E_ARG, "null pointer");
-    if (kv_type > 1) return fail(BCHIP_E_ARG, "element type %u", kv_type);
+    if (kv_type > LAST_TYPE) return fail(BCHIP_E_ARG, "element type %u", kv_type);
     CHECK(check_heads(nh, nkv, hd));
+    if (kv_type == BCHIP_Q4) CHECK(check_q4(nkv, hd));
     if (rope_dim % 2 || rope_dim > hd) return fail(BCHIP_E_ARG, "rope_dim %u for head_dim %u", rope_dim, hd);
     if (!aligned16(q) || !aligned16(out) || !aligned16(kc) || !aligned16(vc))
         return fail(BCHIP_E_ARG, "q, out and the caches must be 16-byte aligned");
@@ -701,13 +779,13 @@ int bchip_rope_append_attention_rows(bchip_ctx* c, float* q, const float* k, con
     CHECK(check_span(c, out, sat_mul(sat_mul(rows, nh), (uint64_t)hd * 4), "out"));
     CHECK(check_span(c, k, sat_mul(rows, kvd * 4), "k"));
     CHECK(check_span(c, v, sat_mul(rows, kvd * 4), "v"));
-    CHECK(check_span(c, kc, sat_mul(slots, kvd * esize(kv_type)), "kc"));
-    CHECK(check_span(c, vc, sat_mul(slots, kvd * esize(kv_type)), "vc"));
+    CHECK(check_span(c, kc, bytes_of(kv_type, sat_mul(slots, kvd)), "kc"));
+    CHECK(check_span(c, vc, bytes_of(kv_type, sat_mul(slots, kvd)), "vc"));
     CHECK(check_span(c, positions, (uint64_t)rows * 4, "positions"));
     CHECK(check_span(c, inv_freq, (uint64_t)(rope_dim / 2) * 4, "inv_freq"));
     if (kv_type == BCHIP_F32 && rows <= 8) {
         // f32 caches: attn_f32_step rotates q and appends the new rows itself (the two calls' bits).
-        const uint64_t limit = std::min(bytes_left(c, kc), bytes_left(c, vc)) / (kvd * esize(kv_type));
+        const uint64_t limit = slots_held(c, kc, vc, kv_type, kvd);
         AttnCall a{q, kc, vc, kv_type, out, nullptr, 0u, rows, nh, nkv, hd, pos, scale, limit};
         const RopeArgs r{q, k, v, inv_freq, positions, rope_dim, neox};
         c->take_marks(a);
@@ -716,7 +794,7 @@ int bchip_rope_append_attention_rows(bchip_ctx* c, float* q, const float* k, con
     }
     // (The one-launch form loads the new k and v rows 16 bytes a lane.)
     if (kv_type == BCHIP_F16 && rows > 1 && aligned16(k) && aligned16(v)) {
-        const uint64_t limit = std::min(bytes_left(c, kc), bytes_left(c, vc)) / (kvd * esize(kv_type));
+        const uint64_t limit = slots_held(c, kc, vc, kv_type, kvd);
         AttnCall a{q, kc, vc, kv_type, out, nullptr, 0u, rows, nh, nkv, hd, pos, scale, limit};
         const RopeArgs r{q, k, v, inv_freq, positions, rope_dim, neox};
         c->take_marks(a);
@@ -742,8 +820,9 @@ static int fused_step(bchip_ctx* c, Workspace& ws, float* q, const float* k, con
                       float* out) {
     CHECK(enter(c));
     if (!q || !k || !v || !kc || !vc || !inv_freq || !positions || !out) return fail(BCHIP_E_ARG, "null pointer");
-    if (kv_type > 1) return fail(BCHIP_E_ARG, "element type %u", kv_type);
+    if (kv_type > LAST_TYPE) return fail(BCHIP_E_ARG, "element type %u", kv_type);
     CHECK(check_heads(nh, nkv, hd));
+    if (kv_type == BCHIP_Q4) CHECK(check_q4(nkv, hd));
     if (rope_dim % 2 || rope_dim > hd) return fail(BCHIP_E_ARG, "rope_dim %u for head_dim %u", rope_dim, hd);
     const bool fuse = kv_type == BCHIP_F16 && row_fusable(nh, nkv, hd, rope_dim, neox);
     if (!aligned16(q) || !aligned16(out) || !aligned16(kc) || !aligned16(vc) || (fuse && (!aligned16(k) || !aligned16(v))))
@@ -754,8 +833,8 @@ static int fused_step(bchip_ctx* c, Workspace& ws, float* q, const float* k, con
     CHECK(check_span(c, out, sat_mul(nh, (uint64_t)hd * 4), "out"));
     CHECK(check_span(c, k, kvd * 4, "k"));
     CHECK(check_span(c, v, kvd * 4, "v"));
-    CHECK(check_span(c, kc, sat_mul(slots, kvd * esize(kv_type)), "kc"));
-    CHECK(check_span(c, vc, sat_mul(slots, kvd * esize(kv_type)), "vc"));
+    CHECK(check_span(c, kc, bytes_of(kv_type, sat_mul(slots, kvd)), "kc"));
+    CHECK(check_span(c, vc, bytes_of(kv_type, sat_mul(slots, kvd)), "vc"));
     CHECK(check_span(c, positions, 4, "positions"));
     CHECK(check_span(c, inv_freq, (uint64_t)(rope_dim / 2) * 4, "inv_freq"));
     if (ws.fixed && kv_type == BCHIP_F16) {
@@ -767,13 +846,19 @@ static int fused_step(bchip_ctx* c, Workspace& ws, float* q, const float* k, con
                         "entry point holds %zu and %zu",
                         need * hdp * 4, fuse ? (size_t)nh * hd * 4 : (size_t)0, ws.o_cap, ws.qrot_cap);
     }
-    const uint64_t limit = std::min(bytes_left(c, kc), bytes_left(c, vc)) / (kvd * esize(kv_type));
+    const uint64_t limit = slots_held(c, kc, vc, kv_type, kvd);
     AttnCall a{q, kc, vc, kv_type, out, nullptr, 0u, 1u, nh, nkv, hd, pos, scale, limit};
     c->take_marks(a);
     if (kv_type == BCHIP_F32) {
         // f32 caches: attn_f32_step rotates q and appends the new row itself (the two calls' bits).
         const RopeArgs r{q, k, v, inv_freq, positions, rope_dim, neox};
         HIP_TRY(f32_attention(a, 0, ws, c->stream, &r), "rope_append_attention");
+        return BCHIP_OK;
+    }
+    if (kv_type == BCHIP_Q4) {
+        HIP_TRY(rope_append_launch(q, k, v, kc, vc, kv_type, inv_freq, positions, 1, nh, nkv, hd, rope_dim, neox, pos, c->stream),
+                "rope_append");
+        HIP_TRY(q4_attention(a, ws, c->stream), "rope_append_attention");
         return BCHIP_OK;
     }
     if (!fuse) {
@@ -818,7 +903,7 @@ static int check_ragged(bchip_ctx* c, const void* kc, const void* vc, uint32_t k
     if (nseq > 256) return fail(BCHIP_E_ARG, "%u sequences (at most 256)", nseq);
     for (uint32_t i = 0; i < nseq; i++) {
         if (seq_lens[i] == 0) return fail(BCHIP_E_ARG, "sequence %u sees no slots", i);
-        const uint64_t end = sat_mul(sat_mul(sat_add(kv_offsets[i], seq_lens[i]), kvd), esize(kv_type));
+        const uint64_t end = bytes_of(kv_type, sat_mul(sat_add(kv_offsets[i], seq_lens[i]), kvd));
         CHECK(check_span(c, kc, end, "kc"));
         CHECK(check_span(c, vc, end, "vc"));
     }
@@ -850,6 +935,10 @@ static int ragged_attention(bchip_ctx* c, AttnCall& a, const uint32_t* seq_lens,
         }
         return BCHIP_OK;
     }
+    if (a.kv_type == BCHIP_Q4) {
+        HIP_TRY(q4_attention_ragged(a, seq_lens, kv_offsets, nseq, c->ws, c->stream), "ragged attention");
+        return BCHIP_OK;
+    }
     for (uint32_t s0 = 0; s0 < nseq; s0 += MAX_ITEMS) {
         const uint32_t ns = std::min<uint32_t>(MAX_ITEMS, nseq - s0);
         Item items[MAX_ITEMS];
@@ -873,15 +962,16 @@ int bchip_attention_ragged(bchip_ctx* c, const float* q, const void* kc, const v
     CHECK(enter(c));
     if (nseq == 0) return BCHIP_OK;
     if (!q || !kc || !vc || !out || !seq_lens || !kv_offsets) return fail(BCHIP_E_ARG, "null pointer");
-    if (kv_type > 1) return fail(BCHIP_E_ARG, "element type %u", kv_type);
+    if (kv_type > LAST_TYPE) return fail(BCHIP_E_ARG, "element type %u", kv_type);
     CHECK(check_heads(nh, nkv, hd));
+    if (kv_type == BCHIP_Q4) CHECK(check_q4(nkv, hd));
     if (!aligned16(q) || !aligned16(out) || !aligned16(kc) || !aligned16(vc))
         return fail(BCHIP_E_ARG, "q, out and the caches must be 16-byte aligned");
     const uint64_t kvd = (uint64_t)nkv * hd;
     CHECK(check_span(c, q, sat_mul(sat_mul(nseq, nh), (uint64_t)hd * 4), "q"));
     CHECK(check_span(c, out, sat_mul(sat_mul(nseq, nh), (uint64_t)hd * 4), "out"));
     CHECK(check_ragged(c, kc, vc, kv_type, seq_lens, kv_offsets, nseq, kvd));
-    const uint64_t limit = std::min(bytes_left(c, kc), bytes_left(c, vc)) / (kvd * esize(kv_type));
+    const uint64_t limit = slots_held(c, kc, vc, kv_type, kvd);
     AttnCall a{q, kc, vc, kv_type, out, nullptr, 0u, 1u, nh, nkv, hd, 0u, scale, limit};
     c->take_marks(a);
     return ragged_attention(c, a, seq_lens, kv_offsets, nseq);
@@ -895,9 +985,13 @@ int bchip_rope_append_ragged(bchip_ctx* c, float* q, const float* k, const float
     if (nseq == 0) return BCHIP_OK;
     if (!q || !k || !v || !kc || !vc || !inv_freq || !positions || !seq_lens || !kv_offsets)
         return fail(BCHIP_E_ARG, "null pointer");
-    if (kv_type > 1) return fail(BCHIP_E_ARG, "element type %u", kv_type);
+    if (kv_type > LAST_TYPE) return fail(BCHIP_E_ARG, "element type %u", kv_type);
     if (hd % 2 || rope_dim % 2 || rope_dim > hd) return fail(BCHIP_E_ARG, "rope_dim %u for head_dim %u", rope_dim, hd);
     if (nh == 0 || nkv == 0) return fail(BCHIP_E_ARG, "no heads");
+    if (kv_type == BCHIP_Q4) {
+        CHECK(check_q4(nkv, hd));
+        if (!aligned16(kc) || !aligned16(vc)) return fail(BCHIP_E_ARG, "4-bit caches must be 16-byte aligned");
+    }
     const uint64_t kvd = (uint64_t)nkv * hd;
     CHECK(check_span(c, q, sat_mul(sat_mul(nseq, nh), (uint64_t)hd * 4), "q"));
     CHECK(check_span(c, k, sat_mul(nseq, kvd * 4), "k"));
@@ -922,8 +1016,9 @@ int bchip_rope_append_attention_ragged(bchip_ctx* c, float* q, const float* k, c
     if (nseq == 0) return BCHIP_OK;
     if (!q || !k || !v || !kc || !vc || !inv_freq || !positions || !seq_lens || !kv_offsets || !out)
         return fail(BCHIP_E_ARG, "null pointer");
-    if (kv_type > 1) return fail(BCHIP_E_ARG, "element type %u", kv_type);
+    if (kv_type > LAST_TYPE) return fail(BCHIP_E_ARG, "element type %u", kv_type);
     CHECK(check_heads(nh, nkv, hd));
+    if (kv_type == BCHIP_Q4) CHECK(check_q4(nkv, hd));
     if (rope_dim % 2 || rope_dim > hd) return fail(BCHIP_E_ARG, "rope_dim %u for head_dim %u", rope_dim, hd);
     const bool fuse = kv_type == BCHIP_F16 && row_fusable(nh, nkv, hd, rope_dim, neox);
     if (!aligned16(q) || !aligned16(out) || !aligned16(kc) || !aligned16(vc) || (fuse && (!aligned16(k) || !aligned16(v))))
@@ -936,7 +1031,7 @@ int bchip_rope_append_attention_ragged(bchip_ctx* c, float* q, const float* k, c
     CHECK(check_span(c, positions, (uint64_t)nseq * 4, "positions"));
     CHECK(check_span(c, inv_freq, (uint64_t)(rope_dim / 2) * 4, "inv_freq"));
     CHECK(check_ragged(c, kc, vc, kv_type, seq_lens, kv_offsets, nseq, kvd));
-    const uint64_t limit = std::min(bytes_left(c, kc), bytes_left(c, vc)) / (kvd * esize(kv_type));
+    const uint64_t limit = slots_held(c, kc, vc, kv_type, kvd);
     AttnCall a{q, kc, vc, kv_type, out, nullptr, 0u, 1u, nh, nkv, hd, 0u, scale, limit};
     c->take_marks(a);
     if (!fuse) {
@@ -991,7 +1086,7 @@ int bchip_fill_normal(bchip_ctx* c, void* dst, uint32_t type, uint64_t n, uint64
     if (n == 0) return BCHIP_OK;
     if (!dst) return fail(BCHIP_E_ARG, "null pointer");
     if (type > 1) return fail(BCHIP_E_ARG, "element type %u", type);
-    CHECK(check_span(c, dst, sat_mul(n, esize(type)), "fill"));
+    CHECK(check_span(c, dst, bytes_of(type, n), "fill"));
     HIP_TRY(fill_normal_launch(dst, type, n, seed, c->stream), "fill_normal");
     return BCHIP_OK;
 }

@@ -1,0 +1,255 @@
+// What a cache in 4 bits (q4.hpp) needs beside attention: the rotation and append of new rows,
+// conversion to and from f32 and f16, and the moves of a cache's rows.
+//
+// k_rope_append_q4 is k_rope_append (rope.hip) over such a cache: q rotates in place with the
+// same expressions, and k, rotated the same, and v go into the cache as codes. A thread takes
+// one pair of a q head or two consecutive elements of a k or v head, so sixteen lanes hold a
+// block and agree on its scale by four shuffles. Bound by q's traffic for many rows (512 rows
+// of 32 + 2 x 8 heads of 128) and by the launch for few.
+#include "common.hpp"
+#include "internal.hpp"
+#include "q4.hpp"
+
+#include <type_traits>
+
+namespace bchip {
+
+struct Q4RowSlots {
+    uint64_t slot[MAX_ITEMS];
+};
+
+// Element e of a head x of hd elements after the rotation of its pairs by pos * inv_freq.
+__device__ __forceinline__ float rotated(const float* x, uint32_t e, float pos, const float* inv_freq,
+                                         uint32_t rope_dim, uint32_t neox) {
+    if (e >= rope_dim) return x[e];
+    const uint32_t hh = rope_dim / 2;
+    const uint32_t i = neox ? (e < hh ? e : e - hh) : e / 2;
+    const uint32_t a = neox ? i : 2 * i, b = neox ? i + hh : 2 * i + 1;
+    float y0, y1;
+    rotate(x[a], x[b], pos * inv_freq[i], y0, y1);
+    return e == a ? y0 : y1;
+}
+
+// Row r goes to slot slot0 + r, or (RAGGED) to sl.slot[r]. hd a multiple of 32.
+template <bool RAGGED>
+__global__ __launch_bounds__(256) void k_rope_append_q4(float* __restrict__ q, const float* __restrict__ k,
+                                                        const float* __restrict__ v, uint8_t* __restrict__ kc,
+                                                        uint8_t* __restrict__ vc, const float* __restrict__ inv_freq,
+                                                        const uint32_t* __restrict__ positions, uint32_t rows,
+                                                        uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t rope_dim,
+                                                        uint32_t neox, uint64_t slot0, const Q4RowSlots sl) {
+    const uint32_t half = hd / 2, heads = nh + 2 * nkv;
+    const uint64_t idx = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (idx >= (uint64_t)rows * heads * half) return;  // (whole blocks of sixteen lanes: half % 16 == 0)
+    const uint32_t p = idx % half, hx = (idx / half) % heads;
+    const uint64_t r = idx / ((uint64_t)half * heads);
+    if (hx < nh) {
+        uint32_t a, b;
+        if (!rope_pair(p, rope_dim, neox, a, b)) return;
+        float* hp = q + (r * nh + hx) * hd;
+        float y0, y1;
+        rotate(hp[a], hp[b], (float)positions[r] * inv_freq[p], y0, y1);
+        hp[a] = y0;
+        hp[b] = y1;
+        return;
+    }
+    const bool isk = hx < nh + nkv;
+    const uint32_t kh = isk ? hx - nh : hx - nh - nkv;
+    const float* hp = (isk ? k : v) + (r * nkv + kh) * hd;
+    float x0, x1;
+    if (!isk) {
+        x0 = hp[2 * p];
+        x1 = hp[2 * p + 1];
+    } else if (!neox && 2 * p < rope_dim) {
+        rotate(hp[2 * p], hp[2 * p + 1], (float)positions[r] * inv_freq[p], x0, x1);
+    } else {
+        const float pos = (float)positions[r];
+        x0 = rotated(hp, 2 * p, pos, inv_freq, rope_dim, neox);
+        x1 = rotated(hp, 2 * p + 1, pos, inv_freq, rope_dim, neox);
+    }
+    uint8_t codes;
+    const f16 d = q4_quantise(x0, x1, codes);
+    const uint64_t e = (RAGGED ? sl.slot[r] : slot0 + r) * ((uint64_t)nkv * hd) + (uint64_t)kh * hd + 2 * p;
+    uint8_t* dst = isk ? kc : vc;
+    dst[q4_code_at(e)] = codes;
+    if (p % 16 == 0) *(f16*)(dst + q4_scale_at(e)) = d;
+}
+
+// dst[off + i] = src[i]: two elements a thread, n and off multiples of 32.
+template <typename S>
+__global__ __launch_bounds__(256) void k_to_q4(const S* __restrict__ src, uint8_t* __restrict__ dst, uint64_t off,
+                                               uint64_t n) {
+    // (n / 2 is a multiple of 16 and so is every stride: blocks stay within sixteen lanes.)
+    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n / 2; i += (uint64_t)gridDim.x * blockDim.x) {
+        uint8_t codes;
+        const f16 d = q4_quantise((float)src[2 * i], (float)src[2 * i + 1], codes);
+        const uint64_t e = off + 2 * i;
+        dst[q4_code_at(e)] = codes;
+        if (i % 16 == 0) *(f16*)(dst + q4_scale_at(e)) = d;
+    }
+}
+
+// dst[i] = src[i]: eight elements a thread. An f16 holds every value exactly.
+template <typename D>
+__global__ __launch_bounds__(256) void k_from_q4(const uint8_t* __restrict__ src, D* __restrict__ dst, uint64_t n) {
+    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n / 8; i += (uint64_t)gridDim.x * blockDim.x) {
+        const uint32_t w = *(const uint32_t*)(src + q4_code_at(8 * i));
+        const float d = (float)*(const f16*)(src + q4_scale_at(8 * i));
+#pragma unroll
+        for (int j = 0; j < 8; j++) dst[8 * i + j] = (D)(((float)((w >> (4 * j)) & 15u) - 8.0f) * d);
+    }
+}
+
+// A block's codes and scale.
+struct Q4Block {
+    uint4 codes;
+    uint16_t scale;
+};
+__device__ __forceinline__ Q4Block q4_block(const uint8_t* b, uint64_t i) {
+    return {*(const uint4*)(b + q4_code_at(i * Q4_BLOCK)), *(const uint16_t*)(b + q4_scale_at(i * Q4_BLOCK))};
+}
+__device__ __forceinline__ void q4_put(uint8_t* b, uint64_t i, const Q4Block& x) {
+    *(uint4*)(b + q4_code_at(i * Q4_BLOCK)) = x.codes;
+    *(uint16_t*)(b + q4_scale_at(i * Q4_BLOCK)) = x.scale;
+}
+
+// dst block to + i = src block from + i, a block a thread; src may be dst where the ranges do
+// not overlap.
+__global__ __launch_bounds__(256) void k_blocks_q4(const uint8_t* src, uint8_t* dst, uint64_t from, uint64_t to,
+                                                   uint64_t n) {
+    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (uint64_t)gridDim.x * blockDim.x)
+        q4_put(dst, to + i, q4_block(src, from + i));
+}
+
+struct Q4KeepArgs {
+    uint8_t* bufs[64];
+    uint32_t rows[64];
+};
+
+// k_keep (kvcache.hip) with a block a thread: the moves of one block column, in order.
+__global__ __launch_bounds__(256) void k_keep_q4(const Q4KeepArgs a, uint32_t nbufs, uint32_t width, uint64_t base,
+                                                 uint32_t nrows) {
+    const uint32_t col = blockIdx.x * blockDim.x + threadIdx.x;
+    if (col >= width || blockIdx.y >= nbufs) return;
+    uint8_t* b = a.bufs[blockIdx.y];
+    for (uint32_t i = 0; i < nrows; i++) {
+        const uint32_t r = a.rows[i];
+        if (r != i) q4_put(b, (base + i) * width + col, q4_block(b, (base + r) * width + col));
+    }
+}
+
+struct Q4GrowArgs {
+    const uint8_t* src[64];
+    uint8_t* dst[64];
+};
+
+// k_grow with a block a thread: the first `keep` blocks copied, zeros behind them.
+__global__ __launch_bounds__(256) void k_grow_q4(const Q4GrowArgs a, uint64_t keep, uint64_t total) {
+    const uint8_t* src = a.src[blockIdx.y];
+    uint8_t* dst = a.dst[blockIdx.y];
+    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x)
+        q4_put(dst, i, i < keep ? q4_block(src, i) : Q4Block{{0u, 0u, 0u, 0u}, 0});
+}
+
+static uint32_t blocks_of(uint64_t n) { return (uint32_t)((n + 255) / 256); }
+static uint32_t grid_of(uint64_t n) {
+    const uint64_t b = (n + 255) / 256;
+    return (uint32_t)(b > 65536 ? 65536 : (b ? b : 1));
+}
+
+hipError_t rope_append_q4_launch(float* q, const float* k, const float* v, void* kc, void* vc, const float* inv_freq,
+                                 const uint32_t* positions, uint32_t rows, uint32_t nh, uint32_t nkv, uint32_t hd,
+                                 uint32_t rope_dim, uint32_t neox, uint64_t slot0, const uint64_t* slots,
+                                 hipStream_t s) {
+    const uint64_t per_row = (uint64_t)(nh + 2 * nkv) * (hd / 2);
+    if (!slots) {
+        if (rows * per_row == 0) return hipSuccess;
+        hipLaunchKernelGGL(k_rope_append_q4<false>, dim3(blocks_of(rows * per_row)), dim3(256), 0, s, q, k, v,
+                           (uint8_t*)kc, (uint8_t*)vc, inv_freq, positions, rows, nh, nkv, hd, rope_dim, neox, slot0,
+                           Q4RowSlots{});
+        return hipGetLastError();
+    }
+    for (uint32_t r0 = 0; r0 < rows; r0 += MAX_ITEMS) {
+        const uint32_t nr = rows - r0 < MAX_ITEMS ? rows - r0 : MAX_ITEMS;
+        Q4RowSlots sl{};
+        for (uint32_t i = 0; i < nr; i++) sl.slot[i] = slots[r0 + i];
+        hipLaunchKernelGGL(k_rope_append_q4<true>, dim3(blocks_of(nr * per_row)), dim3(256), 0, s,
+                           q + (size_t)r0 * nh * hd, k + (size_t)r0 * nkv * hd, v + (size_t)r0 * nkv * hd,
+                           (uint8_t*)kc, (uint8_t*)vc, inv_freq, positions + r0, nr, nh, nkv, hd, rope_dim, neox, 0ull,
+                           sl);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+hipError_t copy_q4_launch(const void* src, uint32_t st, void* dst, uint32_t dt, uint64_t off, uint64_t n,
+                          hipStream_t s) {
+    if (n == 0) return hipSuccess;
+    if (st == 2 && dt == 2)
+        hipLaunchKernelGGL(k_blocks_q4, dim3(grid_of(n / Q4_BLOCK)), dim3(256), 0, s, (const uint8_t*)src,
+                           (uint8_t*)dst, 0ull, off / Q4_BLOCK, n / Q4_BLOCK);
+    else if (dt == 2 && st == 1)
+        hipLaunchKernelGGL(k_to_q4<f16>, dim3(grid_of(n / 2)), dim3(256), 0, s, (const f16*)src, (uint8_t*)dst, off, n);
+    else if (dt == 2)
+        hipLaunchKernelGGL(k_to_q4<float>, dim3(grid_of(n / 2)), dim3(256), 0, s, (const float*)src, (uint8_t*)dst, off,
+                           n);
+    else if (dt == 1)
+        hipLaunchKernelGGL(k_from_q4<f16>, dim3(grid_of(n / 8)), dim3(256), 0, s, (const uint8_t*)src, (f16*)dst + off,
+                           n);
+    else
+        hipLaunchKernelGGL(k_from_q4<float>, dim3(grid_of(n / 8)), dim3(256), 0, s, (const uint8_t*)src,
+                           (float*)dst + off, n);
+    return hipGetLastError();
+}
+
+hipError_t move_q4_launch(void* buf, uint64_t from, uint64_t to, uint64_t n, hipStream_t s) {
+    if (n == 0 || from == to) return hipSuccess;
+    // Overlapping ranges move in pieces of from - to, as in move_launch.
+    const uint64_t f = from / Q4_BLOCK, t = to / Q4_BLOCK, nb = n / Q4_BLOCK, step = f - t < nb ? f - t : nb;
+    for (uint64_t o = 0; o < nb; o += step) {
+        const uint64_t m = nb - o < step ? nb - o : step;
+        hipLaunchKernelGGL(k_blocks_q4, dim3(grid_of(m)), dim3(256), 0, s, (const uint8_t*)buf, (uint8_t*)buf, f + o,
+                           t + o, m);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+hipError_t keep_q4_launch(void* const* bufs, uint32_t nbufs, uint32_t width, uint64_t base, const uint32_t* rows,
+                          uint32_t nrows, hipStream_t s) {
+    if (nbufs == 0 || nrows == 0 || width == 0) return hipSuccess;
+    const uint32_t wb = width / Q4_BLOCK;
+    for (uint32_t b0 = 0; b0 < nbufs; b0 += 64) {
+        Q4KeepArgs a{};
+        const uint32_t nb = nbufs - b0 < 64 ? nbufs - b0 : 64;
+        for (uint32_t i = 0; i < nb; i++) a.bufs[i] = (uint8_t*)bufs[b0 + i];
+        for (uint32_t i = 0; i < nrows; i++) a.rows[i] = rows[i];
+        hipLaunchKernelGGL(k_keep_q4, dim3((wb + 255) / 256, nb), dim3(256), 0, s, a, nb, wb, base, nrows);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+hipError_t grow_q4_launch(const void* const* src, void* const* dst, uint32_t nbufs, uint64_t keep, uint64_t total,
+                          hipStream_t s) {
+    if (nbufs == 0 || total == 0) return hipSuccess;
+    for (uint32_t b0 = 0; b0 < nbufs; b0 += 64) {
+        Q4GrowArgs a{};
+        const uint32_t nb = nbufs - b0 < 64 ? nbufs - b0 : 64;
+        for (uint32_t i = 0; i < nb; i++) {
+            a.src[i] = (const uint8_t*)src[b0 + i];
+            a.dst[i] = (uint8_t*)dst[b0 + i];
+        }
+        const uint64_t blocks = total / Q4_BLOCK;
+        const uint32_t gx = (uint32_t)((blocks + 255) / 256 > 2048 ? 2048 : (blocks + 255) / 256);
+        hipLaunchKernelGGL(k_grow_q4, dim3(gx, nb), dim3(256), 0, s, a, keep / Q4_BLOCK, blocks);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+}  // namespace bchip

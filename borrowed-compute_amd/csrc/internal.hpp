@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <vector>
+
 #include "common.hpp"
 
 namespace bchip {
@@ -48,6 +50,16 @@ struct Workspace {
     hipError_t reserve(size_t need_slots, size_t hd_pad);
     hipError_t reserve_qrot(size_t floats);
     hipError_t reserve_vt(size_t bytes);
+    // The same for a call that has a form without scratch: false where none is to be had, the
+    // memory full or the stream captured over a workspace too small (nothing can be allocated
+    // there). Memory that a capture took stays where it is until the context ends: a graph may
+    // be replayed after a larger call has moved the workspace on.
+    bool reserve_if(size_t need_slots, size_t hd_pad, hipStream_t s);
+    bool reserve_vt_if(size_t bytes, hipStream_t s);
+    bool captured = false;
+    std::vector<void*> retired;
+    void drop(void* p);
+    bool had(hipStream_t s, bool enough);
     void release();
 };
 
@@ -59,7 +71,7 @@ struct AttnCall {
     const float* q;
     const void* kc;
     const void* vc;
-    uint32_t kv_type;  // 0 f32, 1 f16
+    uint32_t kv_type;  // 0 f32, 1 f16, 2 4-bit codes
     float* out;
     const uint32_t* masks;
     uint32_t tree, rows, nh, nkv, hd, pos;
@@ -110,6 +122,12 @@ hipError_t combine_launch(CombineParams& cp, uint32_t groups, uint32_t hd, hipSt
 hipError_t f32_attention(const AttnCall& a, uint64_t kvoff, Workspace& ws, hipStream_t s,
                          const RopeArgs* rope = nullptr);
 
+// Every call on a 4-bit cache (attention_q4.hip): lines, trees, one row; and a ragged batch of
+// one-row calls over a pool.
+hipError_t q4_attention(const AttnCall& a, Workspace& ws, hipStream_t s);
+hipError_t q4_attention_ragged(const AttnCall& a, const uint32_t* lens, const uint64_t* offs, uint32_t nseq,
+                               Workspace& ws, hipStream_t s);
+
 hipError_t rope_launch(float* x, const float* inv_freq, const uint32_t* positions, uint32_t rows,
                        uint32_t heads, uint32_t hd, uint32_t rope_dim, uint32_t neox, hipStream_t s);
 hipError_t rope_append_launch(float* q, const float* k, const float* v, void* kc, void* vc, uint32_t kv_type,
@@ -128,6 +146,19 @@ hipError_t keep_launch(void* const* bufs, uint32_t nbufs, uint32_t type, uint32_
                        const uint32_t* rows, uint32_t nrows, hipStream_t s);
 hipError_t grow_launch(const void* const* src, void* const* dst, uint32_t nbufs, uint64_t keep_bytes,
                        uint64_t total_bytes, hipStream_t s);
+// The same over 4-bit caches (cache_q4.hip); offsets and counts in elements, multiples of 32.
+// slots: a slot for each row (a ragged append), or null for slots slot0 + r.
+hipError_t rope_append_q4_launch(float* q, const float* k, const float* v, void* kc, void* vc, const float* inv_freq,
+                                 const uint32_t* positions, uint32_t rows, uint32_t nh, uint32_t nkv, uint32_t hd,
+                                 uint32_t rope_dim, uint32_t neox, uint64_t slot0, const uint64_t* slots,
+                                 hipStream_t s);
+hipError_t copy_q4_launch(const void* src, uint32_t st, void* dst, uint32_t dt, uint64_t off, uint64_t n,
+                          hipStream_t s);
+hipError_t move_q4_launch(void* buf, uint64_t from, uint64_t to, uint64_t n, hipStream_t s);
+hipError_t keep_q4_launch(void* const* bufs, uint32_t nbufs, uint32_t width, uint64_t base, const uint32_t* rows,
+                          uint32_t nrows, hipStream_t s);
+hipError_t grow_q4_launch(const void* const* src, void* const* dst, uint32_t nbufs, uint64_t keep, uint64_t total,
+                          hipStream_t s);
 hipError_t fill_normal_launch(void* dst, uint32_t type, uint64_t n, uint64_t seed, hipStream_t s);
 
 // The sampler (sample.hip): ids[r] = sample.rs's pick for row r of scores [rows][vocab] at step

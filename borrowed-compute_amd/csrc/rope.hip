@@ -105,6 +105,9 @@ hipError_t rope_append_launch(float* q, const float* k, const float* v, void* kc
                               hipStream_t s) {
     const uint64_t n = (uint64_t)rows * (nh + 2 * nkv) * (hd / 2);
     if (n == 0) return hipSuccess;
+    if (kv_type == 2)
+        return rope_append_q4_launch(q, k, v, kc, vc, inv_freq, positions, rows, nh, nkv, hd, rope_dim, neox, slot0,
+                                     nullptr, s);
     const RowSlots none{};
     if (kv_type == 1)
         hipLaunchKernelGGL((k_rope_append<f16, false>), dim3(blocks_of(n)), dim3(256), 0, s, q, k, v, (f16*)kc,
@@ -119,6 +122,9 @@ hipError_t rope_append_ragged_launch(float* q, const float* k, const float* v, v
                                      const float* inv_freq, const uint32_t* positions, uint32_t rows, uint32_t nh,
                                      uint32_t nkv, uint32_t hd, uint32_t rope_dim, uint32_t neox,
                                      const uint64_t* slots, hipStream_t s) {
+    if (kv_type == 2)
+        return rope_append_q4_launch(q, k, v, kc, vc, inv_freq, positions, rows, nh, nkv, hd, rope_dim, neox, 0, slots,
+                                     s);
     for (uint32_t r0 = 0; r0 < rows; r0 += MAX_ITEMS) {
         const uint32_t nr = rows - r0 < MAX_ITEMS ? rows - r0 : MAX_ITEMS;
         RowSlots sl{};

@@ -15,10 +15,21 @@
  *  - All kernels run in order on the context's one stream (cuda.rs:40, one stream);
  *    launches return before the work ends; bchip_sync waits (cuda.rs:93). The caller
  *    serialises calls on one context, as the reference's Gpu mutex does (mod.rs:105-107).
- *  - Element types of cache buffers: BCHIP_F32 (the reference's f32 cache, mod.rs:409-421)
- *    or BCHIP_F16 (IEEE binary16, rounded to nearest even: new with this backend).
+ *  - Element types of cache buffers: BCHIP_F32 (the reference's f32 cache, mod.rs:409-421),
+ *    BCHIP_F16 (IEEE binary16, rounded to nearest even: new with this backend) or BCHIP_Q4
+ *    (4-bit codes in blocks of 32 that share a scale: 9/32 of an f16 cache's bytes, below).
  *  - Cache layout is the reference's: per layer, K and V each [slots][n_head_kv*head_dim]
  *    (slot t of KV head h at t*kvd + h*head_dim, mod.rs:473-475, kernels.h:287,310).
+ *  - A BCHIP_Q4 buffer of n elements is ceil(n / 256) units of 144 bytes, 16-byte aligned: 128
+ *    bytes of codes (two a byte, the even element in the low four bits), then the f16 scales of
+ *    the unit's eight blocks of 32 elements. An element is (code - 8) * scale. The library writes
+ *    as a block's scale the value of its largest magnitude over -8 (of two, the positive one),
+ *    rounded to 7 significant bits and held within 2^-14 .. 896 (values past 7168 saturate), and
+ *    as a code the value over the scale to the nearest even; a block with an element that is not
+ *    finite gets the scale NaN and reads as NaN. A buffer written elsewhere has to keep to such
+ *    scales. Element offsets, counts and row widths are multiples of 32, and cache calls take
+ *    head dims that are multiples of 32 and slots of at most 2^24 elements (else
+ *    BCHIP_E_UNSUPPORTED).
  */
 #ifndef BCHIP_H
 #define BCHIP_H
@@ -32,7 +43,7 @@ extern "C" {
 
 #define BCHIP_ABI_VERSION 6
 
-enum bchip_type { BCHIP_F32 = 0, BCHIP_F16 = 1 }; /* T_F32 / T_F16 of kernels.h:14-15 */
+enum bchip_type { BCHIP_F32 = 0, BCHIP_F16 = 1, BCHIP_Q4 = 2 }; /* T_F32 / T_F16 of kernels.h:14-15 */
 
 enum bchip_status {
     BCHIP_OK = 0,
@@ -84,7 +95,8 @@ int bchip_rope(bchip_ctx* ctx, float* x, const float* inv_freq, const uint32_t* 
 
 /* k_copy (kernels.h:332, entry cuda.cu:90; mod.rs:413-420, 473-475):
  * dst[dst_off + i] = src[i] for i < n (element offsets and counts), converting from
- * src_type to dst_type (f32 -> f16 rounds to nearest even). */
+ * src_type to dst_type (f32 -> f16 rounds to nearest even; to and from 4-bit codes as above:
+ * an f16 holds every 4-bit value exactly). */
 int bchip_copy(bchip_ctx* ctx, const void* src, uint32_t src_type, void* dst,
                uint32_t dst_type, uint64_t dst_off, uint64_t n);
 
@@ -141,7 +153,16 @@ int bchip_rope_append(bchip_ctx* ctx, float* q, const float* k, const float* v, 
  * token. A one-row call (a decode step) cuts its list into at most 256 chunks (their length
  * set by the list length and nkv alone) and folds the chunk states in a fixed order:
  * deterministic, and within rounding of the same row in a batch (the reference allows
- * 1e-4, model.rs:641-642). */
+ * 1e-4, model.rs:641-642).
+ * 4-bit caches: K and V are exact f16 MFMA operands, q and the softmax weights two f16 each (22
+ * bits), f32 accumulation: results within f32 rounding of the formula. Lists are cut into chunks
+ * by the call's size, so a row alone, in a batch, in a tree or a ragged call agrees within f32
+ * rounding, not bit for bit; reruns give the same bits. A row that sees no slot gives zeros; a
+ * row whose q is not finite NaN; a NaN block of K or V reaches the rows that see its slot, and
+ * no other. No slot past the highest that a mask names is read; one past the end of a
+ * bchip_alloc buffer is left out. Where scratch cannot be had (memory full, a call under graph
+ * capture that has not run before at its size) lists run uncut. Scratch that a captured call
+ * took stays valid until the context is destroyed; replays run one at a time. */
 int bchip_attention(bchip_ctx* ctx, const float* q, const void* kc, const void* vc,
                     uint32_t kv_type, float* out, const uint32_t* masks, uint32_t tree,
                     uint32_t rows, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t pos,
@@ -155,8 +176,8 @@ int bchip_attention(bchip_ctx* ctx, const float* q, const void* kc, const void* 
  * and the append run inside the attention kernel, which takes the new row from registers
  * (f16 caches) or LDS (f32 caches: attn_f32_step rotates q as it stages it and the fold leaves q
  * rotated). f16 shapes the fused kernel does not take (hd % 32 != 0, neox pairs with
- * rope_dim/2 not a multiple of 32, or more than 8 query heads per KV head) run as the two
- * calls. positions: device u32 [1]. */
+ * rope_dim/2 not a multiple of 32, or more than 8 query heads per KV head) and 4-bit caches run
+ * as the two calls. positions: device u32 [1]. */
 int bchip_rope_append_attention(bchip_ctx* ctx, float* q, const float* k, const float* v, void* kc, void* vc,
                                 uint32_t kv_type, const float* inv_freq, const uint32_t* positions, uint32_t nh,
                                 uint32_t nkv, uint32_t hd, uint32_t rope_dim, uint32_t neox, uint32_t pos,
@@ -199,8 +220,8 @@ int bchip_rope_append_attention_noalloc(bchip_ctx* ctx, float* q, const float* k
  * k_attention per KV stream, crates/bc-mesh/src/engine.rs:25,305-309): sequence i's row
  * q[i] [nh][hd] sees the seq_lens[i] slots kv_offsets[i] .. kv_offsets[i]+seq_lens[i]-1 of
  * the shared kc/vc pool (a ragged layout). Each sequence's result equals bchip_attention
- * with rows = 1, pos = seq_lens[i]-1 on its own slots, bit for bit. seq_lens and
- * kv_offsets are host arrays; nseq <= 256. Not for graph capture across calls with
+ * with rows = 1, pos = seq_lens[i]-1 on its own slots, bit for bit (4-bit caches: within f32
+ * rounding). seq_lens and kv_offsets are host arrays; nseq <= 256. Not for graph capture across calls with
  * different lengths: the plan is made on the host from seq_lens. */
 int bchip_attention_ragged(bchip_ctx* ctx, const float* q, const void* kc, const void* vc,
                            uint32_t kv_type, float* out, const uint32_t* seq_lens,
