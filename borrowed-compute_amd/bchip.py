@@ -90,6 +90,7 @@ def lib() -> ctypes.CDLL:
                                                 P], i32),
         "bchip_fill_normal": ([P, P, u32, u64, u64], i32),
         "bchip_sample": ([P, P, u32, u32, f32, f32, u64, u64, P], i32),
+        "bchip_logprobs": ([P, P, u32, u32, f32, P, P, P, u32, P, P], i32),
         "bchip_matmul": ([P, P, u32, P, P, u32, u32, u32], i32),
         "bchip_rms_norm": ([P, P, P, P, u32, u32, f32], i32),
         "bchip_bias_add": ([P, P, P, u64, u32], i32),
@@ -301,6 +302,12 @@ class Ctx:
         """sample.rs on the device: ids (device u32 [rows]) from scores (device f32 [rows][vocab])."""
         check(lib().bchip_sample(self.h, _ptr(scores), rows, vocab, temperature, top_p, seed & 0xFFFFFFFFFFFFFFFF,
                                  step0 & 0xFFFFFFFFFFFFFFFF, _ptr(ids)))
+
+    def logprobs(self, scores, rows, vocab, temperature, tokens, logprob, entropy, top, top_ids, top_logprobs) -> None:
+        """Log probabilities of tokens, entropies and the `top` most likely tokens of device f32 scores
+        [rows][vocab]; tokens and logprob, entropy, and the last two may be None (top 0)."""
+        check(lib().bchip_logprobs(self.h, _ptr(scores), rows, vocab, temperature, _ptr(tokens), _ptr(logprob), _ptr(entropy),
+                                   top, _ptr(top_ids), _ptr(top_logprobs)))
 
     def fill_normal(self, dst, t, n, seed) -> None:
         check(lib().bchip_fill_normal(self.h, _ptr(dst), t, n, seed))

@@ -1081,6 +1081,42 @@ int bchip_sample(bchip_ctx* c, const float* scores, uint32_t rows, uint32_t voca
     return BCHIP_OK;
 }
 
+int bchip_logprobs(bchip_ctx* c, const float* scores, uint32_t rows, uint32_t vocab, float temperature,
+                   const uint32_t* tokens, float* logprob, float* entropy, uint32_t top, uint32_t* top_ids,
+                   float* top_logprobs) {
+    CHECK(enter(c));
+    if (rows == 0) return BCHIP_OK;
+    if (!scores) return fail(BCHIP_E_ARG, "null pointer");
+    if (vocab == 0) return fail(BCHIP_E_ARG, "an empty vocabulary");
+    if (rows > 65535) return fail(BCHIP_E_ARG, "%u rows (at most 65535 a call)", rows);
+    if (!(temperature >= 1e-6f && temperature <= 1e6f)) return fail(BCHIP_E_ARG, "temperature %g (within 1e-6 .. 1e6)", (double)temperature);
+    if (!tokens != !logprob) return fail(BCHIP_E_ARG, "tokens and their log probabilities go together");
+    if (top > 64 || top > vocab) return fail(BCHIP_E_ARG, "%u most likely tokens of %u (at most 64)", top, vocab);
+    if (top > 0 && (!top_ids || !top_logprobs)) return fail(BCHIP_E_ARG, "null pointer");
+    CHECK(check_span(c, scores, sat_mul(rows, (uint64_t)vocab * 4), "scores"));
+    if (tokens) CHECK(check_span(c, tokens, (uint64_t)rows * 4, "tokens"));
+    if (logprob) CHECK(check_span(c, logprob, (uint64_t)rows * 4, "logprob"));
+    if (entropy) CHECK(check_span(c, entropy, (uint64_t)rows * 4, "entropy"));
+    if (top > 0) {
+        CHECK(check_span(c, top_ids, (uint64_t)rows * top * 4, "top_ids"));
+        CHECK(check_span(c, top_logprobs, (uint64_t)rows * top * 4, "top_logprobs"));
+    }
+    // As many rows a launch as keep its scratch small beside the scores.
+    const size_t one = logprobs_scratch_bytes(1, vocab, top);
+    const uint32_t most = one ? (uint32_t)std::max<size_t>(1, ((size_t)64 << 20) / one) : rows;
+    const uint32_t each = std::min(rows, most);
+    void* scratch = one && c->ws.reserve_vt_if(each * one, c->stream) ? c->ws.vt : nullptr;
+    for (uint32_t r = 0; r < rows; r += each) {
+        const uint32_t n = std::min(each, rows - r);
+        HIP_TRY(logprobs_launch(scores + (size_t)r * vocab, n, vocab, temperature, tokens ? tokens + r : nullptr,
+                                logprob ? logprob + r : nullptr, entropy ? entropy + r : nullptr, top,
+                                top ? top_ids + (size_t)r * top : nullptr, top ? top_logprobs + (size_t)r * top : nullptr,
+                                scratch, c->stream),
+                "logprobs");
+    }
+    return BCHIP_OK;
+}
+
 int bchip_fill_normal(bchip_ctx* c, void* dst, uint32_t type, uint64_t n, uint64_t seed) {
     CHECK(enter(c));
     if (n == 0) return BCHIP_OK;

@@ -168,6 +168,13 @@ hipError_t sample_launch(const float* scores, uint32_t rows, uint32_t vocab, flo
                          uint64_t seed, uint64_t step0, uint32_t* ids, void* scratch, size_t scratch_bytes,
                          hipStream_t s);
 
+// Log probabilities, entropies and best tokens (logprobs.hip); logprob, entropy and top may be
+// left out (null, null, 0). scratch null: a workgroup takes a whole row.
+size_t logprobs_scratch_bytes(uint32_t rows, uint32_t vocab, uint32_t top);
+hipError_t logprobs_launch(const float* scores, uint32_t rows, uint32_t vocab, float temperature, const uint32_t* tokens,
+                           float* logprob, float* entropy, uint32_t top, uint32_t* ids, float* tops, void* scratch,
+                           hipStream_t s);
+
 // The rest of a layer (layer.hip).
 bool ggml_block(uint32_t type, uint32_t& weights, uint32_t& bytes);
 // Input rows one product call takes: passes of 8 rows over the grid's y dimension (65535).

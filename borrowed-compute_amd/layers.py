@@ -1,7 +1,7 @@
 """One pipeline stage's layers on the GPU: bc-infer's Layers::forward
 (crates/bc-infer/src/gpu/mod.rs:428-495), its logits head (mod.rs:499-508, the product
-of model.rs:361-370) and the sampler after it (sample.rs, engine.rs:341-350), issued as this
-library's entry points instead of a Cmd list.
+of model.rs:361-370) and the sampler after it (sample.rs, engine.rs:341-350), or the log probabilities of
+tokens in its place, issued as this library's entry points instead of a Cmd list.
 
 Per layer, in the reference's order: RMSNorm, the q/k/v products, their biases, RoPE of q
 and k with the append of k and v at slot `pos` (the four commands at mod.rs:464-475 as one
@@ -212,6 +212,33 @@ class GpuLayers:
         scores.free()
         ids.free()
         return got
+
+    def logprobs(self, x: np.ndarray, rows: int, tokens=None, top: int = 0, temperature: float = 1.0, upto: int | None = None):
+        """What the scores of each row say of tokens, on the device (bchip_logprobs): the logits head,
+        then the log probability of tokens[r] (None without tokens), the entropy, and the `top` most
+        likely tokens with their log probabilities. Only these come back to the host."""
+        if self.head is None:
+            raise ValueError("this stage has no output head")
+        if tokens is not None and len(tokens) != rows:
+            raise ValueError(f"{len(tokens)} tokens for {rows} rows")
+        norm, out, ty, vr, vc = self.head
+        upto = vr if upto is None else min(upto, vr)
+        s = self._scratch(rows)
+        ctx = self.ctx
+        ctx.upload(np.ascontiguousarray(x, np.float32), s["x"])
+        ctx.rms_norm(s["x"], norm, s["n"], rows, self.cfg.n_embd, self.cfg.eps)
+        scores, vals, ids = ctx.zeros(rows * upto * 4), ctx.zeros(rows * (2 + top) * 4), ctx.zeros(rows * max(top, 1) * 4)
+        tk = None if tokens is None else ctx.upload(np.ascontiguousarray(tokens, np.uint32))
+        try:
+            ctx.matmul(out, ty, s["n"], scores, upto, vc, rows)
+            ctx.logprobs(scores, rows, upto, temperature, tk, vals if tk else None, vals.offset(rows * 4), top, ids,
+                         vals.offset(2 * rows * 4))
+            got = ctx.read(vals, rows * (2 + top))
+            best = ctx.read(ids, (rows, max(top, 1)), np.uint32)[:, :top]
+        finally:
+            for b in (scores, vals, ids) + ((tk,) if tk else ()):
+                b.free()
+        return (got[:rows] if tk else None), got[rows:2 * rows], best, got[2 * rows:].reshape(rows, top)
 
     def free(self) -> None:
         for l in self.layers:

@@ -314,6 +314,20 @@ int bchip_add(bchip_ctx* ctx, float* x, const float* y, uint64_t n);
 int bchip_sample(bchip_ctx* ctx, const float* scores, uint32_t rows, uint32_t vocab, float temperature,
                  float top_p, uint64_t seed, uint64_t step0, uint32_t* ids);
 
+/* Beside the sampler: what rows of scores (device f32 [rows][vocab]) say of tokens, under the
+ * softmax of score / temperature (within 1e-6 .. 1e6). logprob[r] = the log probability of
+ * tokens[r] (device u32 [rows]; NaN for an id past the vocabulary), entropy[r] = the
+ * distribution's entropy in nats, top_ids / top_logprobs [rows][top] the `top` (at most 64 and
+ * vocab) most likely tokens in descending order and their log probabilities, equal scores by
+ * ascending id, NaN behind every number. tokens and logprob, entropy, and the last two may be
+ * left out (null, null, 0). f32 sums in a fixed order, one pass over the scores. A score of -inf
+ * has probability 0; a row with a NaN, a score of +inf or nothing above -inf gives NaN log
+ * probabilities and entropy. rows <= 65535. Takes scratch as bchip_attention does over 4-bit
+ * caches, and without it gives the same ids and values within f32 rounding. */
+int bchip_logprobs(bchip_ctx* ctx, const float* scores, uint32_t rows, uint32_t vocab, float temperature,
+                   const uint32_t* tokens, float* logprob, float* entropy, uint32_t top, uint32_t* top_ids,
+                   float* top_logprobs);
+
 /* Seeded N(0,1) draws into dst (n elements of type): splitmix64 (Steele, Lea and Flood
  * 2014) + Box-Muller (1958), the generator of the benchmark inputs; draw i of seed s is
  * the oracle's draw i of s up to the last bit of the device's log/sin/cos. */
