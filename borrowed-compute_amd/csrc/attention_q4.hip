@@ -38,7 +38,7 @@ namespace bchip {
 
 // A sequence's rows over its cache: row r of the item (q and out row row0 + r) sees the slots
 // below base + r (a line), or those below base and the named ones (a tree). Each of its lists is
-// cut into nchunk chunks of `chunk` tiles.
+// cut into nchunk chunks of `chunk` tiles; block0 is the first of its rows of eight blocks.
 struct Q4Item {
     uint32_t row0, rows, base, unit0, block0, nchunk, chunk, pad;
     uint64_t kvoff;
@@ -49,13 +49,13 @@ struct Q4Params {
     const uint8_t* kc;
     const uint8_t* vc;
     float* out;
-    float* part_o;   // [unit][QT][HD]: chunk states, QT query rows a unit
-    float* part_ml;  // [unit][QT][2]: their references and sums
+    float* part_o;   // [unit][qt / 16][HD / 16][64][4]: chunk states, qt query rows a unit
+    float* part_ml;  // [unit][qt][2]: their references and sums
     const uint32_t* masks;
     uint32_t tree;
     uint32_t nh, nkv, G;
     uint32_t nqt;  // units of query rows a KV head (attn_q4_tile)
-    uint32_t qt;   // query rows a unit (the fold)
+    uint32_t qt;   // query rows a unit
     float sc;      // scale * log2(e)
     uint64_t slot_limit;
     uint32_t nitems;
@@ -67,10 +67,19 @@ namespace {
 constexpr float Q4_BIAS = 11.0f;  // log2 of the weight of a row's largest score when ref is set
 constexpr float Q4_MOST = 15.0f;  // of any weight: an f16 holds it
 
+// The constants of the unpacking, in registers so that one instruction takes both.
+struct Q4Bits {
+    uint32_t field, sixty4;
+    __device__ __forceinline__ Q4Bits() {
+        asm("v_mov_b32 %0, 0x00f000f0" : "=v"(field));
+        asm("s_mov_b32 %0, 0x54005400" : "=s"(sixty4));
+    }
+};
+
 // Two values of a word pair's 4-bit field k (bits 4k .. 4k + 3 of each half) times their scales.
-__device__ __forceinline__ uint32_t unpack2(uint32_t w, int k, half2 d, half2 c) {
+__device__ __forceinline__ uint32_t unpack2(const Q4Bits& b, uint32_t w, int k, half2 d, half2 c) {
     const uint32_t f = k == 0 ? w << 4 : k == 1 ? w : k == 2 ? w >> 4 : w >> 8;
-    const half2 x = __builtin_bit_cast(half2, (f & 0x00f000f0u) | 0x54005400u);  // 64 + code
+    const half2 x = __builtin_bit_cast(half2, (f & b.field) | b.sixty4);  // 64 + code
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(x, d, c));
 }
 
@@ -79,9 +88,9 @@ __device__ __forceinline__ half8 as_half8(uint32_t a, uint32_t b, uint32_t c, ui
 }
 
 // A K operand's eight dims from their word: elements 0, 4, 1, 5, 2, 6, 3, 7.
-__device__ __forceinline__ half8 unpack_k(uint32_t w, f16 scale) {
+__device__ __forceinline__ half8 unpack_k(const Q4Bits& b, uint32_t w, f16 scale) {
     const half2 d = {scale, scale}, c = d * (f16)-72.0f;
-    return as_half8(unpack2(w, 0, d, c), unpack2(w, 1, d, c), unpack2(w, 2, d, c), unpack2(w, 3, d, c));
+    return as_half8(unpack2(b, w, 0, d, c), unpack2(b, w, 1, d, c), unpack2(b, w, 2, d, c), unpack2(b, w, 3, d, c));
 }
 
 __device__ __forceinline__ bool odd_scale(f16 d) {  // an infinity or a NaN
@@ -98,67 +107,94 @@ struct Seg {
     static constexpr int frag(int s) { return s < N128 ? 8 * s : (H64 && s == N128) ? 8 * N128 : 8 * N128 + 4 * H64; }
 };
 
-template <int W>
-__device__ __forceinline__ uint32_t load_codes(const uint8_t* p) {
-    if constexpr (W == 8) return *(const uint32_t*)p;
-    else if constexpr (W == 4) return *(const uint16_t*)p;
-    else return *p;
+// The columns of operand f that result registers 0 .. 3 of lane group g hold: the first, and how
+// far they are apart.
+template <int NB>
+__device__ __forceinline__ uint32_t stride(uint32_t f) {
+    using S = Seg<NB>;
+    return f < 8u * S::N128 ? 8 : S::H64 && f < 8u * S::N128 + 4u ? 4 : 2;
+}
+template <int NB>
+__device__ __forceinline__ uint32_t column(uint32_t f, uint32_t g) {
+    using S = Seg<NB>;
+    if (f < 8u * S::N128) return 128 * (f / 8) + f % 8 + 32 * g;
+    if (S::H64 && f < 8u * S::N128 + 4u) return 128 * S::N128 + f % 4 + 16 * g;
+    return 32 * (NB - 1) + f % 2 + 8 * g;
 }
 
 // Operands of W columns from the words of eight slots and their scales.
 template <int W>
-__device__ __forceinline__ void unpack_v(const uint32_t (&raw)[8], const f16 (&sc)[8], half8 (&out)[W]) {
+__device__ __forceinline__ void unpack_v(const Q4Bits& b, const uint32_t (&raw)[8], const f16 (&sc)[8], half8 (&out)[W]) {
     uint32_t r[W][4];
 #pragma unroll
     for (int p = 0; p < 4; p++) {
         const half2 d = {sc[2 * p], sc[2 * p + 1]}, c = d * (f16)-72.0f;
         const uint32_t lo = __builtin_amdgcn_perm(raw[2 * p + 1], raw[2 * p], 0x05040100u);
 #pragma unroll
-        for (int k = 0; k < (W < 4 ? W : 4); k++) r[k][p] = unpack2(lo, k, d, c);
+        for (int k = 0; k < (W < 4 ? W : 4); k++) r[k][p] = unpack2(b, lo, k, d, c);
         if constexpr (W == 8) {
             const uint32_t hi = __builtin_amdgcn_perm(raw[2 * p + 1], raw[2 * p], 0x07060302u);
 #pragma unroll
-            for (int k = 0; k < 4; k++) r[4 + k][p] = unpack2(hi, k, d, c);
+            for (int k = 0; k < 4; k++) r[4 + k][p] = unpack2(b, hi, k, d, c);
         }
     }
 #pragma unroll
     for (int k = 0; k < W; k++) out[k] = as_half8(r[k][0], r[k][1], r[k][2], r[k][3]);
 }
 
-// A lane's dims of one query row (8 words of NB, dims 8 (NB g + j) ..) as two f16 parts; back
-// comes the power of two that scores are to be multiplied by.
-template <int NB>
-__device__ __forceinline__ float load_q(const float* qrow, uint32_t g, float sc, half8 (&hi)[NB], half8 (&lo)[NB]) {
-    float x[NB][8];
-    float top = 0.0f;
-#pragma unroll
-    for (int j = 0; j < NB; j++) {
-        float4 a{}, b{};
-        if (qrow) {
-            a = *(const float4*)(qrow + 8 * (NB * g + j));
-            b = *(const float4*)(qrow + 8 * (NB * g + j) + 4);
-        }
-        const float v[8] = {a.x, b.x, a.y, b.y, a.z, b.z, a.w, b.w};
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            x[j][i] = v[i] * sc;
-            top = fmaxf(top, fabsf(x[j][i]));
-        }
+// The larger of two, a number before a NaN: fmaxf without the quieting of its operands.
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// Eight dims of a query row from `at`, in the order of a K word's, and the largest magnitude of
+// them and `top`.
+__device__ __forceinline__ float q_dims(const float* at, bool valid, float (&x)[8], float top) {
+    float4 a{}, b{};
+    if (valid) {
+        a = *(const float4*)at;
+        b = *(const float4*)(at + 4);
     }
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    int e = (int)(__float_as_uint(top) >> 23) - 127;  // (of an infinity 128: its row is NaN)
+    x[0] = a.x, x[1] = b.x, x[2] = a.y, x[3] = b.y, x[4] = a.z, x[5] = b.z, x[6] = a.w, x[7] = b.w;
+#pragma unroll
+    for (int i = 0; i < 8; i++) top = larger(top, fabsf(x[i]));
+    return top;
+}
+
+// From a row's largest |q|: q times k is q scale log2 e brought to 2^13 .. 2^14, c takes it back.
+__device__ __forceinline__ void q_scale(float top, float sc, float& k, float& c) {
+    int e = (int)(__float_as_uint(top * fabsf(sc)) >> 23) - 127;  // (of an infinity 128: its row is NaN)
     e = e < -100 ? -100 : e;
-    const float up = __uint_as_float((uint32_t)(13 - e + 127) << 23);
+    k = sc * __uint_as_float((uint32_t)(13 - e + 127) << 23);
+    c = __uint_as_float((uint32_t)(e - 13 + 127) << 23);
+}
+
+__device__ __forceinline__ void q_parts(const float (&x)[8], float k, half8& hi, half8& lo) {
 #pragma unroll
-    for (int j = 0; j < NB; j++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float y = x[j][i] * up;
-            hi[j][i] = (f16)y;
-            lo[j][i] = (f16)(y - (float)hi[j][i]);
-        }
-    return __uint_as_float((uint32_t)(e - 13 + 127) << 23);
+    for (int i = 0; i < 8; i += 2) {
+        const half2 h = __builtin_convertvector((f32x2{x[i] * k, x[i + 1] * k}), half2);
+        const half2 r = __builtin_convertvector((f32x2{__builtin_fmaf(x[i], k, -(float)h[0]), __builtin_fmaf(x[i + 1], k, -(float)h[1])}), half2);
+        hi[i] = h[0], hi[i + 1] = h[1];
+        lo[i] = r[0], lo[i + 1] = r[1];
+    }
+}
+
+// A list's codes and scales are read through buffer descriptors that end with its last slot's
+// unit: what a tile reaches past that comes back as zero, whatever lies there.
+typedef __amdgpu_buffer_rsrc_t q4_rsrc;
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ q4_rsrc q4_from(const uint8_t* base, uint64_t at, uint64_t end) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)(base + at), 0, (uint32_t)min(end - at, (uint64_t)0x7fffffffu), 0x00020000);
+}
+template <int W>
+__device__ __forceinline__ uint32_t load_codes(q4_rsrc r, uint32_t lane, uint32_t all) {
+    if constexpr (W == 8) return __builtin_amdgcn_raw_buffer_load_b32(r, lane, all, 0);
+    else if constexpr (W == 4) return __builtin_amdgcn_raw_buffer_load_b16(r, lane, all, 0);
+    else return __builtin_amdgcn_raw_buffer_load_b8(r, lane, all, 0);
+}
+__device__ __forceinline__ f16 load_scale(q4_rsrc r, uint32_t lane, uint32_t all) {
+    return __builtin_bit_cast(f16, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, lane, all, 0));
 }
 
 // Byte offsets, within a tile, of what a lane reads of a slot: its K words and scales.
@@ -175,45 +211,53 @@ struct KLoad {
             scale[j] = q4_scale_at32(e + 8 * (NB * g + j));
         }
     }
-    __device__ __forceinline__ void load(const uint8_t* tile, uint32_t (&w)[NB], f16 (&s)[NS]) const {
+    __device__ __forceinline__ void load(q4_rsrc r, uint32_t at, uint32_t (&w)[NB], f16 (&s)[NS]) const {
         if constexpr (NB == 1) {
-            w[0] = *(const uint32_t*)(tile + code[0]);
+            w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, code[0], at, 0);
         } else if constexpr (NB == 2) {
-            const uint2 a = *(const uint2*)(tile + code[0]);
+            const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, code[0], at, 0));
             w[0] = a.x, w[1] = a.y;
         } else if constexpr (NB == 4 || NB == 8) {
 #pragma unroll
             for (int j = 0; j < NB; j += 4) {
-                const uint4 a = *(const uint4*)(tile + code[0] + 4 * j);
+                const u32x4 a = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, code[0] + 4 * j, at, 0));
                 w[j] = a.x, w[j + 1] = a.y, w[j + 2] = a.z, w[j + 3] = a.w;
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < NB; j++) w[j] = *(const uint32_t*)(tile + code[j]);
+            for (int j = 0; j < NB; j++) w[j] = __builtin_amdgcn_raw_buffer_load_b32(r, code[j], at, 0);
         }
         if constexpr (NB == 8) {
-            const half2 a = *(const half2*)(tile + scale[0]);  // blocks 2g, 2g + 1
-            s[0] = a[0], s[1] = a[1];
+            const half2 a = __builtin_bit_cast(half2, (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, scale[0], at, 0));
+            s[0] = a[0], s[1] = a[1];  // blocks 2g, 2g + 1
         } else {
 #pragma unroll
-            for (int j = 0; j < NS; j++) s[j] = *(const f16*)(tile + scale[j]);
+            for (int j = 0; j < NS; j++) s[j] = load_scale(r, scale[j], at);
         }
     }
     static __device__ __forceinline__ f16 of(const f16 (&s)[NS], int j) { return s[NB == 8 ? j / 4 : NS == 1 ? 0 : j]; }
 };
 
-// What query row n (of an item's rows x G) of this lane sees.
+// What a query row sees: the slots below vis, and in a tree those of `mask` from base on.
 struct Sees {
-    uint32_t vis;     // slots below this
-    uint32_t lo, hi;  // a tree: and these from `base` on
-    __device__ __forceinline__ bool at(uint32_t slot, uint32_t base, uint32_t end, uint32_t tree) const {
-        if (slot >= end) return false;
-        if (slot < vis) return true;
-        if (!tree) return false;
+    uint32_t vis, base;
+    uint64_t mask;
+    __device__ __forceinline__ bool at(uint32_t slot) const {
         const uint32_t j = slot - base;
-        return j < 64 && (((j < 32 ? lo >> j : hi >> (j - 32)) & 1u) != 0);
+        return (slot < vis) | ((uint32_t)(mask >> (j & 63)) & (uint32_t)(j < 64));
     }
 };
+
+// Of row r of an item (end: of its farthest list).
+__device__ __forceinline__ Sees sees(const Q4Params& p, const Q4Item& it, uint32_t r, bool valid, uint32_t end) {
+    Sees s{valid ? it.base + (p.tree ? 0 : r) : end, it.base, 0};
+    if (p.tree && valid) {
+        const uint32_t row = it.row0 + r, named = end - it.base;
+        s.mask = p.masks[2 * row] | (uint64_t)p.masks[2 * row + 1] << 32;
+        if (named < 64) s.mask &= (1ull << named) - 1;
+    }
+    return s;
+}
 
 // The end of an item's farthest list. A tree's is its highest named slot's: no slot past that is
 // read. Every lane of the wave calls it.
@@ -226,15 +270,16 @@ __device__ __forceinline__ uint32_t tree_end(const Q4Params& p, const Q4Item& it
     }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-    return (uint32_t)min((uint64_t)it.base + top, p.slot_limit);
+    return __builtin_amdgcn_readfirstlane((uint32_t)min((uint64_t)it.base + top, p.slot_limit));
 }
 
-// A row's weights are 2^(s - ref). Where some score of these 32 slots passes ref by more than
-// Q4_MOST, the refs rise to Q4_BIAS under their rows' maxima (to the maxima themselves where
-// those are so large that the difference would be lost), and what was summed against the old one
-// is to be multiplied by f.
-__device__ __forceinline__ bool raise(const float (&s)[8], float& ref, float& f) {
-    float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+// A row's scores are c s (c a power of two), its weights 2^(c s - ref). Where some score of these
+// 32 slots passes ref by more than Q4_MOST, the refs rise to Q4_BIAS under their rows' maxima (to
+// the maxima themselves where those are so large that the difference would be lost), and what
+// was summed against the old one is to be multiplied by f.
+__device__ __forceinline__ bool raise(const f32x4 (&s)[2], float c, float& ref, float& f) {
+    float top = larger(larger(larger(s[0][0], s[0][1]), larger(s[0][2], s[0][3])),
+                       larger(larger(s[1][0], s[1][1]), larger(s[1][2], s[1][3]))) * c;
     if (!__any(top > ref + Q4_MOST)) return false;
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
@@ -244,114 +289,200 @@ __device__ __forceinline__ bool raise(const float (&s)[8], float& ref, float& f)
     return true;
 }
 
+// The weights' B operand, the rounded values (hi) and the rest (lo); their sum goes to l. With
+// PART, hi comes back as the rounded values times 1 - keep plus the rest times keep (0 or 1): a
+// lane holds one part.
+template <bool PART>
+__device__ __forceinline__ void weights(const f32x4 (&s)[2], float c, float ref, float keep, float& l, half8& hi, half8& lo) {
+    const float base = ref == -INFINITY ? 0.0f : ref;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const float w0 = exp2_hw(__builtin_fmaf(s[i >> 2][i & 3], c, -base));
+        const float w1 = exp2_hw(__builtin_fmaf(s[i >> 2][(i & 3) + 1], c, -base));
+        l += w0;
+        l += w1;
+        const half2 h = __builtin_convertvector((f32x2{w0, w1}), half2);
+        const float k = PART ? -keep : -1.0f;
+        const half2 r = __builtin_convertvector((f32x2{__builtin_fmaf((float)h[0], k, w0), __builtin_fmaf((float)h[1], k, w1)}), half2);
+        hi[i] = PART ? r[0] : h[0];
+        hi[i + 1] = PART ? r[1] : h[1];
+        lo[i] = r[0];
+        lo[i + 1] = r[1];
+    }
+}
+
 __device__ __forceinline__ float ror8(float x) {  // lane n of each 16 gets lane (n + 8) % 16's
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false));
 }
 
-constexpr int Q4_WAVES = 4;
 constexpr uint32_t Q4_TILE = 32;
 
-template <int NB, bool PK>
-__global__ __launch_bounds__(64 * Q4_WAVES) void attn_q4_row(const Q4Params p) {
-    constexpr int HD = 32 * NB, NF = 2 * NB, ROWS = PK ? 8 : 16, LD = HD + 4;
+// Where a lane reads eight slots of V, 4g .. 4g + 3 and 16 more of each, in a tile of 32
+// slots: its columns' words and their scales. Slots 4g + j lie the same way within their
+// units for every g where four slots are whole units and a segment lies within one (heads of 64,
+// 128 or 256): a lane's offset is then one for all, beside a uniform one. HALF: half the columns of
+// every segment but those of 32, whose words both halves read.
+template <int NB, bool HALF>
+struct VLoad {
     using S = Seg<NB>;
-    __shared__ float so[Q4_WAVES][ROWS][LD];
-    __shared__ float sm[Q4_WAVES][16], sl[Q4_WAVES][16];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m16 = lane & 15, g = lane >> 4;
+    static constexpr bool SAME = NB == 2 || NB == 4 || NB == 8;
+    static constexpr int w(int si) { return HALF && S::w(si) > 2 ? S::w(si) / 2 : S::w(si); }
+    uint32_t code[S::N][SAME ? 1 : 8], scale[S::N][SAME ? 1 : 8];
+    uint32_t ucode[S::N][4], uscale[S::N][4];
+    __device__ __forceinline__ void set(uint32_t rem, uint32_t kvd, uint32_t m16, uint32_t g, uint32_t half) {
+#pragma unroll
+        for (int si = 0; si < S::N; si++) {
+            const uint32_t c = S::w(si) * m16 + (S::w(si) > 2 ? w(si) * half : 0);
+            if constexpr (SAME) {
+                code[si][0] = g * (kvd / 4 * 9) + c / 2;
+                scale[si][0] = g * (kvd / 4 * 9) + c / 32 * 2;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    ucode[si][j] = q4_code_at32(rem + j * kvd + S::col(si));
+                    uscale[si][j] = q4_scale_at32(rem + j * kvd + S::col(si));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const uint32_t e = rem + (4 * g + (i & 3) + 16 * (i >> 2)) * kvd + S::col(si) + c;
+                    code[si][i] = q4_code_at32(e);
+                    scale[si][i] = q4_scale_at32(e);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void load(q4_rsrc r, uint32_t kvd, uint32_t (&vw)[S::N][8], f16 (&vs)[S::N][8]) const {
+#pragma unroll
+        for (int si = 0; si < S::N; si++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint32_t lc = code[si][SAME ? 0 : i], ls = scale[si][SAME ? 0 : i];
+                const uint32_t uc = SAME ? ucode[si][i & 3] + (i >> 2) * 9 * kvd : 0;  // (16 slots are whole units)
+                const uint32_t us = SAME ? uscale[si][i & 3] + (i >> 2) * 9 * kvd : 0;
+                vw[si][i] = w(si) == 8 ? load_codes<8>(r, lc, uc) : w(si) == 4 ? load_codes<4>(r, lc, uc) : load_codes<2>(r, lc, uc);
+                vs[si][i] = load_scale(r, ls, us);
+            }
+    }
+};
+
+// Bytes of `slots` slots from the start of their first unit (rem elements into it).
+__device__ __forceinline__ uint64_t q4_bytes(uint64_t slots, uint32_t rem, uint32_t kvd) {
+    return (slots * kvd + rem + Q4_UNIT - 1) / Q4_UNIT * Q4_UNIT_BYTES;
+}
+
+template <int NB, bool PK, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void attn_q4_row(const Q4Params p) {
+    constexpr int HD = 32 * NB, NF = 2 * NB, QW = NB < WAVES ? NB : WAVES, QJ = (NB + WAVES - 1) / WAVES;
+    using S = Seg<NB>;
+    __shared__ union {
+        half8 q[PK ? 1 : 2][NB][64];
+        f32x4 o[WAVES > 4 ? WAVES / 2 : 4][NF][64];
+    } sh;
+    __shared__ float stop[QW][16], sr[WAVES][64], sl[WAVES][64];
+    const Q4Bits bits;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t m16 = lane & 15, g = lane >> 4;
 
     uint32_t ii = 0;
     if (p.nitems > 1) {  // the last item whose first block is at most this one
-        const bool before = lane < p.nitems && p.items[lane].block0 <= blockIdx.x;
+        const bool before = lane < p.nitems && p.items[lane].block0 <= blockIdx.z;
         ii = __builtin_amdgcn_readfirstlane(__popcll(__ballot(before)) - 1);
     }
     const Q4Item& it = p.items[ii];
     // Blocks 8 apart (one XCD) take the KV heads of one chunk: their bytes share cache lines.
-    const uint32_t b = blockIdx.x - it.block0, oct = b / (8 * p.nkv), rest = b % (8 * p.nkv);
-    const uint32_t kvh = rest / 8, chunk = oct * 8 + rest % 8;
+    const uint32_t kvh = blockIdx.y, chunk = (blockIdx.z - it.block0) * 8 + blockIdx.x;
     if (chunk >= it.nchunk) return;
     const uint32_t kvd = p.nkv * HD, nq = it.rows * p.G, end = p.tree ? tree_end(p, it) : it.base + it.rows - 1;
+    const uint32_t all = (uint32_t)(((uint64_t)end + Q4_TILE - 1) / Q4_TILE), first = chunk * it.chunk;
+    const uint32_t tiles = first < all ? min(it.chunk, all - first) : 0;
 
-    const uint32_t n = PK ? (m16 & 7) : m16;
-    const bool valid = n < nq;
-    const uint32_t row = it.row0 + (valid ? n / p.G : 0), head = kvh * p.G + (valid ? n % p.G : 0);
-    Sees see{valid ? it.base + (p.tree ? 0 : n / p.G) : end, 0, 0};
-    if (p.tree && valid) {
-        see.lo = p.masks[2 * row];
-        see.hi = p.masks[2 * row + 1];
-    }
-    half8 qa[NB], qb[NB];
-    const float c = load_q<NB>(valid ? p.q + ((size_t)row * p.nh + head) * HD : nullptr, g, p.sc, qa, qb);
-    if constexpr (PK) {
-#pragma unroll
-        for (int j = 0; j < NB; j++)
-            if (m16 >= 8) qa[j] = qb[j];
-    }
-
+    // The chunk's bytes, from its first slot's unit to the end of the list.
     const uint64_t e0 = it.kvoff * kvd;
-    const uint32_t rem = (uint32_t)(e0 & 255) + kvh * HD;
-    const uint64_t tile_bytes = (uint64_t)kvd * 18;  // 32 slots
-    const uint8_t* kbase = p.kc + (e0 >> 8) * Q4_UNIT_BYTES;
-    const uint8_t* vbase = p.vc + (e0 >> 8) * Q4_UNIT_BYTES;
+    const uint32_t rem0 = (uint32_t)(e0 & 255), rem = rem0 + kvh * HD;
+    const uint64_t base = (e0 >> 8) * Q4_UNIT_BYTES, tile_bytes = (uint64_t)kvd * 18;
+    const uint64_t from = base + first * tile_bytes, to = base + q4_bytes(end, rem0, kvd);
+    KLoad<NB> kl;
+    VLoad<NB, false> vl;
+    kl.set(rem + m16 * kvd, g);
+    vl.set(rem, kvd, m16, g, 0);
+    uint32_t kw[2][NB], vw[S::N][8];
+    f16 ks[2][KLoad<NB>::NS], vs[S::N][8];
+    auto load_k = [&](uint32_t t) {
+        const q4_rsrc r = q4_from(p.kc, from + t * tile_bytes, to);
+#pragma unroll
+        for (int h = 0; h < 2; h++) kl.load(r, h * 9 * kvd, kw[h], ks[h]);
+    };
+    auto load_v = [&](uint32_t t) { vl.load(q4_from(p.vc, from + t * tile_bytes, to), kvd, vw, vs); };
+    if (wave < tiles) {  // the first tile is on its way while q is made ready
+        load_k(wave);
+        load_v(wave);
+    }
 
-    const uint32_t ntiles = (uint32_t)(((uint64_t)end + Q4_TILE - 1) / Q4_TILE);
-    const uint32_t t0 = chunk * it.chunk, t1 = min(t0 + it.chunk, ntiles);
-    KLoad<NB> kl[2];
-    uint32_t vcode[S::N][8], vscale[S::N][8];
-    auto place = [&](uint32_t last) {  // slots past `last` read it instead (their weights are 0)
+    // q's operands, each wave some of the steps for all.
+    const uint32_t n = PK ? (m16 & 7) : m16, r = (n * (65536 / p.G + 1)) >> 16;  // n / G
+    const bool valid = n < nq;
+    const uint32_t row = it.row0 + (valid ? r : 0), head = kvh * p.G + (valid ? n - r * p.G : 0);
+    const Sees see = sees(p, it, r, valid, end);
+    const size_t qrow = ((size_t)row * p.nh + head) * HD;
+    float x[QJ][8], top = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 2; r++) kl[r].set(rem + min(16 * r + m16, last) * kvd, g);
+    for (int i = 0; i < QJ; i++) {
+        const uint32_t j = i * WAVES + wave;
+        if (j < NB) top = q_dims(p.q + qrow + 8 * (NB * g + j), valid, x[i], top);
+    }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    if (wave < QW && lane < 16) stop[wave][lane] = top;
+    __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t e = rem + min(4 * g + (i & 3) + 16 * (i >> 2), last) * kvd;
+    for (int w = 0; w < QW; w++) top = fmaxf(top, stop[w][m16]);
+    float k, c;
+    q_scale(top, p.sc, k, c);
+    const float keep = PK && m16 >= 8 ? 1.0f : 0.0f;
 #pragma unroll
-            for (int si = 0; si < S::N; si++) {
-                const uint32_t ec = e + S::col(si) + S::w(si) * m16;
-                vcode[si][i] = q4_code_at32(ec);
-                vscale[si][i] = q4_scale_at32(ec);
+    for (int i = 0; i < QJ; i++) {
+        const uint32_t j = i * WAVES + wave;
+        if (j < NB) {
+            half8 hi, lo;
+            q_parts(x[i], k, hi, lo);
+            if constexpr (PK) {
+                sh.q[0][j][lane] = m16 < 8 ? hi : lo;
+            } else {
+                sh.q[0][j][lane] = hi;
+                sh.q[1][j][lane] = lo;
             }
         }
-    };
-    place(Q4_TILE - 1);
+    }
+    __syncthreads();
+    half8 qa[NB], qb[NB];
+#pragma unroll
+    for (int j = 0; j < NB; j++) {
+        qa[j] = sh.q[0][j][lane];
+        if constexpr (!PK) qb[j] = sh.q[1][j][lane];
+    }
 
     f32x4 o[NF];
 #pragma unroll
     for (int f = 0; f < NF; f++) o[f] = f32x4{0, 0, 0, 0};
     float ref = -INFINITY, l = 0.0f;
 
-    for (uint32_t t = t0 + wave; t < t1; t += Q4_WAVES) {
-        const uint32_t ts = t * Q4_TILE;
-        if (end - ts < Q4_TILE) place(end - 1 - ts);
-        const uint8_t* kt = kbase + t * tile_bytes;
-        const uint8_t* vt = vbase + t * tile_bytes;
-        uint32_t kw[2][NB], vw[S::N][8];
-        f16 ks[2][KLoad<NB>::NS], vs[S::N][8];
+    for (uint32_t t = wave; t < tiles; t += WAVES) {
+        const uint32_t ts = (first + t) * Q4_TILE;
+        const bool more = t + WAVES < tiles;
+        f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, s2[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-        for (int r = 0; r < 2; r++) kl[r].load(kt, kw[r], ks[r]);
+        for (int j = 0; j < NB; j++)
 #pragma unroll
-        for (int si = 0; si < S::N; si++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                vw[si][i] = S::w(si) == 8   ? load_codes<8>(vt + vcode[si][i])
-                            : S::w(si) == 4 ? load_codes<4>(vt + vcode[si][i])
-                                            : load_codes<2>(vt + vcode[si][i]);
-                vs[si][i] = *(const f16*)(vt + vscale[si][i]);
+            for (int h = 0; h < 2; h++) {
+                const half8 a = unpack_k(bits, kw[h][j], KLoad<NB>::of(ks[h], j));
+                s[h] = mfma16(a, qa[j], s[h]);
+                if constexpr (!PK) s2[h] = mfma16(a, qb[j], s2[h]);
             }
-        float s[8];
+        if (more) load_k(t + WAVES);
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
-            f32x4 acc = {0, 0, 0, 0};
+        for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int j = 0; j < NB; j++) {
-                const half8 k = unpack_k(kw[r][j], KLoad<NB>::of(ks[r], j));
-                acc = mfma16(k, qa[j], acc);
-                if constexpr (!PK) acc = mfma16(k, qb[j], acc);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if constexpr (PK) acc[i] += ror8(acc[i]);
-                s[4 * r + i] = acc[i] * c;
-            }
-        }
+            for (int i = 0; i < 4; i++) s[h][i] += PK ? ror8(s[h][i]) : s2[h][i];
         // A tile that some row does not see whole: scores of unseen slots become -inf, and V
         // scales that are not finite 0, their blocks put back as NaN for the rows that see them.
         const bool edge = ts + Q4_TILE > it.base;
@@ -359,7 +490,7 @@ __global__ __launch_bounds__(64 * Q4_WAVES) void attn_q4_row(const Q4Params p) {
         if (edge) {
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                if (!see.at(ts + 16 * (i >> 2) + 4 * g + (i & 3), it.base, end, p.tree)) s[i] = -INFINITY;
+                if (!see.at(ts + 16 * (i >> 2) + 4 * g + (i & 3))) s[i >> 2][i & 3] = -INFINITY;
 #pragma unroll
             for (int si = 0; si < S::N; si++)
 #pragma unroll
@@ -370,34 +501,22 @@ __global__ __launch_bounds__(64 * Q4_WAVES) void attn_q4_row(const Q4Params p) {
                     }
         }
         float f;
-        if (raise(s, ref, f)) {
+        if (raise(s, c, ref, f)) {
             l *= f;
 #pragma unroll
-            for (int k = 0; k < NF; k++) o[k] *= f;
+            for (int i = 0; i < NF; i++) o[i] *= f;
         }
-        const float base = ref == -INFINITY ? 0.0f : ref;
         half8 ph, pl;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float w = exp2_hw(s[i] - base);
-            l += w;
-            const f16 h = (f16)w;
-            if constexpr (PK) {
-                ph[i] = m16 < 8 ? h : (f16)(w - (float)h);
-            } else {
-                ph[i] = h;
-                pl[i] = (f16)(w - (float)h);
-            }
-        }
+        weights<PK>(s, c, ref, keep, l, ph, pl);
         auto pv = [&](auto width, int si) {
             constexpr int W = decltype(width)::value;
             half8 vf[W];
-            unpack_v<W>(vw[si], vs[si], vf);
+            unpack_v<W>(bits, vw[si], vs[si], vf);
 #pragma unroll
-            for (int k = 0; k < W; k++) {
-                f32x4& acc = o[S::frag(si) + k];
-                acc = mfma16(vf[k], ph, acc);
-                if constexpr (!PK) acc = mfma16(vf[k], pl, acc);
+            for (int i = 0; i < W; i++) o[S::frag(si) + i] = mfma16(vf[i], ph, o[S::frag(si) + i]);
+            if constexpr (!PK) {
+#pragma unroll
+                for (int i = 0; i < W; i++) o[S::frag(si) + i] = mfma16(vf[i], pl, o[S::frag(si) + i]);
             }
         };
 #pragma unroll
@@ -406,21 +525,24 @@ __global__ __launch_bounds__(64 * Q4_WAVES) void attn_q4_row(const Q4Params p) {
             else if (S::w(si) == 4) pv(std::integral_constant<int, 4>{}, si);
             else pv(std::integral_constant<int, 2>{}, si);
         }
+        if (more) load_v(t + WAVES);
         if (edge && __any(odd)) {
+            const q4_rsrc vr = q4_from(p.vc, from + t * tile_bytes, to);
             for (uint32_t i = 0; i < Q4_TILE && ts + i < end; i++) {
-                const bool seen = see.at(ts + i, it.base, end, p.tree);
+                const bool seen = see.at(ts + i);
 #pragma unroll
                 for (int si = 0; si < S::N; si++) {  // (a lane's columns of a segment lie in one block)
-                    const uint32_t e = rem + i * kvd + S::col(si) + S::w(si) * 4 * g;
-                    if (seen && odd_scale(*(const f16*)(vt + q4_scale_at32(e))))
+                    const f16 d = load_scale(vr, q4_scale_at32(rem + i * kvd + S::col(si) + S::w(si) * 4 * g), 0);
+                    if (seen && odd_scale(d))
 #pragma unroll
-                        for (int k = 0; k < S::w(si); k++) o[S::frag(si) + k] = f32x4{NAN, NAN, NAN, NAN};
+                        for (int w = 0; w < S::w(si); w++) o[S::frag(si) + w] = f32x4{NAN, NAN, NAN, NAN};
                 }
             }
         }
     }
 
-    // The four waves' states.
+    // The waves' states, lane by lane: the upper half of more than four to the lower, then each of
+    // four waves brings some of the columns together.
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     if constexpr (PK) {
@@ -429,48 +551,60 @@ __global__ __launch_bounds__(64 * Q4_WAVES) void attn_q4_row(const Q4Params p) {
 #pragma unroll
             for (int i = 0; i < 4; i++) o[f][i] += ror8(o[f][i]);
     }
-    if (lane < 16) {
-        sm[wave][lane] = ref;
-        sl[wave][lane] = l;
-    }
-    if (valid && m16 < ROWS) {
 #pragma unroll
-        for (int si = 0; si < S::N; si++)
+    for (uint32_t half = WAVES / 2; half >= 4; half /= 2) {
+        __syncthreads();
+        if (wave >= half && wave < 2 * half) {
+            sr[wave][lane] = ref;
+            sl[wave][lane] = l;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int f = 0; f < NF; f++) sh.o[wave - half][f][lane] = o[f];
+        }
+        __syncthreads();
+        if (wave < half) {
+            const float other = sr[wave + half][lane], to = fmaxf(ref, other), ts = to == -INFINITY ? 0.0f : to;
+            const float a = exp2_hw(ref - ts), e = exp2_hw(other - ts);
+            l = l * a + sl[wave + half][lane] * e;
 #pragma unroll
-                for (int k = 0; k < S::w(si); k++)
-                    so[wave][m16][S::col(si) + S::w(si) * (4 * g + i) + k] = o[S::frag(si) + k][i];
+            for (int f = 0; f < NF; f++) o[f] = o[f] * a + sh.o[wave][f][lane] * e;
+            ref = to;
+        }
     }
     __syncthreads();
-    const uint32_t unit = it.unit0 + kvh * it.nchunk + chunk;
-    for (uint32_t x = threadIdx.x; x < nq * (HD / 4); x += 64 * Q4_WAVES) {
-        const uint32_t r = x / (HD / 4), col = 4 * (x % (HD / 4));
-        float M = sm[0][r];
+    if (wave < 4) {
+        sr[wave][lane] = ref;
+        sl[wave][lane] = l;
 #pragma unroll
-        for (int w = 1; w < Q4_WAVES; w++) M = fmaxf(M, sm[w][r]);
-        const float Ms = M == -INFINITY ? 0.0f : M;
-        float L = 0.0f;
-        f32x4 a = {0, 0, 0, 0};
+        for (int f = 0; f < NF; f++) sh.o[wave][f][lane] = o[f];
+    }
+    __syncthreads();
+    if (wave >= 4 || !valid || (PK && m16 >= 8)) return;
+    float a[4], L = 0.0f;
+    const float R = fmaxf(fmaxf(sr[0][lane], sr[1][lane]), fmaxf(sr[2][lane], sr[3][lane])), Rs = R == -INFINITY ? 0.0f : R;
 #pragma unroll
-        for (int w = 0; w < Q4_WAVES; w++) {
-            const float k = exp2_hw(sm[w][r] - Ms);
-            L += k * sl[w][r];
-            a += k * *(const f32x4*)&so[w][r][col];
-        }
-        if (it.nchunk == 1) {
-            const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // (a row that sees nothing: zeros)
-            const uint32_t orow = it.row0 + r / p.G, oh = kvh * p.G + r % p.G;
-            *(f32x4*)(p.out + ((size_t)orow * p.nh + oh) * HD + col) = a * inv;
+    for (int w = 0; w < 4; w++) {
+        a[w] = exp2_hw(sr[w][lane] - Rs);
+        L += sl[w][lane] * a[w];
+    }
+    const size_t unit = it.unit0 + kvh * it.nchunk + chunk;
+    const float inv = it.nchunk > 1 ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;  // (a row that sees nothing: zeros)
+    if (it.nchunk > 1 && wave == 0 && g == 0) *(float2*)(p.part_ml + 2 * (unit * 16 + n)) = float2{R, L};
+    for (uint32_t f = wave; f < NF; f += 4) {
+        f32x4 v = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < 4; w++) v += sh.o[w][f][lane] * a[w];
+        v *= inv;
+        if (it.nchunk > 1) {
+            *(f32x4*)(p.part_o + ((unit * NF + f) * 64 + lane) * 4) = v;
         } else {
-            *(f32x4*)(p.part_o + ((size_t)unit * 16 + r) * HD + col) = a;
-            if (col == 0) {
-                p.part_ml[2 * ((size_t)unit * 16 + r)] = M;
-                p.part_ml[2 * ((size_t)unit * 16 + r) + 1] = L;
-            }
+            const uint32_t col = column<NB>(f, g), step = stride<NB>(f);
+#pragma unroll
+            for (int i = 0; i < 4; i++) p.out[qrow + col + i * step] = v[i];
         }
     }
 }
+
+constexpr int Q4_WAVES = 4;
 
 // More query rows: a tile of 64 slots unpacked once into LDS for the workgroup's four waves of
 // 16 RT query rows each.
@@ -484,78 +618,61 @@ __global__ __launch_bounds__(64 * Q4_WAVES, NB <= 4 ? 2 : 1) void attn_q4_tile(c
     __shared__ half8 kf[2][4][NB][64];
     __shared__ half8 vf[2][2][NF][64];
     __shared__ uint32_t odd_tile[2];  // 1 + the tile of each buffer that held a scale that is not finite
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m16 = lane & 15, g = lane >> 4;
+    const Q4Bits bits;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t m16 = lane & 15, g = lane >> 4;
     const Q4Item& it = p.items[0];
-    // Blocks 8 apart take one KV head's units of query rows, the longest lists first.
-    uint32_t b = blockIdx.x;
-    const uint32_t kvh = b % p.nkv;
-    b /= p.nkv;
-    const uint32_t qt = p.nqt - 1 - b / it.nchunk, chunk = b % it.nchunk;
+    // The longest lists first.
+    const uint32_t kvh = blockIdx.x, chunk = blockIdx.y, qt = p.nqt - 1 - blockIdx.z;
     const uint32_t kvd = p.nkv * HD, nq = it.rows * p.G, q0 = qt * QT, q1 = min(q0 + QT, nq);
-    const uint32_t first = p.tree ? it.base : it.base + q0 / p.G;  // slots every row here sees
+    const uint32_t r0 = q0 / p.G, h0 = q0 - r0 * p.G;
+    const uint32_t seen = p.tree ? it.base : it.base + r0;  // slots every row here sees
     const uint32_t end = p.tree ? tree_end(p, it) : it.base + (q1 - 1) / p.G;
+    const uint32_t all = (uint32_t)(((uint64_t)end + Q4_TILE_B - 1) / Q4_TILE_B), t0 = chunk * it.chunk;
+    const uint32_t t1 = t0 < all ? min(t0 + it.chunk, all) : t0;
+
+    const uint64_t e0 = it.kvoff * kvd;
+    const uint32_t rem0 = (uint32_t)(e0 & 255), rem = rem0 + kvh * HD;
+    const uint64_t base = (e0 >> 8) * Q4_UNIT_BYTES, tile_bytes = (uint64_t)kvd * 36, to = base + q4_bytes(end, rem0, kvd);
+
+    // This wave's share of a tile: K's slots 16 wave .. + 15, and of V's half wave / 2 half the
+    // columns of every lane.
+    const uint32_t half = wave & 1, step = wave >> 1;
+    KLoad<NB> kl;
+    VLoad<NB, true> vl;
+    kl.set(rem + m16 * kvd, g);
+    vl.set(rem, kvd, m16, g, half);
+    uint32_t kw[NB], vw[S::N][8];
+    f16 ks[KLoad<NB>::NS], vs[S::N][8];
+    auto fetch = [&](uint32_t t) {  // (16 slots are whole units)
+        const uint64_t at = base + t * tile_bytes, ka = at + wave * 9 * kvd, va = at + step * 18 * kvd;
+        kl.load(q4_from(p.kc, min(ka, to), to), 0, kw, ks);
+        vl.load(q4_from(p.vc, min(va, to), to), kvd, vw, vs);
+    };
+    if (t0 < t1) fetch(t0);
 
     Sees see[RT];
     half8 qh[RT][NB], ql[RT][NB];
     float c[RT];
 #pragma unroll
     for (int r = 0; r < RT; r++) {
-        const uint32_t n = q0 + (wave * RT + r) * 16 + m16;
-        const bool valid = n < nq;
-        const uint32_t row = it.row0 + (valid ? n / p.G : 0), head = kvh * p.G + (valid ? n % p.G : 0);
-        see[r] = Sees{valid ? it.base + (p.tree ? 0 : n / p.G) : end, 0, 0};
-        if (p.tree && valid) {
-            see[r].lo = p.masks[2 * row];
-            see[r].hi = p.masks[2 * row + 1];
-        }
-        c[r] = load_q<NB>(valid ? p.q + ((size_t)row * p.nh + head) * HD : nullptr, g, p.sc, qh[r], ql[r]);
+        const uint32_t x = (wave * RT + r) * 16 + m16, y = h0 + x, dr = (y * (65536 / p.G + 1)) >> 16;  // y / G
+        const bool valid = q0 + x < nq;
+        const uint32_t row = it.row0 + (valid ? r0 + dr : 0), head = kvh * p.G + (valid ? y - dr * p.G : 0);
+        see[r] = sees(p, it, r0 + dr, valid, end);
+        const float* q = p.q + ((size_t)row * p.nh + head) * HD;
+        float v[NB][8], top = 0.0f, k;
+#pragma unroll
+        for (int j = 0; j < NB; j++) top = q_dims(q + 8 * (NB * g + j), valid, v[j], top);
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        q_scale(top, p.sc, k, c[r]);
+#pragma unroll
+        for (int j = 0; j < NB; j++) q_parts(v[j], k, qh[r][j], ql[r][j]);
     }
 
-    const uint64_t e0 = it.kvoff * kvd;
-    const uint32_t rem = (uint32_t)(e0 & 255) + kvh * HD;
-    const uint64_t tile_bytes = (uint64_t)kvd * 36;  // 64 slots
-    const uint8_t* kbase = p.kc + (e0 >> 8) * Q4_UNIT_BYTES;
-    const uint8_t* vbase = p.vc + (e0 >> 8) * Q4_UNIT_BYTES;
-    const uint32_t ntiles = (uint32_t)(((uint64_t)end + Q4_TILE_B - 1) / Q4_TILE_B);
-    const uint32_t t0 = chunk * it.chunk, t1 = min(t0 + it.chunk, ntiles);
-
-    // This wave's share of a tile: K's slots 16 wave .. + 15, and of V's half wave / 2 half the
-    // columns of every lane.
-    const uint32_t half = wave & 1, step = wave >> 1;
-    KLoad<NB> kl;
-    uint32_t vcode[S::N][8], vscale[S::N][8];
-    auto place = [&](uint32_t last) {
-        kl.set(rem + min(16 * wave + m16, last) * kvd, g);
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t e = rem + min(32 * step + 4 * g + (i & 3) + 16 * (i >> 2), last) * kvd;
-#pragma unroll
-            for (int si = 0; si < S::N; si++) {
-                const uint32_t W = S::w(si), ec = e + S::col(si) + W * m16 + (W == 2 ? 0 : W / 2 * half);
-                vcode[si][i] = q4_code_at32(ec);
-                vscale[si][i] = q4_scale_at32(ec);
-            }
-        }
-    };
-    place(Q4_TILE_B - 1);
-    uint32_t kw[NB], vw[S::N][8];
-    f16 ks[KLoad<NB>::NS], vs[S::N][8];
-    auto fetch = [&](uint32_t t) {
-        const uint32_t ts = t * Q4_TILE_B;
-        if (end - ts < Q4_TILE_B) place(end - 1 - ts);
-        const uint8_t* kt = kbase + t * tile_bytes;
-        const uint8_t* vt = vbase + t * tile_bytes;
-        kl.load(kt, kw, ks);
-#pragma unroll
-        for (int si = 0; si < S::N; si++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                vw[si][i] = S::w(si) == 8 ? load_codes<4>(vt + vcode[si][i]) : load_codes<2>(vt + vcode[si][i]);
-                vs[si][i] = *(const f16*)(vt + vscale[si][i]);
-            }
-    };
     auto unpack = [&](uint32_t t, int buf) {
-        if (t * Q4_TILE_B + Q4_TILE_B > first) {  // some row here does not see all of it
+        if (t * Q4_TILE_B + Q4_TILE_B > seen) {  // some row here does not see all of it
             bool odd = false;
 #pragma unroll
             for (int si = 0; si < S::N; si++)
@@ -568,22 +685,22 @@ __global__ __launch_bounds__(64 * Q4_WAVES, NB <= 4 ? 2 : 1) void attn_q4_tile(c
             if (odd) odd_tile[buf] = t + 1;
         }
 #pragma unroll
-        for (int j = 0; j < NB; j++) kf[buf][wave][j][lane] = unpack_k(kw[j], KLoad<NB>::of(ks, j));
+        for (int j = 0; j < NB; j++) kf[buf][wave][j][lane] = unpack_k(bits, kw[j], KLoad<NB>::of(ks, j));
 #pragma unroll
         for (int si = 0; si < S::N; si++) {
             if (S::w(si) == 8) {
                 half8 x[4];
-                unpack_v<4>(vw[si], vs[si], x);
+                unpack_v<4>(bits, vw[si], vs[si], x);
 #pragma unroll
                 for (int k = 0; k < 4; k++) vf[buf][step][S::frag(si) + 4 * half + k][lane] = x[k];
             } else if (S::w(si) == 4) {
                 half8 x[2];
-                unpack_v<2>(vw[si], vs[si], x);
+                unpack_v<2>(bits, vw[si], vs[si], x);
 #pragma unroll
                 for (int k = 0; k < 2; k++) vf[buf][step][S::frag(si) + 2 * half + k][lane] = x[k];
             } else {
                 half8 x[2];
-                unpack_v<2>(vw[si], vs[si], x);
+                unpack_v<2>(bits, vw[si], vs[si], x);
                 vf[buf][step][S::frag(si) + half][lane] = half ? x[1] : x[0];
             }
         }
@@ -599,7 +716,6 @@ __global__ __launch_bounds__(64 * Q4_WAVES, NB <= 4 ? 2 : 1) void attn_q4_tile(c
         for (int f = 0; f < NF; f++) o[r][f] = f32x4{0, 0, 0, 0};
     }
     if (threadIdx.x < 2) odd_tile[threadIdx.x] = 0;
-    if (t0 < t1) fetch(t0);
     __syncthreads();
     if (t0 < t1) unpack(t0, 0);
     __syncthreads();
@@ -607,68 +723,73 @@ __global__ __launch_bounds__(64 * Q4_WAVES, NB <= 4 ? 2 : 1) void attn_q4_tile(c
         const int buf = (t - t0) & 1;
         const uint32_t ts = t * Q4_TILE_B;
         if (t + 1 < t1) fetch(t + 1);
-        const bool edge = ts + Q4_TILE_B > first;
+        const bool edge = ts + Q4_TILE_B > seen;
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            f32x4 acc[RT][2];
+            // (Four sums in turn, so that no MFMA waits for the one before: one set of rows takes the
+            // parts of q apart.)
+            constexpr int LO = RT == 1 ? 1 : 0;
+            f32x4 s[RT][2], s2[2];
 #pragma unroll
-            for (int r = 0; r < RT; r++) acc[r][0] = acc[r][1] = f32x4{0, 0, 0, 0};
+            for (int r = 0; r < RT; r++) s[r][0] = s[r][1] = s2[0] = s2[1] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int j = 0; j < NB; j++)
+            for (int j = 0; j < NB; j++) {
+                const half8 k0 = kf[buf][2 * u][j][lane], k1 = kf[buf][2 * u + 1][j][lane];
 #pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const half8 k = kf[buf][2 * u + x][j][lane];
-#pragma unroll
-                    for (int r = 0; r < RT; r++) {
-                        acc[r][x] = mfma16(k, qh[r][j], acc[r][x]);
-                        acc[r][x] = mfma16(k, ql[r][j], acc[r][x]);
-                    }
+                for (int r = 0; r < RT; r++) {
+                    s[r][0] = mfma16(k0, qh[r][j], s[r][0]);
+                    s[r][1] = mfma16(k1, qh[r][j], s[r][1]);
                 }
+#pragma unroll
+                for (int r = 0; r < RT; r++) {
+                    f32x4(&to)[2] = LO ? s2 : s[r];
+                    to[0] = mfma16(k0, ql[r][j], to[0]);
+                    to[1] = mfma16(k1, ql[r][j], to[1]);
+                }
+            }
             half8 ph[RT], pl[RT];
 #pragma unroll
             for (int r = 0; r < RT; r++) {
-                float s[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) s[i] = acc[r][i >> 2][i & 3] * c[r];
+                if (LO) {
+                    s[r][0] += s2[0];
+                    s[r][1] += s2[1];
+                }
                 if (edge)
 #pragma unroll
                     for (int i = 0; i < 8; i++)
-                        if (!see[r].at(ts + 32 * u + 16 * (i >> 2) + 4 * g + (i & 3), it.base, end, p.tree)) s[i] = -INFINITY;
+                        if (!see[r].at(ts + 32 * u + 16 * (i >> 2) + 4 * g + (i & 3))) s[r][i >> 2][i & 3] = -INFINITY;
                 float f;
-                if (raise(s, ref[r], f)) {
+                if (raise(s[r], c[r], ref[r], f)) {
                     l[r] *= f;
 #pragma unroll
                     for (int k = 0; k < NF; k++) o[r][k] *= f;
                 }
-                const float base = ref[r] == -INFINITY ? 0.0f : ref[r];
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float w = exp2_hw(s[i] - base);
-                    l[r] += w;
-                    ph[r][i] = (f16)w;
-                    pl[r][i] = (f16)(w - (float)ph[r][i]);
-                }
+                weights<false>(s[r], c[r], ref[r], 0.0f, l[r], ph[r], pl[r]);
             }
 #pragma unroll
-            for (int f = 0; f < NF; f++) {
-                const half8 v = vf[buf][u][f][lane];
+            for (int f = 0; f < NF; f += 2) {
+                const half8 v0 = vf[buf][u][f][lane], v1 = vf[buf][u][f + 1][lane];
 #pragma unroll
                 for (int r = 0; r < RT; r++) {
-                    o[r][f] = mfma16(v, ph[r], o[r][f]);
-                    o[r][f] = mfma16(v, pl[r], o[r][f]);
+                    o[r][f] = mfma16(v0, ph[r], o[r][f]);
+                    o[r][f + 1] = mfma16(v1, ph[r], o[r][f + 1]);
+                }
+#pragma unroll
+                for (int r = 0; r < RT; r++) {
+                    o[r][f] = mfma16(v0, pl[r], o[r][f]);
+                    o[r][f + 1] = mfma16(v1, pl[r], o[r][f + 1]);
                 }
             }
         }
         if (edge && odd_tile[buf] == t + 1) {
-            const uint8_t* vt = vbase + t * tile_bytes;
+            const q4_rsrc vr = q4_from(p.vc, base + t * tile_bytes, to);
             for (uint32_t i = 0; i < Q4_TILE_B && ts + i < end; i++)
 #pragma unroll
                 for (int si = 0; si < S::N; si++) {
-                    const uint32_t e = rem + i * kvd + S::col(si) + S::w(si) * 4 * g;
-                    const bool odd = odd_scale(*(const f16*)(vt + q4_scale_at32(e)));
+                    const bool odd = odd_scale(load_scale(vr, q4_scale_at32(rem + i * kvd + S::col(si) + S::w(si) * 4 * g), 0));
 #pragma unroll
                     for (int r = 0; r < RT; r++)
-                        if (odd && see[r].at(ts + i, it.base, end, p.tree))
+                        if (odd && see[r].at(ts + i))
 #pragma unroll
                             for (int k = 0; k < S::w(si); k++) o[r][S::frag(si) + k] = f32x4{NAN, NAN, NAN, NAN};
                 }
@@ -677,25 +798,23 @@ __global__ __launch_bounds__(64 * Q4_WAVES, NB <= 4 ? 2 : 1) void attn_q4_tile(c
         __syncthreads();
     }
 
-    const uint32_t unit = (kvh * p.nqt + qt) * it.nchunk + chunk;
+    const size_t unit = ((size_t)kvh * p.nqt + qt) * it.nchunk + chunk;
 #pragma unroll
     for (int r = 0; r < RT; r++) {
         l[r] += __shfl_xor(l[r], 16);
         l[r] += __shfl_xor(l[r], 32);
-        const uint32_t sl = (wave * RT + r) * 16 + m16, n = q0 + sl;
-        if (n >= nq) continue;
-        float* dst;
-        float k = 1.0f;
-        if (it.nchunk == 1) {
-            dst = p.out + ((size_t)(it.row0 + n / p.G) * p.nh + kvh * p.G + n % p.G) * HD;
-            k = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
-        } else {
-            dst = p.part_o + ((size_t)unit * QT + sl) * HD;
-            if (g == 0) {
-                p.part_ml[2 * ((size_t)unit * QT + sl)] = ref[r];
-                p.part_ml[2 * ((size_t)unit * QT + sl) + 1] = l[r];
-            }
+        const uint32_t sl = (wave * RT + r) * 16 + m16;
+        if (q0 + sl >= nq) continue;
+        if (it.nchunk > 1) {
+            f32x4* part = (f32x4*)p.part_o + (unit * (QT / 16) + sl / 16) * NF * 64 + lane;
+#pragma unroll
+            for (int f = 0; f < NF; f++) part[64 * f] = o[r][f];
+            if (g == 0) *(float2*)(p.part_ml + 2 * (unit * QT + sl)) = float2{ref[r], l[r]};
+            continue;
         }
+        const uint32_t y = h0 + sl, dr = (y * (65536 / p.G + 1)) >> 16;
+        float* dst = p.out + ((size_t)(it.row0 + r0 + dr) * p.nh + kvh * p.G + y - dr * p.G) * HD;
+        const float k = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
 #pragma unroll
         for (int si = 0; si < S::N; si++)
 #pragma unroll
@@ -706,61 +825,86 @@ __global__ __launch_bounds__(64 * Q4_WAVES, NB <= 4 ? 2 : 1) void attn_q4_tile(c
     }
 }
 
-// One output row of one head from its chunks' states.
+// The chunks of 16 query rows of a list brought together, two operands' columns a workgroup, its
+// waves a share of the chunks each; states lie as their waves held them.
 constexpr uint32_t Q4_MAX_CHUNKS = 256;
+constexpr int Q4_FOLD_WAVES = 8;
 
-__global__ __launch_bounds__(256) void attn_q4_fold(const Q4Params p, uint32_t hd) {
-    __shared__ float wt[Q4_MAX_CHUNKS];
-    __shared__ float red[8];
-    __shared__ f32x4 sum[256];
-    const uint32_t tid = threadIdx.x, head = blockIdx.x, kvh = head / p.G;
-    const Q4Item& it = p.items[p.nitems > 1 ? blockIdx.y : 0];
+template <int NB>
+__global__ __launch_bounds__(64 * Q4_FOLD_WAVES) void attn_q4_fold(const Q4Params p) {
+    constexpr int HD = 32 * NB, NF = 2 * NB;
+    __shared__ float wt[Q4_MAX_CHUNKS][16];
+    __shared__ float red[2][4 * Q4_FOLD_WAVES][16];
+    __shared__ f32x4 sum[Q4_FOLD_WAVES][2][64];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m16 = lane & 15, g = lane >> 4;
+    const uint32_t f = 2 * blockIdx.x, kvh = blockIdx.y, z = blockIdx.z;
+    const Q4Item& it = p.items[p.nitems > 1 ? z : 0];
     if (it.nchunk == 1) return;  // written by its workgroup
-    const uint32_t r = p.nitems > 1 ? 0 : blockIdx.y, n = r * p.G + head % p.G;
-    const size_t u0 = it.unit0 + (size_t)(kvh * p.nqt + n / p.qt) * it.nchunk;
-    const uint32_t sl = n % p.qt;
-    float mc = -INFINITY, lc = 0.0f;
-    if (tid < it.nchunk) {
-        const float2 ml = *(const float2*)(p.part_ml + 2 * ((u0 + tid) * p.qt + sl));
-        mc = ml.x;
-        lc = ml.y;
-    }
-    float M = mc;
+    const uint32_t n0 = p.nitems > 1 ? 0 : 16 * z, n = n0 + m16, nq = it.rows * p.G;  // this row of the item's
+    const size_t u0 = it.unit0 + ((size_t)kvh * p.nqt + n0 / p.qt) * it.nchunk;
+    const uint32_t sl = n0 % p.qt;
+    const bool valid = n < nq;
+    // Weights of the chunks: thread (part, row) takes every 32nd.
+    constexpr uint32_t PARTS = 4 * Q4_FOLD_WAVES;
+    const uint32_t part = tid >> 4;
+    float2 ml[Q4_MAX_CHUNKS / PARTS];
+    float R = -INFINITY, L = 0.0f;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) M = fmaxf(M, __shfl_xor(M, d));
-    if ((tid & 63) == 0) red[tid >> 6] = M;
-    __syncthreads();
-    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float w = exp2_hw(mc - (M == -INFINITY ? 0.0f : M));
-    wt[tid] = w;
-    float L = w * lc;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) L += __shfl_xor(L, d);
-    if ((tid & 63) == 0) red[4 + (tid >> 6)] = L;
-    __syncthreads();
-    L = (red[4] + red[5]) + (red[6] + red[7]);
-    const uint32_t q = hd / 4, parts = 256 / q, part = tid / q, col = 4 * (tid % q);
-    f32x4 a = {0, 0, 0, 0};
-    if (part < parts)
-        for (uint32_t c = part; c < it.nchunk; c += parts)
-            a += wt[c] * *(const f32x4*)(p.part_o + ((u0 + c) * p.qt + sl) * hd + col);
-    sum[tid] = a;
-    __syncthreads();
-    if (part == 0) {
-        for (uint32_t k = 1; k < parts; k++) a += sum[k * q + tid];
-        *(f32x4*)(p.out + ((size_t)(it.row0 + r) * p.nh + head) * hd + col) = a * (L == 0.0f ? 0.0f : 1.0f / L);
+    for (uint32_t i = 0; i < Q4_MAX_CHUNKS / PARTS; i++) {
+        const uint32_t c = part + PARTS * i;
+        ml[i] = c < it.nchunk && valid ? *(const float2*)(p.part_ml + 2 * ((u0 + c) * p.qt + sl + m16)) : float2{-INFINITY, 0.0f};
+        R = fmaxf(R, ml[i].x);
     }
+    red[0][part][m16] = R;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < PARTS; i++) R = fmaxf(R, red[0][i][m16]);
+    const float Rs = R == -INFINITY ? 0.0f : R;
+#pragma unroll
+    for (uint32_t i = 0; i < Q4_MAX_CHUNKS / PARTS; i++) {
+        const float w = exp2_hw(ml[i].x - Rs);
+        wt[part + PARTS * i][m16] = w;
+        L += w * ml[i].y;
+    }
+    red[1][part][m16] = L;
+    __syncthreads();
+    f32x4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+    if (valid) {
+        const f32x4* at = (const f32x4*)p.part_o + ((u0 * (p.qt / 16) + sl / 16) * NF + f) * 64 + lane;
+        const size_t next = (size_t)(p.qt / 16) * NF * 64;
+#pragma unroll 4
+        for (uint32_t c = wave; c < it.nchunk; c += Q4_FOLD_WAVES) {
+            const float w = wt[c][m16];
+            a += w * at[c * next];
+            b += w * at[c * next + 64];
+        }
+    }
+    sum[wave][0][lane] = a;
+    sum[wave][1][lane] = b;
+    __syncthreads();
+    if (wave >= 2 || !valid) return;
+    L = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < PARTS; i++) L += red[1][i][m16];
+    a = sum[0][wave][lane];
+#pragma unroll
+    for (int w = 1; w < Q4_FOLD_WAVES; w++) a += sum[w][wave][lane];
+    a *= L == 0.0f ? 0.0f : 1.0f / L;
+    const uint32_t r = n / p.G, col = column<NB>(f + wave, g), step = stride<NB>(f);
+    float* dst = p.out + ((size_t)(it.row0 + r) * p.nh + kvh * p.G + n - r * p.G) * HD + col;
+#pragma unroll
+    for (int i = 0; i < 4; i++) dst[i * step] = a[i];
 }
 
-template <int NB>
-void launch_row(const Q4Params& p, uint32_t blocks, bool pk, const AttnCall& a, hipStream_t s) {
-    const dim3 grid(blocks), wg(64 * Q4_WAVES);
-    if (pk) hipExtLaunchKernelGGL((attn_q4_row<NB, true>), grid, wg, 0, s, a.ev_before, a.ev_after, 0, p);
-    else hipExtLaunchKernelGGL((attn_q4_row<NB, false>), grid, wg, 0, s, a.ev_before, a.ev_after, 0, p);
+template <int NB, int WAVES>
+void launch_row(const Q4Params& p, uint32_t octs, bool pk, const AttnCall& a, hipStream_t s) {
+    const dim3 grid(8, p.nkv, octs), wg(64 * WAVES);
+    if (pk) hipExtLaunchKernelGGL((attn_q4_row<NB, true, WAVES>), grid, wg, 0, s, a.ev_before, a.ev_after, 0, p);
+    else hipExtLaunchKernelGGL((attn_q4_row<NB, false, WAVES>), grid, wg, 0, s, a.ev_before, a.ev_after, 0, p);
 }
 template <int NB>
-void launch_tile(const Q4Params& p, uint32_t blocks, uint32_t rt, const AttnCall& a, hipStream_t s) {
-    const dim3 grid(blocks), wg(64 * Q4_WAVES);
+void launch_tile(const Q4Params& p, uint32_t rt, const AttnCall& a, hipStream_t s) {
+    const dim3 grid(p.nkv, p.items[0].nchunk, p.nqt), wg(64 * Q4_WAVES);
     if constexpr (NB <= 4) {
         if (rt == 2) {
             hipExtLaunchKernelGGL((attn_q4_tile<NB, 2>), grid, wg, 0, s, a.ev_before, a.ev_after, 0, p);
@@ -768,6 +912,11 @@ void launch_tile(const Q4Params& p, uint32_t blocks, uint32_t rt, const AttnCall
         }
     }
     hipExtLaunchKernelGGL((attn_q4_tile<NB, 1>), grid, wg, 0, s, a.ev_before, a.ev_after, 0, p);
+}
+
+template <int NB>
+void launch_fold(const Q4Params& p, uint32_t groups, hipStream_t s) {
+    hipLaunchKernelGGL(attn_q4_fold<NB>, dim3(NB, p.nkv, groups), dim3(64 * Q4_FOLD_WAVES), 0, s, p);
 }
 
 Q4Params params(const AttnCall& a) {
@@ -824,32 +973,34 @@ hipError_t launch_items(Q4Params& p, const AttnCall& a, const uint64_t* lens, Wo
     uint64_t total = 0;
     for (uint32_t i = 0; i < p.nitems; i++) total += (lens[i] + Q4_TILE - 1) / Q4_TILE;
     const uint32_t want = std::max(1u, Q4_ROW_GROUPS / a.nkv);
-    uint32_t units, blocks;
+    uint32_t units, octs;
     bool split;
     auto plan = [&](uint64_t all) {
-        units = blocks = 0;
+        units = octs = 0;
         split = false;
         for (uint32_t i = 0; i < p.nitems; i++) {
             Q4Item& it = p.items[i];
             const uint64_t tiles = (lens[i] + Q4_TILE - 1) / Q4_TILE;
             it.unit0 = units;
-            it.block0 = blocks;
+            it.block0 = octs;
             // A list's share of the workgroups is its share of the tiles.
             cut(it, tiles, (uint32_t)std::max<uint64_t>(1, all * tiles / std::max<uint64_t>(1, total)), Q4_WAVES);
             units += it.nchunk * a.nkv;
-            blocks += (it.nchunk + 7) / 8 * 8 * a.nkv;
+            octs += (it.nchunk + 7) / 8;
             split |= it.nchunk > 1;
         }
     };
     plan(want);
     if (split && !reserve(p, (uint64_t)units * 16, a.hd, ws, s)) plan(0);
     const bool pk = p.items[0].rows * p.G <= 8;
-#define Q4_ROW(NB) launch_row<NB>(p, blocks, pk, a, s)
+#define Q4_ROW(NB) launch_row<NB, Q4_WAVES>(p, octs, pk, a, s)
     Q4_BY_DIM(a.hd / 32, Q4_ROW)
 #undef Q4_ROW
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !split) return e;
-    hipLaunchKernelGGL(attn_q4_fold, dim3(a.nh, p.nitems > 1 ? p.nitems : a.rows), dim3(256), 0, s, p, a.hd);
+#define Q4_FOLD(NB) launch_fold<NB>(p, p.nitems, s)
+    Q4_BY_DIM(a.hd / 32, Q4_FOLD)
+#undef Q4_FOLD
     return hipGetLastError();
 }
 
@@ -864,6 +1015,20 @@ hipError_t q4_attention(const AttnCall& a, Workspace& ws, hipStream_t s) {
     const uint64_t far = std::min<uint64_t>((uint64_t)a.pos + (a.tree ? 64 : a.rows), a.slot_limit);
     const uint64_t nq = (uint64_t)a.rows * p.G;
     if (nq <= 16) return launch_items(p, a, &far, ws, s);
+    const uint32_t most = 65535 * 64 / p.G;  // rows whose units of query rows a grid holds
+    if (a.rows > most) {
+        AttnCall part = a;
+        for (uint32_t r = 0; r < a.rows; r += most) {
+            part.rows = std::min(most, a.rows - r);
+            part.pos = a.pos + r;
+            part.q = a.q + (size_t)r * a.nh * a.hd;
+            part.out = a.out + (size_t)r * a.nh * a.hd;
+            const hipError_t e = q4_attention(part, ws, s);
+            if (e != hipSuccess) return e;
+            part.ev_before = part.ev_after = nullptr;
+        }
+        return hipSuccess;
+    }
     // 32 query rows a wave where that still makes a workgroup for every CU.
     const uint32_t rt = a.hd <= 128 && (nq + 127) / 128 * a.nkv >= 256 ? 2 : 1;
     p.qt = 64 * rt;
@@ -871,14 +1036,14 @@ hipError_t q4_attention(const AttnCall& a, Workspace& ws, hipStream_t s) {
     const uint64_t groups = (uint64_t)p.nqt * a.nkv, tiles = (far + Q4_TILE_B - 1) / Q4_TILE_B;
     cut(it, tiles, (uint32_t)std::max<uint64_t>(1, Q4_TILE_GROUPS / groups), 2);
     if (it.nchunk > 1 && !reserve(p, groups * it.nchunk * p.qt, a.hd, ws, s)) cut(it, tiles, 1, 2);
-    const uint64_t blocks = groups * it.nchunk;
-    if (blocks > 0x7fffffffull) return hipErrorInvalidValue;
-#define Q4_TILES(NB) launch_tile<NB>(p, (uint32_t)blocks, rt, a, s)
+#define Q4_TILES(NB) launch_tile<NB>(p, rt, a, s)
     Q4_BY_DIM(a.hd / 32, Q4_TILES)
 #undef Q4_TILES
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || it.nchunk == 1) return e;
-    hipLaunchKernelGGL(attn_q4_fold, dim3(a.nh, a.rows), dim3(256), 0, s, p, a.hd);
+#define Q4_FOLD(NB) launch_fold<NB>(p, (uint32_t)((nq + 15) / 16), s)
+    Q4_BY_DIM(a.hd / 32, Q4_FOLD)
+#undef Q4_FOLD
     return hipGetLastError();
 }
 

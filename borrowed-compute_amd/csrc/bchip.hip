@@ -189,7 +189,8 @@ int check_heads(uint32_t nh, uint32_t nkv, uint32_t hd) {
 // What a 4-bit cache asks beside: heads of whole blocks, and tile offsets within 32 bits.
 int check_q4(uint32_t nkv, uint32_t hd) {
     if (hd % Q4_BLOCK) return fail(BCHIP_E_UNSUPPORTED, "head_dim %u (a 4-bit cache takes multiples of %u)", hd, Q4_BLOCK);
-    if ((uint64_t)nkv * hd > (1u << 24)) return fail(BCHIP_E_UNSUPPORTED, "%u KV heads of %u (a 4-bit cache's slot holds at most 2^24 elements)", nkv, hd);
+    if ((uint64_t)nkv * hd > (1u << 20))
+        return fail(BCHIP_E_UNSUPPORTED, "%u KV heads of %u (a 4-bit cache's slot holds at most 2^20 elements)", nkv, hd);
     return BCHIP_OK;
 }
 

@@ -28,7 +28,7 @@
  *    as a code the value over the scale to the nearest even; a block with an element that is not
  *    finite gets the scale NaN and reads as NaN. A buffer written elsewhere has to keep to such
  *    scales. Element offsets, counts and row widths are multiples of 32, and cache calls take
- *    head dims that are multiples of 32 and slots of at most 2^24 elements (else
+ *    head dims that are multiples of 32 and slots of at most 2^20 elements (else
  *    BCHIP_E_UNSUPPORTED).
  */
 #ifndef BCHIP_H
