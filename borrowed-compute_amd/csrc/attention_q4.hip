@@ -187,55 +187,116 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ q4_rsrc q4_from(const uint8_t* base, uint64_t at, uint64_t end) {
     return __builtin_amdgcn_make_buffer_rsrc((void*)(base + at), 0, (uint32_t)min(end - at, (uint64_t)0x7fffffffu), 0x00020000);
 }
-template <int W>
-__device__ __forceinline__ uint32_t load_codes(q4_rsrc r, uint32_t lane, uint32_t all) {
-    if constexpr (W == 8) return __builtin_amdgcn_raw_buffer_load_b32(r, lane, all, 0);
-    else if constexpr (W == 4) return __builtin_amdgcn_raw_buffer_load_b16(r, lane, all, 0);
-    else return __builtin_amdgcn_raw_buffer_load_b8(r, lane, all, 0);
-}
-__device__ __forceinline__ f16 load_scale(q4_rsrc r, uint32_t lane, uint32_t all) {
-    return __builtin_bit_cast(f16, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, lane, all, 0));
+__device__ __forceinline__ f16 load_scale(q4_rsrc r, uint32_t at) {
+    return __builtin_bit_cast(f16, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0));
 }
 
-// Byte offsets, within a tile, of what a lane reads of a slot: its K words and scales.
+// One head's part of SLOTS slots of K or V on its way into LDS: a thread takes blocks of a slot,
+// 16 bytes of codes and their scale, so consecutive lanes read consecutive bytes (loads of a few
+// bytes a lane at the operands' own places cost the memory path 30 to 60 cycles each). In LDS a slot
+// takes SLOT bytes, its codes and then its scales: an odd multiple of 16 for heads of 64 to 256,
+// so the operands' lanes read every bank once.
+template <int NB, int SLOTS, int THREADS>
+struct Raw {
+    static constexpr int SLOT = 16 * NB + 16, BYTES = SLOT * SLOTS;
+    static constexpr int N = (SLOTS * NB + THREADS - 1) / THREADS, STEP = THREADS / NB;  // slots from load to load
+    static constexpr bool SAME = THREADS % NB == 0 && STEP % 8 == 0;  // (8 slots are whole units)
+    static constexpr int M = SAME ? 1 : N;
+    uint32_t code[M], scale[M], to[M], tod[M];
+    u32x4 c[N];
+    uint16_t d[N];
+    __device__ __forceinline__ void set(uint32_t rem, uint32_t kvd, uint32_t thread) {
+#pragma unroll
+        for (int i = 0; i < M; i++) {
+            const uint32_t x = min((uint32_t)(i * THREADS) + thread, (uint32_t)(SLOTS * NB - 1)), slot = x / NB, b = x % NB;
+            const uint32_t e = rem + slot * kvd + 32 * b;
+            code[i] = q4_code_at32(e);
+            scale[i] = q4_scale_at32(e);
+            to[i] = slot * SLOT + 16 * b;
+            tod[i] = slot * SLOT + 16 * NB + 2 * b;
+        }
+    }
+    __device__ __forceinline__ void load(q4_rsrc r, uint32_t kvd) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const uint32_t at = SAME ? i * (STEP / 8) * (kvd / 2 * 9) : 0;
+            c[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, code[SAME ? 0 : i], at, 0));
+            d[i] = __builtin_amdgcn_raw_buffer_load_b16(r, scale[SAME ? 0 : i], at, 0);
+        }
+    }
+    __device__ __forceinline__ void store(uint8_t* lds) const {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int at = SAME ? i * STEP * SLOT : 0;
+            *(u32x4*)(lds + to[SAME ? 0 : i] + at) = c[i];
+            *(uint16_t*)(lds + tod[SAME ? 0 : i] + at) = d[i];
+        }
+    }
+};
+
+// K's operands of a slot in LDS: lane group g takes the words NB g .. NB g + NB - 1 of its codes.
 template <int NB>
-struct KLoad {
-    static constexpr bool WHOLE = NB == 1 || NB == 2 || NB == 4 || NB == 8;  // consecutive bytes
-    static constexpr int NC = WHOLE ? 1 : NB;                                // code offsets
-    static constexpr int NS = NB == 8 ? 2 : WHOLE ? 1 : NB;                  // scales
-    uint32_t code[NC], scale[NC];
-    __device__ __forceinline__ void set(uint32_t e, uint32_t g) {
+__device__ __forceinline__ void read_k(const uint8_t* slot, uint32_t g, uint32_t (&w)[NB], f16 (&s)[NB]) {
+    constexpr int ALIGN = NB % 4 == 0 ? 4 : NB % 2 == 0 ? 2 : 1;
+    if constexpr (ALIGN == 4) {
 #pragma unroll
-        for (int j = 0; j < NC; j++) {
-            code[j] = q4_code_at32(e + 8 * (NB * g + j));
-            scale[j] = q4_scale_at32(e + 8 * (NB * g + j));
+        for (int j = 0; j < NB; j += 4) {
+            const u32x4 a = *(const u32x4*)(slot + 4 * (NB * g + j));
+            w[j] = a.x, w[j + 1] = a.y, w[j + 2] = a.z, w[j + 3] = a.w;
         }
-    }
-    __device__ __forceinline__ void load(q4_rsrc r, uint32_t at, uint32_t (&w)[NB], f16 (&s)[NS]) const {
-        if constexpr (NB == 1) {
-            w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, code[0], at, 0);
-        } else if constexpr (NB == 2) {
-            const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, code[0], at, 0));
-            w[0] = a.x, w[1] = a.y;
-        } else if constexpr (NB == 4 || NB == 8) {
+    } else if constexpr (ALIGN == 2) {
 #pragma unroll
-            for (int j = 0; j < NB; j += 4) {
-                const u32x4 a = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, code[0] + 4 * j, at, 0));
-                w[j] = a.x, w[j + 1] = a.y, w[j + 2] = a.z, w[j + 3] = a.w;
+        for (int j = 0; j < NB; j += 2) {
+            const u32x2 a = *(const u32x2*)(slot + 4 * (NB * g + j));
+            w[j] = a.x, w[j + 1] = a.y;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NB; j++) w[j] = *(const uint32_t*)(slot + 4 * (NB * g + j));
+    }
+    constexpr int SAME = NB == 1 || NB == 2 || NB == 4 || NB == 8 ? (NB < 4 ? NB : 4) : 1;  // words of one block
+#pragma unroll
+    for (int j = 0; j < NB; j++) s[j] = j % SAME ? s[j - 1] : *(const f16*)(slot + 16 * NB + 2 * ((NB * g + j) >> 2));
+}
+
+// W columns of V's segment si in LDS (W: the segment's, or half of them from the half'th on), for
+// the operands of 32 slots from `tile`: slots 4g .. 4g + 3 and 16 + 4g ... .
+template <int NB, bool HALF>
+struct VRead {
+    using S = Seg<NB>;
+    static constexpr int w(int si) { return HALF && S::w(si) > 2 ? S::w(si) / 2 : S::w(si); }
+    uint32_t word[S::N][8];
+    f16 scale[S::N][8];
+    __device__ __forceinline__ void read(const uint8_t* tile, uint32_t m16, uint32_t g, uint32_t half) {
+        constexpr int SLOT = 16 * NB + 16;
+#pragma unroll
+        for (int si = 0; si < S::N; si++) {
+            const uint32_t c = S::col(si) + S::w(si) * m16;
+            const uint8_t* at = tile + 4 * g * SLOT;
+            const uint32_t code = c / 2 + (w(si) < S::w(si) ? w(si) / 2 * half : 0), d = 16 * NB + c / 32 * 2;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint8_t* x = at + ((i & 3) + 16 * (i >> 2)) * SLOT;
+                word[si][i] = w(si) == 8   ? *(const uint32_t*)(x + code)
+                              : w(si) == 4 ? *(const uint16_t*)(x + code)
+                                           : (uint32_t) * (x + code);
+                scale[si][i] = *(const f16*)(x + d);
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < NB; j++) w[j] = __builtin_amdgcn_raw_buffer_load_b32(r, code[j], at, 0);
-        }
-        if constexpr (NB == 8) {
-            const half2 a = __builtin_bit_cast(half2, (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, scale[0], at, 0));
-            s[0] = a[0], s[1] = a[1];  // blocks 2g, 2g + 1
-        } else {
-#pragma unroll
-            for (int j = 0; j < NS; j++) s[j] = load_scale(r, scale[j], at);
         }
     }
-    static __device__ __forceinline__ f16 of(const f16 (&s)[NS], int j) { return s[NB == 8 ? j / 4 : NS == 1 ? 0 : j]; }
+    // Scales that are not finite become 0; whether there were any.
+    __device__ __forceinline__ bool drop_odd() {
+        bool odd = false;
+#pragma unroll
+        for (int si = 0; si < S::N; si++)
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (odd_scale(scale[si][i])) {
+                    scale[si][i] = (f16)0.0f;
+                    odd = true;
+                }
+        return odd;
+    }
 };
 
 // What a query row sees: the slots below vis, and in a tree those of `mask` from base on.
@@ -317,54 +378,6 @@ __device__ __forceinline__ float ror8(float x) {  // lane n of each 16 gets lane
 
 constexpr uint32_t Q4_TILE = 32;
 
-// Where a lane reads eight slots of V, 4g .. 4g + 3 and 16 more of each, in a tile of 32
-// slots: its columns' words and their scales. Slots 4g + j lie the same way within their
-// units for every g where four slots are whole units and a segment lies within one (heads of 64,
-// 128 or 256): a lane's offset is then one for all, beside a uniform one. HALF: half the columns of
-// every segment but those of 32, whose words both halves read.
-template <int NB, bool HALF>
-struct VLoad {
-    using S = Seg<NB>;
-    static constexpr bool SAME = NB == 2 || NB == 4 || NB == 8;
-    static constexpr int w(int si) { return HALF && S::w(si) > 2 ? S::w(si) / 2 : S::w(si); }
-    uint32_t code[S::N][SAME ? 1 : 8], scale[S::N][SAME ? 1 : 8];
-    uint32_t ucode[S::N][4], uscale[S::N][4];
-    __device__ __forceinline__ void set(uint32_t rem, uint32_t kvd, uint32_t m16, uint32_t g, uint32_t half) {
-#pragma unroll
-        for (int si = 0; si < S::N; si++) {
-            const uint32_t c = S::w(si) * m16 + (S::w(si) > 2 ? w(si) * half : 0);
-            if constexpr (SAME) {
-                code[si][0] = g * (kvd / 4 * 9) + c / 2;
-                scale[si][0] = g * (kvd / 4 * 9) + c / 32 * 2;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    ucode[si][j] = q4_code_at32(rem + j * kvd + S::col(si));
-                    uscale[si][j] = q4_scale_at32(rem + j * kvd + S::col(si));
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const uint32_t e = rem + (4 * g + (i & 3) + 16 * (i >> 2)) * kvd + S::col(si) + c;
-                    code[si][i] = q4_code_at32(e);
-                    scale[si][i] = q4_scale_at32(e);
-                }
-            }
-        }
-    }
-    __device__ __forceinline__ void load(q4_rsrc r, uint32_t kvd, uint32_t (&vw)[S::N][8], f16 (&vs)[S::N][8]) const {
-#pragma unroll
-        for (int si = 0; si < S::N; si++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const uint32_t lc = code[si][SAME ? 0 : i], ls = scale[si][SAME ? 0 : i];
-                const uint32_t uc = SAME ? ucode[si][i & 3] + (i >> 2) * 9 * kvd : 0;  // (16 slots are whole units)
-                const uint32_t us = SAME ? uscale[si][i & 3] + (i >> 2) * 9 * kvd : 0;
-                vw[si][i] = w(si) == 8 ? load_codes<8>(r, lc, uc) : w(si) == 4 ? load_codes<4>(r, lc, uc) : load_codes<2>(r, lc, uc);
-                vs[si][i] = load_scale(r, ls, us);
-            }
-    }
-};
-
 // Bytes of `slots` slots from the start of their first unit (rem elements into it).
 __device__ __forceinline__ uint64_t q4_bytes(uint64_t slots, uint32_t rem, uint32_t kvd) {
     return (slots * kvd + rem + Q4_UNIT - 1) / Q4_UNIT * Q4_UNIT_BYTES;
@@ -374,10 +387,12 @@ template <int NB, bool PK, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void attn_q4_row(const Q4Params p) {
     constexpr int HD = 32 * NB, NF = 2 * NB, QW = NB < WAVES ? NB : WAVES, QJ = (NB + WAVES - 1) / WAVES;
     using S = Seg<NB>;
-    __shared__ union {
-        half8 q[PK ? 1 : 2][NB][64];
+    using B = Raw<NB, Q4_TILE, 64>;
+    __shared__ __attribute__((aligned(16))) union {
+        uint8_t raw[WAVES][2][B::BYTES];
         f32x4 o[WAVES > 4 ? WAVES / 2 : 4][NF][64];
     } sh;
+    __shared__ half8 sq[PK ? 1 : 2][NB][64];
     __shared__ float stop[QW][16], sr[WAVES][64], sl[WAVES][64];
     const Q4Bits bits;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -401,22 +416,15 @@ __global__ __launch_bounds__(64 * WAVES) void attn_q4_row(const Q4Params p) {
     const uint32_t rem0 = (uint32_t)(e0 & 255), rem = rem0 + kvh * HD;
     const uint64_t base = (e0 >> 8) * Q4_UNIT_BYTES, tile_bytes = (uint64_t)kvd * 18;
     const uint64_t from = base + first * tile_bytes, to = base + q4_bytes(end, rem0, kvd);
-    KLoad<NB> kl;
-    VLoad<NB, false> vl;
-    kl.set(rem + m16 * kvd, g);
-    vl.set(rem, kvd, m16, g, 0);
-    uint32_t kw[2][NB], vw[S::N][8];
-    f16 ks[2][KLoad<NB>::NS], vs[S::N][8];
-    auto load_k = [&](uint32_t t) {
-        const q4_rsrc r = q4_from(p.kc, from + t * tile_bytes, to);
-#pragma unroll
-        for (int h = 0; h < 2; h++) kl.load(r, h * 9 * kvd, kw[h], ks[h]);
+    B kraw, vraw;
+    kraw.set(rem, kvd, lane);
+    vraw.set(rem, kvd, lane);
+    auto load = [&](uint32_t t) {
+        const uint64_t at = from + t * tile_bytes;
+        kraw.load(q4_from(p.kc, at, to), kvd);
+        vraw.load(q4_from(p.vc, at, to), kvd);
     };
-    auto load_v = [&](uint32_t t) { vl.load(q4_from(p.vc, from + t * tile_bytes, to), kvd, vw, vs); };
-    if (wave < tiles) {  // the first tile is on its way while q is made ready
-        load_k(wave);
-        load_v(wave);
-    }
+    if (wave < tiles) load(wave);  // the first tile is on its way while q is made ready
 
     // q's operands, each wave some of the steps for all.
     const uint32_t n = PK ? (m16 & 7) : m16, r = (n * (65536 / p.G + 1)) >> 16;  // n / G
@@ -446,10 +454,10 @@ __global__ __launch_bounds__(64 * WAVES) void attn_q4_row(const Q4Params p) {
             half8 hi, lo;
             q_parts(x[i], k, hi, lo);
             if constexpr (PK) {
-                sh.q[0][j][lane] = m16 < 8 ? hi : lo;
+                sq[0][j][lane] = m16 < 8 ? hi : lo;
             } else {
-                sh.q[0][j][lane] = hi;
-                sh.q[1][j][lane] = lo;
+                sq[0][j][lane] = hi;
+                sq[1][j][lane] = lo;
             }
         }
     }
@@ -457,8 +465,8 @@ __global__ __launch_bounds__(64 * WAVES) void attn_q4_row(const Q4Params p) {
     half8 qa[NB], qb[NB];
 #pragma unroll
     for (int j = 0; j < NB; j++) {
-        qa[j] = sh.q[0][j][lane];
-        if constexpr (!PK) qb[j] = sh.q[1][j][lane];
+        qa[j] = sq[0][j][lane];
+        if constexpr (!PK) qb[j] = sq[1][j][lane];
     }
 
     f32x4 o[NF];
@@ -468,17 +476,31 @@ __global__ __launch_bounds__(64 * WAVES) void attn_q4_row(const Q4Params p) {
 
     for (uint32_t t = wave; t < tiles; t += WAVES) {
         const uint32_t ts = (first + t) * Q4_TILE;
-        const bool more = t + WAVES < tiles;
+        // The tile's bytes are the wave's own, and LDS serves a wave in order: its lanes' writes come
+        // after their reads of the tile before and before those of this one.
+        uint8_t *kt = sh.raw[wave][0], *vt = sh.raw[wave][1];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        kraw.store(kt);
+        vraw.store(vt);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (t + WAVES < tiles) load(t + WAVES);
         f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, s2[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        uint32_t kw[2][NB];
+        f16 ks[2][NB];
+#pragma unroll
+        for (int h = 0; h < 2; h++) read_k<NB>(kt + (16 * h + m16) * B::SLOT, g, kw[h], ks[h]);
 #pragma unroll
         for (int j = 0; j < NB; j++)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const half8 a = unpack_k(bits, kw[h][j], KLoad<NB>::of(ks[h], j));
+                const half8 a = unpack_k(bits, kw[h][j], ks[h][j]);
                 s[h] = mfma16(a, qa[j], s[h]);
                 if constexpr (!PK) s2[h] = mfma16(a, qb[j], s2[h]);
             }
-        if (more) load_k(t + WAVES);
+        VRead<NB, false> v;
+        v.read(vt, m16, g, 0);
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
@@ -491,14 +513,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_q4_row(const Q4Params p) {
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 if (!see.at(ts + 16 * (i >> 2) + 4 * g + (i & 3))) s[i >> 2][i & 3] = -INFINITY;
-#pragma unroll
-            for (int si = 0; si < S::N; si++)
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (odd_scale(vs[si][i])) {
-                        vs[si][i] = (f16)0.0f;
-                        odd = true;
-                    }
+            odd = v.drop_odd();
         }
         float f;
         if (raise(s, c, ref, f)) {
@@ -511,7 +526,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_q4_row(const Q4Params p) {
         auto pv = [&](auto width, int si) {
             constexpr int W = decltype(width)::value;
             half8 vf[W];
-            unpack_v<W>(bits, vw[si], vs[si], vf);
+            unpack_v<W>(bits, v.word[si], v.scale[si], vf);
 #pragma unroll
             for (int i = 0; i < W; i++) o[S::frag(si) + i] = mfma16(vf[i], ph, o[S::frag(si) + i]);
             if constexpr (!PK) {
@@ -525,14 +540,12 @@ __global__ __launch_bounds__(64 * WAVES) void attn_q4_row(const Q4Params p) {
             else if (S::w(si) == 4) pv(std::integral_constant<int, 4>{}, si);
             else pv(std::integral_constant<int, 2>{}, si);
         }
-        if (more) load_v(t + WAVES);
         if (edge && __any(odd)) {
-            const q4_rsrc vr = q4_from(p.vc, from + t * tile_bytes, to);
             for (uint32_t i = 0; i < Q4_TILE && ts + i < end; i++) {
                 const bool seen = see.at(ts + i);
 #pragma unroll
                 for (int si = 0; si < S::N; si++) {  // (a lane's columns of a segment lie in one block)
-                    const f16 d = load_scale(vr, q4_scale_at32(rem + i * kvd + S::col(si) + S::w(si) * 4 * g), 0);
+                    const f16 d = *(const f16*)(vt + i * B::SLOT + 16 * NB + (S::col(si) + S::w(si) * 4 * g) / 32 * 2);
                     if (seen && odd_scale(d))
 #pragma unroll
                         for (int w = 0; w < S::w(si); w++) o[S::frag(si) + w] = f32x4{NAN, NAN, NAN, NAN};
@@ -617,6 +630,8 @@ __global__ __launch_bounds__(64 * Q4_WAVES, NB <= 4 ? 2 : 1) void attn_q4_tile(c
     using S = Seg<NB>;
     __shared__ half8 kf[2][4][NB][64];
     __shared__ half8 vf[2][2][NF][64];
+    using R = Raw<NB, Q4_TILE_B, 64 * Q4_WAVES>;
+    __shared__ __attribute__((aligned(16))) uint8_t raw[2][R::BYTES];
     __shared__ uint32_t odd_tile[2];  // 1 + the tile of each buffer that held a scale that is not finite
     const Q4Bits bits;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -635,19 +650,13 @@ __global__ __launch_bounds__(64 * Q4_WAVES, NB <= 4 ? 2 : 1) void attn_q4_tile(c
     const uint32_t rem0 = (uint32_t)(e0 & 255), rem = rem0 + kvh * HD;
     const uint64_t base = (e0 >> 8) * Q4_UNIT_BYTES, tile_bytes = (uint64_t)kvd * 36, to = base + q4_bytes(end, rem0, kvd);
 
-    // This wave's share of a tile: K's slots 16 wave .. + 15, and of V's half wave / 2 half the
-    // columns of every lane.
-    const uint32_t half = wave & 1, step = wave >> 1;
-    KLoad<NB> kl;
-    VLoad<NB, true> vl;
-    kl.set(rem + m16 * kvd, g);
-    vl.set(rem, kvd, m16, g, half);
-    uint32_t kw[NB], vw[S::N][8];
-    f16 ks[KLoad<NB>::NS], vs[S::N][8];
-    auto fetch = [&](uint32_t t) {  // (16 slots are whole units)
-        const uint64_t at = base + t * tile_bytes, ka = at + wave * 9 * kvd, va = at + step * 18 * kvd;
-        kl.load(q4_from(p.kc, min(ka, to), to), 0, kw, ks);
-        vl.load(q4_from(p.vc, min(va, to), to), kvd, vw, vs);
+    R kraw, vraw;
+    kraw.set(rem, kvd, threadIdx.x);
+    vraw.set(rem, kvd, threadIdx.x);
+    auto fetch = [&](uint32_t t) {
+        const uint64_t at = base + t * tile_bytes;
+        kraw.load(q4_from(p.kc, at, to), kvd);
+        vraw.load(q4_from(p.vc, at, to), kvd);
     };
     if (t0 < t1) fetch(t0);
 
@@ -671,36 +680,33 @@ __global__ __launch_bounds__(64 * Q4_WAVES, NB <= 4 ? 2 : 1) void attn_q4_tile(c
         for (int j = 0; j < NB; j++) q_parts(v[j], k, qh[r][j], ql[r][j]);
     }
 
+    // This wave's share of a tile's operands: K's of slots 16 wave .. + 15, and of V's of slots 32 step ..
+    // + 31 half the columns of every lane.
+    const uint32_t half = wave & 1, step = wave >> 1;
     auto unpack = [&](uint32_t t, int buf) {
-        if (t * Q4_TILE_B + Q4_TILE_B > seen) {  // some row here does not see all of it
-            bool odd = false;
+        uint32_t kw[NB];
+        f16 ks[NB];
+        read_k<NB>(raw[0] + (16 * wave + m16) * R::SLOT, g, kw, ks);
+        VRead<NB, true> v;
+        v.read(raw[1] + 32 * step * R::SLOT, m16, g, half);
+        if (t * Q4_TILE_B + Q4_TILE_B > seen && v.drop_odd()) odd_tile[buf] = t + 1;  // some row does not see all of it
 #pragma unroll
-            for (int si = 0; si < S::N; si++)
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (odd_scale(vs[si][i])) {
-                        vs[si][i] = (f16)0.0f;
-                        odd = true;
-                    }
-            if (odd) odd_tile[buf] = t + 1;
-        }
-#pragma unroll
-        for (int j = 0; j < NB; j++) kf[buf][wave][j][lane] = unpack_k(bits, kw[j], KLoad<NB>::of(ks, j));
+        for (int j = 0; j < NB; j++) kf[buf][wave][j][lane] = unpack_k(bits, kw[j], ks[j]);
 #pragma unroll
         for (int si = 0; si < S::N; si++) {
             if (S::w(si) == 8) {
                 half8 x[4];
-                unpack_v<4>(bits, vw[si], vs[si], x);
+                unpack_v<4>(bits, v.word[si], v.scale[si], x);
 #pragma unroll
                 for (int k = 0; k < 4; k++) vf[buf][step][S::frag(si) + 4 * half + k][lane] = x[k];
             } else if (S::w(si) == 4) {
                 half8 x[2];
-                unpack_v<2>(bits, vw[si], vs[si], x);
+                unpack_v<2>(bits, v.word[si], v.scale[si], x);
 #pragma unroll
                 for (int k = 0; k < 2; k++) vf[buf][step][S::frag(si) + 2 * half + k][lane] = x[k];
             } else {
                 half8 x[2];
-                unpack_v<2>(bits, vw[si], vs[si], x);
+                unpack_v<2>(bits, v.word[si], v.scale[si], x);
                 vf[buf][step][S::frag(si) + half][lane] = half ? x[1] : x[0];
             }
         }
@@ -716,13 +722,25 @@ __global__ __launch_bounds__(64 * Q4_WAVES, NB <= 4 ? 2 : 1) void attn_q4_tile(c
         for (int f = 0; f < NF; f++) o[r][f] = f32x4{0, 0, 0, 0};
     }
     if (threadIdx.x < 2) odd_tile[threadIdx.x] = 0;
+    if (t0 < t1) {
+        kraw.store(raw[0]);
+        vraw.store(raw[1]);
+    }
     __syncthreads();
-    if (t0 < t1) unpack(t0, 0);
+    if (t0 < t1) {
+        if (t0 + 1 < t1) fetch(t0 + 1);
+        unpack(t0, 0);
+    }
     __syncthreads();
     for (uint32_t t = t0; t < t1; t++) {
         const int buf = (t - t0) & 1;
         const uint32_t ts = t * Q4_TILE_B;
-        if (t + 1 < t1) fetch(t + 1);
+        if (t + 1 < t1) {  // the next tile's bytes, unpacked behind this tile's products
+            kraw.store(raw[0]);
+            vraw.store(raw[1]);
+            __syncthreads();
+            if (t + 2 < t1) fetch(t + 2);
+        }
         const bool edge = ts + Q4_TILE_B > seen;
 #pragma unroll
         for (int u = 0; u < 2; u++) {
@@ -786,7 +804,7 @@ __global__ __launch_bounds__(64 * Q4_WAVES, NB <= 4 ? 2 : 1) void attn_q4_tile(c
             for (uint32_t i = 0; i < Q4_TILE_B && ts + i < end; i++)
 #pragma unroll
                 for (int si = 0; si < S::N; si++) {
-                    const bool odd = odd_scale(load_scale(vr, q4_scale_at32(rem + i * kvd + S::col(si) + S::w(si) * 4 * g), 0));
+                    const bool odd = odd_scale(load_scale(vr, q4_scale_at32(rem + i * kvd + S::col(si) + S::w(si) * 4 * g)));
 #pragma unroll
                     for (int r = 0; r < RT; r++)
                         if (odd && see[r].at(ts + i))
