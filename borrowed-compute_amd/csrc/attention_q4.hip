@@ -147,15 +147,17 @@ __device__ __forceinline__ float larger(float a, float b) { return __builtin_amd
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-// Eight dims of a query row from `at`, in the order of a K word's, and the largest magnitude of
-// them and `top`.
-__device__ __forceinline__ float q_dims(const float* at, bool valid, float (&x)[8], float top) {
+// Eight dims of a query row from `at`, in the order of a K word's.
+__device__ __forceinline__ void q_load(const float* at, bool valid, float (&x)[8]) {
     float4 a{}, b{};
     if (valid) {
         a = *(const float4*)at;
         b = *(const float4*)(at + 4);
     }
     x[0] = a.x, x[1] = b.x, x[2] = a.y, x[3] = b.y, x[4] = a.z, x[5] = b.z, x[6] = a.w, x[7] = b.w;
+}
+// The largest magnitude of them and `top`.
+__device__ __forceinline__ float q_top(const float (&x)[8], float top) {
 #pragma unroll
     for (int i = 0; i < 8; i++) top = larger(top, fabsf(x[i]));
     return top;
@@ -416,6 +418,15 @@ __global__ __launch_bounds__(64 * WAVES) void attn_q4_row(const Q4Params p) {
     const uint32_t rem0 = (uint32_t)(e0 & 255), rem = rem0 + kvh * HD;
     const uint64_t base = (e0 >> 8) * Q4_UNIT_BYTES, tile_bytes = (uint64_t)kvd * 18;
     const uint64_t from = base + first * tile_bytes, to = base + q4_bytes(end, rem0, kvd);
+    // q's operands, each wave some of the steps for all; q's rows and the first tile are asked for together.
+    const uint32_t n = PK ? (m16 & 7) : m16, r = (n * (65536 / p.G + 1)) >> 16;  // n / G
+    const bool valid = n < nq;
+    const uint32_t row = it.row0 + (valid ? r : 0), head = kvh * p.G + (valid ? n - r * p.G : 0);
+    const Sees see = sees(p, it, r, valid, end);
+    const size_t qrow = ((size_t)row * p.nh + head) * HD;
+    float x[QJ][8], top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < QJ; i++) q_load(p.q + qrow + 8 * (NB * g + i * WAVES + wave), valid && i * WAVES + wave < NB, x[i]);
     B kraw, vraw;
     kraw.set(rem, kvd, lane);
     vraw.set(rem, kvd, lane);
@@ -424,20 +435,9 @@ __global__ __launch_bounds__(64 * WAVES) void attn_q4_row(const Q4Params p) {
         kraw.load(q4_from(p.kc, at, to), kvd);
         vraw.load(q4_from(p.vc, at, to), kvd);
     };
-    if (wave < tiles) load(wave);  // the first tile is on its way while q is made ready
-
-    // q's operands, each wave some of the steps for all.
-    const uint32_t n = PK ? (m16 & 7) : m16, r = (n * (65536 / p.G + 1)) >> 16;  // n / G
-    const bool valid = n < nq;
-    const uint32_t row = it.row0 + (valid ? r : 0), head = kvh * p.G + (valid ? n - r * p.G : 0);
-    const Sees see = sees(p, it, r, valid, end);
-    const size_t qrow = ((size_t)row * p.nh + head) * HD;
-    float x[QJ][8], top = 0.0f;
+    if (wave < tiles) load(wave);
 #pragma unroll
-    for (int i = 0; i < QJ; i++) {
-        const uint32_t j = i * WAVES + wave;
-        if (j < NB) top = q_dims(p.q + qrow + 8 * (NB * g + j), valid, x[i], top);
-    }
+    for (int i = 0; i < QJ; i++) top = q_top(x[i], top);
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
     if (wave < QW && lane < 16) stop[wave][lane] = top;
@@ -619,22 +619,25 @@ __global__ __launch_bounds__(64 * WAVES) void attn_q4_row(const Q4Params p) {
 
 constexpr int Q4_WAVES = 4;
 
-// More query rows: a tile of 64 slots unpacked once into LDS for the workgroup's four waves of
-// 16 RT query rows each.
+// More query rows: a tile of 64 slots unpacked once into LDS for the workgroup's waves of 16 RT
+// query rows each: four of 32 rows, or eight of 16, of which four take each half of the slots.
 constexpr uint32_t Q4_TILE_B = 64;
 
 template <int NB, int RT>
-__global__ __launch_bounds__(64 * Q4_WAVES, NB <= 4 ? 2 : 1) void attn_q4_tile(const Q4Params p) {
-    constexpr int HD = 32 * NB, NF = 2 * NB;
+__global__ __launch_bounds__(RT == 1 ? 512 : 256, 2) void attn_q4_tile(const Q4Params p) {
+    constexpr int HD = 32 * NB, NF = 2 * NB, KS = RT == 1 ? 2 : 1;
     constexpr uint32_t QT = 64 * RT;
     using S = Seg<NB>;
-    __shared__ half8 kf[2][4][NB][64];
-    __shared__ half8 vf[2][2][NF][64];
+    __shared__ struct {
+        half8 k[2][4][NB][64], v[2][2][NF][64];
+    } fr;
+    static_assert(KS == 1 || sizeof fr >= sizeof(f32x4) * 4 * NF * 64, "the second waves' states");
     using R = Raw<NB, Q4_TILE_B, 64 * Q4_WAVES>;
     __shared__ __attribute__((aligned(16))) uint8_t raw[2][R::BYTES];
     __shared__ uint32_t odd_tile[2];  // 1 + the tile of each buffer that held a scale that is not finite
     const Q4Bits bits;
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) & 3);
+    const uint32_t ks = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);  // KS 2: the second four waves
     const uint32_t m16 = lane & 15, g = lane >> 4;
     const Q4Item& it = p.items[0];
     // The longest lists first.
@@ -644,70 +647,90 @@ __global__ __launch_bounds__(64 * Q4_WAVES, NB <= 4 ? 2 : 1) void attn_q4_tile(c
     const uint32_t seen = p.tree ? it.base : it.base + r0;  // slots every row here sees
     const uint32_t end = p.tree ? tree_end(p, it) : it.base + (q1 - 1) / p.G;
     const uint32_t all = (uint32_t)(((uint64_t)end + Q4_TILE_B - 1) / Q4_TILE_B), t0 = chunk * it.chunk;
-    const uint32_t t1 = t0 < all ? min(t0 + it.chunk, all) : t0;
+    const size_t unit = ((size_t)kvh * p.nqt + qt) * it.nchunk + chunk;
+    if (t0 >= all && it.nchunk > 1) {  // nothing of these rows' lists
+        if (threadIdx.x < QT) *(float2*)(p.part_ml + 2 * (unit * QT + threadIdx.x)) = float2{-INFINITY, 0.0f};
+        return;
+    }
+    const uint32_t t1 = min(t0 + it.chunk, all);
 
     const uint64_t e0 = it.kvoff * kvd;
     const uint32_t rem0 = (uint32_t)(e0 & 255), rem = rem0 + kvh * HD;
     const uint64_t base = (e0 >> 8) * Q4_UNIT_BYTES, tile_bytes = (uint64_t)kvd * 36, to = base + q4_bytes(end, rem0, kvd);
 
-    R kraw, vraw;
-    kraw.set(rem, kvd, threadIdx.x);
-    vraw.set(rem, kvd, threadIdx.x);
-    auto fetch = [&](uint32_t t) {
-        const uint64_t at = base + t * tile_bytes;
-        kraw.load(q4_from(p.kc, at, to), kvd);
-        vraw.load(q4_from(p.vc, at, to), kvd);
-    };
-    if (t0 < t1) fetch(t0);
-
+    // q's rows and the first tile are asked for together.
     Sees see[RT];
     half8 qh[RT][NB], ql[RT][NB];
-    float c[RT];
+    float c[RT], x[RT][NB][8], top[RT];
 #pragma unroll
     for (int r = 0; r < RT; r++) {
-        const uint32_t x = (wave * RT + r) * 16 + m16, y = h0 + x, dr = (y * (65536 / p.G + 1)) >> 16;  // y / G
-        const bool valid = q0 + x < nq;
+        const uint32_t i = (wave * RT + r) * 16 + m16, y = h0 + i, dr = (y * (65536 / p.G + 1)) >> 16;  // y / G
+        const bool valid = q0 + i < nq;
         const uint32_t row = it.row0 + (valid ? r0 + dr : 0), head = kvh * p.G + (valid ? y - dr * p.G : 0);
         see[r] = sees(p, it, r0 + dr, valid, end);
         const float* q = p.q + ((size_t)row * p.nh + head) * HD;
-        float v[NB][8], top = 0.0f, k;
+        top[r] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < NB; j++) top = q_dims(q + 8 * (NB * g + j), valid, v[j], top);
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        q_scale(top, p.sc, k, c[r]);
+        for (int j = 0; j < NB; j++) q_load(q + 8 * (NB * g + j), valid, x[r][j]);
+    }
+    // (KS 2: four waves fetch and unpack K, four V.)
+    R kraw, vraw;
+    const uint32_t thread = threadIdx.x & 255;
+    kraw.set(rem, kvd, thread);
+    if constexpr (KS == 1) vraw.set(rem, kvd, thread);
+    auto fetch = [&](uint32_t t) {
+        const uint64_t at = base + t * tile_bytes;
+        kraw.load(q4_from(KS == 2 && ks ? p.vc : p.kc, at, to), kvd);
+        if constexpr (KS == 1) vraw.load(q4_from(p.vc, at, to), kvd);
+    };
+    auto store = [&]() {
+        kraw.store(raw[KS == 2 ? ks : 0]);
+        if constexpr (KS == 1) vraw.store(raw[1]);
+    };
+    if (t0 < t1) fetch(t0);
 #pragma unroll
-        for (int j = 0; j < NB; j++) q_parts(v[j], k, qh[r][j], ql[r][j]);
+    for (int r = 0; r < RT; r++) {
+        float k;
+#pragma unroll
+        for (int j = 0; j < NB; j++) top[r] = q_top(x[r][j], top[r]);
+        top[r] = fmaxf(top[r], __shfl_xor(top[r], 16));
+        top[r] = fmaxf(top[r], __shfl_xor(top[r], 32));
+        q_scale(top[r], p.sc, k, c[r]);
+#pragma unroll
+        for (int j = 0; j < NB; j++) q_parts(x[r][j], k, qh[r][j], ql[r][j]);
     }
 
     // This wave's share of a tile's operands: K's of slots 16 wave .. + 15, and of V's of slots 32 step ..
     // + 31 half the columns of every lane.
     const uint32_t half = wave & 1, step = wave >> 1;
     auto unpack = [&](uint32_t t, int buf) {
-        uint32_t kw[NB];
-        f16 ks[NB];
-        read_k<NB>(raw[0] + (16 * wave + m16) * R::SLOT, g, kw, ks);
+        if (KS == 1 || ks == 0) {
+            uint32_t kw[NB];
+            f16 kd[NB];
+            read_k<NB>(raw[0] + (16 * wave + m16) * R::SLOT, g, kw, kd);
+#pragma unroll
+            for (int j = 0; j < NB; j++) fr.k[buf][wave][j][lane] = unpack_k(bits, kw[j], kd[j]);
+        }
+        if (KS == 2 && ks == 0) return;
         VRead<NB, true> v;
         v.read(raw[1] + 32 * step * R::SLOT, m16, g, half);
         if (t * Q4_TILE_B + Q4_TILE_B > seen && v.drop_odd()) odd_tile[buf] = t + 1;  // some row does not see all of it
-#pragma unroll
-        for (int j = 0; j < NB; j++) kf[buf][wave][j][lane] = unpack_k(bits, kw[j], ks[j]);
 #pragma unroll
         for (int si = 0; si < S::N; si++) {
             if (S::w(si) == 8) {
                 half8 x[4];
                 unpack_v<4>(bits, v.word[si], v.scale[si], x);
 #pragma unroll
-                for (int k = 0; k < 4; k++) vf[buf][step][S::frag(si) + 4 * half + k][lane] = x[k];
+                for (int k = 0; k < 4; k++) fr.v[buf][step][S::frag(si) + 4 * half + k][lane] = x[k];
             } else if (S::w(si) == 4) {
                 half8 x[2];
                 unpack_v<2>(bits, v.word[si], v.scale[si], x);
 #pragma unroll
-                for (int k = 0; k < 2; k++) vf[buf][step][S::frag(si) + 2 * half + k][lane] = x[k];
+                for (int k = 0; k < 2; k++) fr.v[buf][step][S::frag(si) + 2 * half + k][lane] = x[k];
             } else {
                 half8 x[2];
                 unpack_v<2>(bits, v.word[si], v.scale[si], x);
-                vf[buf][step][S::frag(si) + half][lane] = half ? x[1] : x[0];
+                fr.v[buf][step][S::frag(si) + half][lane] = half ? x[1] : x[0];
             }
         }
     };
@@ -722,10 +745,7 @@ __global__ __launch_bounds__(64 * Q4_WAVES, NB <= 4 ? 2 : 1) void attn_q4_tile(c
         for (int f = 0; f < NF; f++) o[r][f] = f32x4{0, 0, 0, 0};
     }
     if (threadIdx.x < 2) odd_tile[threadIdx.x] = 0;
-    if (t0 < t1) {
-        kraw.store(raw[0]);
-        vraw.store(raw[1]);
-    }
+    if (t0 < t1) store();
     __syncthreads();
     if (t0 < t1) {
         if (t0 + 1 < t1) fetch(t0 + 1);
@@ -736,14 +756,14 @@ __global__ __launch_bounds__(64 * Q4_WAVES, NB <= 4 ? 2 : 1) void attn_q4_tile(c
         const int buf = (t - t0) & 1;
         const uint32_t ts = t * Q4_TILE_B;
         if (t + 1 < t1) {  // the next tile's bytes, unpacked behind this tile's products
-            kraw.store(raw[0]);
-            vraw.store(raw[1]);
+            store();
             __syncthreads();
             if (t + 2 < t1) fetch(t + 2);
         }
         const bool edge = ts + Q4_TILE_B > seen;
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
+        for (int i = 0; i < 2 / KS; i++) {
+            const uint32_t u = KS == 2 ? ks : i;  // 32 of the tile's slots
             // (Four sums in turn, so that no MFMA waits for the one before: one set of rows takes the
             // parts of q apart.)
             constexpr int LO = RT == 1 ? 1 : 0;
@@ -752,7 +772,7 @@ __global__ __launch_bounds__(64 * Q4_WAVES, NB <= 4 ? 2 : 1) void attn_q4_tile(c
             for (int r = 0; r < RT; r++) s[r][0] = s[r][1] = s2[0] = s2[1] = f32x4{0, 0, 0, 0};
 #pragma unroll
             for (int j = 0; j < NB; j++) {
-                const half8 k0 = kf[buf][2 * u][j][lane], k1 = kf[buf][2 * u + 1][j][lane];
+                const half8 k0 = fr.k[buf][2 * u][j][lane], k1 = fr.k[buf][2 * u + 1][j][lane];
 #pragma unroll
                 for (int r = 0; r < RT; r++) {
                     s[r][0] = mfma16(k0, qh[r][j], s[r][0]);
@@ -786,7 +806,7 @@ __global__ __launch_bounds__(64 * Q4_WAVES, NB <= 4 ? 2 : 1) void attn_q4_tile(c
             }
 #pragma unroll
             for (int f = 0; f < NF; f += 2) {
-                const half8 v0 = vf[buf][u][f][lane], v1 = vf[buf][u][f + 1][lane];
+                const half8 v0 = fr.v[buf][u][f][lane], v1 = fr.v[buf][u][f + 1][lane];
 #pragma unroll
                 for (int r = 0; r < RT; r++) {
                     o[r][f] = mfma16(v0, ph[r], o[r][f]);
@@ -816,7 +836,24 @@ __global__ __launch_bounds__(64 * Q4_WAVES, NB <= 4 ? 2 : 1) void attn_q4_tile(c
         __syncthreads();
     }
 
-    const size_t unit = ((size_t)kvh * p.nqt + qt) * it.nchunk + chunk;
+    if constexpr (KS == 2) {  // the two halves of the slots
+        f32x4(*so)[NF][64] = (f32x4(*)[NF][64])&fr;
+        float(*sr)[2][64] = (float(*)[2][64])raw;
+        if (ks) {
+            sr[wave][0][lane] = ref[0];
+            sr[wave][1][lane] = l[0];
+#pragma unroll
+            for (int f = 0; f < NF; f++) so[wave][f][lane] = o[0][f];
+        }
+        __syncthreads();
+        if (ks) return;
+        const float other = sr[wave][0][lane], R2 = fmaxf(ref[0], other), Rs = R2 == -INFINITY ? 0.0f : R2;
+        const float a = exp2_hw(ref[0] - Rs), e = exp2_hw(other - Rs);
+        ref[0] = R2;
+        l[0] = l[0] * a + sr[wave][1][lane] * e;
+#pragma unroll
+        for (int f = 0; f < NF; f++) o[0][f] = o[0][f] * a + so[wave][f][lane] * e;
+    }
 #pragma unroll
     for (int r = 0; r < RT; r++) {
         l[r] += __shfl_xor(l[r], 16);
@@ -843,98 +880,110 @@ __global__ __launch_bounds__(64 * Q4_WAVES, NB <= 4 ? 2 : 1) void attn_q4_tile(c
     }
 }
 
-// The chunks of 16 query rows of a list brought together, two operands' columns a workgroup, its
-// waves a share of the chunks each; states lie as their waves held them.
+// The chunks of 16 query rows of a list brought together, two operands' columns a workgroup, each
+// wave a share of the chunks; states lie as their waves held them. A chunk without a weight left
+// its columns unwritten.
 constexpr uint32_t Q4_MAX_CHUNKS = 256;
-constexpr int Q4_FOLD_WAVES = 8;
 
-template <int NB>
-__global__ __launch_bounds__(64 * Q4_FOLD_WAVES) void attn_q4_fold(const Q4Params p) {
-    constexpr int HD = 32 * NB, NF = 2 * NB;
-    __shared__ float wt[Q4_MAX_CHUNKS][16];
-    __shared__ float red[2][4 * Q4_FOLD_WAVES][16];
-    __shared__ f32x4 sum[Q4_FOLD_WAVES][2][64];
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m16 = lane & 15, g = lane >> 4;
+template <int NB, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void attn_q4_fold(const Q4Params p) {
+    constexpr int HD = 32 * NB, NF = 2 * NB, AHEAD = 4;
+    __shared__ f32x4 sum[WAVES][2][64];
+    __shared__ float sr[WAVES][64], sl[WAVES][64];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m16 = lane & 15, g = lane >> 4;
     const uint32_t f = 2 * blockIdx.x, kvh = blockIdx.y, z = blockIdx.z;
     const Q4Item& it = p.items[p.nitems > 1 ? z : 0];
-    if (it.nchunk == 1) return;  // written by its workgroup
-    const uint32_t n0 = p.nitems > 1 ? 0 : 16 * z, n = n0 + m16, nq = it.rows * p.G;  // this row of the item's
-    const size_t u0 = it.unit0 + ((size_t)kvh * p.nqt + n0 / p.qt) * it.nchunk;
-    const uint32_t sl = n0 % p.qt;
-    const bool valid = n < nq;
-    // Weights of the chunks: thread (part, row) takes every 32nd.
-    constexpr uint32_t PARTS = 4 * Q4_FOLD_WAVES;
-    const uint32_t part = tid >> 4;
-    float2 ml[Q4_MAX_CHUNKS / PARTS];
-    float R = -INFINITY, L = 0.0f;
-#pragma unroll
-    for (uint32_t i = 0; i < Q4_MAX_CHUNKS / PARTS; i++) {
-        const uint32_t c = part + PARTS * i;
-        ml[i] = c < it.nchunk && valid ? *(const float2*)(p.part_ml + 2 * ((u0 + c) * p.qt + sl + m16)) : float2{-INFINITY, 0.0f};
-        R = fmaxf(R, ml[i].x);
-    }
-    red[0][part][m16] = R;
-    __syncthreads();
-#pragma unroll
-    for (uint32_t i = 0; i < PARTS; i++) R = fmaxf(R, red[0][i][m16]);
-    const float Rs = R == -INFINITY ? 0.0f : R;
-#pragma unroll
-    for (uint32_t i = 0; i < Q4_MAX_CHUNKS / PARTS; i++) {
-        const float w = exp2_hw(ml[i].x - Rs);
-        wt[part + PARTS * i][m16] = w;
-        L += w * ml[i].y;
-    }
-    red[1][part][m16] = L;
-    __syncthreads();
+    const uint32_t chunks = it.nchunk;
+    if (chunks == 1) return;  // written by its workgroup
+    const uint32_t n0 = p.nitems > 1 ? 0 : 16 * z, n = n0 + m16, sl0 = n0 & (p.qt - 1);  // this row of the item's
+    const bool valid = n < it.rows * p.G;
+    const size_t u0 = it.unit0 + ((size_t)kvh * p.nqt + n0 / p.qt) * chunks;
+    const float2* ml = (const float2*)p.part_ml + u0 * p.qt + sl0 + m16;
+    const f32x4* at = (const f32x4*)p.part_o + ((u0 * (p.qt / 16) + sl0 / 16) * NF + f) * 64 + lane;
+    const size_t next = (size_t)(p.qt / 16) * NF * 64;
     f32x4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
-    if (valid) {
-        const f32x4* at = (const f32x4*)p.part_o + ((u0 * (p.qt / 16) + sl / 16) * NF + f) * 64 + lane;
-        const size_t next = (size_t)(p.qt / 16) * NF * 64;
-#pragma unroll 4
-        for (uint32_t c = wave; c < it.nchunk; c += Q4_FOLD_WAVES) {
-            const float w = wt[c][m16];
-            a += w * at[c * next];
-            b += w * at[c * next + 64];
+    float R = -INFINITY, L = 0.0f;
+    for (uint32_t c0 = wave; c0 < chunks; c0 += AHEAD * WAVES) {
+        float2 s[AHEAD];
+        f32x4 x[AHEAD], y[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            const uint32_t c = c0 + i * WAVES;
+            const bool there = valid && c < chunks;
+            s[i] = there ? ml[(size_t)c * p.qt] : float2{-INFINITY, 0.0f};
+            x[i] = there ? at[c * next] : f32x4{0, 0, 0, 0};
+            y[i] = there ? at[c * next + 64] : f32x4{0, 0, 0, 0};
+        }
+        float to = R;
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) to = fmaxf(to, s[i].x);
+        const float ts = to == -INFINITY ? 0.0f : to, w = exp2_hw(R - ts);
+        a *= w;
+        b *= w;
+        L *= w;
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            const float e = exp2_hw(s[i].x - ts);
+            L += e * s[i].y;
+            a += s[i].y == 0.0f ? f32x4{0, 0, 0, 0} : e * x[i];
+            b += s[i].y == 0.0f ? f32x4{0, 0, 0, 0} : e * y[i];
+        }
+        R = to;
+    }
+    if constexpr (WAVES > 1) {
+        sr[wave][lane] = R;
+        sl[wave][lane] = L;
+        sum[wave][0][lane] = a;
+        sum[wave][1][lane] = b;
+        __syncthreads();
+        if (wave > 0) return;
+        for (int w = 1; w < WAVES; w++) R = fmaxf(R, sr[w][lane]);
+        const float Rs = R == -INFINITY ? 0.0f : R;
+        a = b = f32x4{0, 0, 0, 0};
+        L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            const float e = exp2_hw(sr[w][lane] - Rs);
+            L += e * sl[w][lane];
+            a += e * sum[w][0][lane];
+            b += e * sum[w][1][lane];
         }
     }
-    sum[wave][0][lane] = a;
-    sum[wave][1][lane] = b;
-    __syncthreads();
-    if (wave >= 2 || !valid) return;
-    L = 0.0f;
+    if (!valid) return;
+    const float k = L == 0.0f ? 0.0f : 1.0f / L;
+    const uint32_t r = n / p.G, step = stride<NB>(f);
+    float* dst = p.out + ((size_t)(it.row0 + r) * p.nh + kvh * p.G + n - r * p.G) * HD + column<NB>(f, g);
 #pragma unroll
-    for (uint32_t i = 0; i < PARTS; i++) L += red[1][i][m16];
-    a = sum[0][wave][lane];
-#pragma unroll
-    for (int w = 1; w < Q4_FOLD_WAVES; w++) a += sum[w][wave][lane];
-    a *= L == 0.0f ? 0.0f : 1.0f / L;
-    const uint32_t r = n / p.G, col = column<NB>(f + wave, g), step = stride<NB>(f);
-    float* dst = p.out + ((size_t)(it.row0 + r) * p.nh + kvh * p.G + n - r * p.G) * HD + col;
-#pragma unroll
-    for (int i = 0; i < 4; i++) dst[i * step] = a[i];
+    for (int i = 0; i < 4; i++) *(float2*)(dst + i * step) = float2{a[i] * k, b[i] * k};  // (neighbours: f is even)
 }
 
 template <int NB, int WAVES>
 void launch_row(const Q4Params& p, uint32_t octs, bool pk, const AttnCall& a, hipStream_t s) {
     const dim3 grid(8, p.nkv, octs), wg(64 * WAVES);
+    // (Eight waves have 256 registers a lane; more than eight query rows of heads past 192 want more.)
+    constexpr int W = NB > 6 ? Q4_WAVES : WAVES;
     if (pk) hipExtLaunchKernelGGL((attn_q4_row<NB, true, WAVES>), grid, wg, 0, s, a.ev_before, a.ev_after, 0, p);
-    else hipExtLaunchKernelGGL((attn_q4_row<NB, false, WAVES>), grid, wg, 0, s, a.ev_before, a.ev_after, 0, p);
+    else hipExtLaunchKernelGGL((attn_q4_row<NB, false, W>), grid, dim3(64 * W), 0, s, a.ev_before, a.ev_after, 0, p);
 }
 template <int NB>
 void launch_tile(const Q4Params& p, uint32_t rt, const AttnCall& a, hipStream_t s) {
-    const dim3 grid(p.nkv, p.items[0].nchunk, p.nqt), wg(64 * Q4_WAVES);
+    const dim3 grid(p.nkv, p.items[0].nchunk, p.nqt);
     if constexpr (NB <= 4) {
         if (rt == 2) {
-            hipExtLaunchKernelGGL((attn_q4_tile<NB, 2>), grid, wg, 0, s, a.ev_before, a.ev_after, 0, p);
+            hipExtLaunchKernelGGL((attn_q4_tile<NB, 2>), grid, dim3(256), 0, s, a.ev_before, a.ev_after, 0, p);
             return;
         }
     }
-    hipExtLaunchKernelGGL((attn_q4_tile<NB, 1>), grid, wg, 0, s, a.ev_before, a.ev_after, 0, p);
+    hipExtLaunchKernelGGL((attn_q4_tile<NB, 1>), grid, dim3(512), 0, s, a.ev_before, a.ev_after, 0, p);
 }
-
 template <int NB>
 void launch_fold(const Q4Params& p, uint32_t groups, hipStream_t s) {
-    hipLaunchKernelGGL(attn_q4_fold<NB>, dim3(NB, p.nkv, groups), dim3(64 * Q4_FOLD_WAVES), 0, s, p);
+    // A wave alone holds a few chunks' states at once; more chunks are shared out.
+    uint32_t most = 0;
+    for (uint32_t i = 0; i < p.nitems; i++) most = std::max(most, p.items[i].nchunk);
+    const dim3 grid(NB, p.nkv, groups);
+    if (most <= 8) hipLaunchKernelGGL((attn_q4_fold<NB, 1>), grid, dim3(64), 0, s, p);
+    else hipLaunchKernelGGL((attn_q4_fold<NB, 8>), grid, dim3(512), 0, s, p);
 }
 
 Q4Params params(const AttnCall& a) {
@@ -955,9 +1004,18 @@ Q4Params params(const AttnCall& a) {
     return p;
 }
 
-// Workgroups of attn_q4_row that keep the GPU busy: chunks of a list are made to come near it.
-constexpr uint32_t Q4_ROW_GROUPS = 1024;
-constexpr uint32_t Q4_TILE_GROUPS = 512;
+// Workgroups that keep the GPU busy without more states than they are worth: of attn_q4_row two a CU
+// (a step of 32 x 8 heads of 128 at 32768 slots: 18.0 us at 512, 20.7 at 256, 21.4 at 1024), of
+// attn_q4_tile, eight waves each, one (8 rows of 64 x 8 heads at 20000: 27 us at 256, 31 at 192, 33
+// at 512).
+constexpr uint32_t Q4_ROW_GROUPS = 512;
+constexpr uint32_t Q4_TILE_GROUPS = 256;
+// Lists in two chunks cost more in states and a second launch than they save (200 rows of 32 x 8
+// heads at 300: 22 us in two, 18.5 in one).
+constexpr uint32_t Q4_LEAST_CHUNKS = 3;
+// Tiles of a list up to which one workgroup of eight waves takes it whole, without a second launch
+// (32 x 8 heads of 128: 8.0 us at 16 tiles against 9.4, 11.3 at 32 against 10).
+constexpr uint32_t Q4_BRIEF = 20;
 
 // Chunks for a list of `tiles` tiles, `least` at least a chunk, for `want` of them.
 void cut(Q4Item& it, uint64_t tiles, uint32_t want, uint32_t least) {
@@ -1008,12 +1066,20 @@ hipError_t launch_items(Q4Params& p, const AttnCall& a, const uint64_t* lens, Wo
             split |= it.nchunk > 1;
         }
     };
-    plan(want);
+    // Lists that eight waves take in a few tiles each are not cut: no second launch.
+    const bool brief = total <= (uint64_t)p.nitems * Q4_BRIEF;
+    plan(brief ? 0 : want);
     if (split && !reserve(p, (uint64_t)units * 16, a.hd, ws, s)) plan(0);
     const bool pk = p.items[0].rows * p.G <= 8;
+#define Q4_BRIEF_ROW(NB) launch_row<NB, 2 * Q4_WAVES>(p, octs, pk, a, s)
 #define Q4_ROW(NB) launch_row<NB, Q4_WAVES>(p, octs, pk, a, s)
-    Q4_BY_DIM(a.hd / 32, Q4_ROW)
+    if (brief) {
+        Q4_BY_DIM(a.hd / 32, Q4_BRIEF_ROW)
+    } else {
+        Q4_BY_DIM(a.hd / 32, Q4_ROW)
+    }
 #undef Q4_ROW
+#undef Q4_BRIEF_ROW
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !split) return e;
 #define Q4_FOLD(NB) launch_fold<NB>(p, p.nitems, s)
@@ -1052,7 +1118,8 @@ hipError_t q4_attention(const AttnCall& a, Workspace& ws, hipStream_t s) {
     p.qt = 64 * rt;
     p.nqt = (uint32_t)((nq + p.qt - 1) / p.qt);
     const uint64_t groups = (uint64_t)p.nqt * a.nkv, tiles = (far + Q4_TILE_B - 1) / Q4_TILE_B;
-    cut(it, tiles, (uint32_t)std::max<uint64_t>(1, Q4_TILE_GROUPS / groups), 2);
+    const uint64_t want = Q4_TILE_GROUPS / groups;
+    cut(it, tiles, want < Q4_LEAST_CHUNKS ? 1 : (uint32_t)want, 2);
     if (it.nchunk > 1 && !reserve(p, groups * it.nchunk * p.qt, a.hd, ws, s)) cut(it, tiles, 1, 2);
 #define Q4_TILES(NB) launch_tile<NB>(p, rt, a, s)
     Q4_BY_DIM(a.hd / 32, Q4_TILES)

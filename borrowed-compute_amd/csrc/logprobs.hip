@@ -9,12 +9,13 @@
 // L -> e^d L, A -> e^d (A + d L) with d = (m' - m) / T.
 //
 // One pass over the scores. A workgroup holds 8192 of them in registers (32 a thread) and takes
-// from them their maximum, the sums and the block's best tokens: with the threads in at least
-// `top` groups, the smallest of the groups' maxima has `top` scores at or above it, so only
-// those (a few times `top`) go into LDS, where each one's rank is the number of better ones. Rows whose candidates
-// are too many (most scores equal, as under a mask) pick the block's best one at a time. Keys of
-// score over inverted index make every order total: ties go to the lowest index, a NaN is
-// behind every number. Rows are cut over workgroups; k_logprobs_join brings a row's parts together.
+// from them their maximum, the sums and the block's best tokens: of the maxima of 64 groups of
+// threads, or of all 256 threads, the top'th largest has `top` scores at or above it, so only
+// those, little more than `top`, go into LDS, where each one's rank is the number of better ones.
+// Rows whose candidates are too many (most scores equal, as under a mask) pick the block's best one
+// at a time. Keys of score over inverted index make every order total: ties go to the lowest
+// index, a NaN is behind every number. Rows are cut over workgroups; k_logprobs_join brings a
+// row's parts together.
 #include "common.hpp"
 #include "internal.hpp"
 
@@ -95,8 +96,11 @@ __device__ __forceinline__ void lp_finish(const LpParams& p, uint32_t row, const
 __device__ __forceinline__ void lp_rank(const uint64_t* pool, uint32_t n, uint64_t* out, uint32_t top) {
     for (uint32_t i = threadIdx.x; i < n; i += LP_THREADS) {
         const uint64_t k = pool[i];
-        uint32_t rank = 0;
-        for (uint32_t j = 0; j < n; j++) rank += pool[j] > k;
+        uint32_t rank = 0, j = 0;
+        for (; j + 8 <= n; j += 8)  // (the reads of eight do not wait for each other)
+#pragma unroll
+            for (int e = 0; e < 8; e++) rank += pool[j + e] > k;
+        for (; j < n; j++) rank += pool[j] > k;
         if (k != 0 && rank < top) out[rank] = k;
     }
 }
@@ -119,6 +123,7 @@ struct __attribute__((packed, aligned(4))) Float4Any {  // rows of an odd vocabu
 __global__ __launch_bounds__(LP_THREADS) void k_logprobs(const LpParams p) {
     __shared__ uint64_t pool[LP_TOP + LP_POOL], best[LP_TOP], pick[4];
     __shared__ float red[4][4];
+    __shared__ __attribute__((aligned(16))) float gmax[LP_THREADS];
     __shared__ uint32_t count;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.y, part = blockIdx.x;
     const float* s = p.scores + (size_t)row * p.vocab;
@@ -154,29 +159,48 @@ __global__ __launch_bounds__(LP_THREADS) void k_logprobs(const LpParams p) {
             st.a += w * fmaxf(x, -1e4f);  // (0 for a score of -inf; a NaN stays one)
         }
         if (p.top == 0) continue;
-        // At least `top` of the block's scores reach the smallest of its groups' maxima.
-        const uint32_t width = p.top <= 8 ? 32 : p.top <= 32 ? 8 : 4;  // lanes a group: 8, 32 or 64 groups
+        // At least `top` of the block's scores reach the top'th largest of its groups' maxima.
+        const uint32_t groups = p.top <= 32 ? 64 : LP_THREADS;
         float gm = top;
-        for (uint32_t d = 1; d < width; d *= 2) gm = fmaxf(gm, __shfl_xor(gm, (int)d));
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) gm = fminf(gm, __shfl_xor(gm, d));
-        __syncthreads();  // (the block before has done with red, pool and count)
-        if (lane == 0) red[0][wave] = gm;
+        if (groups == 64) {  // four threads a group
+            gm = fmaxf(gm, __shfl_xor(gm, 1));
+            gm = fmaxf(gm, __shfl_xor(gm, 2));
+        }
+        __syncthreads();  // (the block before has done with gmax, pool and count)
+        if (groups == LP_THREADS) gmax[tid] = gm;
+        else if ((tid & 3) == 0) gmax[tid >> 2] = gm;
         if (tid == 0) count = kept;
         if (tid < kept) pool[tid] = best[tid];
         __syncthreads();
-        const float least = fminf(fminf(red[0][0], red[0][1]), fminf(red[0][2], red[0][3]));
-        const uint64_t last = kept == p.top ? best[p.top - 1] : 0;  // (later tokens of its score lose to it)
+        // The smallest of those that fewer than `top` are larger than; a wave looks at 64 of them.
+        const float mine = gmax[(groups == 64 ? 0 : 64 * wave) + lane];
+        uint32_t above = 0;
+        for (uint32_t j = 0; j < groups; j += 16)
 #pragma unroll
-        for (int e = 0; e < LP_EACH; e++) {
-            // Under a mask of -inf the numbers alone, if they are enough, else the picks below.
-            if (v[e] >= least && v[e] > -INFINITY) {
-                const uint64_t k = lp_key(v[e], index(e));
-                if (k > last) {
-                    const uint32_t at = atomicAdd(&count, 1u);
-                    if (at < LP_TOP + LP_POOL) pool[at] = k;
-                }
+            for (int e = 0; e < 16; e += 4) {
+                const float4 x = *(const float4*)&gmax[j + e];
+                above += (uint32_t)(x.x > mine) + (uint32_t)(x.y > mine) + (uint32_t)(x.z > mine) + (uint32_t)(x.w > mine);
             }
+        float least = -wave_max(above < p.top ? -mine : -INFINITY);
+        if (groups != 64) {
+            if (lane == 0) red[0][wave] = least;
+            __syncthreads();
+            least = fminf(fminf(red[0][0], red[0][1]), fminf(red[0][2], red[0][3]));
+        }
+        // Numbers above -inf (under a mask those alone, if they are enough), and above the worst key
+        // kept, whose score beats its equals of later blocks.
+        const float worst = kept == p.top ? lp_score(best[p.top - 1]) : -INFINITY, floor = worst != worst ? -INFINITY : worst;
+        uint32_t pass = 0;
+#pragma unroll
+        for (int e = 0; e < LP_EACH; e++) pass |= (uint32_t)(v[e] >= least && v[e] > floor) << e;
+        if (__any(pass)) {
+            uint32_t at = pass ? atomicAdd(&count, (uint32_t)__popc(pass)) : 0;
+#pragma unroll
+            for (int e = 0; e < LP_EACH; e++)
+                if (pass >> e & 1u) {
+                    if (at < LP_TOP + LP_POOL) pool[at] = lp_key(v[e], index(e));
+                    at++;
+                }
         }
         __syncthreads();
         uint32_t n = count;
