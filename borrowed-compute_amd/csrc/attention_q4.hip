@@ -38,9 +38,10 @@ namespace bchip {
 
 // A sequence's rows over its cache: row r of the item (q and out row row0 + r) sees the slots
 // below base + r (a line), or those below base and the named ones (a tree). Each of its lists is
-// cut into nchunk chunks of `chunk` tiles; block0 is the first of its rows of eight blocks.
+// cut into nchunk chunks of `chunk` tiles; block0 is the first of its rows of eight blocks,
+// turned by `turn` so that an item's first chunk lies behind the last of the item before.
 struct Q4Item {
-    uint32_t row0, rows, base, unit0, block0, nchunk, chunk, pad;
+    uint32_t row0, rows, base, unit0, block0, nchunk, chunk, turn;
     uint64_t kvoff;
 };
 
@@ -407,7 +408,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_q4_row(const Q4Params p) {
     }
     const Q4Item& it = p.items[ii];
     // Blocks 8 apart (one XCD) take the KV heads of one chunk: their bytes share cache lines.
-    const uint32_t kvh = blockIdx.y, chunk = (blockIdx.z - it.block0) * 8 + blockIdx.x;
+    const uint32_t kvh = blockIdx.y, chunk = (blockIdx.z - it.block0) * 8 + ((blockIdx.x - it.turn) & 7);
     if (chunk >= it.nchunk) return;
     const uint32_t kvd = p.nkv * HD, nq = it.rows * p.G, end = p.tree ? tree_end(p, it) : it.base + it.rows - 1;
     const uint32_t all = (uint32_t)(((uint64_t)end + Q4_TILE - 1) / Q4_TILE), first = chunk * it.chunk;
@@ -880,18 +881,19 @@ __global__ __launch_bounds__(RT == 1 ? 512 : 256, 2) void attn_q4_tile(const Q4P
     }
 }
 
-// The chunks of 16 query rows of a list brought together, two operands' columns a workgroup, each
-// wave a share of the chunks; states lie as their waves held them. A chunk without a weight left
+// The chunks of 16 query rows of a list brought together, one operand's columns a workgroup (two took
+// 0.4 to 1.9 us more, few workgroups reading much each), each wave a share of the chunks; states lie as
+// their waves held them. A chunk without a weight left
 // its columns unwritten.
 constexpr uint32_t Q4_MAX_CHUNKS = 256;
 
 template <int NB, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void attn_q4_fold(const Q4Params p) {
-    constexpr int HD = 32 * NB, NF = 2 * NB, AHEAD = 4;
-    __shared__ f32x4 sum[WAVES][2][64];
+    constexpr int HD = 32 * NB, NF = 2 * NB, AHEAD = 8;
+    __shared__ f32x4 sum[WAVES][64];
     __shared__ float sr[WAVES][64], sl[WAVES][64];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m16 = lane & 15, g = lane >> 4;
-    const uint32_t f = 2 * blockIdx.x, kvh = blockIdx.y, z = blockIdx.z;
+    const uint32_t f = blockIdx.x, kvh = blockIdx.y, z = blockIdx.z;
     const Q4Item& it = p.items[p.nitems > 1 ? z : 0];
     const uint32_t chunks = it.nchunk;
     if (chunks == 1) return;  // written by its workgroup
@@ -901,52 +903,47 @@ __global__ __launch_bounds__(64 * WAVES) void attn_q4_fold(const Q4Params p) {
     const float2* ml = (const float2*)p.part_ml + u0 * p.qt + sl0 + m16;
     const f32x4* at = (const f32x4*)p.part_o + ((u0 * (p.qt / 16) + sl0 / 16) * NF + f) * 64 + lane;
     const size_t next = (size_t)(p.qt / 16) * NF * 64;
-    f32x4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+    f32x4 a = {0, 0, 0, 0};
     float R = -INFINITY, L = 0.0f;
     for (uint32_t c0 = wave; c0 < chunks; c0 += AHEAD * WAVES) {
         float2 s[AHEAD];
-        f32x4 x[AHEAD], y[AHEAD];
+        f32x4 x[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
             const uint32_t c = c0 + i * WAVES;
             const bool there = valid && c < chunks;
             s[i] = there ? ml[(size_t)c * p.qt] : float2{-INFINITY, 0.0f};
             x[i] = there ? at[c * next] : f32x4{0, 0, 0, 0};
-            y[i] = there ? at[c * next + 64] : f32x4{0, 0, 0, 0};
         }
         float to = R;
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) to = fmaxf(to, s[i].x);
         const float ts = to == -INFINITY ? 0.0f : to, w = exp2_hw(R - ts);
         a *= w;
-        b *= w;
         L *= w;
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
             const float e = exp2_hw(s[i].x - ts);
             L += e * s[i].y;
             a += s[i].y == 0.0f ? f32x4{0, 0, 0, 0} : e * x[i];
-            b += s[i].y == 0.0f ? f32x4{0, 0, 0, 0} : e * y[i];
         }
         R = to;
     }
     if constexpr (WAVES > 1) {
         sr[wave][lane] = R;
         sl[wave][lane] = L;
-        sum[wave][0][lane] = a;
-        sum[wave][1][lane] = b;
+        sum[wave][lane] = a;
         __syncthreads();
         if (wave > 0) return;
         for (int w = 1; w < WAVES; w++) R = fmaxf(R, sr[w][lane]);
         const float Rs = R == -INFINITY ? 0.0f : R;
-        a = b = f32x4{0, 0, 0, 0};
+        a = f32x4{0, 0, 0, 0};
         L = 0.0f;
 #pragma unroll
         for (int w = 0; w < WAVES; w++) {
             const float e = exp2_hw(sr[w][lane] - Rs);
             L += e * sl[w][lane];
-            a += e * sum[w][0][lane];
-            b += e * sum[w][1][lane];
+            a += e * sum[w][lane];
         }
     }
     if (!valid) return;
@@ -954,7 +951,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_q4_fold(const Q4Params p) {
     const uint32_t r = n / p.G, step = stride<NB>(f);
     float* dst = p.out + ((size_t)(it.row0 + r) * p.nh + kvh * p.G + n - r * p.G) * HD + column<NB>(f, g);
 #pragma unroll
-    for (int i = 0; i < 4; i++) *(float2*)(dst + i * step) = float2{a[i] * k, b[i] * k};  // (neighbours: f is even)
+    for (int i = 0; i < 4; i++) dst[i * step] = a[i] * k;
 }
 
 template <int NB, int WAVES>
@@ -981,7 +978,7 @@ void launch_fold(const Q4Params& p, uint32_t groups, hipStream_t s) {
     // A wave alone holds a few chunks' states at once; more chunks are shared out.
     uint32_t most = 0;
     for (uint32_t i = 0; i < p.nitems; i++) most = std::max(most, p.items[i].nchunk);
-    const dim3 grid(NB, p.nkv, groups);
+    const dim3 grid(2 * NB, p.nkv, groups);
     if (most <= 8) hipLaunchKernelGGL((attn_q4_fold<NB, 1>), grid, dim3(64), 0, s, p);
     else hipLaunchKernelGGL((attn_q4_fold<NB, 8>), grid, dim3(512), 0, s, p);
 }
@@ -1009,6 +1006,9 @@ Q4Params params(const AttnCall& a) {
 // attn_q4_tile, eight waves each, one (8 rows of 64 x 8 heads at 20000: 27 us at 256, 31 at 192, 33
 // at 512).
 constexpr uint32_t Q4_ROW_GROUPS = 512;
+// Lists of several lengths end at different times: more workgroups (16 of 28 x 4 heads of 128 at 1 to 16384
+// slots: 38 us at 768, 46 at 512, 40 at 1024).
+constexpr uint32_t Q4_RAGGED_GROUPS = 768;
 constexpr uint32_t Q4_TILE_GROUPS = 256;
 // Lists in two chunks cost more in states and a second launch than they save (200 rows of 32 x 8
 // heads at 300: 22 us in two, 18.5 in one).
@@ -1017,10 +1017,16 @@ constexpr uint32_t Q4_LEAST_CHUNKS = 3;
 // (32 x 8 heads of 128: 8.0 us at 16 tiles against 9.4, 11.3 at 32 against 10).
 constexpr uint32_t Q4_BRIEF = 20;
 
-// Chunks for a list of `tiles` tiles, `least` at least a chunk, for `want` of them.
-void cut(Q4Item& it, uint64_t tiles, uint32_t want, uint32_t least) {
-    const uint64_t n = std::max<uint64_t>(1, std::min<uint64_t>({(uint64_t)want, tiles / least, Q4_MAX_CHUNKS}));
-    it.chunk = (uint32_t)std::max<uint64_t>(1, (tiles + n - 1) / n);
+// Chunks that attn_q4_fold reads at once, and the tiles a chunk past them is worth (28 x 4 heads of 128 at
+// 24000 slots: 13.4 us in 62 chunks, 15.2 in 125).
+constexpr uint32_t Q4_FOLD_CHUNKS = 64, Q4_FOLD_TILES = 16;
+
+// Chunks for a list of `tiles` tiles, `least` at least a chunk, for `want` of them; of multiples of `of` (a
+// chunk of attn_q4_row takes as long as its first wave, so fewer chunks of whole rounds: 9.6 us for 10.2 at
+// 1300 slots of 32 x 8 heads).
+void cut(Q4Item& it, uint64_t tiles, uint32_t want, uint32_t least, uint32_t of) {
+    const uint64_t n = std::max<uint64_t>(1, std::min<uint64_t>({(uint64_t)want, tiles / least, std::max<uint64_t>(Q4_FOLD_CHUNKS, tiles / Q4_FOLD_TILES), Q4_MAX_CHUNKS}));
+    it.chunk = (uint32_t)std::max<uint64_t>(1, ((tiles + n - 1) / n + of - 1) / of * of);
     it.nchunk = (uint32_t)std::max<uint64_t>(1, (tiles + it.chunk - 1) / it.chunk);
 }
 
@@ -1048,7 +1054,7 @@ bool reserve(Q4Params& p, uint64_t states, uint32_t hd, Workspace& ws, hipStream
 hipError_t launch_items(Q4Params& p, const AttnCall& a, const uint64_t* lens, Workspace& ws, hipStream_t s) {
     uint64_t total = 0;
     for (uint32_t i = 0; i < p.nitems; i++) total += (lens[i] + Q4_TILE - 1) / Q4_TILE;
-    const uint32_t want = std::max(1u, Q4_ROW_GROUPS / a.nkv);
+    const uint32_t want = std::max(1u, (p.nitems > 1 ? Q4_RAGGED_GROUPS : Q4_ROW_GROUPS) / a.nkv);
     uint32_t units, octs;
     bool split;
     auto plan = [&](uint64_t all) {
@@ -1059,8 +1065,9 @@ hipError_t launch_items(Q4Params& p, const AttnCall& a, const uint64_t* lens, Wo
             const uint64_t tiles = (lens[i] + Q4_TILE - 1) / Q4_TILE;
             it.unit0 = units;
             it.block0 = octs;
+            it.turn = units / a.nkv % 8;
             // A list's share of the workgroups is its share of the tiles.
-            cut(it, tiles, (uint32_t)std::max<uint64_t>(1, all * tiles / std::max<uint64_t>(1, total)), Q4_WAVES);
+            cut(it, tiles, (uint32_t)std::max<uint64_t>(1, all * tiles / std::max<uint64_t>(1, total)), Q4_WAVES, Q4_WAVES);
             units += it.nchunk * a.nkv;
             octs += (it.nchunk + 7) / 8;
             split |= it.nchunk > 1;
@@ -1119,8 +1126,8 @@ hipError_t q4_attention(const AttnCall& a, Workspace& ws, hipStream_t s) {
     p.nqt = (uint32_t)((nq + p.qt - 1) / p.qt);
     const uint64_t groups = (uint64_t)p.nqt * a.nkv, tiles = (far + Q4_TILE_B - 1) / Q4_TILE_B;
     const uint64_t want = Q4_TILE_GROUPS / groups;
-    cut(it, tiles, want < Q4_LEAST_CHUNKS ? 1 : (uint32_t)want, 2);
-    if (it.nchunk > 1 && !reserve(p, groups * it.nchunk * p.qt, a.hd, ws, s)) cut(it, tiles, 1, 2);
+    cut(it, tiles, want < Q4_LEAST_CHUNKS ? 1 : (uint32_t)want, 2, 1);
+    if (it.nchunk > 1 && !reserve(p, groups * it.nchunk * p.qt, a.hd, ws, s)) cut(it, tiles, 1, 2, 1);
 #define Q4_TILES(NB) launch_tile<NB>(p, rt, a, s)
     Q4_BY_DIM(a.hd / 32, Q4_TILES)
 #undef Q4_TILES
