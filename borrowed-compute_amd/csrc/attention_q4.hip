@@ -1014,7 +1014,9 @@ constexpr uint32_t Q4_TILE_GROUPS = 256;
 // heads at 300: 22 us in two, 18.5 in one).
 constexpr uint32_t Q4_LEAST_CHUNKS = 3;
 // Tiles of a list up to which one workgroup of eight waves takes it whole, without a second launch
-// (32 x 8 heads of 128: 8.0 us at 16 tiles against 9.4, 11.3 at 32 against 10).
+// (32 x 8 heads of 128: 8.0 us at 16 tiles against 9.4, 11.3 at 32 against 10). Of several lists their
+// average, if the longest has at most twice that (8 lists of 28 x 4 heads, one of 1500 slots and the
+// rest of 200: 9.8 us cut, 13.4 whole).
 constexpr uint32_t Q4_BRIEF = 20;
 
 // Chunks that attn_q4_fold reads at once, and the tiles a chunk past them is worth (28 x 4 heads of 128 at
@@ -1052,8 +1054,12 @@ bool reserve(Q4Params& p, uint64_t states, uint32_t hd, Workspace& ws, hipStream
 // One launch of attn_q4_row over p's items of `lens` entries, and the fold of its chunks. A
 // call whose scratch cannot be had takes each list in one chunk.
 hipError_t launch_items(Q4Params& p, const AttnCall& a, const uint64_t* lens, Workspace& ws, hipStream_t s) {
-    uint64_t total = 0;
-    for (uint32_t i = 0; i < p.nitems; i++) total += (lens[i] + Q4_TILE - 1) / Q4_TILE;
+    uint64_t total = 0, most = 0;
+    for (uint32_t i = 0; i < p.nitems; i++) {
+        const uint64_t tiles = (lens[i] + Q4_TILE - 1) / Q4_TILE;
+        total += tiles;
+        most = std::max(most, tiles);
+    }
     const uint32_t want = std::max(1u, (p.nitems > 1 ? Q4_RAGGED_GROUPS : Q4_ROW_GROUPS) / a.nkv);
     uint32_t units, octs;
     bool split;
@@ -1074,7 +1080,7 @@ hipError_t launch_items(Q4Params& p, const AttnCall& a, const uint64_t* lens, Wo
         }
     };
     // Lists that eight waves take in a few tiles each are not cut: no second launch.
-    const bool brief = total <= (uint64_t)p.nitems * Q4_BRIEF;
+    const bool brief = total <= (uint64_t)p.nitems * Q4_BRIEF && most <= 2 * Q4_BRIEF;
     plan(brief ? 0 : want);
     if (split && !reserve(p, (uint64_t)units * 16, a.hd, ws, s)) plan(0);
     const bool pk = p.items[0].rows * p.G <= 8;

@@ -152,6 +152,7 @@ uint64_t bytes_of(uint32_t type, uint64_t n) {
     return sat_mul(n, type == BCHIP_F16 ? 2u : 4u);
 }
 constexpr uint32_t LAST_TYPE = BCHIP_Q4;
+constexpr uint64_t Q4_SLOTS = 0xffffff00u;  // slots that a list in 4 bits may reach
 
 // Bytes from p to the end of the bchip_alloc allocation holding it, or UINT64_MAX for
 // memory this library did not allocate.
@@ -167,7 +168,7 @@ uint64_t bytes_left(const bchip_ctx* c, const void* p) {
 // Slots of kvd elements that both caches hold, as far as is known.
 uint64_t slots_held(const bchip_ctx* c, const void* kc, const void* vc, uint32_t type, uint64_t kvd) {
     const uint64_t bytes = std::min(bytes_left(c, kc), bytes_left(c, vc));
-    if (type == BCHIP_Q4) return sat_mul(bytes / Q4_UNIT_BYTES, Q4_UNIT) / kvd;
+    if (type == BCHIP_Q4) return std::min(sat_mul(bytes / Q4_UNIT_BYTES, Q4_UNIT) / kvd, Q4_SLOTS);
     return bytes / bytes_of(type, kvd);
 }
 
@@ -186,8 +187,10 @@ int check_heads(uint32_t nh, uint32_t nkv, uint32_t hd) {
     return BCHIP_OK;
 }
 
-// What a 4-bit cache asks beside: heads of whole blocks, and tile offsets within 32 bits.
-int check_q4(uint32_t nkv, uint32_t hd) {
+// What a 4-bit cache asks beside: heads of whole blocks, tile offsets within 32 bits, and slots whose
+// tile ends within 32 bits.
+int check_q4(uint32_t nkv, uint32_t hd, uint64_t slots = 0) {
+    if (slots > Q4_SLOTS) return fail(BCHIP_E_UNSUPPORTED, "a list up to slot %llu of a 4-bit cache (at most %llu slots)", (unsigned long long)slots, (unsigned long long)Q4_SLOTS);
     if (hd % Q4_BLOCK) return fail(BCHIP_E_UNSUPPORTED, "head_dim %u (a 4-bit cache takes multiples of %u)", hd, Q4_BLOCK);
     if ((uint64_t)nkv * hd > (1u << 20))
         return fail(BCHIP_E_UNSUPPORTED, "%u KV heads of %u (a 4-bit cache's slot holds at most 2^20 elements)", nkv, hd);
@@ -700,7 +703,7 @@ int bchip_attention(bchip_ctx* c, const float* q, const void* kc, const void* vc
     if (!q || !kc || !vc || !out) return fail(BCHIP_E_ARG, "null pointer");
     if (kv_type > LAST_TYPE) return fail(BCHIP_E_ARG, "element type %u", kv_type);
     CHECK(check_heads(nh, nkv, hd));
-    if (kv_type == BCHIP_Q4) CHECK(check_q4(nkv, hd));
+    if (kv_type == BCHIP_Q4) CHECK(check_q4(nkv, hd, (uint64_t)pos + rows));
     if (!aligned16(q) || !aligned16(out) || !aligned16(kc) || !aligned16(vc))
         return fail(BCHIP_E_ARG, "q, out and the caches must be 16-byte aligned");
     if ((uint64_t)pos + rows > 0xffffffffull) return fail(BCHIP_E_ARG, "position past 2^32");
@@ -770,7 +773,7 @@ int bchip_rope_append_attention_rows(bchip_ctx* c, float* q, const float* k, con
     if (!q || !k || !v || !kc || !vc || !inv_freq || !positions || !out) return fail(BCHIP_E_ARG, "null pointer");
     if (kv_type > LAST_TYPE) return fail(BCHIP_E_ARG, "element type %u", kv_type);
     CHECK(check_heads(nh, nkv, hd));
-    if (kv_type == BCHIP_Q4) CHECK(check_q4(nkv, hd));
+    if (kv_type == BCHIP_Q4) CHECK(check_q4(nkv, hd, (uint64_t)pos + rows));
     if (rope_dim % 2 || rope_dim > hd) return fail(BCHIP_E_ARG, "rope_dim %u for head_dim %u", rope_dim, hd);
     if (!aligned16(q) || !aligned16(out) || !aligned16(kc) || !aligned16(vc))
         return fail(BCHIP_E_ARG, "q, out and the caches must be 16-byte aligned");
@@ -823,7 +826,7 @@ static int fused_step(bchip_ctx* c, Workspace& ws, float* q, const float* k, con
     if (!q || !k || !v || !kc || !vc || !inv_freq || !positions || !out) return fail(BCHIP_E_ARG, "null pointer");
     if (kv_type > LAST_TYPE) return fail(BCHIP_E_ARG, "element type %u", kv_type);
     CHECK(check_heads(nh, nkv, hd));
-    if (kv_type == BCHIP_Q4) CHECK(check_q4(nkv, hd));
+    if (kv_type == BCHIP_Q4) CHECK(check_q4(nkv, hd, (uint64_t)pos + 1));
     if (rope_dim % 2 || rope_dim > hd) return fail(BCHIP_E_ARG, "rope_dim %u for head_dim %u", rope_dim, hd);
     const bool fuse = kv_type == BCHIP_F16 && row_fusable(nh, nkv, hd, rope_dim, neox);
     if (!aligned16(q) || !aligned16(out) || !aligned16(kc) || !aligned16(vc) || (fuse && (!aligned16(k) || !aligned16(v))))
@@ -904,6 +907,7 @@ static int check_ragged(bchip_ctx* c, const void* kc, const void* vc, uint32_t k
     if (nseq > 256) return fail(BCHIP_E_ARG, "%u sequences (at most 256)", nseq);
     for (uint32_t i = 0; i < nseq; i++) {
         if (seq_lens[i] == 0) return fail(BCHIP_E_ARG, "sequence %u sees no slots", i);
+        if (kv_type == BCHIP_Q4 && seq_lens[i] > Q4_SLOTS) return fail(BCHIP_E_UNSUPPORTED, "sequence %u: a list of %u (a 4-bit cache's have at most %llu slots)", i, seq_lens[i], (unsigned long long)Q4_SLOTS);
         const uint64_t end = bytes_of(kv_type, sat_mul(sat_add(kv_offsets[i], seq_lens[i]), kvd));
         CHECK(check_span(c, kc, end, "kc"));
         CHECK(check_span(c, vc, end, "vc"));

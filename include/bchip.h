@@ -28,8 +28,8 @@
  *    as a code the value over the scale to the nearest even; a block with an element that is not
  *    finite gets the scale NaN and reads as NaN. A buffer written elsewhere has to keep to such
  *    scales. Element offsets, counts and row widths are multiples of 32, and cache calls take
- *    head dims that are multiples of 32 and slots of at most 2^20 elements (else
- *    BCHIP_E_UNSUPPORTED).
+ *    head dims that are multiples of 32, slots of at most 2^20 elements and lists of at most
+ *    2^32 - 256 slots (else BCHIP_E_UNSUPPORTED).
  */
 #ifndef BCHIP_H
 #define BCHIP_H
@@ -162,7 +162,8 @@ int bchip_rope_append(bchip_ctx* ctx, float* q, const float* k, const float* v, 
  * no other. No slot past the highest that a mask names is read; one past the end of a
  * bchip_alloc buffer is left out. Where scratch cannot be had (memory full, a call under graph
  * capture that has not run before at its size) lists run uncut. Scratch that a captured call
- * took stays valid until the context is destroyed; replays run one at a time. */
+ * took stays valid until the context is destroyed; a replay shares it with the context's other
+ * calls and replays, so they run one after another, not beside each other. */
 int bchip_attention(bchip_ctx* ctx, const float* q, const void* kc, const void* vc,
                     uint32_t kv_type, float* out, const uint32_t* masks, uint32_t tree,
                     uint32_t rows, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t pos,

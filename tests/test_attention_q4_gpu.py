@@ -143,6 +143,40 @@ def test_ragged(ctx, nh, nkv, hd, seqs, longest):
         b.free()
 
 
+@pytest.mark.parametrize("lens", [[20000] + [100] * 63, [33, 6000] + [100] * 15, [1300] * 3 + [640] * 9, [2561] * 65])
+def test_ragged_lists_of_unlike_lengths(ctx, lens):
+    """One long list among brief ones is cut, whatever their average; more lists than a launch takes."""
+    nh, nkv, hd = 14, 2, 64
+    lens = np.array(lens, np.uint32)
+    offs = np.concatenate([[0], np.cumsum(lens)[:-1]]).astype(np.uint64)
+    n, kvd, scale, r = int(lens.sum()), nkv * hd, hd ** -0.5, np.random.default_rng(len(lens))
+    q = (r.standard_normal((len(lens), nh, hd)) * 2).astype(np.float32)
+    kbuf, k = cache(n, kvd, 17)
+    vbuf, v = cache(n, kvd, 18)
+    qb, kb, vb, ob = ctx.upload(q), ctx.upload(kbuf), ctx.upload(vbuf), ctx.zeros(q.nbytes)
+    ctx.attention_ragged(qb, kb, vb, bchip.Q4, ob, lens, offs, nh, nkv, hd, scale)
+    got = ctx.read(ob, q.shape)
+    whole = np.linalg.norm(got - np.concatenate([ragged_row(q, k, v, nkv, hd, scale, i, o, l, got) for i, (o, l) in enumerate(zip(offs, lens))]))
+    assert whole <= 8e-6 * np.linalg.norm(got)
+    for b in (qb, kb, vb, ob):
+        b.free()
+
+
+def test_more_rows_than_a_grid_holds(ctx):
+    """65535 units of 64 query rows a KV head are a grid's most: a longer pass runs in parts."""
+    nh, nkv, hd, rows = 16, 1, 32, 65535 * 4 + 70
+    r = np.random.default_rng(2)
+    q = np.resize((r.standard_normal((1000, nh, hd)) * 2).astype(np.float32), (rows, nh, hd))
+    kbuf, k = cache(rows, hd, 19)
+    vbuf, v = cache(rows, hd, 20)
+    got = run(ctx, q, kbuf, vbuf, nkv, 0, hd ** -0.5)
+    some = np.array([0, 65535 * 4 - 1, 65535 * 4, rows - 1])
+    see = np.arange(rows)[None] <= some[:, None]
+    want, mass, top = P.attention(q[some], k.reshape(rows, nkv, hd), v.reshape(rows, nkv, hd), nkv, see, hd ** -0.5)
+    gate(got[some], want, mass, top, hd, "rows in parts")
+    assert np.isfinite(got).all()
+
+
 def test_a_pool_past_4_gib(ctx):
     """Slots whose bytes lie past 2^32."""
     nh, nkv, hd, length = 8, 8, 128, 700
@@ -269,5 +303,8 @@ def test_bad_arguments_are_refused(ctx):
     refused(bchip.E_ARG, lambda: ctx.attention_ragged(q, kc, kc, bchip.Q4, out, [0], [1], 32, 8, 128, 0.1))
     refused(bchip.E_ARG, lambda: ctx.attention_ragged(q, kc, kc, bchip.Q4, out, [3], [(1 << 64) // 1024], 32, 8, 128, 0.1))
     refused(bchip.E_UNSUPPORTED, lambda: ctx.attention_ragged(q, kc, kc, bchip.Q4, out, [3], [0], 32, 8, 48, 0.1))
+    # Lists whose last tile would end past 2^32.
+    refused(bchip.E_UNSUPPORTED, lambda: ctx.attention(q, kc, kc, bchip.Q4, out, None, False, 1, 1, 1, 32, (1 << 32) - 256, 0.1))
+    refused(bchip.E_UNSUPPORTED, lambda: ctx.attention_ragged(q, kc, kc, bchip.Q4, out, [(1 << 32) - 255], [0], 1, 1, 32, 0.1))
     for b in (kc, q, out):
         b.free()
