@@ -223,8 +223,14 @@ void Workspace::set_fixed(void* base, size_t o_bytes, size_t ml_bytes, size_t q_
 
 void Workspace::drop(void* p) {
     if (!p) return;
-    if (captured) retired.push_back(p);
-    else (void)hipFree(p);
+    if (!captured) {
+        (void)hipFree(p);
+        return;
+    }
+    try {
+        retired.push_back(p);
+    } catch (...) {  // (no memory for the note: the block stays until the process ends)
+    }
 }
 
 bool Workspace::had(hipStream_t s, bool enough) {
