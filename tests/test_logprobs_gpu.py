@@ -161,6 +161,31 @@ def test_many_rows(ctx):
     np.testing.assert_array_equal(got[0][:40], one[0])
 
 
+def test_rows_of_several_blocks_a_workgroup(ctx):
+    """More rows than workgroups: each takes a row's blocks in turn and keeps the best of them. Rows whose
+    best come in order, equal ones, masks that leave few numbers, and NaNs beside -inf alone."""
+    rows, vocab, top = 1030, 20001, 20
+    r = np.random.default_rng(11)
+    x = (r.standard_normal((rows, vocab)) * 3).astype(np.float32)
+    x[1] = np.linspace(-5, 5, vocab)
+    x[2] = x[1][::-1]
+    x[3] = 0.5
+    x[4, :19000] = -np.inf
+    x[5] = -np.inf
+    x[5, [3, 8200, 16500]] = 1.0, 3.0, 2.0
+    x[6, :17000] = 1.0
+    x[7] = np.floor(x[7])
+    x[8] = np.nan                        # -inf and one number among NaNs
+    x[8, 9000:9030], x[8, 20000] = -np.inf, 7.0
+    x[9, 10000] = np.nan
+    tokens = r.integers(0, vocab, rows).astype(np.uint32)
+    tokens[3:8] = 5, 19500, 8200, 17500, 1
+    check(call(ctx, x, 1.0, tokens, top), plain(x, 1.0, tokens, top), "several blocks")
+    few = call(ctx, x[:40], 1.0, tokens[:40], top)
+    for a, b in zip(call(ctx, x, 1.0, tokens, top), few):
+        np.testing.assert_array_equal(a[:40], b)  # the bits do not depend on the rows beside
+
+
 def test_a_captured_call(ctx):
     """Under capture a fresh context has no scratch: a workgroup takes each row. The same ids; values
     within rounding; and once scratch is there, a graph that took it survives a larger call."""
