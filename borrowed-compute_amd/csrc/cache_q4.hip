@@ -3,9 +3,10 @@
 //
 // k_rope_append_q4 is k_rope_append (rope.hip) over such a cache: q rotates in place with the
 // same expressions, and k, rotated the same, and v go into the cache as codes. A thread takes
-// one pair of a q head or two consecutive elements of a k or v head, so sixteen lanes hold a
-// block and agree on its scale by four shuffles. Bound by q's traffic for many rows (512 rows
-// of 32 + 2 x 8 heads of 128) and by the launch for few.
+// one pair of q heads or two consecutive elements of k or v heads, so sixteen lanes hold a
+// block and agree on its scale by four shuffles. Bound by q's traffic for many rows (4096 rows
+// of 32 + 2 x 8 heads of 128: 42 us, 4.1 TB/s, of 56 with a sine and cosine for every head; 512
+// rows 8.6 us) and by the launch for few (5 us up to 128 rows).
 #include "common.hpp"
 #include "internal.hpp"
 #include "q4.hpp"
@@ -14,65 +15,101 @@
 
 namespace bchip {
 
+// Pairs of a call from which a thread takes four heads' for one sine and cosine (32 + 2 x 8 heads of 128,
+// 1024 rows: 12.1 us against 16.1; 256 rows: 6.7 against 6.0, 28 + 2 x 4 heads, 512 rows: 8.6 against 8.1,
+// where the launch has too few threads).
+constexpr uint64_t Q4_SHARED_PAIRS = 5 << 18;
+
 struct Q4RowSlots {
     uint64_t slot[MAX_ITEMS];
 };
 
-// Element e of a head x of hd elements after the rotation of its pairs by pos * inv_freq.
-__device__ __forceinline__ float rotated(const float* x, uint32_t e, float pos, const float* inv_freq,
-                                         uint32_t rope_dim, uint32_t neox) {
-    if (e >= rope_dim) return x[e];
-    const uint32_t hh = rope_dim / 2;
-    const uint32_t i = neox ? (e < hh ? e : e - hh) : e / 2;
-    const uint32_t a = neox ? i : 2 * i, b = neox ? i + hh : 2 * i + 1;
-    float y0, y1;
-    rotate(x[a], x[b], pos * inv_freq[i], y0, y1);
-    return e == a ? y0 : y1;
-}
-
-// Row r goes to slot slot0 + r, or (RAGGED) to sl.slot[r]. hd a multiple of 32.
-template <bool RAGGED>
+// Row r goes to slot slot0 + r, or (RAGGED) to sl.slot[r]. hd a multiple of 32. A thread takes its
+// pair of up to HG heads, whose rotation is the same.
+template <bool RAGGED, int HG>
 __global__ __launch_bounds__(256) void k_rope_append_q4(float* __restrict__ q, const float* __restrict__ k,
                                                         const float* __restrict__ v, uint8_t* __restrict__ kc,
                                                         uint8_t* __restrict__ vc, const float* __restrict__ inv_freq,
                                                         const uint32_t* __restrict__ positions, uint32_t rows,
                                                         uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t rope_dim,
                                                         uint32_t neox, uint64_t slot0, const Q4RowSlots sl) {
-    const uint32_t half = hd / 2, heads = nh + 2 * nkv;
+    const uint32_t half = hd / 2, qg = (nh + HG - 1) / HG, kg = (nkv + HG - 1) / HG, groups = qg + 2 * kg;
     const uint64_t idx = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (idx >= (uint64_t)rows * heads * half) return;  // (whole blocks of sixteen lanes: half % 16 == 0)
-    const uint32_t p = idx % half, hx = (idx / half) % heads;
-    const uint64_t r = idx / ((uint64_t)half * heads);
-    if (hx < nh) {
+    if (idx >= (uint64_t)rows * groups * half) return;  // (whole blocks of sixteen lanes: half % 16 == 0)
+    const uint32_t p = idx % half, gx = (idx / half) % groups;
+    const uint64_t r = idx / ((uint64_t)half * groups);
+    if (gx < qg) {
         uint32_t a, b;
         if (!rope_pair(p, rope_dim, neox, a, b)) return;
-        float* hp = q + (r * nh + hx) * hd;
-        float y0, y1;
-        rotate(hp[a], hp[b], (float)positions[r] * inv_freq[p], y0, y1);
-        hp[a] = y0;
-        hp[b] = y1;
+        float* hp = q + (r * nh + gx * HG) * hd;
+        float x[HG][2], s, c;
+#pragma unroll
+        for (int h = 0; h < HG; h++)
+            if (gx * HG + h < nh) x[h][0] = hp[h * hd + a], x[h][1] = hp[h * hd + b];
+        sincosf((float)positions[r] * inv_freq[p], &s, &c);
+#pragma unroll
+        for (int h = 0; h < HG; h++)
+            if (gx * HG + h < nh) {
+                float y0, y1;
+                rotate_sc(x[h][0], x[h][1], s, c, y0, y1);
+                hp[h * hd + a] = y0;
+                hp[h * hd + b] = y1;
+            }
         return;
     }
-    const bool isk = hx < nh + nkv;
-    const uint32_t kh = isk ? hx - nh : hx - nh - nkv;
-    const float* hp = (isk ? k : v) + (r * nkv + kh) * hd;
-    float x0, x1;
-    if (!isk) {
-        x0 = hp[2 * p];
-        x1 = hp[2 * p + 1];
-    } else if (!neox && 2 * p < rope_dim) {
-        rotate(hp[2 * p], hp[2 * p + 1], (float)positions[r] * inv_freq[p], x0, x1);
-    } else {
-        const float pos = (float)positions[r];
-        x0 = rotated(hp, 2 * p, pos, inv_freq, rope_dim, neox);
-        x1 = rotated(hp, 2 * p + 1, pos, inv_freq, rope_dim, neox);
-    }
-    uint8_t codes;
-    const f16 d = q4_quantise(x0, x1, codes);
-    const uint64_t e = (RAGGED ? sl.slot[r] : slot0 + r) * ((uint64_t)nkv * hd) + (uint64_t)kh * hd + 2 * p;
+    const bool isk = gx < qg + kg;
+    const uint32_t h0 = (isk ? gx - qg : gx - qg - kg) * HG;
+    const float* hp = (isk ? k : v) + (r * nkv + h0) * hd;
     uint8_t* dst = isk ? kc : vc;
-    dst[q4_code_at(e)] = codes;
-    if (p % 16 == 0) *(f16*)(dst + q4_scale_at(e)) = d;
+    const uint64_t e0 = (RAGGED ? sl.slot[r] : slot0 + r) * ((uint64_t)nkv * hd) + 2 * p;
+    // Elements 2p and 2p + 1 of each head: a pair, or (neox) the same half of two pairs.
+    const uint32_t hh = rope_dim / 2;
+    const float pos = (float)positions[r];
+    uint32_t other[2] = {2 * p + 1, 2 * p};
+    float s[2] = {0, 0}, c[2] = {1, 1};
+    bool first[2] = {true, false}, turn[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint32_t e = 2 * p + i;
+        turn[i] = isk && e < rope_dim;
+        if (neox && turn[i]) {
+            first[i] = e < hh;
+            other[i] = first[i] ? e + hh : e - hh;
+            sincosf(pos * inv_freq[first[i] ? e : e - hh], &s[i], &c[i]);
+        }
+    }
+    if (!neox && turn[0]) {
+        sincosf(pos * inv_freq[p], &s[0], &c[0]);
+        s[1] = s[0], c[1] = c[0];
+    }
+    float x[HG][2], y[HG][2];
+#pragma unroll
+    for (int h = 0; h < HG; h++)
+        if (h0 + h < nkv) {
+            x[h][0] = hp[h * hd + 2 * p], x[h][1] = hp[h * hd + 2 * p + 1];
+            if (neox) {
+#pragma unroll
+                for (int i = 0; i < 2; i++) y[h][i] = turn[i] ? hp[h * hd + other[i]] : 0.0f;
+            } else {
+                y[h][0] = x[h][1], y[h][1] = x[h][0];
+            }
+        }
+#pragma unroll
+    for (int h = 0; h < HG; h++)
+        if (h0 + h < nkv) {
+            float z[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                float y0, y1;
+                rotate_sc(first[i] ? x[h][i] : y[h][i], first[i] ? y[h][i] : x[h][i], s[i], c[i], y0, y1);
+                z[i] = !turn[i] ? x[h][i] : first[i] ? y0 : y1;
+            }
+            uint8_t codes;
+            const f16 d = q4_quantise(z[0], z[1], codes);
+            const uint64_t e = e0 + (uint64_t)(h0 + h) * hd;
+            dst[q4_code_at(e)] = codes;
+            if (p % 16 == 0) *(f16*)(dst + q4_scale_at(e)) = d;
+        }
 }
 
 // dst[off + i] = src[i]: two elements a thread, n and off multiples of 32.
@@ -157,14 +194,14 @@ static uint32_t grid_of(uint64_t n) {
     return (uint32_t)(b > 65536 ? 65536 : (b ? b : 1));
 }
 
-hipError_t rope_append_q4_launch(float* q, const float* k, const float* v, void* kc, void* vc, const float* inv_freq,
-                                 const uint32_t* positions, uint32_t rows, uint32_t nh, uint32_t nkv, uint32_t hd,
-                                 uint32_t rope_dim, uint32_t neox, uint64_t slot0, const uint64_t* slots,
-                                 hipStream_t s) {
-    const uint64_t per_row = (uint64_t)(nh + 2 * nkv) * (hd / 2);
+template <int HG>
+static hipError_t rope_append_q4_heads(float* q, const float* k, const float* v, void* kc, void* vc, const float* inv_freq,
+                                       const uint32_t* positions, uint32_t rows, uint32_t nh, uint32_t nkv, uint32_t hd,
+                                       uint32_t rope_dim, uint32_t neox, uint64_t slot0, const uint64_t* slots,
+                                       hipStream_t s) {
+    const uint64_t per_row = ((nh + HG - 1) / HG + 2 * (uint64_t)((nkv + HG - 1) / HG)) * (hd / 2);
     if (!slots) {
-        if (rows * per_row == 0) return hipSuccess;
-        hipLaunchKernelGGL(k_rope_append_q4<false>, dim3(blocks_of(rows * per_row)), dim3(256), 0, s, q, k, v,
+        hipLaunchKernelGGL((k_rope_append_q4<false, HG>), dim3(blocks_of(rows * per_row)), dim3(256), 0, s, q, k, v,
                            (uint8_t*)kc, (uint8_t*)vc, inv_freq, positions, rows, nh, nkv, hd, rope_dim, neox, slot0,
                            Q4RowSlots{});
         return hipGetLastError();
@@ -173,7 +210,7 @@ hipError_t rope_append_q4_launch(float* q, const float* k, const float* v, void*
         const uint32_t nr = rows - r0 < MAX_ITEMS ? rows - r0 : MAX_ITEMS;
         Q4RowSlots sl{};
         for (uint32_t i = 0; i < nr; i++) sl.slot[i] = slots[r0 + i];
-        hipLaunchKernelGGL(k_rope_append_q4<true>, dim3(blocks_of(nr * per_row)), dim3(256), 0, s,
+        hipLaunchKernelGGL((k_rope_append_q4<true, HG>), dim3(blocks_of(nr * per_row)), dim3(256), 0, s,
                            q + (size_t)r0 * nh * hd, k + (size_t)r0 * nkv * hd, v + (size_t)r0 * nkv * hd,
                            (uint8_t*)kc, (uint8_t*)vc, inv_freq, positions + r0, nr, nh, nkv, hd, rope_dim, neox, 0ull,
                            sl);
@@ -181,6 +218,16 @@ hipError_t rope_append_q4_launch(float* q, const float* k, const float* v, void*
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
+}
+
+hipError_t rope_append_q4_launch(float* q, const float* k, const float* v, void* kc, void* vc, const float* inv_freq,
+                                 const uint32_t* positions, uint32_t rows, uint32_t nh, uint32_t nkv, uint32_t hd,
+                                 uint32_t rope_dim, uint32_t neox, uint64_t slot0, const uint64_t* slots,
+                                 hipStream_t s) {
+    if (rows == 0) return hipSuccess;
+    const uint64_t pairs = (uint64_t)rows * (nh + 2 * (uint64_t)nkv) * (hd / 2);
+    const auto launch = pairs >= Q4_SHARED_PAIRS ? rope_append_q4_heads<4> : rope_append_q4_heads<1>;
+    return launch(q, k, v, kc, vc, inv_freq, positions, rows, nh, nkv, hd, rope_dim, neox, slot0, slots, s);
 }
 
 hipError_t copy_q4_launch(const void* src, uint32_t st, void* dst, uint32_t dt, uint64_t off, uint64_t n,

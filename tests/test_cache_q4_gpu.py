@@ -127,6 +127,30 @@ def test_append_is_the_rotated_row_in_4_bits(ctx, nh, nkv, hd, rd, neox, rows, s
         b.free()
 
 
+@pytest.mark.parametrize("nh,nkv,hd,rd,neox,rows", [(32, 8, 128, 128, False, 517), (14, 2, 64, 64, True, 2333), (13, 1, 128, 64, True, 1401),
+                                                    (9, 3, 96, 40, False, 1900), (6, 6, 32, 32, True, 4600)])
+def test_an_append_of_many_rows(ctx, nh, nkv, hd, rd, neox, rows):
+    """Rows from which a thread takes several heads: the bits of appends of a few rows each."""
+    r = np.random.default_rng(rows)
+    kvd, n = nkv * hd, rows * nkv * hd
+    q, k, v = (r.standard_normal((rows, x * hd)).astype(np.float32) for x in (nh, nkv, nkv))
+    pos = (np.arange(rows) * 31 + 5).astype(np.uint32)
+    ib, pb, kb, vb = ctx.upload(O.inv_freq(rd, 1e4)), ctx.upload(pos), ctx.upload(k), ctx.upload(v)
+    got = []
+    for step in (rows, 100):
+        qb, kc, vc = ctx.upload(q), ctx.zeros(bchip.nbytes_of(bchip.Q4, n)), ctx.zeros(bchip.nbytes_of(bchip.Q4, n))
+        for i in range(0, rows, step):
+            ctx.rope_append(qb.offset(i * nh * hd * 4), kb.offset(i * kvd * 4), vb.offset(i * kvd * 4), kc, vc, bchip.Q4, ib,
+                            pb.offset(i * 4), min(step, rows - i), nh, nkv, hd, rd, neox, i)
+        got.append([ctx.read(qb, q.shape), raw(ctx, kc, n), raw(ctx, vc, n)])
+        for b in (qb, kc, vc):
+            b.free()
+    for x, y in zip(*got):
+        np.testing.assert_array_equal(x, y)
+    for b in (ib, pb, kb, vb):
+        b.free()
+
+
 def test_ragged_append_is_each_rows_own(ctx):
     nh, nkv, hd, n = 8, 2, 64, 70
     kvd = nkv * hd
