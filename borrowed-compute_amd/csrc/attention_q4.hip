@@ -20,7 +20,7 @@
 // nothing.
 //
 // attn_q4_row: at most 16 query rows a KV head (a decode step, a short verify pass of few heads):
-// a wave takes tiles of 32 slots of its workgroup's chunk, its four waves' states meet in LDS. Up
+// a wave takes tiles of 32 slots of its workgroup's chunk, the waves' states meet in LDS. Up
 // to eight query rows put q's and the weights' two parts side by side in the MFMA's 16 columns:
 // half the matrix work. attn_q4_tile: more query rows: a workgroup unpacks each tile of 64 slots
 // once, into LDS in the order of the operands, and its waves take 16 or 32 query rows each.
@@ -386,6 +386,13 @@ __device__ __forceinline__ uint64_t q4_bytes(uint64_t slots, uint32_t rem, uint3
     return (slots * kvd + rem + Q4_UNIT - 1) / Q4_UNIT * Q4_UNIT_BYTES;
 }
 
+// What bounds it, measured at 32 x 8 heads of 128. Long lists: a tile is some 300 vector instructions
+// a wave, most of them unpacking, against 256 cycles of MFMA; at 131072 slots the arithmetic alone takes
+// 25 us and the loads alone 25, and two waves a SIMD overlap them to 40 (3.8 TB/s; the call 44). At 32768
+// slots 14.4 (the call 17.4). Short ones: the chain from the launch over q, the first tile and the states
+// to the result, 7.4 us at 1000 slots. Tried: two tiles on their way to a wave instead of one (15.1 us for
+// 14.5 at 32768, and spills for heads past 160); operands read from memory where the lanes need them
+// (1.6 times the time a tile); 1024 workgroups (two more waves a SIMD: 16.1 and 44.5 us, the states double).
 template <int NB, bool PK, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void attn_q4_row(const Q4Params p) {
     constexpr int HD = 32 * NB, NF = 2 * NB, QW = NB < WAVES ? NB : WAVES, QJ = (NB + WAVES - 1) / WAVES;
@@ -622,6 +629,12 @@ constexpr int Q4_WAVES = 4;
 
 // More query rows: a tile of 64 slots unpacked once into LDS for the workgroup's waves of 16 RT
 // query rows each: four of 32 rows, or eight of 16, of which four take each half of the slots.
+//
+// What bounds it. Prompts: the matrix cores, which q's and the weights' two parts give twice the work:
+// 4096 rows of 32 x 8 heads of 128 take 283 us, 485 TFLOP/s of the 549 that half of a large f16 product's
+// rate leaves. Verify passes: latency. 8 rows of 64 x 8 heads at 5003 slots take 14 us, of which the first
+// tile's way in some 6, three tiles 0.85 each (two barriers a tile) and 7 MB of states 1.5; eight waves
+// a workgroup instead of four took 2 us off, 32 rows a wave there would leave half of the waves idle.
 constexpr uint32_t Q4_TILE_B = 64;
 
 template <int NB, int RT>
@@ -883,7 +896,8 @@ __global__ __launch_bounds__(RT == 1 ? 512 : 256, 2) void attn_q4_tile(const Q4P
 
 // The chunks of 16 query rows of a list brought together, one operand's columns a workgroup (two took
 // 0.4 to 1.9 us more, few workgroups reading much each), each wave a share of the chunks; states lie as
-// their waves held them. A chunk without a weight left
+// their waves held them: 3 to 4 us of a call, a launch behind the other kernel and one read of the states.
+// A chunk without a weight left
 // its columns unwritten.
 constexpr uint32_t Q4_MAX_CHUNKS = 256;
 
@@ -1126,8 +1140,10 @@ hipError_t q4_attention(const AttnCall& a, Workspace& ws, hipStream_t s) {
         }
         return hipSuccess;
     }
-    // 32 query rows a wave where that still makes a workgroup for every CU.
-    const uint32_t rt = a.hd <= 128 && (nq + 127) / 128 * a.nkv >= 256 ? 2 : 1;
+    // 32 query rows a wave halve the LDS reads a product, where enough such workgroups keep every CU busy
+    // (32 x 8 heads of 128, 4096 rows: 271 us, 397 with 16; 1000 rows: 51, 39 with 16; they meet at 1300.
+    // Heads of 64 read less: 14 x 2 of them, 4096 rows, 124 us and 100 with 16, 8192 rows 314 and 329).
+    const uint32_t rt = a.hd <= 128 && (nq + 127) / 128 * a.nkv >= (a.hd > 64 ? 352u : 768u) ? 2 : 1;
     p.qt = 64 * rt;
     p.nqt = (uint32_t)((nq + p.qt - 1) / p.qt);
     const uint64_t groups = (uint64_t)p.nqt * a.nkv, tiles = (far + Q4_TILE_B - 1) / Q4_TILE_B;

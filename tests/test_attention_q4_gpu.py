@@ -177,6 +177,50 @@ def test_more_rows_than_a_grid_holds(ctx):
     assert np.isfinite(got).all()
 
 
+# Enough rows that a wave takes 32 of them.
+@pytest.mark.parametrize("nh,nkv,hd,rows,pos", [(32, 8, 128, 1500, 0), (28, 4, 128, 1701, 333), (14, 2, 64, 7100, 77), (12, 4, 96, 3800, 0),
+                                                (16, 8, 32, 6200, 5)])
+def test_passes_of_32_rows_a_wave(ctx, nh, nkv, hd, rows, pos):
+    """Against the formula in some rows; a V block that is not finite reaches the rows that see its
+    slot, and no other."""
+    r = np.random.default_rng(rows)
+    q = (r.standard_normal((rows, nh, hd)) * 2).astype(np.float32)
+    n, kvd, odd = pos + rows, nkv * hd, pos + rows - 41
+    kbuf, k = cache(n, kvd, 21)
+    x = np.random.default_rng(22).standard_normal((n, nkv, hd)).astype(np.float32)
+    x[odd, nkv - 1, hd - 1] = np.inf  # the last block of the last head
+    vbuf = P.pack(*P.quantise(x.reshape(n, kvd)))
+    v = P.unpack(vbuf, n * kvd).reshape(n, nkv, hd)
+    got = run(ctx, q, kbuf, vbuf, nkv, pos, hd ** -0.5)
+    some = np.unique(np.concatenate([[0, rows - 1, 31, 32, rows - 41, rows - 42], r.integers(0, rows, 16)]))
+    see = np.arange(n)[None] <= (pos + some)[:, None]
+    want, mass, top = P.attention(q[some], k.reshape(n, nkv, hd), v, nkv, see, hd ** -0.5)
+    bad = np.zeros(got.shape, bool)
+    bad[rows - 41:, nh - nh // nkv:, hd - 32:] = True
+    np.testing.assert_array_equal(np.isnan(got), bad)
+    fine = ~bad[some]
+    assert (np.abs(got[some] - want)[fine] <= P.bound(mass, top, hd)[fine]).all()
+    assert np.linalg.norm((got[some] - want)[fine]) <= 8e-6 * np.linalg.norm(want[fine])
+
+
+def test_a_tree_of_many_heads(ctx):
+    """A tree whose KV heads alone make enough workgroups for 32 rows a wave."""
+    nh, nkv, hd, rows, pos = 768, 48, 96, 64, 70
+    r = np.random.default_rng(5)
+    q = (r.standard_normal((rows, nh, hd)) * 2).astype(np.float32)
+    masks = r.integers(0, 1 << 63, rows, dtype=np.uint64) * np.uint64(2)
+    n, kvd = pos + 64, nkv * hd
+    kbuf, k = cache(n, kvd, 23)
+    vbuf, v = cache(n, kvd, 24)
+    got = run(ctx, q, kbuf, vbuf, nkv, pos, hd ** -0.5, masks)
+    some = np.array([0, 1, 17, 31, 32, 63])
+    bits = (masks[some][:, None] >> np.arange(64, dtype=np.uint64)[None]) & np.uint64(1)
+    see = np.concatenate([np.ones((len(some), pos), bool), bits.astype(bool)], 1)
+    want, mass, top = P.attention(q[some], k.reshape(n, nkv, hd), v.reshape(n, nkv, hd), nkv, see, hd ** -0.5)
+    gate(got[some], want, mass, top, hd, "a tree of 768 heads")
+    assert np.isfinite(got).all()
+
+
 def test_a_pool_past_4_gib(ctx):
     """Slots whose bytes lie past 2^32."""
     nh, nkv, hd, length = 8, 8, 128, 700
