@@ -1015,18 +1015,12 @@ Q4Params params(const AttnCall& a) {
     return p;
 }
 
-// Workgroups that keep the GPU busy without more states than they are worth: of attn_q4_row two a CU
-// (a step of 32 x 8 heads of 128 at 32768 slots: 18.0 us at 512, 20.7 at 256, 21.4 at 1024), of
-// attn_q4_tile, eight waves each, one (8 rows of 64 x 8 heads at 20000: 27 us at 256, 31 at 192, 33
-// at 512).
+// Workgroups of attn_q4_row that keep the GPU busy without more states than they are worth: two a CU (a
+// step of 32 x 8 heads of 128 at 32768 slots: 18.0 us at 512, 20.7 at 256, 21.4 at 1024).
 constexpr uint32_t Q4_ROW_GROUPS = 512;
 // Lists of several lengths end at different times: more workgroups (16 of 28 x 4 heads of 128 at 1 to 16384
 // slots: 38 us at 768, 46 at 512, 40 at 1024).
 constexpr uint32_t Q4_RAGGED_GROUPS = 768;
-constexpr uint32_t Q4_TILE_GROUPS = 256;
-// Lists in two chunks cost more in states and a second launch than they save (200 rows of 32 x 8
-// heads at 300: 22 us in two, 18.5 in one).
-constexpr uint32_t Q4_LEAST_CHUNKS = 3;
 // Tiles of a list up to which one workgroup of eight waves takes it whole, without a second launch
 // (32 x 8 heads of 128: 8.0 us at 16 tiles against 9.4, 11.3 at 32 against 10). Of several lists their
 // average, if the longest has at most twice that (8 lists of 28 x 4 heads, one of 1500 slots and the
@@ -1044,6 +1038,25 @@ void cut(Q4Item& it, uint64_t tiles, uint32_t want, uint32_t least, uint32_t of)
     const uint64_t n = std::max<uint64_t>(1, std::min<uint64_t>({(uint64_t)want, tiles / least, std::max<uint64_t>(Q4_FOLD_CHUNKS, tiles / Q4_FOLD_TILES), Q4_MAX_CHUNKS}));
     it.chunk = (uint32_t)std::max<uint64_t>(1, ((tiles + n - 1) / n + of - 1) / of * of);
     it.nchunk = (uint32_t)std::max<uint64_t>(1, (tiles + it.chunk - 1) / it.chunk);
+}
+
+// Chunks of attn_q4_tile's lists of `tiles` tiles for `units` workgroups a chunk: those of the least time
+// by what was measured (us): 0.6 + 0.006 hd a tile and 7 a workgroup beside, one at a time a CU; for
+// a second launch 2 + 0.0006 hd a unit, and the states' write and read at 5 TB/s. So 200 rows of 32 x 8 heads of
+// 128 run whole at 300 slots (18 us, in two chunks 25) and in two at 4000 (63, whole 96, in four 68), 340 rows at
+// 16000 in four (288, whole 352, in two 367), 8 rows of 64 x 8 at 500 in four (12.5, whole 17.5).
+uint32_t tile_chunks(uint64_t tiles, uint64_t units, uint32_t hd) {
+    constexpr uint64_t CUS = 256;
+    const float tile = 0.6f + 0.006f * hd, launch = 2.0f + 0.0006f * hd * units, states = 64.0f * 8.0f / 5e6f * hd * units;
+    uint64_t best = 1;
+    float least = (float)((units + CUS - 1) / CUS) * (tile * tiles + 7.0f);
+    for (uint64_t half = 1; half <= 8; half++) {  // as many as half a round holds, one round, ... four
+        const uint64_t n = std::min<uint64_t>({CUS * half / 2 / units, tiles / 2, Q4_MAX_CHUNKS});
+        if (n < 2) continue;
+        const float t = (float)((units * n + CUS - 1) / CUS) * (tile * ((tiles + n - 1) / n) + 7.0f) + launch + states * n;
+        if (t < least) least = t, best = n;
+    }
+    return (uint32_t)best;
 }
 
 bool reserve(Q4Params& p, uint64_t states, uint32_t hd, Workspace& ws, hipStream_t s) {
@@ -1147,8 +1160,7 @@ hipError_t q4_attention(const AttnCall& a, Workspace& ws, hipStream_t s) {
     p.qt = 64 * rt;
     p.nqt = (uint32_t)((nq + p.qt - 1) / p.qt);
     const uint64_t groups = (uint64_t)p.nqt * a.nkv, tiles = (far + Q4_TILE_B - 1) / Q4_TILE_B;
-    const uint64_t want = Q4_TILE_GROUPS / groups;
-    cut(it, tiles, want < Q4_LEAST_CHUNKS ? 1 : (uint32_t)want, 2, 1);
+    cut(it, tiles, rt == 2 ? 1 : tile_chunks(tiles, groups, a.hd), 2, 1);
     if (it.nchunk > 1 && !reserve(p, groups * it.nchunk * p.qt, a.hd, ws, s)) cut(it, tiles, 1, 2, 1);
 #define Q4_TILES(NB) launch_tile<NB>(p, rt, a, s)
     Q4_BY_DIM(a.hd / 32, Q4_TILES)

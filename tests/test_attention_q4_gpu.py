@@ -203,6 +203,23 @@ def test_passes_of_32_rows_a_wave(ctx, nh, nkv, hd, rows, pos):
     assert np.linalg.norm((got[some] - want)[fine]) <= 8e-6 * np.linalg.norm(want[fine])
 
 
+@pytest.mark.parametrize("nh,nkv,hd,rows,pos", [(32, 8, 128, 200, 4000), (32, 8, 128, 340, 9001), (14, 2, 64, 777, 3999), (12, 4, 96, 600, 7000),
+                                                (16, 4, 256, 400, 3500)])
+def test_pieces_of_a_prompt_behind_a_long_history(ctx, nh, nkv, hd, rows, pos):
+    """Passes of many workgroups whose lists are cut all the same."""
+    r = np.random.default_rng(rows)
+    q = (r.standard_normal((rows, nh, hd)) * 2).astype(np.float32)
+    n, kvd = pos + rows, nkv * hd
+    kbuf, k = cache(n, kvd, 25)
+    vbuf, v = cache(n, kvd, 26)
+    got = run(ctx, q, kbuf, vbuf, nkv, pos, hd ** -0.5)
+    some = np.unique(np.concatenate([[0, rows - 1, rows // 2], r.integers(0, rows, 12)]))
+    see = np.arange(n)[None] <= (pos + some)[:, None]
+    want, mass, top = P.attention(q[some], k.reshape(n, nkv, hd), v.reshape(n, nkv, hd), nkv, see, hd ** -0.5)
+    gate(got[some], want, mass, top, hd, f"{nh}/{nkv} x {hd}, {rows} at {pos}")
+    assert np.isfinite(got).all()
+
+
 def test_a_tree_of_many_heads(ctx):
     """A tree whose KV heads alone make enough workgroups for 32 rows a wave."""
     nh, nkv, hd, rows, pos = 768, 48, 96, 64, 70
