@@ -227,8 +227,8 @@ class GpuLayers:
         ctx = self.ctx
         ctx.upload(np.ascontiguousarray(x, np.float32), s["x"])
         ctx.rms_norm(s["x"], norm, s["n"], rows, self.cfg.n_embd, self.cfg.eps)
-        scores, vals, ids = ctx.zeros(rows * upto * 4), ctx.zeros(rows * (2 + top) * 4), ctx.zeros(rows * max(top, 1) * 4)
         tk = None if tokens is None else ctx.upload(np.ascontiguousarray(tokens, np.uint32))
+        scores, vals, ids = ctx.zeros(rows * upto * 4), ctx.zeros(rows * (2 + top) * 4), ctx.zeros(rows * max(top, 1) * 4)
         try:
             ctx.matmul(out, ty, s["n"], scores, upto, vc, rows)
             ctx.logprobs(scores, rows, upto, temperature, tk, vals if tk else None, vals.offset(rows * 4), top, ids,

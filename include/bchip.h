@@ -210,7 +210,7 @@ int bchip_rope_append_attention_rows(bchip_ctx* ctx, float* q, const float* k, c
  * dims: any plan with n_head_kv <= 1024), 128 KiB of their maxima and sums, 256 KiB of q
  * (nh * hd <= 65536 for the fused kernel). A step that needs more is refused with BCHIP_E_ARG
  * before anything is launched; an f32 cache never needs more (its pass then runs unsplit, the
- * same bits). Every call on one device shares that array, so calls on one device that overlap
+ * same bits), nor does a 4-bit one (at most 512 units). Every call on one device shares that array, so calls on one device that overlap
  * in time (from several contexts, threads or streams) race. */
 int bchip_rope_append_attention_noalloc(bchip_ctx* ctx, float* q, const float* k, const float* v, void* kc,
                                         void* vc, uint32_t kv_type, const float* inv_freq,
