@@ -212,6 +212,21 @@ def test_a_captured_call(ctx):
             hip("hipGraphExecDestroy", graph)
 
 
+def test_a_row_without_scratch_gives_the_same_bits(ctx):
+    from test_matmul_scratch_gpu import captured, hip
+    s, tokens = rows_of(3, 70000, 9), [69999, 0, 35000]
+    want = call(ctx, s, 0.7, tokens, 20)
+    with bchip.Ctx(0) as c:  # nothing has run here: under capture no scratch can be had
+        sb, tb = c.upload(s), c.upload(np.array(tokens, np.uint32))
+        lb, eb, ib, pb = c.zeros(12), c.zeros(12), c.zeros(240), c.zeros(240)
+        stream, graph = captured(c, lambda: c.logprobs(sb, 3, 70000, 0.7, tb, lb, eb, 20, ib, pb))
+        hip("hipGraphLaunch", graph, stream)
+        got = c.read(lb, 3), c.read(eb, 3), c.read(ib, (3, 20), np.uint32), c.read(pb, (3, 20))
+        hip("hipGraphExecDestroy", graph)
+    for a, b in zip(got, want):
+        np.testing.assert_array_equal(a, b)
+
+
 def test_bad_arguments_are_refused(ctx):
     s, o, w = ctx.zeros(4 * 2000), ctx.zeros(4 * 100), ctx.zeros(4 * 1)
 
