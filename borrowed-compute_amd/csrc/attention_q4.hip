@@ -1059,8 +1059,8 @@ uint32_t tile_chunks(uint64_t tiles, uint64_t units, uint32_t hd) {
     return (uint32_t)best;
 }
 
-bool reserve(Q4Params& p, uint64_t states, uint32_t hd, Workspace& ws, hipStream_t s) {
-    const bool had = ws.reserve_if(states, hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256, s);
+bool reserve(Q4Params& p, uint64_t states, uint32_t hd, Workspace& ws) {
+    const bool had = ws.reserve_if(states, hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256);
     p.part_o = ws.o;
     p.part_ml = ws.ml;
     return had;
@@ -1109,7 +1109,7 @@ hipError_t launch_items(Q4Params& p, const AttnCall& a, const uint64_t* lens, Wo
     // Lists that eight waves take in a few tiles each are not cut: no second launch.
     const bool brief = total <= (uint64_t)p.nitems * Q4_BRIEF && most <= 2 * Q4_BRIEF;
     plan(brief ? 0 : want);
-    if (split && !reserve(p, (uint64_t)units * 16, a.hd, ws, s)) plan(0);
+    if (split && !reserve(p, (uint64_t)units * 16, a.hd, ws)) plan(0);
     const bool pk = p.items[0].rows * p.G <= 8;
 #define Q4_BRIEF_ROW(NB) launch_row<NB, 2 * Q4_WAVES>(p, octs, pk, a, s)
 #define Q4_ROW(NB) launch_row<NB, Q4_WAVES>(p, octs, pk, a, s)
@@ -1161,7 +1161,7 @@ hipError_t q4_attention(const AttnCall& a, Workspace& ws, hipStream_t s) {
     p.nqt = (uint32_t)((nq + p.qt - 1) / p.qt);
     const uint64_t groups = (uint64_t)p.nqt * a.nkv, tiles = (far + Q4_TILE_B - 1) / Q4_TILE_B;
     cut(it, tiles, rt == 2 ? 1 : tile_chunks(tiles, groups, a.hd), 2, 1);
-    if (it.nchunk > 1 && !reserve(p, groups * it.nchunk * p.qt, a.hd, ws, s)) cut(it, tiles, 1, 2, 1);
+    if (it.nchunk > 1 && !reserve(p, groups * it.nchunk * p.qt, a.hd, ws)) cut(it, tiles, 1, 2, 1);
 #define Q4_TILES(NB) launch_tile<NB>(p, rt, a, s)
     Q4_BY_DIM(a.hd / 32, Q4_TILES)
 #undef Q4_TILES

@@ -221,9 +221,15 @@ void Workspace::set_fixed(void* base, size_t o_bytes, size_t ml_bytes, size_t q_
     gerr_host = owner.gerr_host;
 }
 
-void Workspace::drop(void* p) {
+bool Workspace::capturing() const {
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream, &cap) != hipSuccess) (void)hipGetLastError();
+    return cap != hipStreamCaptureStatusNone;
+}
+
+void Workspace::drop(void* p, bool held) {
     if (!p) return;
-    if (!captured) {
+    if (!held) {
         (void)hipFree(p);
         return;
     }
@@ -233,23 +239,15 @@ void Workspace::drop(void* p) {
     }
 }
 
-bool Workspace::had(hipStream_t s, bool enough) {
-    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(s, &cap) != hipSuccess) (void)hipGetLastError();
-    if (cap == hipStreamCaptureStatusNone) return true;
-    captured |= enough && !fixed;
-    return enough;
-}
-
-bool Workspace::reserve_if(size_t need_slots, size_t hd_pad, hipStream_t s) {
-    if (!fixed && !had(s, need_slots <= slots && hd_pad <= hdp && o)) return false;
+bool Workspace::reserve_if(size_t need_slots, size_t hd_pad) {
+    if (!fixed && !(need_slots <= slots && hd_pad <= hdp && o) && capturing()) return false;
     if (reserve(need_slots, hd_pad) == hipSuccess) return true;
     (void)hipGetLastError();
     return false;
 }
 
-bool Workspace::reserve_vt_if(size_t bytes, hipStream_t s) {
-    if (!fixed && !had(s, bytes <= vt_bytes && vt)) return false;
+bool Workspace::reserve_vt_if(size_t bytes) {
+    if (!fixed && !(bytes <= vt_bytes && vt) && capturing()) return false;
     if (reserve_vt(bytes) == hipSuccess) return true;
     (void)hipGetLastError();
     return false;
@@ -263,11 +261,15 @@ hipError_t Workspace::reserve(size_t need_slots, size_t hd_pad) {
         hdp = hd_pad;
         return hipSuccess;
     }
-    if (need_slots <= slots && hd_pad <= hdp && o) return hipSuccess;
+    if (need_slots <= slots && hd_pad <= hdp && o) {
+        o_held |= capturing();
+        return hipSuccess;
+    }
     const size_t ns = std::max(need_slots, slots), nh = std::max(hd_pad, hdp);
-    drop(o);
-    drop(ml);
+    drop(o, o_held);
+    drop(ml, o_held);
     o = ml = nullptr;
+    o_held = capturing();
     slots = 0;
     hdp = nh;
     hipError_t e = hipMalloc((void**)&o, ns * hdp * sizeof(float));
@@ -280,9 +282,13 @@ hipError_t Workspace::reserve(size_t need_slots, size_t hd_pad) {
 
 hipError_t Workspace::reserve_vt(size_t bytes) {
     if (fixed) return hipErrorOutOfMemory;
-    if (bytes <= vt_bytes && vt) return hipSuccess;
-    drop(vt);
+    if (bytes <= vt_bytes && vt) {
+        vt_held |= capturing();
+        return hipSuccess;
+    }
+    drop(vt, vt_held);
     vt = nullptr;
+    vt_held = capturing();
     vt_bytes = 0;
     hipError_t e = hipMalloc(&vt, bytes);
     if (e != hipSuccess) return e;
@@ -296,9 +302,13 @@ hipError_t Workspace::reserve_qrot(size_t floats) {
         qrot_floats = floats;
         return hipSuccess;
     }
-    if (floats <= qrot_floats && qrot) return hipSuccess;
-    if (qrot) (void)hipFree(qrot);
+    if (floats <= qrot_floats && qrot) {
+        qrot_held |= capturing();
+        return hipSuccess;
+    }
+    drop(qrot, qrot_held);
     qrot = nullptr;
+    qrot_held = capturing();
     qrot_floats = 0;
     hipError_t e = hipMalloc((void**)&qrot, floats * sizeof(float));
     if (e != hipSuccess) return e;
@@ -306,7 +316,8 @@ hipError_t Workspace::reserve_qrot(size_t floats) {
     return hipSuccess;
 }
 
-hipError_t Workspace::init(int device) {
+hipError_t Workspace::init(int device, hipStream_t on) {
+    stream = on;
     hipError_t e = hipMalloc(&zero, ZERO_BYTES);
     if (e == hipSuccess) e = hipMemset(zero, 0, ZERO_BYTES);
     if (e == hipSuccess) e = hipMalloc((void**)&gcnt, (size_t)GROUP_COUNTERS * GROUP_STRIDE * sizeof(uint32_t));
@@ -379,7 +390,7 @@ int bchip_init(int device, bchip_ctx** out) {
     c->name = std::string(prop.name[0] ? prop.name : prop.gcnArchName) + " (" +
               std::to_string(prop.multiProcessorCount) + " CUs)";
     hipError_t e = hipStreamCreateWithFlags(&c->stream, hipStreamNonBlocking);
-    if (e == hipSuccess) e = c->ws.init(device);
+    if (e == hipSuccess) e = c->ws.init(device, c->stream);
     if (e == hipSuccess) {
         // This device's copy of the no-allocation scratch (the device is current here).
         void* sp = nullptr;
@@ -530,15 +541,7 @@ int bchip_matmul(bchip_ctx* c, const void* w, uint32_t type, const float* x, flo
     CHECK(check_span(c, out, sat_mul(n, (uint64_t)rows * 4), "out"));
     // Scratch may not be had: device memory may be full, and nothing can be allocated while the
     // stream is captured. The call then runs without it, to the same bits.
-    auto scratch = [&](size_t bytes) -> void* {
-        if (bytes <= c->ws.vt_bytes) return c->ws.vt;
-        hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-        if (hipStreamIsCapturing(c->stream, &cap) == hipSuccess && cap == hipStreamCaptureStatusNone &&
-            c->ws.reserve_vt(bytes) == hipSuccess)
-            return c->ws.vt;
-        (void)hipGetLastError();
-        return nullptr;
-    };
+    auto scratch = [&](size_t bytes) -> void* { return c->ws.reserve_vt_if(bytes) ? c->ws.vt : nullptr; };
     bool tile = matmul_uses_tile(type, rows, cols, n);
     void* work = tile ? scratch(matmul_scratch_bytes(type, rows, cols, n, true)) : nullptr;
     if (!work) {
@@ -1116,7 +1119,7 @@ int bchip_logprobs(bchip_ctx* c, const float* scores, uint32_t rows, uint32_t vo
     const size_t one = logprobs_scratch_bytes(1, vocab, top);
     const uint32_t most = one ? (uint32_t)std::max<size_t>(1, ((size_t)64 << 20) / one) : rows;
     const uint32_t each = std::min(rows, most);
-    void* scratch = one && c->ws.reserve_vt_if(each * one, c->stream) ? c->ws.vt : nullptr;
+    void* scratch = one && c->ws.reserve_vt_if(each * one) ? c->ws.vt : nullptr;
     for (uint32_t r = 0; r < rows; r += each) {
         const uint32_t n = std::min(each, rows - r);
         HIP_TRY(logprobs_launch(scores + (size_t)r * vocab, n, vocab, temperature, tokens ? tokens + r : nullptr,

@@ -43,7 +43,8 @@ struct Workspace {
     size_t slots = 0, hdp = 0, vt_bytes = 0, qrot_floats = 0;
     bool fixed = false;
     size_t o_cap = 0, ml_cap = 0, qrot_cap = 0;  // fixed: bytes of o, ml and qrot
-    hipError_t init(int device);  // allocates the zero page, the counters and the error word
+    // Allocates the zero page, the counters and the error word for calls on `on`.
+    hipError_t init(int device, hipStream_t on);
     // The fixed view: o, ml and qrot at base (o_bytes, ml_bytes, q_bytes each); the zero page,
     // counters and error word of `owner`.
     void set_fixed(void* base, size_t o_bytes, size_t ml_bytes, size_t q_bytes, const Workspace& owner);
@@ -52,14 +53,17 @@ struct Workspace {
     hipError_t reserve_vt(size_t bytes);
     // The same for a call that has a form without scratch: false where none is to be had, the
     // memory full or the stream captured over a workspace too small (nothing can be allocated
-    // there). Memory that a capture took stays where it is until the context ends: a graph may
-    // be replayed after a larger call has moved the workspace on.
-    bool reserve_if(size_t need_slots, size_t hd_pad, hipStream_t s);
-    bool reserve_vt_if(size_t bytes, hipStream_t s);
-    bool captured = false;
+    // there).
+    bool reserve_if(size_t need_slots, size_t hd_pad);
+    bool reserve_vt_if(size_t bytes);
+    // A block that was handed out while the stream was captured stays where it is until the
+    // context ends: its graph may be replayed after a larger call has moved the workspace on.
+    // Blocks that no capture took are freed when they are outgrown.
+    hipStream_t stream = nullptr;
+    bool o_held = false, vt_held = false, qrot_held = false;  // (o's stands for ml too)
     std::vector<void*> retired;
-    void drop(void* p);
-    bool had(hipStream_t s, bool enough);
+    bool capturing() const;
+    void drop(void* p, bool held);
     void release();
 };
 

@@ -15,6 +15,10 @@
  *  - All kernels run in order on the context's one stream (cuda.rs:40, one stream);
  *    launches return before the work ends; bchip_sync waits (cuda.rs:93). The caller
  *    serialises calls on one context, as the reference's Gpu mutex does (mod.rs:105-107).
+ *  - A context's calls share scratch that grows on demand. What a call took while the stream was
+ *    captured stays valid until the context is destroyed, whichever call outgrows it; what no
+ *    capture took is freed when it is outgrown. A graph's replay uses the same scratch as the
+ *    context's other calls and replays, so they run one after another, not beside each other.
  *  - Element types of cache buffers: BCHIP_F32 (the reference's f32 cache, mod.rs:409-421),
  *    BCHIP_F16 (IEEE binary16, rounded to nearest even: new with this backend) or BCHIP_Q4
  *    (4-bit codes in blocks of 32 that share a scale: 9/32 of an f16 cache's bytes, below).
@@ -161,9 +165,7 @@ int bchip_rope_append(bchip_ctx* ctx, float* q, const float* k, const float* v, 
  * row whose q is not finite NaN; a NaN block of K or V reaches the rows that see its slot, and
  * no other. No slot past the highest that a mask names is read; one past the end of a
  * bchip_alloc buffer is left out. Where scratch cannot be had (memory full, a call under graph
- * capture that has not run before at its size) lists run uncut. Scratch that a captured call
- * took stays valid until the context is destroyed; a replay shares it with the context's other
- * calls and replays, so they run one after another, not beside each other. */
+ * capture that has not run before at its size) lists run uncut. */
 int bchip_attention(bchip_ctx* ctx, const float* q, const void* kc, const void* vc,
                     uint32_t kv_type, float* out, const uint32_t* masks, uint32_t tree,
                     uint32_t rows, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t pos,
@@ -285,8 +287,8 @@ int bchip_rope_append_attention_ragged(bchip_ctx* ctx, float* q, const float* k,
  * row agrees with the same row passed alone within f32 rounding (as the reference's). Reruns
  * give the same bits, also where scratch cannot be had (memory full, a call under graph
  * capture): the call then runs without. The context keeps the scratch of its largest call (prepared
- * x, at most 256 MiB plus its sums and partial sums) until it is destroyed; a larger call replaces
- * it, so a graph captured over calls that use it is replayed only before that. */
+ * x, at most 256 MiB plus its sums and partial sums) until it is destroyed or a larger call
+ * replaces it. */
 int bchip_matmul(bchip_ctx* ctx, const void* w, uint32_t type, const float* x, float* out,
                  uint32_t rows, uint32_t cols, uint32_t n);
 
