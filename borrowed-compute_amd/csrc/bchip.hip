@@ -1115,19 +1115,11 @@ int bchip_logprobs(bchip_ctx* c, const float* scores, uint32_t rows, uint32_t vo
         CHECK(check_span(c, top_ids, (uint64_t)rows * top * 4, "top_ids"));
         CHECK(check_span(c, top_logprobs, (uint64_t)rows * top * 4, "top_logprobs"));
     }
-    // As many rows a launch as keep its scratch small beside the scores.
-    const size_t one = logprobs_scratch_bytes(1, vocab, top);
-    const uint32_t most = one ? (uint32_t)std::max<size_t>(1, ((size_t)64 << 20) / one) : rows;
-    const uint32_t each = std::min(rows, most);
-    void* scratch = one && c->ws.reserve_vt_if(each * one) ? c->ws.vt : nullptr;
-    for (uint32_t r = 0; r < rows; r += each) {
-        const uint32_t n = std::min(each, rows - r);
-        HIP_TRY(logprobs_launch(scores + (size_t)r * vocab, n, vocab, temperature, tokens ? tokens + r : nullptr,
-                                logprob ? logprob + r : nullptr, entropy ? entropy + r : nullptr, top,
-                                top ? top_ids + (size_t)r * top : nullptr, top ? top_logprobs + (size_t)r * top : nullptr,
-                                scratch, c->stream),
-                "logprobs");
-    }
+    const size_t need = logprobs_scratch_bytes(rows, vocab, top);
+    void* scratch = need && c->ws.reserve_vt_if(need) ? c->ws.vt : nullptr;
+    HIP_TRY(logprobs_launch(scores, rows, vocab, temperature, tokens, logprob, entropy, top, top_ids, top_logprobs,
+                            scratch, c->stream),
+            "logprobs");
     return BCHIP_OK;
 }
 

@@ -422,6 +422,8 @@ void lp_plan(uint32_t rows, uint32_t vocab, LpParams& p) {
 
 }  // namespace
 
+// At most 4.2 MB: parts times rows is below 2 LP_GROUPS, and from LP_GROUPS rows on a row has one
+// workgroup and the call no scratch.
 size_t logprobs_scratch_bytes(uint32_t rows, uint32_t vocab, uint32_t top) {
     LpParams p{};
     lp_plan(rows, vocab, p);

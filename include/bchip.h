@@ -326,7 +326,7 @@ int bchip_sample(bchip_ctx* ctx, const float* scores, uint32_t rows, uint32_t vo
  * left out (null, null, 0). f32 sums in a fixed order, one pass over the scores. A score of -inf
  * has probability 0; a row with a NaN, a score of +inf or nothing above -inf gives NaN log
  * probabilities and entropy. rows <= 65535. Takes scratch as bchip_attention does over 4-bit
- * caches. A row's bits depend neither on that nor on the rows beside it. */
+ * caches, at most 4.2 MB. A row's bits depend neither on that nor on the rows beside it. */
 int bchip_logprobs(bchip_ctx* ctx, const float* scores, uint32_t rows, uint32_t vocab, float temperature,
                    const uint32_t* tokens, float* logprob, float* entropy, uint32_t top, uint32_t* top_ids,
                    float* top_logprobs);
