@@ -641,6 +641,7 @@ template <int NB, int RT>
 __global__ __launch_bounds__(RT == 1 ? 512 : 256, 2) void attn_q4_tile(const Q4Params p) {
     constexpr int HD = 32 * NB, NF = 2 * NB, KS = RT == 1 ? 2 : 1;
     constexpr uint32_t QT = 64 * RT;
+    constexpr bool CUT = RT == 1;  // lists may be cut (32 rows a wave are taken where every CU has work)
     using S = Seg<NB>;
     __shared__ struct {
         half8 k[2][4][NB][64], v[2][2][NF][64];
@@ -655,14 +656,16 @@ __global__ __launch_bounds__(RT == 1 ? 512 : 256, 2) void attn_q4_tile(const Q4P
     const uint32_t m16 = lane & 15, g = lane >> 4;
     const Q4Item& it = p.items[0];
     // The longest lists first.
-    const uint32_t kvh = blockIdx.x, chunk = blockIdx.y, qt = p.nqt - 1 - blockIdx.z;
+    const uint32_t kvh = blockIdx.x, chunk = CUT ? blockIdx.y : 0, qt = p.nqt - 1 - blockIdx.z;
     const uint32_t kvd = p.nkv * HD, nq = it.rows * p.G, q0 = qt * QT, q1 = min(q0 + QT, nq);
     const uint32_t r0 = q0 / p.G, h0 = q0 - r0 * p.G;
     const uint32_t seen = p.tree ? it.base : it.base + r0;  // slots every row here sees
     const uint32_t end = p.tree ? tree_end(p, it) : it.base + (q1 - 1) / p.G;
     const uint32_t all = (uint32_t)(((uint64_t)end + Q4_TILE_B - 1) / Q4_TILE_B), t0 = chunk * it.chunk;
     const size_t unit = ((size_t)kvh * p.nqt + qt) * it.nchunk + chunk;
-    if (t0 >= all && it.nchunk > 1) {  // nothing of these rows' lists
+    // Nothing of these rows' lists. (Only cut ones get here; compiled for CUT alone, the other form's loop
+    // is ordered another way and 4096 rows of 32 x 8 heads take 276 us, not 272.)
+    if (t0 >= all && it.nchunk > 1) {
         if (threadIdx.x < QT) *(float2*)(p.part_ml + 2 * (unit * QT + threadIdx.x)) = float2{-INFINITY, 0.0f};
         return;
     }
@@ -874,7 +877,7 @@ __global__ __launch_bounds__(RT == 1 ? 512 : 256, 2) void attn_q4_tile(const Q4P
         l[r] += __shfl_xor(l[r], 32);
         const uint32_t sl = (wave * RT + r) * 16 + m16;
         if (q0 + sl >= nq) continue;
-        if (it.nchunk > 1) {
+        if (CUT && it.nchunk > 1) {
             f32x4* part = (f32x4*)p.part_o + (unit * (QT / 16) + sl / 16) * NF * 64 + lane;
 #pragma unroll
             for (int f = 0; f < NF; f++) part[64 * f] = o[r][f];
@@ -1160,6 +1163,7 @@ hipError_t q4_attention(const AttnCall& a, Workspace& ws, hipStream_t s) {
     p.qt = 64 * rt;
     p.nqt = (uint32_t)((nq + p.qt - 1) / p.qt);
     const uint64_t groups = (uint64_t)p.nqt * a.nkv, tiles = (far + Q4_TILE_B - 1) / Q4_TILE_B;
+    // (attn_q4_tile<., 2> knows whole lists only.)
     cut(it, tiles, rt == 2 ? 1 : tile_chunks(tiles, groups, a.hd), 2, 1);
     if (it.nchunk > 1 && !reserve(p, groups * it.nchunk * p.qt, a.hd, ws)) cut(it, tiles, 1, 2, 1);
 #define Q4_TILES(NB) launch_tile<NB>(p, rt, a, s)
