@@ -118,6 +118,9 @@ def check(code: int) -> None:
 
 
 def esize(t: int) -> int:
+    """Bytes of an element of F32 or F16 (4-bit codes come in whole units: nbytes_of)."""
+    if t not in (F32, F16):
+        raise ValueError(f"an element of type {t} has no size of its own")
     return 2 if t == F16 else 4
 
 
