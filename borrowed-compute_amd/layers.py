@@ -14,6 +14,7 @@ growth, mod.rs:404-423); positions and the tree's visibility masks come from the
 Shape (model.rs:405-443), as in the reference."""
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import ctypes.util
 import math
@@ -82,6 +83,8 @@ class GpuLayers:
     `layers` holds per layer: attn_norm, ffn_norm (f32 vectors), wq, wk, wv, wo, gate, up,
     down (Matrix), and bq, bk, bv (f32 vectors or None). `head` is (output_norm, output)
     or None."""
+
+    SCORE_BYTES = 256 << 20  # of scores that sample and logprobs hold at once
 
     def __init__(self, ctx: bchip.Ctx, cfg: Config, layers: list[dict], head=None, kv_type: int = bchip.F32):
         self.ctx, self.cfg, self.kv_type = ctx, cfg, kv_type
@@ -192,6 +195,31 @@ class GpuLayers:
         scores.free()
         return got
 
+    @contextlib.contextmanager
+    def _score_rows(self, x: np.ndarray, rows: int, upto: int, *words: int):
+        """The logits head of `rows` rows in pieces whose scores take at most SCORE_BYTES (and two rows:
+        a row passed alone may differ in its last bits from the same row in a batch, whose size does not
+        matter). Gives result buffers of `words` u32s each, and an iterator that computes a piece's scores
+        and yields (first row, rows, scores). Every buffer is freed at the end."""
+        norm, out, ty, _, vc = self.head
+        s, ctx, bufs = self._scratch(rows), self.ctx, []
+        ctx.upload(np.ascontiguousarray(x, np.float32), s["x"])
+        ctx.rms_norm(s["x"], norm, s["n"], rows, self.cfg.n_embd, self.cfg.eps)
+        count = max(1, min(-(-rows * upto * 4 // self.SCORE_BYTES), rows // 2))
+        ends = [rows * i // count for i in range(count + 1)]
+
+        def pieces():
+            for r, end in zip(ends, ends[1:]):
+                ctx.matmul(out, ty, s["n"].offset(r * vc * 4), bufs[-1], upto, vc, end - r)
+                yield r, end - r, bufs[-1]
+        try:
+            for n in (*words, max(b - a for a, b in zip(ends, ends[1:])) * upto):
+                bufs.append(ctx.zeros(4 * n))
+            yield bufs[:-1], pieces()
+        finally:
+            for b in bufs:
+                b.free()
+
     def sample(self, x: np.ndarray, rows: int, temperature: float, top_p: float, seed: int, step0: int,
                upto: int | None = None) -> np.ndarray:
         """The last stage's next tokens (engine.rs:341-350): the logits head, then sample.rs's
@@ -199,46 +227,35 @@ class GpuLayers:
         come back to the host, not the rows x vocab scores."""
         if self.head is None:
             raise ValueError("this stage has no output head")
-        norm, out, ty, vr, vc = self.head
+        vr = self.head[3]
         upto = vr if upto is None else min(upto, vr)
-        s = self._scratch(rows)
-        ctx = self.ctx
-        ctx.upload(np.ascontiguousarray(x, np.float32), s["x"])
-        ctx.rms_norm(s["x"], norm, s["n"], rows, self.cfg.n_embd, self.cfg.eps)
-        scores, ids = ctx.zeros(rows * upto * 4), ctx.zeros(rows * 4)
-        ctx.matmul(out, ty, s["n"], scores, upto, vc, rows)
-        ctx.sample(scores, rows, upto, temperature, top_p, seed, step0, ids)
-        got = ctx.read(ids, (rows,), np.uint32)
-        scores.free()
-        ids.free()
-        return got
+        with self._score_rows(x, rows, upto, rows) as ((ids,), pieces):
+            for r, n, scores in pieces:
+                self.ctx.sample(scores, n, upto, temperature, top_p, seed, step0 + r, ids.offset(4 * r))
+            return self.ctx.read(ids, (rows,), np.uint32)
 
     def logprobs(self, x: np.ndarray, rows: int, tokens=None, top: int = 0, temperature: float = 1.0, upto: int | None = None):
         """What the scores of each row say of tokens, on the device (bchip_logprobs): the logits head,
         then the log probability of tokens[r] (None without tokens), the entropy, and the `top` most
-        likely tokens with their log probabilities. Only these come back to the host."""
+        likely tokens with their log probabilities. Only these come back to the host; rows are scored in
+        pieces (SCORE_BYTES), with the same results."""
         if self.head is None:
             raise ValueError("this stage has no output head")
         if tokens is not None and len(tokens) != rows:
             raise ValueError(f"{len(tokens)} tokens for {rows} rows")
-        norm, out, ty, vr, vc = self.head
+        vr = self.head[3]
         upto = vr if upto is None else min(upto, vr)
-        s = self._scratch(rows)
-        ctx = self.ctx
-        ctx.upload(np.ascontiguousarray(x, np.float32), s["x"])
-        ctx.rms_norm(s["x"], norm, s["n"], rows, self.cfg.n_embd, self.cfg.eps)
-        tk = None if tokens is None else ctx.upload(np.ascontiguousarray(tokens, np.uint32))
-        scores, vals, ids = ctx.zeros(rows * upto * 4), ctx.zeros(rows * (2 + top) * 4), ctx.zeros(rows * max(top, 1) * 4)
-        try:
-            ctx.matmul(out, ty, s["n"], scores, upto, vc, rows)
-            ctx.logprobs(scores, rows, upto, temperature, tk, vals if tk else None, vals.offset(rows * 4), top, ids,
-                         vals.offset(2 * rows * 4))
-            got = ctx.read(vals, rows * (2 + top))
-            best = ctx.read(ids, (rows, max(top, 1)), np.uint32)[:, :top]
-        finally:
-            for b in (scores, vals, ids) + ((tk,) if tk else ()):
-                b.free()
-        return (got[:rows] if tk else None), got[rows:2 * rows], best, got[2 * rows:].reshape(rows, top)
+        given = () if tokens is None else (rows,)
+        with self._score_rows(x, rows, upto, rows * (2 + top), rows * top, *given) as ((vals, ids, *tk), pieces):
+            for b in tk:
+                self.ctx.upload(np.ascontiguousarray(tokens, np.uint32), b)
+            for r, n, scores in pieces:
+                given = (tk[0].offset(4 * r), vals.offset(4 * r)) if tk else (None, None)
+                self.ctx.logprobs(scores, n, upto, temperature, *given, vals.offset(4 * (rows + r)), top,
+                                  ids.offset(4 * r * top), vals.offset(4 * (2 * rows + r * top)))
+            got = self.ctx.read(vals, rows * (2 + top))
+            best = self.ctx.read(ids, (rows, top), np.uint32)
+        return (None if tokens is None else got[:rows]), got[rows:2 * rows], best, got[2 * rows:].reshape(rows, top)
 
     def free(self) -> None:
         for l in self.layers:
