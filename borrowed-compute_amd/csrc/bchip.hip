@@ -74,7 +74,9 @@ int fail(int code, const char* fmt, ...) {
     return code;
 }
 
+// The error is reported here: what the runtime still holds of it would fail the next call's launches.
 int hip_fail(hipError_t e, const char* what) {
+    (void)hipGetLastError();
     if (e == hipErrorOutOfMemory) return fail(BCHIP_E_OOM, "%s: %s", what, hipGetErrorString(e));
     return fail(BCHIP_E_HIP, "%s: %s", what, hipGetErrorString(e));
 }

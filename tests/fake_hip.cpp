@@ -21,6 +21,7 @@ std::vector<std::string> launches;
 std::vector<Block> mallocs;
 size_t serial = 0;
 bool capturing = false;
+hipError_t last = hipSuccess;  // of a call that failed, until hipGetLastError takes it
 size_t budget = SIZE_MAX;  // what hipMalloc may still give
 dim3 grid_, block_;
 size_t shared_;
@@ -64,8 +65,8 @@ hipError_t __hipPopCallConfiguration(dim3* g, dim3* b, size_t* shared, hipStream
 }
 
 hipError_t hipMalloc(void** p, size_t n) {
-    if (capturing) return hipErrorStreamCaptureUnsupported;
-    if (n > budget) return hipErrorOutOfMemory;
+    if (capturing) return last = hipErrorStreamCaptureUnsupported;
+    if (n > budget) return last = hipErrorOutOfMemory;
     *p = aligned_alloc(256, (n + 255) / 256 * 256);
     live[*p] = ++serial;
     mallocs.push_back({*p, n, serial});
@@ -98,7 +99,11 @@ hipError_t hipGetDevicePropertiesR0600(hipDeviceProp_tR0600* p, int) {
     p->multiProcessorCount = 256;
     return hipSuccess;
 }
-hipError_t hipGetLastError() { return hipSuccess; }
+hipError_t hipGetLastError() {
+    const hipError_t e = last;
+    last = hipSuccess;
+    return e;
+}
 const char* hipGetErrorString(hipError_t) { return "an error"; }
 
 hipError_t hipStreamCreateWithFlags(hipStream_t* s, unsigned) { return *s = (hipStream_t)&stream_, hipSuccess; }
