@@ -147,8 +147,7 @@ int check_span(const bchip_ctx* c, const void* p, uint64_t bytes, const char* wh
     return check_at(c, p, 0, bytes, what);
 }
 
-// Bytes of n elements of a type (a 4-bit cache: whole units), and the types that bchip_fill_normal
-// takes, or a cache may have.
+// Bytes of n elements of a type (a 4-bit cache: whole units), and the last type that a cache may have.
 uint64_t bytes_of(uint32_t type, uint64_t n) {
     if (type == BCHIP_Q4) return n > UINT64_MAX - Q4_UNIT ? UINT64_MAX : sat_mul((n + Q4_UNIT - 1) / Q4_UNIT, Q4_UNIT_BYTES);
     return sat_mul(n, type == BCHIP_F16 ? 2u : 4u);

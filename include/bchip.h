@@ -29,11 +29,12 @@
  *    the unit's eight blocks of 32 elements. An element is (code - 8) * scale. The library writes
  *    as a block's scale the value of its largest magnitude over -8 (of two, the positive one),
  *    rounded to 7 significant bits and held within 2^-14 .. 896 (values past 7168 saturate), and
- *    as a code the value over the scale to the nearest even; a block with an element that is not
- *    finite gets the scale NaN and reads as NaN. A buffer written elsewhere has to keep to such
- *    scales. Element offsets, counts and row widths are multiples of 32, and cache calls take
- *    head dims that are multiples of 32, slots of at most 2^20 elements and lists of at most
- *    2^32 - 256 slots (else BCHIP_E_UNSUPPORTED).
+ *    as a code the value times the scale's reciprocal, both rounded to f32, to the nearest even (so a
+ *    value is at most 1/2 + 2^-20 scales from its code's, where nothing saturates); a block with
+ *    an element that is not finite gets the scale NaN and reads as NaN. A buffer written elsewhere
+ *    has to keep to such scales. Element offsets, counts and row widths are multiples of 32, and cache
+ *    calls take head dims that are multiples of 32, slots of at most 2^20 elements and lists of at
+ *    most 2^32 - 256 slots (else BCHIP_E_UNSUPPORTED).
  */
 #ifndef BCHIP_H
 #define BCHIP_H
