@@ -32,9 +32,12 @@
  *    as a code the value times the scale's reciprocal, both rounded to f32, to the nearest even (so a
  *    value is at most 1/2 + 2^-20 scales from its code's, where nothing saturates); a block with
  *    an element that is not finite gets the scale NaN and reads as NaN. A buffer written elsewhere
- *    has to keep to such scales. Element offsets, counts and row widths are multiples of 32, and cache
- *    calls take head dims that are multiples of 32, slots of at most 2^20 elements and lists of at
- *    most 2^32 - 256 slots (else BCHIP_E_UNSUPPORTED).
+ *    has to keep to such scales. A pointer to 4-bit codes is the start of a buffer or of one of
+ *    its units, which the library cannot tell from the address (a bchip_alloc block may hold
+ *    several buffers): an address inside a unit reads and writes other bytes than meant. Element
+ *    offsets, counts and row widths are multiples of 32, and cache calls take head dims that are
+ *    multiples of 32, slots of at most 2^20 elements and lists of at most 2^32 - 256 slots (else
+ *    BCHIP_E_UNSUPPORTED).
  */
 #ifndef BCHIP_H
 #define BCHIP_H
@@ -101,7 +104,8 @@ int bchip_rope(bchip_ctx* ctx, float* x, const float* inv_freq, const uint32_t* 
 /* k_copy (kernels.h:332, entry cuda.cu:90; mod.rs:413-420, 473-475):
  * dst[dst_off + i] = src[i] for i < n (element offsets and counts), converting from
  * src_type to dst_type (f32 -> f16 rounds to nearest even; to and from 4-bit codes as above:
- * an f16 holds every 4-bit value exactly). */
+ * an f16 holds every 4-bit value exactly). A 4-bit src is read from the start of a unit: a row
+ * that starts inside one comes with the elements of its unit before it. */
 int bchip_copy(bchip_ctx* ctx, const void* src, uint32_t src_type, void* dst,
                uint32_t dst_type, uint64_t dst_off, uint64_t n);
 
