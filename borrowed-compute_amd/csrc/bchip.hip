@@ -713,7 +713,7 @@ int bchip_attention(bchip_ctx* c, const float* q, const void* kc, const void* vc
     if (!q || !kc || !vc || !out) return fail(BCHIP_E_ARG, "null pointer");
     if (kv_type > LAST_TYPE) return fail(BCHIP_E_ARG, "element type %u", kv_type);
     CHECK(check_heads(nh, nkv, hd));
-    if (kv_type == BCHIP_Q4) CHECK(check_q4(nkv, hd, (uint64_t)pos + rows));
+    if (kv_type == BCHIP_Q4) CHECK(check_q4(nkv, hd, (uint64_t)pos + (tree ? MAX_ITEMS : rows)));
     if (!aligned16(q) || !aligned16(out) || !aligned16(kc) || !aligned16(vc))
         return fail(BCHIP_E_ARG, "q, out and the caches must be 16-byte aligned");
     if ((uint64_t)pos + rows > 0xffffffffull) return fail(BCHIP_E_ARG, "position past 2^32");

@@ -36,8 +36,8 @@
  *    its units, which the library cannot tell from the address (a bchip_alloc block may hold
  *    several buffers): an address inside a unit reads and writes other bytes than meant. Element
  *    offsets, counts and row widths are multiples of 32, and cache calls take head dims that are
- *    multiples of 32, slots of at most 2^20 elements and lists of at most 2^32 - 256 slots (else
- *    BCHIP_E_UNSUPPORTED).
+ *    multiples of 32, slots of at most 2^20 elements and lists of at most 2^32 - 256 slots, in a
+ *    tree pos + 64 (else BCHIP_E_UNSUPPORTED).
  */
 #ifndef BCHIP_H
 #define BCHIP_H

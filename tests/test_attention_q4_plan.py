@@ -51,3 +51,15 @@ def test_a_tree_of_many_heads_takes_whole_lists(fake):
 got = kernels(64, 768, 48, 96, 70, tree=True)
 assert got == [("tile", 3, 2, 48, 1, 8)], got
 """)
+
+
+def test_a_tree_whose_masks_could_name_slots_past_the_longest_list_is_refused(fake):
+    """A mask names slots up to 63 behind pos; lists reach slot 2^32 - 256 at most. What was named past
+    that was left out in silence."""
+    host_side.run(fake, SETUP + """
+most = (1 << 32) - 256
+kernels(2, 1, 1, 32, most - 64, tree=True)
+kernels(2, 1, 1, 32, most - 2)
+refused(bchip.E_UNSUPPORTED, lambda: kernels(2, 1, 1, 32, most - 63, tree=True))
+refused(bchip.E_UNSUPPORTED, lambda: kernels(2, 1, 1, 32, most - 1))
+""")
