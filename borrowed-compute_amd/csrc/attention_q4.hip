@@ -197,8 +197,12 @@ __device__ __forceinline__ f16 load_scale(q4_rsrc r, uint32_t at) {
 // One head's part of SLOTS slots of K or V on its way into LDS: a thread takes blocks of a slot,
 // 16 bytes of codes and their scale, so consecutive lanes read consecutive bytes (loads of a few
 // bytes a lane at the operands' own places cost the memory path 30 to 60 cycles each). In LDS a slot
-// takes SLOT bytes, its codes and then its scales: an odd multiple of 16 for heads of 64 to 256,
-// so the operands' lanes read every bank once.
+// takes SLOT bytes, its codes and then its scales. For heads of 64, 128, 192 and 256 that is an odd
+// multiple of 16, so the operands' lanes read every bank once. For heads of an odd number of blocks it is
+// 32, 64, 96 or 128, and a group's lanes share banks (four of them start the 16 slots of heads of 96, two
+// those of 224), a word at a time: 16 x 4 heads of 96, 160 and 224 take 9.1, 11.0 and 18.2 us for a step at
+// 512 slots, the next even ones 8.0, 11.2 and 11.9; 2000 rows 60, 79 and 123, the next ones 60, 83 and 98.
+// (Heads of 224 also spill: a vector register in a step's short form.)
 template <int NB, int SLOTS, int THREADS>
 struct Raw {
     static constexpr int SLOT = 16 * NB + 16, BYTES = SLOT * SLOTS;
@@ -386,13 +390,16 @@ __device__ __forceinline__ uint64_t q4_bytes(uint64_t slots, uint32_t rem, uint3
     return (slots * kvd + rem + Q4_UNIT - 1) / Q4_UNIT * Q4_UNIT_BYTES;
 }
 
-// What bounds it, measured at 32 x 8 heads of 128. Long lists: a tile is some 300 vector instructions
-// a wave, most of them unpacking, against 256 cycles of MFMA; at 131072 slots the arithmetic alone takes
-// 25 us and the loads alone 25, and two waves a SIMD overlap them to 40 (3.8 TB/s; the call 44). At 32768
-// slots 14.4 (the call 17.4). Short ones: the chain from the launch over q, the first tile and the states
-// to the result, 7.4 us at 1000 slots. Tried: two tiles on their way to a wave instead of one (15.1 us for
-// 14.5 at 32768, and spills for heads past 160); operands read from memory where the lanes need them
-// (1.6 times the time a tile); 1024 workgroups (two more waves a SIMD: 16.1 and 44.5 us, the states double).
+// What bounds it, measured at 32 x 8 heads of 128, calls one after another over four layers' caches. Long
+// lists: a tile is some 300 vector instructions a wave, most of them unpacking, against 256 cycles of MFMA;
+// at 131072 slots the arithmetic alone takes 25 us and the loads alone 25, and two waves a SIMD overlap
+// them to 41 (3.7 TB/s; the call 45). At 32768 slots 14.6 (the call 17.5; 19.7 where other caches come in
+// between and nothing of these is left in the memory-side cache). Short ones: the chain from the launch over
+// q, the first tile and the states to the result, 6.8 us at 1000 slots. Tried: two tiles on their way to a wave
+// instead of one (15.1 us for 14.5 at 32768, and spills for heads past 160); operands read from memory where
+// the lanes need them (1.6 times the time a tile); three waves a SIMD, the most that 155 registers allow
+// (768 workgroups: 42.0 us at 131072 and the call 47.0, the states half as many again; 1024 are a second
+// round for the last 256: 43.5 and 47.7).
 template <int NB, bool PK, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void attn_q4_row(const Q4Params p) {
     constexpr int HD = 32 * NB, NF = 2 * NB, QW = NB < WAVES ? NB : WAVES, QJ = (NB + WAVES - 1) / WAVES;
@@ -631,8 +638,9 @@ constexpr int Q4_WAVES = 4;
 // query rows each: four of 32 rows, or eight of 16, of which four take each half of the slots.
 //
 // What bounds it. Prompts: the matrix cores, which q's and the weights' two parts give twice the work:
-// 4096 rows of 32 x 8 heads of 128 take 283 us, 485 TFLOP/s of the 549 that half of a large f16 product's
-// rate leaves. Verify passes: latency. 8 rows of 64 x 8 heads at 5003 slots take 14 us, of which the first
+// 4096 rows of 32 x 8 heads of 128 take 272 to 278 us in a row of calls, 283 with other inputs in between: 485 to
+// 505 TFLOP/s of the 549 that half of a large f16 product's rate leaves. Verify passes: latency. 8 rows of 64
+// x 8 heads at 5003 slots take 14.6 us (the call 18.6), of which the first
 // tile's way in some 6, three tiles 0.85 each (two barriers a tile) and 7 MB of states 1.5; eight waves
 // a workgroup instead of four took 2 us off, 32 rows a wave there would leave half of the waves idle.
 constexpr uint32_t Q4_TILE_B = 64;
@@ -1019,7 +1027,8 @@ Q4Params params(const AttnCall& a) {
 }
 
 // Workgroups of attn_q4_row that keep the GPU busy without more states than they are worth: two a CU (a
-// step of 32 x 8 heads of 128 at 32768 slots: 18.0 us at 512, 20.7 at 256, 21.4 at 1024).
+// step of 32 x 8 heads of 128 at 131072 slots: 45.5 us at 512 and at 256, 47.0 at 768, 47.7 at 1024; at 32768
+// 17.5 at 512, which Q4_FOLD_CHUNKS holds it to, 17.0 at 256).
 constexpr uint32_t Q4_ROW_GROUPS = 512;
 // Lists of several lengths end at different times: more workgroups (16 of 28 x 4 heads of 128 at 1 to 16384
 // slots: 38 us at 768, 46 at 512, 40 at 1024).
@@ -1031,7 +1040,7 @@ constexpr uint32_t Q4_RAGGED_GROUPS = 768;
 constexpr uint32_t Q4_BRIEF = 20;
 
 // Chunks that attn_q4_fold reads at once, and the tiles a chunk past them is worth (28 x 4 heads of 128 at
-// 24000 slots: 13.4 us in 62 chunks, 15.2 in 125).
+// 24000 slots: 12.5 us in 63 chunks, 14.7 in 94).
 constexpr uint32_t Q4_FOLD_CHUNKS = 64, Q4_FOLD_TILES = 16;
 
 // Chunks for a list of `tiles` tiles, `least` at least a chunk, for `want` of them; of multiples of `of` (a
@@ -1157,7 +1166,7 @@ hipError_t q4_attention(const AttnCall& a, Workspace& ws, hipStream_t s) {
         return hipSuccess;
     }
     // 32 query rows a wave halve the LDS reads a product, where enough such workgroups keep every CU busy
-    // (32 x 8 heads of 128, 4096 rows: 271 us, 397 with 16; 1000 rows: 51, 39 with 16; they meet at 1300.
+    // (32 x 8 heads of 128, 4096 rows, in a row of calls: 272 us, 397 with 16; 1000 rows: 51, 39 with 16; they meet at 1300.
     // Heads of 64 read less: 14 x 2 of them, 4096 rows, 124 us and 100 with 16, 8192 rows 314 and 329).
     const uint32_t rt = a.hd <= 128 && (nq + 127) / 128 * a.nkv >= (a.hd > 64 ? 352u : 768u) ? 2 : 1;
     p.qt = 64 * rt;
