@@ -49,6 +49,8 @@
 extern "C" {
 #endif
 
+/* BCHIP_Q4 and bchip_logprobs were added under version 6: a program that may meet an older library of
+ * that version looks bchip_logprobs up before it uses either. */
 #define BCHIP_ABI_VERSION 6
 
 enum bchip_type { BCHIP_F32 = 0, BCHIP_F16 = 1, BCHIP_Q4 = 2 }; /* T_F32 / T_F16 of kernels.h:14-15 */

@@ -118,3 +118,24 @@ clear()
 small()
 assert not mallocs()
 """)
+
+
+def test_where_memory_is_full_lists_run_whole(fake):
+    """A call whose scratch cannot be had runs without it, one after it that can takes it again, and a
+    graph's block is not given up for an attempt that fails."""
+    host_side.run(fake, SETUP + """
+small, large, lp, mm = attention(bchip.Q4, 1, 3000), attention(bchip.Q4, 1, 120000), logprobs(3, 70000, 20), matmul(300)
+took = blocks(small)
+with capturing():
+    small()
+fake.fake_budget(1000)
+for call, most in ((large, 1), (lp, 1), (mm, None)):
+    got = blocks(call)
+    assert not got and (most is None or len(launches()) == most), launches()
+fake.fake_budget(1 << 40)
+assert all(live(m) for m in took), "the graph's block was freed"
+for call in (small, large, lp):
+    clear()
+    call()
+    assert len(launches()) == 2, launches()  # the fold, the join
+""")
