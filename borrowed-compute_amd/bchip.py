@@ -88,6 +88,10 @@ def lib() -> ctypes.CDLL:
         "bchip_rope_append_ragged": ([P, P, P, P, P, P, u32, P, P, P, P, u32, u32, u32, u32, u32, u32], i32),
         "bchip_rope_append_attention_ragged": ([P, P, P, P, P, P, u32, P, P, P, P, u32, u32, u32, u32, u32, u32, f32,
                                                 P], i32),
+        "bchip_rope_append_paged": ([P, P, P, P, P, P, u32, P, P, P, P, P, u32, u32, u32, u32, u32, u32, u32, u32, u32], i32),
+        "bchip_attention_paged": ([P, P, P, P, u32, P, P, P, P, u32, u32, u32, u32, u32, u32, u32, f32], i32),
+        "bchip_copy_pages": ([P, P, u32, u32, u64, u32, P, P, u32], i32),
+        "bchip_beam_select": ([P, P, P, u32, u32, u32, u32, P, P, P], i32),
         "bchip_fill_normal": ([P, P, u32, u64, u64], i32),
         "bchip_sample": ([P, P, u32, u32, f32, f32, u64, u64, P], i32),
         "bchip_logprobs": ([P, P, u32, u32, f32, P, P, P, u32, P, P], i32),
@@ -286,6 +290,31 @@ class Ctx:
                                                        offs.ctypes.data_as(ctypes.c_void_p), len(lens), nh, nkv, hd,
                                                        rope_dim, int(neox), scale, _ptr(out)))
 
+    def rope_append_paged(self, q, k, v, kc, vc, kv_type, inv_freq, positions, row_starts, seq_lens, pages, page_stride,
+                          page_slots, npages, nh, nkv, hd, rope_dim, neox) -> None:
+        """rope_append of several sequences' rows to a cache in pages: sequence i's rows are row_starts[i] ..
+        row_starts[i + 1] - 1 and the last of its seq_lens[i] slots; pages: device u32 [nseq][page_stride]."""
+        starts, lens = _batch(row_starts, seq_lens)
+        check(lib().bchip_rope_append_paged(self.h, _ptr(q), _ptr(k), _ptr(v), _ptr(kc), _ptr(vc), kv_type, _ptr(inv_freq),
+                                            _ptr(positions), starts.ctypes.data, lens.ctypes.data, _ptr(pages), page_stride,
+                                            page_slots, npages, len(lens), nh, nkv, hd, rope_dim, int(neox)))
+
+    def attention_paged(self, q, kc, vc, kv_type, out, row_starts, seq_lens, pages, page_stride, page_slots, npages, nh, nkv,
+                        hd, scale) -> None:
+        """Attention of several sequences' new rows over a cache in pages (arguments as rope_append_paged)."""
+        starts, lens = _batch(row_starts, seq_lens)
+        check(lib().bchip_attention_paged(self.h, _ptr(q), _ptr(kc), _ptr(vc), kv_type, _ptr(out), starts.ctypes.data,
+                                          lens.ctypes.data, _ptr(pages), page_stride, page_slots, npages, len(lens), nh, nkv,
+                                          hd, scale))
+
+    def copy_pages(self, bufs, t, page_elems, npages, src, dst) -> None:
+        """Page dst[i] becomes page src[i] in every buffer of a pool, pages of page_elems elements of type t."""
+        arr = (ctypes.c_void_p * len(bufs))(*[_ptr(b) for b in bufs])
+        s, d = np.ascontiguousarray(src, np.uint32), np.ascontiguousarray(dst, np.uint32)
+        if s.shape != d.shape or s.ndim != 1:
+            raise ValueError(f"{s.shape} source pages for {d.shape} destinations")
+        check(lib().bchip_copy_pages(self.h, arr, len(bufs), t, page_elems, npages, s.ctypes.data, d.ctypes.data, len(s)))
+
     def matmul(self, w, wtype, x, out, rows, cols, n) -> None:
         check(lib().bchip_matmul(self.h, _ptr(w), wtype, _ptr(x), _ptr(out), rows, cols, n))
 
@@ -311,6 +340,11 @@ class Ctx:
         [rows][vocab]; tokens and logprob, entropy, and the last two may be None (top 0)."""
         check(lib().bchip_logprobs(self.h, _ptr(scores), rows, vocab, temperature, _ptr(tokens), _ptr(logprob), _ptr(entropy),
                                    top, _ptr(top_ids), _ptr(top_logprobs)))
+
+    def beam_select(self, scores, sums, batch, beams, vocab, k, best, beam, token) -> None:
+        """The k best continuations of each of `batch` beam searches, from device f32 scores [batch * beams][vocab]
+        and the beams' sums [batch][beams]: their scores, beams and tokens, device [batch][k]."""
+        check(lib().bchip_beam_select(self.h, _ptr(scores), _ptr(sums), batch, beams, vocab, k, _ptr(best), _ptr(beam), _ptr(token)))
 
     def fill_normal(self, dst, t, n, seed) -> None:
         check(lib().bchip_fill_normal(self.h, _ptr(dst), t, n, seed))
@@ -378,6 +412,14 @@ class KvCache:
         for b in self.k + self.v:
             b.free()
         self.k, self.v, self.cap = [], [], 0
+
+
+def _batch(row_starts, seq_lens):
+    """The host arrays of a call over pages: one more start than lengths."""
+    starts, lens = np.ascontiguousarray(row_starts, np.uint32), np.ascontiguousarray(seq_lens, np.uint32)
+    if len(starts) != len(lens) + 1:
+        raise ValueError(f"{len(starts)} row starts for {len(lens)} sequences (one more is needed)")
+    return starts, lens
 
 
 def _ptr(x):

@@ -1,0 +1,753 @@
+// Attention over a cache in pages (paged.hpp) of many query rows a KV head: prompts, pieces of them,
+// verify passes; the fold of chunks, and the plan of a call.
+//
+// Mathematics and layout as in attention_paged_row.hip. A workgroup takes 64 or 128 query rows of one
+// KV head and its waves share each tile of K and V, two of which are in LDS: the next one arrives
+// while this one is computed.
+#include "internal.hpp"
+#include "paged.hpp"
+#include "paged_launch.hpp"
+#include "parts.hpp"
+
+#include <algorithm>
+#include <vector>
+
+namespace bchip {
+
+namespace {
+
+// A block of query rows: q0 .. q1 - 1 of a KV head's (rows x G), its tiles t0 .. t1 - 1.
+struct PgBlock {
+    uint32_t kvh, q0, q1, r0, h0, seen, end, nchunk, t0, t1;
+    size_t unit;  // of its first 16 query rows' states
+    size_t next;  // from 16 query rows to the next
+};
+
+template <uint32_t QT, uint32_t SLOTS>
+__device__ __forceinline__ PgBlock block_of(const PgParams& p, const PgItem& it, uint32_t block) {
+    PgBlock b;
+    const uint32_t rows = it.rows_seq >> 8, nq = rows * p.G, nqt = (nq - 1) / QT + 1, local = block - it.block0;
+    b.kvh = blockIdx.x % p.nkv;
+    const uint32_t qt = nqt - 1 - local % nqt, chunk = local / nqt;  // the longest lists first
+    b.q0 = qt * QT;
+    b.q1 = min(b.q0 + QT, nq);
+    b.r0 = b.q0 / p.G;
+    b.h0 = b.q0 - b.r0 * p.G;
+    b.seen = it.len - rows + b.r0 + 1;                // slots that every row here sees,
+    b.end = it.len - rows + (b.q1 - 1) / p.G + 1;     // and the last one
+    b.nchunk = ((it.len - 1) / SLOTS) / p.chunk + 1;
+    const uint32_t all = (b.end - 1) / SLOTS + 1;
+    b.t0 = min(chunk * p.chunk, all);
+    b.t1 = min(b.t0 + p.chunk, all);
+    b.next = b.nchunk;
+    b.unit = ((size_t)it.block0 * p.nkv + (size_t)b.kvh * nqt * b.nchunk + (size_t)qt * b.nchunk) * (QT / 16) + chunk;
+    return b;
+}
+
+// A block's 16 query rows from `first`: this lane's row.
+struct PgRow {
+    bool valid;
+    uint32_t vis;  // slots it sees
+    size_t at;     // its elements of q and out
+};
+__device__ __forceinline__ PgRow row_of(const PgParams& p, const PgItem& it, const PgBlock& b, uint32_t i) {
+    const uint32_t y = b.h0 + i, dr = (y * (65536 / p.G + 1)) >> 16;  // y / G
+    const bool valid = b.q0 + i < b.q1;
+    const uint32_t row = it.row0 + b.r0 + (valid ? dr : 0), head = b.kvh * p.G + (valid ? y - dr * p.G : 0);
+    return PgRow{valid, valid ? b.seen + dr : b.end, ((size_t)row * p.nh + head) * p.hd};
+}
+
+// Every wave's LDS writes and reads are done, its loads have arrived.
+__device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// f16 caches. RT 2: four waves of 32 query rows; RT 1: eight waves, four of them 16 query rows each over
+// half of a tile's slots and four the same rows over the other half.
+template <int NB, int RT>
+__global__ __launch_bounds__(RT == 1 ? 512 : 256, 2) void attn_paged_tile16(const PgParams p) {
+    using T = PgTile<f16, NB>;
+    constexpr int NF = 2 * NB, KS = RT == 1 ? 2 : 1;
+    constexpr uint32_t QT = 64 * RT, SLOTS = 64;
+    __shared__ __attribute__((aligned(16))) uint8_t kt[2][4 * T::GRANULE];
+    __shared__ __attribute__((aligned(16))) uint8_t vt[2][4 * T::GRANULE];
+    __shared__ uint32_t odd_tile[2];  // 1 + the tile of each buffer whose V holds an infinity or a NaN
+    static_assert(KS == 1 || sizeof kt >= sizeof(f32x4) * 4 * NF * 64, "the second waves' states");
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) & 3);
+    const uint32_t ks = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    const uint32_t m16 = lane & 15, g = lane >> 4;
+    const uint32_t block = blockIdx.x / p.nkv;
+    const PgItem& it = p.items[item_of<false>(p, block)];
+    const PgBlock b = block_of<QT, SLOTS>(p, it, block);
+    if (b.t0 >= b.t1) {  // nothing of these rows' lists
+        if (threadIdx.x < QT) {
+            const size_t u = b.unit + threadIdx.x / 16 * b.next;
+            *(float2*)(p.part_ml + 2 * (u * 16 + (threadIdx.x & 15))) = float2{-INFINITY, 0.0f};
+        }
+        return;
+    }
+    PgList list = list_of(p, it, b.kvh, 2);
+    list.end = b.end;
+
+    // A wave brings granule `wave` of a tile, K's and V's (KS 2: K's or V's).
+    uint32_t kfrom[T::LOADS], vfrom[KS == 1 ? T::LOADS : 1], page;
+#pragma unroll
+    for (int i = 0; i < T::LOADS; i++) {
+        kfrom[i] = KS == 2 && ks ? T::template from<true>(i, lane, list.row_bytes, p.hd * 2) : T::template from<false>(i, lane, list.row_bytes, p.hd * 2);
+        if constexpr (KS == 1) vfrom[i] = T::template from<true>(i, lane, list.row_bytes, p.hd * 2);
+    }
+    const uint32_t kl = (uint32_t)(uintptr_t)(pg_lds*)&kt[0][0], vl = (uint32_t)(uintptr_t)(pg_lds*)&vt[0][0];
+    auto look = [&](uint32_t t) { page = list.page(t * SLOTS + 16 * wave); };
+    auto fetch = [&](uint32_t t, uint32_t buf) {
+        const uint32_t slot = t * SLOTS + 16 * wave, at = buf * 4 * T::GRANULE + wave * T::GRANULE;
+        const bool k = KS == 1 || !ks, v = KS == 1 || ks;
+        if (k && list.bad(slot, page)) {  // a page past the pool: the rows that see its slots are NaN
+#pragma unroll
+            for (int i = 0; i < T::LOADS; i++) *(pg_u32x4*)(&kt[0][0] + at + 1024 * i + 16 * lane) = pg_u32x4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
+        } else if (k) {
+            const pg_u32x4 r = list.granule(p.kc, slot, page);
+#pragma unroll
+            for (int i = 0; i < T::LOADS; i++) load_lds(r, kfrom[i], kl + at + 1024 * i);
+        }
+        if (v) {
+            const pg_u32x4 r = list.granule(p.vc, slot, page);
+#pragma unroll
+            for (int i = 0; i < T::LOADS; i++) load_lds(r, KS == 1 ? vfrom[KS == 1 ? i : 0] : kfrom[i], vl + at + 1024 * i);
+        }
+    };
+    look(b.t0);
+    if (threadIdx.x < 2) odd_tile[threadIdx.x] = 0;
+
+    PgRow row[RT];
+    half8 qh[RT][NB], ql[RT][NB];
+    float c[RT];
+    {
+        float x[RT][NB][8];
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            row[r] = row_of(p, it, b, (wave * RT + r) * 16 + m16);
+#pragma unroll
+            for (int j = 0; j < NB; j++) {
+                const uint32_t d = 32 * j + 8 * g;
+                f32x4 lo{0, 0, 0, 0}, hi{0, 0, 0, 0};
+                if (row[r].valid && d < p.hd) {
+                    lo = *(const f32x4*)(p.q + row[r].at + d);
+                    hi = *(const f32x4*)(p.q + row[r].at + d + 4);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[r][j][e] = e < 4 ? lo[e & 3] : hi[e & 3];
+            }
+        }
+        fetch(b.t0, 0);
+        look(b.t0 + 1);
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            float top = 0.0f, k;
+#pragma unroll
+            for (int j = 0; j < NB; j++) top = q_top(x[r][j], top);
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            q_scale(top, p.sc, k, c[r]);
+#pragma unroll
+            for (int j = 0; j < NB; j++) q_parts(x[r][j], k, qh[r][j], ql[r][j]);
+        }
+    }
+    uint32_t kat[NB], vat[NF];
+#pragma unroll
+    for (int j = 0; j < NB; j++) kat[j] = T::at(m16, 4 * j + g, T::turn_k(m16));
+    {
+        const uint32_t slot = 4 * g + (m16 >> 2);
+#pragma unroll
+        for (int f = 0; f < NF; f++) vat[f] = T::at(slot, 2 * f + ((m16 >> 1) & 1), T::turn_v(slot)) + 8 * (m16 & 1);
+    }
+
+    f32x4 o[RT][NF];
+    float ref[RT], l[RT];
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+        ref[r] = -INFINITY;
+        l[r] = 0.0f;
+#pragma unroll
+        for (int f = 0; f < NF; f++) o[r][f] = f32x4{0, 0, 0, 0};
+    }
+    for (uint32_t t = b.t0; t < b.t1; t++) {
+        const uint32_t buf = (t - b.t0) & 1, ts = t * SLOTS;
+        tile_barrier();
+        if (t + 1 < b.t1) {
+            fetch(t + 1, buf ^ 1);
+            look(t + 2);
+        }
+        const uint8_t *kb = kt[buf], *vb = vt[buf];
+        const bool edge = ts + SLOTS > b.seen;
+        if (edge && b.seen < b.end) {
+            // Some row does not see all of the tile: an infinity or a NaN in V, which a weight of 0
+            // would not silence, reaches the rows that see its slot and is 0 from then on.
+            constexpr int EACH = 4 * T::GRANULE / (16 * 256 * KS);
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < EACH; i++) {
+                const pg_u32x4 w = *(const pg_u32x4*)(vb + 16 * (threadIdx.x + 256 * KS * i));
+                odd = odd || odd16(w.x) || odd16(w.y) || odd16(w.z) || odd16(w.w);
+            }
+            if (odd) odd_tile[buf] = t + 1;
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+            if (odd_tile[buf] == t + 1) {
+                for (uint32_t i = KS == 2 ? 32 * ks : 0; i < (KS == 2 ? 32 * ks + 32 : 64u); i++)
+#pragma unroll
+                    for (int f = 0; f < NF; f++) {
+                        const half4 v = *(const half4*)(vb + (i >> 4) * T::GRANULE + T::at(i & 15, 2 * f + (g >> 1), T::turn_v(i)) + 8 * (g & 1));
+#pragma unroll
+                        for (int r = 0; r < RT; r++)
+                            if (ts + i < row[r].vis)
+#pragma unroll
+                                for (int e = 0; e < 4; e++)
+                                    if (odd16(__builtin_bit_cast(uint16_t, v[e]))) o[r][f][e] = NAN;
+                    }
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+                __builtin_amdgcn_s_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+                for (int i = 0; i < EACH; i++) {
+                    pg_u32x4* at = (pg_u32x4*)(vb + 16 * (threadIdx.x + 256 * KS * i));
+                    pg_u32x4 w = *at;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        if ((w[e] & 0x7c00u) == 0x7c00u) w[e] &= 0xffff0000u;
+                        if ((w[e] & 0x7c000000u) == 0x7c000000u) w[e] &= 0xffffu;
+                    }
+                    *at = w;
+                }
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+                __builtin_amdgcn_s_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2 / KS; i++) {
+            const uint32_t u = KS == 2 ? ks : i;  // 32 of the tile's slots
+            // (Four sums in turn, so that no MFMA waits for the one before: one set of rows takes the
+            // parts of q apart.)
+            constexpr bool APART = RT == 1;
+            f32x4 s[RT][2], s2[2];
+#pragma unroll
+            for (int r = 0; r < RT; r++) s[r][0] = s[r][1] = s2[0] = s2[1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < NB; j++) {
+                const half8 k0 = *(const half8*)(kb + 2 * u * T::GRANULE + kat[j]), k1 = *(const half8*)(kb + (2 * u + 1) * T::GRANULE + kat[j]);
+#pragma unroll
+                for (int r = 0; r < RT; r++) {
+                    s[r][0] = mfma16(k0, qh[r][j], s[r][0]);
+                    s[r][1] = mfma16(k1, qh[r][j], s[r][1]);
+                }
+#pragma unroll
+                for (int r = 0; r < RT; r++) {
+                    f32x4(&to)[2] = APART ? s2 : s[r];
+                    to[0] = mfma16(k0, ql[r][j], to[0]);
+                    to[1] = mfma16(k1, ql[r][j], to[1]);
+                }
+            }
+            half8 ph[RT], pl[RT];
+#pragma unroll
+            for (int r = 0; r < RT; r++) {
+                if (APART) {
+                    s[r][0] += s2[0];
+                    s[r][1] += s2[1];
+                }
+                if (edge)
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (ts + 32 * u + 16 * (e >> 2) + 4 * g + (e & 3) >= row[r].vis) s[r][e >> 2][e & 3] = -INFINITY;
+                float f;
+                if (raise(s[r], c[r], ref[r], f)) {
+                    l[r] *= f;
+#pragma unroll
+                    for (int k = 0; k < NF; k++) o[r][k] *= f;
+                }
+                weights<false>(s[r], c[r], ref[r], 0.0f, l[r], ph[r], pl[r]);
+            }
+            const uint8_t* vu = vb + 2 * u * T::GRANULE;
+#pragma unroll
+            for (int f = 0; f < NF; f += 2) {
+                half8 v[2];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const half4 x = read_transposed(vu + vat[f + e]), y = read_transposed(vu + T::GRANULE + vat[f + e]);
+                    v[e] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+                }
+#pragma unroll
+                for (int r = 0; r < RT; r++) {
+                    o[r][f] = mfma16(v[0], ph[r], o[r][f]);
+                    o[r][f + 1] = mfma16(v[1], ph[r], o[r][f + 1]);
+                }
+#pragma unroll
+                for (int r = 0; r < RT; r++) {
+                    o[r][f] = mfma16(v[0], pl[r], o[r][f]);
+                    o[r][f + 1] = mfma16(v[1], pl[r], o[r][f + 1]);
+                }
+            }
+        }
+    }
+
+    if constexpr (KS == 2) {  // the two halves of the slots
+        f32x4(*so)[NF][64] = (f32x4(*)[NF][64]) & kt;
+        float(*sr)[2][64] = (float(*)[2][64]) & vt;
+        __syncthreads();
+        if (ks) {
+            sr[wave][0][lane] = ref[0];
+            sr[wave][1][lane] = l[0];
+#pragma unroll
+            for (int f = 0; f < NF; f++) so[wave][f][lane] = o[0][f];
+        }
+        __syncthreads();
+        if (ks) return;
+        const float other = sr[wave][0][lane], R2 = fmaxf(ref[0], other), Rs = R2 == -INFINITY ? 0.0f : R2;
+        const float a = exp2_hw(ref[0] - Rs), e = exp2_hw(other - Rs);
+        ref[0] = R2;
+        l[0] = l[0] * a + sr[wave][1][lane] * e;
+#pragma unroll
+        for (int f = 0; f < NF; f++) o[0][f] = o[0][f] * a + so[wave][f][lane] * e;
+    }
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+        l[r] += __shfl_xor(l[r], 16);
+        l[r] += __shfl_xor(l[r], 32);
+        if (!row[r].valid) continue;
+        if (b.nchunk > 1) {
+            const size_t u = b.unit + (wave * RT + r) * b.next;
+            f32x4* part = (f32x4*)p.part_o + u * NF * 64 + lane;
+#pragma unroll
+            for (int f = 0; f < NF; f++) part[64 * f] = o[r][f];
+            if (g == 0) *(float2*)(p.part_ml + 2 * (u * 16 + m16)) = float2{ref[r], l[r]};
+            continue;
+        }
+        const float k = 1.0f / l[r];
+#pragma unroll
+        for (int f = 0; f < NF; f++) {
+            const uint32_t d = 16 * f + 4 * g;
+            if (d < p.hd) *(f32x4*)(p.out + row[r].at + d) = o[r][f] * k;
+        }
+    }
+}
+
+// f32 caches: four waves of 16 query rows, tiles of 32 slots.
+template <int NB>
+__global__ __launch_bounds__(256, NB > 4 ? 1 : 2) void attn_paged_tile32(const PgParams p) {
+    using T = PgTile<float, NB>;
+    constexpr int NF = 2 * NB, NJ = 2 * NB, NS = NB / 2, TAIL = NB % 2;
+    constexpr uint32_t QT = 64, SLOTS = 32;
+    __shared__ __attribute__((aligned(16))) uint8_t kt[2][2 * T::GRANULE];
+    __shared__ __attribute__((aligned(16))) uint8_t vt[2][2 * T::GRANULE];
+    __shared__ uint32_t odd_tile[2];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t m16 = lane & 15, g = lane >> 4;
+    const uint32_t block = blockIdx.x / p.nkv;
+    const PgItem& it = p.items[item_of<false>(p, block)];
+    const PgBlock b = block_of<QT, SLOTS>(p, it, block);
+    if (b.t0 >= b.t1) {
+        if (threadIdx.x < QT) {
+            const size_t u = b.unit + threadIdx.x / 16 * b.next;
+            *(float2*)(p.part_ml + 2 * (u * 16 + (threadIdx.x & 15))) = float2{-INFINITY, 0.0f};
+        }
+        return;
+    }
+    PgList list = list_of(p, it, b.kvh, 4);
+    list.end = b.end;
+
+    // Two waves bring a tile's two granules of K, two V's.
+    const uint32_t half = wave & 1;
+    uint32_t from[T::LOADS], page;
+#pragma unroll
+    for (int i = 0; i < T::LOADS; i++)
+        from[i] = wave < 2 ? T::template from<false>(i, lane, list.row_bytes, p.hd * 4) : T::template from<true>(i, lane, list.row_bytes, p.hd * 4);
+    const uint32_t kl = (uint32_t)(uintptr_t)(pg_lds*)&kt[0][0], vl = (uint32_t)(uintptr_t)(pg_lds*)&vt[0][0];
+    auto look = [&](uint32_t t) { page = list.page(t * SLOTS + 16 * half); };
+    auto fetch = [&](uint32_t t, uint32_t buf) {
+        const uint32_t slot = t * SLOTS + 16 * half, at = buf * 2 * T::GRANULE + half * T::GRANULE;
+        if (wave < 2 && list.bad(slot, page)) {  // a page past the pool: the rows that see its slots are NaN
+#pragma unroll
+            for (int i = 0; i < T::LOADS; i++) *(f32x4*)(&kt[0][0] + at + 1024 * i + 16 * lane) = f32x4{NAN, NAN, NAN, NAN};
+        } else {
+            const pg_u32x4 r = list.granule(wave < 2 ? p.kc : p.vc, slot, page);
+            const uint32_t to = (wave < 2 ? kl : vl) + at;
+#pragma unroll
+            for (int i = 0; i < T::LOADS; i++) load_lds(r, from[i], to + 1024 * i);
+        }
+    };
+    look(b.t0);
+    if (threadIdx.x < 2) odd_tile[threadIdx.x] = 0;
+    const PgRow row = row_of(p, it, b, wave * 16 + m16);
+    f32x4 q[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; j++) q[j] = row.valid && 16 * j + 4 * g < p.hd ? *(const f32x4*)(p.q + row.at + 16 * j + 4 * g) : f32x4{0, 0, 0, 0};
+    fetch(b.t0, 0);
+    look(b.t0 + 1);
+    uint32_t kat[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; j++) kat[j] = T::at(m16, 4 * j + g, T::turn_k(m16));
+
+    f32x4 o[NF];
+#pragma unroll
+    for (int f = 0; f < NF; f++) o[f] = f32x4{0, 0, 0, 0};
+    float ref = -INFINITY, l = 0.0f;
+    for (uint32_t t = b.t0; t < b.t1; t++) {
+        const uint32_t buf = (t - b.t0) & 1, ts = t * SLOTS;
+        tile_barrier();
+        if (t + 1 < b.t1) {
+            fetch(t + 1, buf ^ 1);
+            look(t + 2);
+        }
+        const uint8_t *kb = kt[buf], *vb = vt[buf];
+        const bool edge = ts + SLOTS > b.seen;
+        if (edge && b.seen < b.end) {  // (as in attn_paged_tile16)
+            constexpr int EACH = 2 * T::GRANULE / (16 * 256);
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < EACH; i++) {
+                const pg_u32x4 w = *(const pg_u32x4*)(vb + 16 * (threadIdx.x + 256 * i));
+                odd = odd || odd32(w.x) || odd32(w.y) || odd32(w.z) || odd32(w.w);
+            }
+            if (odd) odd_tile[buf] = t + 1;
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+            if (odd_tile[buf] == t + 1) {
+                for (uint32_t i = 0; i < SLOTS && ts + i < row.vis; i++)
+#pragma unroll
+                    for (int f = 0; f < NF; f++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (odd32(*(const uint32_t*)(vb + i * T::PITCH + 4 * dim_of<float, NB>(f, g, e)))) o[f][e] = NAN;
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+                __builtin_amdgcn_s_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+                for (int i = 0; i < EACH; i++) {
+                    pg_u32x4* at = (pg_u32x4*)(vb + 16 * (threadIdx.x + 256 * i));
+                    pg_u32x4 w = *at;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) w[e] = odd32(w[e]) ? 0u : w[e];
+                    *at = w;
+                }
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+                __builtin_amdgcn_s_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+            }
+        }
+        f32x4 s[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            f32x4 a[4] = {};
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                const f32x4 k = *(const f32x4*)(kb + h * T::GRANULE + kat[j]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) a[e] = mfma_f32(k[e], q[j][e], a[e]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                s[h][i] = ((a[0][i] + a[1][i]) + (a[2][i] + a[3][i])) * p.sc;
+                if (edge && ts + 16 * h + 4 * g + i >= row.vis) s[h][i] = -INFINITY;
+            }
+        }
+        float f;
+        if (raise(s, 1.0f, ref, f)) {
+            l *= f;
+#pragma unroll
+            for (int k = 0; k < NF; k++) o[k] *= f;
+        }
+        const float base = ref == -INFINITY ? 0.0f : ref;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                s[h][i] = exp2_hw(s[h][i] - base);
+                l += s[h][i];
+            }
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint8_t* at = vb + (16 * h + 4 * g + i) * T::PITCH;
+#pragma unroll
+                for (int z = 0; z < NS; z++) {
+                    const f32x4 v = *(const f32x4*)(at + 256 * z + 16 * m16);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[4 * z + e] = mfma_f32(v[e], s[h][i], o[4 * z + e]);
+                }
+                if constexpr (TAIL) {
+                    const f32x2 v = *(const f32x2*)(at + 256 * NS + 8 * m16);
+#pragma unroll
+                    for (int e = 0; e < 2; e++) o[4 * NS + e] = mfma_f32(v[e], s[h][i], o[4 * NS + e]);
+                }
+            }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (!row.valid) return;
+    if (b.nchunk > 1) {
+        const size_t u = b.unit + wave * b.next;
+        f32x4* part = (f32x4*)p.part_o + u * NF * 64 + lane;
+#pragma unroll
+        for (int f = 0; f < NF; f++) part[64 * f] = o[f];
+        if (g == 0) *(float2*)(p.part_ml + 2 * (u * 16 + m16)) = float2{ref, l};
+        return;
+    }
+    const float k = 1.0f / l;
+#pragma unroll
+    for (int z = 0; z < NS; z++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t d = 64 * z + 16 * g + 4 * i;
+            if (d < p.hd) *(f32x4*)(p.out + row.at + d) = f32x4{o[4 * z][i], o[4 * z + 1][i], o[4 * z + 2][i], o[4 * z + 3][i]} * k;
+        }
+    if constexpr (TAIL)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t d = 64 * NS + 8 * g + 2 * i;
+            if (d < p.hd) *(f32x2*)(p.out + row.at + d) = f32x2{o[4 * NS][i], o[4 * NS + 1][i]} * k;
+        }
+}
+
+// The chunks of 16 query rows of a list brought together, one operand's columns a workgroup, each wave a
+// share of the chunks; states lie as their waves held them. A chunk without a weight left its columns
+// unwritten.
+template <typename KVT, int NB, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void attn_paged_fold(const PgParams p) {
+    constexpr int NF = 2 * NB, AHEAD = 8;
+    __shared__ f32x4 sum[WAVES][64];
+    __shared__ float sr[WAVES][64], sl[WAVES][64];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m16 = lane & 15, g = lane >> 4;
+    const uint32_t f = blockIdx.z, kvh = blockIdx.y;
+    const PgItem& it = p.items[item_of<true>(p, blockIdx.x)];
+    const uint32_t slots = p.qt == 16 ? (sizeof(KVT) == 2 ? 32 : 16) : (sizeof(KVT) == 2 ? 64 : 32);  // of a tile
+    const uint32_t rows = it.rows_seq >> 8, nq = rows * p.G, groups = ((nq - 1) / p.qt + 1) * (p.qt / 16);
+    const uint32_t chunks = ((it.len - 1) / slots) / p.chunk + 1, group = blockIdx.x - it.fold0, n = 16 * group + m16;
+    const bool valid = n < nq;
+    const size_t u0 = (size_t)it.block0 * p.nkv * (p.qt / 16) + ((size_t)kvh * groups + group) * chunks;
+    const float2* ml = (const float2*)p.part_ml + u0 * 16 + m16;
+    const f32x4* at = (const f32x4*)p.part_o + (u0 * NF + f) * 64 + lane;
+    f32x4 a = {0, 0, 0, 0};
+    float R = -INFINITY, L = 0.0f;
+    for (uint32_t c0 = wave; c0 < chunks; c0 += AHEAD * WAVES) {
+        float2 s[AHEAD];
+        f32x4 x[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            const uint32_t c = c0 + i * WAVES;
+            const bool there = valid && c < chunks;
+            s[i] = there ? ml[(size_t)c * 16] : float2{-INFINITY, 0.0f};
+            x[i] = there ? at[(size_t)c * NF * 64] : f32x4{0, 0, 0, 0};
+        }
+        float to = R;
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) to = fmaxf(to, s[i].x);
+        const float ts = to == -INFINITY ? 0.0f : to, w = exp2_hw(R - ts);
+        a *= w;
+        L *= w;
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            const float e = exp2_hw(s[i].x - ts);
+            L += e * s[i].y;
+            a += s[i].y == 0.0f ? f32x4{0, 0, 0, 0} : e * x[i];
+        }
+        R = to;
+    }
+    if constexpr (WAVES > 1) {
+        sr[wave][lane] = R;
+        sl[wave][lane] = L;
+        sum[wave][lane] = a;
+        __syncthreads();
+        if (wave > 0) return;
+        for (int w = 1; w < WAVES; w++) R = fmaxf(R, sr[w][lane]);
+        const float Rs = R == -INFINITY ? 0.0f : R;
+        a = f32x4{0, 0, 0, 0};
+        L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            const float e = exp2_hw(sr[w][lane] - Rs);
+            L += e * sl[w][lane];
+            a += e * sum[w][lane];
+        }
+    }
+    if (!valid) return;
+    const float k = 1.0f / L;
+    const uint32_t r = n / p.G;
+    float* dst = p.out + ((size_t)(it.row0 + r) * p.nh + kvh * p.G + n - r * p.G) * p.hd;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; i++) {
+        const uint32_t d = dim_of<KVT, NB>(f, g, i);
+        if (d < p.hd) dst[d] = a[i] * k;
+    }
+}
+
+template <typename KVT, int NB>
+void launch_fold(const PgParams& p, uint32_t groups, uint32_t most, hipStream_t s) {
+    // A wave alone holds a few chunks' states at once; more chunks are shared out.
+    const dim3 grid(groups, p.nkv, 2 * NB);
+    if (most <= 8) hipLaunchKernelGGL((attn_paged_fold<KVT, NB, 1>), grid, dim3(64), 0, s, p);
+    else hipLaunchKernelGGL((attn_paged_fold<KVT, NB, 8>), grid, dim3(512), 0, s, p);
+}
+
+template <int NB>
+void launch_tile16(const PgParams& p, hipStream_t s) {
+    const dim3 grid(p.blocks * p.nkv);
+    if constexpr (NB <= 4) {
+        if (p.qt == 128) {
+            hipLaunchKernelGGL((attn_paged_tile16<NB, 2>), grid, dim3(256), 0, s, p);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((attn_paged_tile16<NB, 1>), grid, dim3(512), 0, s, p);
+}
+template <int NB>
+void launch_tile32(const PgParams& p, hipStream_t s) {
+    hipLaunchKernelGGL((attn_paged_tile32<NB>), dim3(p.blocks * p.nkv), dim3(256), 0, s, p);
+}
+
+uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
+
+// What a launch over p's items (block rows p.qt, tiles of `slots` slots) takes in chunks of p.chunk
+// tiles: their places, the states, and the groups of the fold (which gives its own places to items
+// whose lists are whole, none of them).
+struct PgPlan {
+    uint64_t states = 0;  // groups of 16 query rows
+    uint32_t groups = 0, most = 1;
+};
+PgPlan place(PgParams& p, uint32_t slots) {
+    PgPlan plan;
+    p.blocks = 0;
+    for (uint32_t i = 0; i < p.nitems; i++) {
+        PgItem& it = p.items[i];
+        const uint32_t nq = (it.rows_seq >> 8) * p.G, nqt = ceil_div(nq, p.qt), chunks = (it.len - 1) / slots / p.chunk + 1;
+        it.block0 = p.blocks;
+        it.fold0 = plan.groups;
+        p.blocks += nqt * chunks;
+        if (chunks > 1) plan.groups += ceil_div(nq, 16);
+        plan.most = std::max(plan.most, chunks);
+    }
+    plan.states = (uint64_t)p.blocks * p.nkv * (p.qt / 16);
+    return plan;
+}
+
+bool reserve(PgParams& p, const PgPlan& plan, Workspace& ws) {
+    const uint32_t hd = p.hd;  // (states are those of the kernel's head, at most the next power of two)
+    const bool had = ws.reserve_if(plan.states * 16, hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256);
+    p.part_o = ws.o;
+    p.part_ml = ws.ml;
+    return had;
+}
+
+constexpr uint32_t WHOLE = 0x40000000u;  // tiles: no list has as many
+
+// Items of at most 16 query rows.
+hipError_t run_rows(PgParams& p, bool f16_cache, Workspace& ws, hipStream_t s) {
+    const uint32_t slots = pg_row_tile(f16_cache);
+    uint64_t total = 0, most = 0;
+    for (uint32_t i = 0; i < p.nitems; i++) {
+        const uint64_t tiles = (p.items[i].len - 1) / slots + 1;
+        total += tiles;
+        most = std::max(most, tiles);
+    }
+    p.qt = 16;
+    // Lists that eight waves take in a few tiles each are not cut: no second launch.
+    const bool brief = most <= 20;
+    p.chunk = brief ? WHOLE : std::max<uint32_t>(4, ceil_div(ceil_div(total * p.nkv, 512), 4) * 4);
+    PgPlan plan = place(p, slots);
+    if (plan.groups && !reserve(p, plan, ws)) {  // whole lists
+        p.chunk = WHOLE;
+        plan = place(p, slots);
+    }
+    paged_rows_launch(p, f16_cache, brief, s);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !plan.groups) return e;
+    paged_fold_launch(p, f16_cache, plan.groups, plan.most, s);
+    return hipGetLastError();
+}
+
+// Items of more.
+hipError_t run_tiles(PgParams& p, bool f16_cache, Workspace& ws, hipStream_t s) {
+    const uint32_t slots = pg_tile(f16_cache);
+    std::sort(p.items, p.items + p.nitems, [](const PgItem& a, const PgItem& b) { return a.len > b.len; });
+    uint64_t big = 0;
+    for (uint32_t i = 0; i < p.nitems; i++) big += ceil_div((uint64_t)(p.items[i].rows_seq >> 8) * p.G, 128) * (uint64_t)p.nkv;
+    p.qt = f16_cache && p.hd <= 128 && big >= 352 ? 128 : 64;
+    uint64_t work = 0, units = 0, longest = 0;  // tiles of the query blocks, as many as there are, the longest list's
+    for (uint32_t i = 0; i < p.nitems; i++) {
+        const PgItem& it = p.items[i];
+        const uint64_t rows = it.rows_seq >> 8, n = ceil_div(rows * p.G, p.qt) * (uint64_t)p.nkv;
+        units += n;
+        work += n * (((uint64_t)it.len - rows / 2) / slots + 1);
+        longest = std::max<uint64_t>(longest, (it.len - 1) / slots + 1);
+    }
+    constexpr uint64_t CUS = 256;
+    const float tile = 0.6f + 0.006f * p.hd, launch = 2.0f + 0.0006f * p.hd * units, states = 64.0f * 8.0f / 5e6f * p.hd * units;
+    auto time = [&](uint64_t chunk, uint64_t n) {
+        return (std::max((float)work / CUS, (float)chunk) + (float)chunk * 0.25f) * tile + 7.0f + (n > 1 ? launch + states * n : 0.0f);
+    };
+    p.chunk = WHOLE;
+    float least = time(longest, 1);
+    for (uint64_t n = 2; n <= 64 && longest / n >= 2; n++) {
+        const uint64_t chunk = ceil_div(longest, n);
+        if (time(chunk, n) < least) {
+            least = time(chunk, n);
+            p.chunk = (uint32_t)chunk;
+        }
+    }
+    PgPlan plan = place(p, slots);
+    if (plan.groups && !reserve(p, plan, ws)) {
+        p.chunk = WHOLE;
+        plan = place(p, slots);
+    }
+    paged_tiles_launch(p, f16_cache, s);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !plan.groups) return e;
+    paged_fold_launch(p, f16_cache, plan.groups, plan.most, s);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+void paged_tiles_launch(const PgParams& p, bool f16_cache, hipStream_t s) {
+#define PG_TILE(NB) (f16_cache ? launch_tile16<NB>(p, s) : launch_tile32<NB>(p, s))
+    PG_BY_DIM(p.hd, PG_TILE)
+#undef PG_TILE
+}
+
+void paged_fold_launch(const PgParams& p, bool f16_cache, uint32_t groups, uint32_t most, hipStream_t s) {
+#define PG_FOLD(NB) (f16_cache ? launch_fold<f16, NB>(p, groups, most, s) : launch_fold<float, NB>(p, groups, most, s))
+    PG_BY_DIM(p.hd, PG_FOLD)
+#undef PG_FOLD
+}
+
+hipError_t paged_attention(const PagedCall& a, Workspace& ws, hipStream_t s) {
+    const bool f16_cache = a.kv_type == 1;
+    PgParams base{};
+    base.q = a.q;
+    base.kc = (const uint8_t*)a.kc;
+    base.vc = (const uint8_t*)a.vc;
+    base.out = a.out;
+    base.pages = a.pages.table;
+    base.page_stride = a.pages.stride;
+    base.page_shift = a.pages.shift;
+    base.npages = a.pages.npages;
+    base.nh = a.nh;
+    base.nkv = a.nkv;
+    base.hd = a.hd;
+    base.G = a.nh / a.nkv;
+    base.sc = a.scale * LOG2E;
+    for (int many = 0; many < 2; many++) {
+        PgParams p = base;
+        for (uint32_t i = 0; i <= a.pages.nseq; i++) {
+            if (p.nitems == PG_ITEMS || (i == a.pages.nseq && p.nitems)) {
+                const hipError_t e = many ? run_tiles(p, f16_cache, ws, s) : run_rows(p, f16_cache, ws, s);
+                if (e != hipSuccess) return e;
+                p.nitems = 0;
+            }
+            if (i == a.pages.nseq) break;
+            const uint32_t rows = a.pages.starts[i + 1] - a.pages.starts[i];
+            if (rows == 0 || ((uint64_t)rows * base.G > 16) != (many == 1)) continue;
+            p.items[p.nitems++] = PgItem{a.pages.starts[i], a.pages.lens[i], rows << 8 | i, 0, 0};
+        }
+    }
+    return hipSuccess;
+}
+
+}  // namespace bchip

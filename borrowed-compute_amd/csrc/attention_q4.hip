@@ -27,6 +27,7 @@
 // Chunks of a list meet in attn_q4_fold.
 #include "common.hpp"
 #include "internal.hpp"
+#include "parts.hpp"
 #include "q4.hpp"
 
 #include <hip/hip_ext.h>
@@ -64,9 +65,6 @@ struct Q4Params {
 };
 
 namespace {
-
-constexpr float Q4_BIAS = 11.0f;  // log2 of the weight of a row's largest score when ref is set
-constexpr float Q4_MOST = 15.0f;  // of any weight: an f16 holds it
 
 // The constants of the unpacking, in registers so that one instruction takes both.
 struct Q4Bits {
@@ -143,11 +141,6 @@ __device__ __forceinline__ void unpack_v(const Q4Bits& b, const uint32_t (&raw)[
     for (int k = 0; k < W; k++) out[k] = as_half8(r[k][0], r[k][1], r[k][2], r[k][3]);
 }
 
-// The larger of two, a number before a NaN: fmaxf without the quieting of its operands.
-__device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
-
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-
 // Eight dims of a query row from `at`, in the order of a K word's.
 __device__ __forceinline__ void q_load(const float* at, bool valid, float (&x)[8]) {
     float4 a{}, b{};
@@ -157,31 +150,6 @@ __device__ __forceinline__ void q_load(const float* at, bool valid, float (&x)[8
     }
     x[0] = a.x, x[1] = b.x, x[2] = a.y, x[3] = b.y, x[4] = a.z, x[5] = b.z, x[6] = a.w, x[7] = b.w;
 }
-// The largest magnitude of them and `top`.
-__device__ __forceinline__ float q_top(const float (&x)[8], float top) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) top = larger(top, fabsf(x[i]));
-    return top;
-}
-
-// From a row's largest |q|: q times k is q scale log2 e brought to 2^13 .. 2^14, c takes it back.
-__device__ __forceinline__ void q_scale(float top, float sc, float& k, float& c) {
-    int e = (int)(__float_as_uint(top * fabsf(sc)) >> 23) - 127;  // (of an infinity 128: its row is NaN)
-    e = e < -100 ? -100 : e;
-    k = sc * __uint_as_float((uint32_t)(13 - e + 127) << 23);
-    c = __uint_as_float((uint32_t)(e - 13 + 127) << 23);
-}
-
-__device__ __forceinline__ void q_parts(const float (&x)[8], float k, half8& hi, half8& lo) {
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        const half2 h = __builtin_convertvector((f32x2{x[i] * k, x[i + 1] * k}), half2);
-        const half2 r = __builtin_convertvector((f32x2{__builtin_fmaf(x[i], k, -(float)h[0]), __builtin_fmaf(x[i + 1], k, -(float)h[1])}), half2);
-        hi[i] = h[0], hi[i + 1] = h[1];
-        lo[i] = r[0], lo[i + 1] = r[1];
-    }
-}
-
 // A list's codes and scales are read through buffer descriptors that end with its last slot's
 // unit: what a tile reaches past that comes back as zero, whatever lies there.
 typedef __amdgpu_buffer_rsrc_t q4_rsrc;
@@ -339,48 +307,6 @@ __device__ __forceinline__ uint32_t tree_end(const Q4Params& p, const Q4Item& it
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
     return __builtin_amdgcn_readfirstlane((uint32_t)min((uint64_t)it.base + top, p.slot_limit));
-}
-
-// A row's scores are c s (c a power of two), its weights 2^(c s - ref). Where some score of these
-// 32 slots passes ref by more than Q4_MOST, the refs rise to Q4_BIAS under their rows' maxima (to
-// the maxima themselves where those are so large that the difference would be lost), and what
-// was summed against the old one is to be multiplied by f.
-__device__ __forceinline__ bool raise(const f32x4 (&s)[2], float c, float& ref, float& f) {
-    float top = larger(larger(larger(s[0][0], s[0][1]), larger(s[0][2], s[0][3])),
-                       larger(larger(s[1][0], s[1][1]), larger(s[1][2], s[1][3]))) * c;
-    if (!__any(top > ref + Q4_MOST)) return false;
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    const float to = fmaxf(ref, fabsf(top) < 0x1p23f ? top - Q4_BIAS : top);
-    f = to == -INFINITY ? 1.0f : exp2_hw(ref - to);
-    ref = to;
-    return true;
-}
-
-// The weights' B operand, the rounded values (hi) and the rest (lo); their sum goes to l. With
-// PART, hi comes back as the rounded values times 1 - keep plus the rest times keep (0 or 1): a
-// lane holds one part.
-template <bool PART>
-__device__ __forceinline__ void weights(const f32x4 (&s)[2], float c, float ref, float keep, float& l, half8& hi, half8& lo) {
-    const float base = ref == -INFINITY ? 0.0f : ref;
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        const float w0 = exp2_hw(__builtin_fmaf(s[i >> 2][i & 3], c, -base));
-        const float w1 = exp2_hw(__builtin_fmaf(s[i >> 2][(i & 3) + 1], c, -base));
-        l += w0;
-        l += w1;
-        const half2 h = __builtin_convertvector((f32x2{w0, w1}), half2);
-        const float k = PART ? -keep : -1.0f;
-        const half2 r = __builtin_convertvector((f32x2{__builtin_fmaf((float)h[0], k, w0), __builtin_fmaf((float)h[1], k, w1)}), half2);
-        hi[i] = PART ? r[0] : h[0];
-        hi[i + 1] = PART ? r[1] : h[1];
-        lo[i] = r[0];
-        lo[i + 1] = r[1];
-    }
-}
-
-__device__ __forceinline__ float ror8(float x) {  // lane n of each 16 gets lane (n + 8) % 16's
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false));
 }
 
 constexpr uint32_t Q4_TILE = 32;

@@ -16,6 +16,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <map>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -1073,6 +1074,134 @@ int bchip_rope_append_attention_ragged(bchip_ctx* c, float* q, const float* k, c
         HIP_TRY(row_attention_fused_items(a, r, items, ns, c->ws, c->stream), "rope_append_attention_ragged");
         a.ev_before = a.ev_after = nullptr;
     }
+    return BCHIP_OK;
+}
+
+// What the calls over a cache in pages ask of their batch and pool; b is filled in. Every page that the
+// table may name lies inside both buffers, and the entries that are read inside the table.
+static int check_paged(const bchip_ctx* c, const void* kc, const void* vc, uint32_t kv_type, const uint32_t* row_starts,
+                       const uint32_t* seq_lens, const uint32_t* pages, uint32_t page_stride, uint32_t page_slots,
+                       uint32_t npages, uint32_t nseq, uint32_t nh, uint32_t nkv, uint32_t hd, PagedBatch& b) {
+    if (kv_type > LAST_TYPE) return fail(BCHIP_E_ARG, "element type %u", kv_type);
+    if (kv_type == BCHIP_Q4) return fail(BCHIP_E_UNSUPPORTED, "a cache in pages holds f32 or f16");
+    CHECK(check_heads(nh, nkv, hd));
+    if ((uint64_t)nkv * hd > (1u << 20) || nkv > 65535)
+        return fail(BCHIP_E_UNSUPPORTED, "%u KV heads of %u (a slot in pages holds at most 2^20 elements and 65535 heads)", nkv, hd);
+    if (!aligned16(kc) || !aligned16(vc)) return fail(BCHIP_E_ARG, "the caches must be 16-byte aligned");
+    if ((uintptr_t)pages % 4) return fail(BCHIP_E_ARG, "the page table must be 4-byte aligned");
+    if (nseq > 256) return fail(BCHIP_E_ARG, "%u sequences (at most 256)", nseq);
+    if (page_slots < 16 || page_slots > (1u << 20) || (page_slots & (page_slots - 1)))
+        return fail(BCHIP_E_UNSUPPORTED, "pages of %u slots (a power of two from 16 to 2^20)", page_slots);
+    if (npages == 0) return fail(BCHIP_E_ARG, "a pool of no pages");
+    if (row_starts[0] != 0) return fail(BCHIP_E_ARG, "the first sequence's rows start at %u", row_starts[0]);
+    b = PagedBatch{row_starts, seq_lens, nseq, pages, page_stride, (uint32_t)__builtin_ctz(page_slots), npages};
+    for (uint32_t i = 0; i < nseq; i++) {
+        if (row_starts[i + 1] < row_starts[i]) return fail(BCHIP_E_ARG, "sequence %u's rows end before they start", i);
+        const uint32_t rows = row_starts[i + 1] - row_starts[i];
+        if (rows == 0) continue;
+        if (seq_lens[i] < rows) return fail(BCHIP_E_ARG, "sequence %u: %u rows of %u slots", i, rows, seq_lens[i]);
+        if (seq_lens[i] > Q4_SLOTS) return fail(BCHIP_E_UNSUPPORTED, "sequence %u: a list of %u slots (at most 2^32 - 256)", i, seq_lens[i]);
+        const uint32_t held = (seq_lens[i] - 1) / page_slots + 1;
+        if (held > page_stride) return fail(BCHIP_E_ARG, "sequence %u: %u slots, but %u pages of %u a line of the table", i, seq_lens[i], page_stride, page_slots);
+        CHECK(check_span(c, pages, ((uint64_t)i * page_stride + held) * 4, "pages"));
+    }
+    const uint64_t rows = row_starts[nseq];
+    if (rows >= (1u << 24) || sat_mul(rows, nh) >= (1ull << 31)) return fail(BCHIP_E_UNSUPPORTED, "%llu rows of %u heads (fewer than 2^24, of 2^31 heads)", (unsigned long long)rows, nh);
+    const uint64_t pool = bytes_of(kv_type, sat_mul(sat_mul(npages, page_slots), (uint64_t)nkv * hd));
+    CHECK(check_span(c, kc, pool, "kc"));
+    CHECK(check_span(c, vc, pool, "vc"));
+    return BCHIP_OK;
+}
+
+int bchip_rope_append_paged(bchip_ctx* c, float* q, const float* k, const float* v, void* kc, void* vc, uint32_t kv_type,
+                            const float* inv_freq, const uint32_t* positions, const uint32_t* row_starts,
+                            const uint32_t* seq_lens, const uint32_t* pages, uint32_t page_stride, uint32_t page_slots,
+                            uint32_t npages, uint32_t nseq, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t rope_dim,
+                            uint32_t neox) {
+    CHECK(enter(c));
+    if (nseq == 0) return BCHIP_OK;
+    if (!q || !k || !v || !kc || !vc || !inv_freq || !positions || !row_starts || !seq_lens || !pages)
+        return fail(BCHIP_E_ARG, "null pointer");
+    PagedBatch b;
+    CHECK(check_paged(c, kc, vc, kv_type, row_starts, seq_lens, pages, page_stride, page_slots, npages, nseq, nh, nkv, hd, b));
+    if (rope_dim % 2 || rope_dim > hd) return fail(BCHIP_E_ARG, "rope_dim %u for head_dim %u", rope_dim, hd);
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v)) return fail(BCHIP_E_ARG, "q, k and v must be 16-byte aligned");
+    const uint64_t rows = row_starts[nseq], kvd = (uint64_t)nkv * hd;
+    CHECK(check_span(c, q, sat_mul(sat_mul(rows, nh), (uint64_t)hd * 4), "q"));
+    CHECK(check_span(c, k, sat_mul(rows, kvd * 4), "k"));
+    CHECK(check_span(c, v, sat_mul(rows, kvd * 4), "v"));
+    CHECK(check_span(c, positions, rows * 4, "positions"));
+    CHECK(check_span(c, inv_freq, (uint64_t)(rope_dim / 2) * 4, "inv_freq"));
+    HIP_TRY(rope_append_paged_launch(q, k, v, kc, vc, kv_type, inv_freq, positions, b, nh, nkv, hd, rope_dim, neox, c->stream),
+            "rope_append_paged");
+    return BCHIP_OK;
+}
+
+int bchip_attention_paged(bchip_ctx* c, const float* q, const void* kc, const void* vc, uint32_t kv_type, float* out,
+                          const uint32_t* row_starts, const uint32_t* seq_lens, const uint32_t* pages, uint32_t page_stride,
+                          uint32_t page_slots, uint32_t npages, uint32_t nseq, uint32_t nh, uint32_t nkv, uint32_t hd,
+                          float scale) {
+    CHECK(enter(c));
+    if (nseq == 0) return BCHIP_OK;
+    if (!q || !kc || !vc || !out || !row_starts || !seq_lens || !pages) return fail(BCHIP_E_ARG, "null pointer");
+    PagedCall a{q, kc, vc, kv_type, out, {}, nh, nkv, hd, scale};
+    CHECK(check_paged(c, kc, vc, kv_type, row_starts, seq_lens, pages, page_stride, page_slots, npages, nseq, nh, nkv, hd, a.pages));
+    if (!aligned16(q) || !aligned16(out)) return fail(BCHIP_E_ARG, "q and out must be 16-byte aligned");
+    const uint64_t bytes = sat_mul(sat_mul(row_starts[nseq], nh), (uint64_t)hd * 4);
+    CHECK(check_span(c, q, bytes, "q"));
+    CHECK(check_span(c, out, bytes, "out"));
+    HIP_TRY(paged_attention(a, c->ws, c->stream), "attention_paged");
+    return BCHIP_OK;
+}
+
+int bchip_copy_pages(bchip_ctx* c, void* const* bufs, uint32_t nbufs, uint32_t type, uint64_t page_elems, uint32_t npages,
+                     const uint32_t* src, const uint32_t* dst, uint32_t n) {
+    CHECK(enter(c));
+    if (nbufs == 0 || n == 0) return BCHIP_OK;
+    if (!bufs || !src || !dst) return fail(BCHIP_E_ARG, "null pointer");
+    if (type > LAST_TYPE) return fail(BCHIP_E_ARG, "element type %u", type);
+    if (type == BCHIP_Q4) return fail(BCHIP_E_UNSUPPORTED, "a cache in pages holds f32 or f16");
+    const uint64_t bytes = bytes_of(type, page_elems);
+    if (bytes == 0 || bytes % 16 || bytes > (1ull << 40)) return fail(BCHIP_E_ARG, "pages of %llu elements: not whole 16-byte pieces, up to 2^40 bytes", (unsigned long long)page_elems);
+    for (uint32_t b = 0; b < nbufs; b++) {
+        if (!bufs[b]) return fail(BCHIP_E_ARG, "null buffer %u", b);
+        if (!aligned16(bufs[b])) return fail(BCHIP_E_ARG, "buffer %u: not 16-byte aligned", b);
+        CHECK(check_span(c, bufs[b], sat_mul(npages, bytes), "pages"));
+    }
+    for (uint32_t i = 0; i < n; i++)
+        if (src[i] >= npages || dst[i] >= npages) return fail(BCHIP_E_ARG, "copy %u: page %u to %u of %u", i, src[i], dst[i], npages);
+    try {
+        std::vector<uint32_t> to(dst, dst + n);
+        std::sort(to.begin(), to.end());
+        for (uint32_t i = 0; i < n; i++) {
+            if (i + 1 < n && to[i] == to[i + 1]) return fail(BCHIP_E_ARG, "page %u is written twice", to[i]);
+            if (std::binary_search(to.begin(), to.end(), src[i])) return fail(BCHIP_E_ARG, "page %u is read and written", src[i]);
+        }
+    } catch (const std::bad_alloc&) {
+        return fail(BCHIP_E_OOM, "no memory to compare %u pages", n);
+    }
+    HIP_TRY(copy_pages_launch(bufs, nbufs, bytes, src, dst, n, c->stream), "copy_pages");
+    return BCHIP_OK;
+}
+
+int bchip_beam_select(bchip_ctx* c, const float* scores, const float* sums, uint32_t batch, uint32_t beams, uint32_t vocab,
+                      uint32_t k, float* best, uint32_t* beam, uint32_t* token) {
+    CHECK(enter(c));
+    if (batch == 0) return BCHIP_OK;
+    if (!scores || !sums || !best || !beam || !token) return fail(BCHIP_E_ARG, "null pointer");
+    if (vocab == 0) return fail(BCHIP_E_ARG, "an empty vocabulary");
+    if (beams == 0 || beams > 64) return fail(BCHIP_E_ARG, "%u beams (1 to 64)", beams);
+    if (k == 0 || k > 64 || k > (uint64_t)beams * vocab) return fail(BCHIP_E_ARG, "the %u best (1 to 64) of %u beams and %u tokens", k, beams, vocab);
+    if ((uint64_t)batch * beams > 65535) return fail(BCHIP_E_ARG, "%u searches of %u beams (at most 65535 rows a call)", batch, beams);
+    const uint64_t rows = (uint64_t)batch * beams, found = (uint64_t)batch * k;
+    CHECK(check_span(c, scores, sat_mul(rows, (uint64_t)vocab * 4), "scores"));
+    CHECK(check_span(c, sums, rows * 4, "sums"));
+    CHECK(check_span(c, best, found * 4, "best"));
+    CHECK(check_span(c, beam, found * 4, "beam"));
+    CHECK(check_span(c, token, found * 4, "token"));
+    const size_t need = beam_scratch_bytes((uint32_t)rows, vocab, k);
+    if (!c->ws.reserve_vt_if(need)) return fail(BCHIP_E_OOM, "%zu bytes of scratch for beam search cannot be had", need);
+    HIP_TRY(beam_launch(scores, sums, batch, beams, vocab, k, best, beam, token, c->ws.vt, c->stream), "beam_select");
     return BCHIP_OK;
 }
 

@@ -132,6 +132,34 @@ hipError_t q4_attention(const AttnCall& a, Workspace& ws, hipStream_t s);
 hipError_t q4_attention_ragged(const AttnCall& a, const uint32_t* lens, const uint64_t* offs, uint32_t nseq,
                                Workspace& ws, hipStream_t s);
 
+// Sequences' new rows over a cache in pages: sequence i's rows are starts[i] .. starts[i + 1] - 1 and its
+// slots lens[i], theirs the last (host arrays); slot t of it lies in page table[i * stride + (t >> shift)] (device).
+struct PagedBatch {
+    const uint32_t* starts;
+    const uint32_t* lens;
+    uint32_t nseq;
+    const uint32_t* table;
+    uint32_t stride, shift, npages;
+};
+struct PagedCall {
+    const float* q;
+    const void* kc;
+    const void* vc;
+    uint32_t kv_type;  // 0 f32, 1 f16
+    float* out;
+    PagedBatch pages;
+    uint32_t nh, nkv, hd;
+    float scale;
+};
+// Attention of every sequence's rows (attention_paged.hip, attention_paged_row.hip).
+hipError_t paged_attention(const PagedCall& a, Workspace& ws, hipStream_t s);
+// The rotation and append of their rows (rope_paged.hip), and whole pages copied (src, dst: host arrays).
+hipError_t rope_append_paged_launch(float* q, const float* k, const float* v, void* kc, void* vc, uint32_t kv_type,
+                                    const float* inv_freq, const uint32_t* positions, const PagedBatch& b, uint32_t nh,
+                                    uint32_t nkv, uint32_t hd, uint32_t rope_dim, uint32_t neox, hipStream_t s);
+hipError_t copy_pages_launch(void* const* bufs, uint32_t nbufs, uint64_t page_bytes, const uint32_t* src, const uint32_t* dst,
+                             uint32_t n, hipStream_t s);
+
 hipError_t rope_launch(float* x, const float* inv_freq, const uint32_t* positions, uint32_t rows,
                        uint32_t heads, uint32_t hd, uint32_t rope_dim, uint32_t neox, hipStream_t s);
 hipError_t rope_append_launch(float* q, const float* k, const float* v, void* kc, void* vc, uint32_t kv_type,
@@ -178,6 +206,11 @@ size_t logprobs_scratch_bytes(uint32_t rows, uint32_t vocab, uint32_t top);
 hipError_t logprobs_launch(const float* scores, uint32_t rows, uint32_t vocab, float temperature, const uint32_t* tokens,
                            float* logprob, float* entropy, uint32_t top, uint32_t* ids, float* tops, void* scratch,
                            hipStream_t s);
+
+// A step of beam search (beam.hip). scratch: beam_scratch_bytes(...) bytes.
+size_t beam_scratch_bytes(uint32_t rows, uint32_t vocab, uint32_t k);
+hipError_t beam_launch(const float* scores, const float* sums, uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t k,
+                       float* best, uint32_t* beam, uint32_t* token, void* scratch, hipStream_t s);
 
 // The rest of a layer (layer.hip).
 bool ggml_block(uint32_t type, uint32_t& weights, uint32_t& bytes);

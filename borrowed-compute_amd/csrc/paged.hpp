@@ -1,0 +1,147 @@
+// A KV cache in pages: the parameters of the kernels that attend over it, and how they bring tiles of
+// it into LDS.
+//
+// A pool's K and V are [pages][page slots][kvd]; slot t of sequence i is slot t % page slots of page
+// table[i][t / page slots]. Pages are powers of two of at least 16 slots, so the 16 slots of a granule
+// lie in one page, one after another: a granule is one buffer descriptor, which ends with the list's
+// last slot (what is asked for past that comes back as zeros, whatever a reused page holds there) and
+// is empty for a page number past the pool.
+//
+// Granules go to LDS by buffer loads that write LDS themselves, 64 lanes x 16 bytes in a row: a slot's
+// bytes follow each other at PITCH, its 16-byte units turned by an amount of its own so that the reads
+// of 16 slots' units at once meet all banks. The loads are inline asm without outputs: the compiler
+// would else wait for all of them before every transposing read, not knowing which tile that reads.
+// Whoever reads waits by wait_loads (and a barrier, for other waves' loads) first.
+#pragma once
+
+#include "common.hpp"
+
+namespace bchip {
+
+// A sequence's new rows (q and out rows row0 ..) over its `len` slots, which end with theirs: row r sees
+// the slots below len - rows + r + 1. block0: the first of its blocks of the launch; fold0: of its
+// groups of 16 query rows in the fold's.
+struct PgItem {
+    uint32_t row0, len, rows_seq, block0, fold0;  // rows << 8 | sequence (its line of the table)
+};
+
+constexpr uint32_t PG_ITEMS = 128;  // of a launch: two a lane
+
+struct PgParams {
+    const float* q;
+    const uint8_t* kc;
+    const uint8_t* vc;
+    float* out;
+    float* part_o;   // chunk states [item, KV head, 16 query rows, chunk][HD / 16][64][4]
+    float* part_ml;  // [...][16][2]: their references and sums
+    const uint32_t* pages;
+    uint32_t page_stride, page_shift, npages;
+    uint32_t nh, nkv, hd, G;
+    float sc;        // scale * log2(e)
+    uint32_t chunk;  // tiles a chunk
+    uint32_t qt;     // query rows a block
+    uint32_t blocks; // blocks of the launch / KV heads
+    uint32_t nitems;
+    PgItem items[PG_ITEMS];
+};
+
+// The last item whose first block (fold: group) is at most x.
+template <bool FOLD>
+__device__ __forceinline__ uint32_t item_of(const PgParams& p, uint32_t x) {
+    if (p.nitems == 1) return 0;
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t n = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < PG_ITEMS; i += 64) {
+        if (i >= p.nitems) break;
+        const uint32_t k = min(lane + i, PG_ITEMS - 1);
+        n += __popcll(__ballot(lane + i < p.nitems && (FOLD ? p.items[k].fold0 : p.items[k].block0) <= x));
+    }
+    return __builtin_amdgcn_readfirstlane(n - 1);
+}
+
+typedef uint32_t pg_u32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) uint8_t pg_lds;
+typedef __attribute__((address_space(3))) int16_t __attribute__((ext_vector_type(4))) pg_s16x4_lds;
+
+// 64 lanes' 16 bytes at their offsets to LDS, one after another from `to`.
+__device__ __forceinline__ void load_lds(pg_u32x4 from, uint32_t offset, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(from), "s"(to) : "memory");
+}
+// Until at most N of this wave's loads are on their way.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// This wave's reads and writes of LDS are done.
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// Granules of heads of 32 NB dims.
+template <typename KVT, int NB>
+struct PgTile {
+    static constexpr int ES = sizeof(KVT), PITCH = 32 * NB * ES, UNITS = PITCH / 16, GRANULE = 16 * PITCH, LOADS = GRANULE / 1024;
+    // Slots after which the units of a row start at the same bank again: 1 << (2 - SHIFT) ... of 16 units.
+    static constexpr int SHIFT = UNITS % 16 == 0 ? 0 : UNITS % 8 == 0 ? 1 : 2;
+    static __device__ __forceinline__ uint32_t turn_k(uint32_t slot) { return (slot & 15) >> SHIFT; }
+    // (f16: a transposing read takes two units of each of eight slots at once; f32: a whole slot's.)
+    static __device__ __forceinline__ uint32_t turn_v(uint32_t slot) { return ES == 2 ? 2 * ((slot & 7) >> SHIFT) : 0; }
+    static __device__ __forceinline__ uint32_t at(uint32_t slot, uint32_t unit, uint32_t turn) {
+        return slot * PITCH + (unit + turn) % UNITS * 16;
+    }
+    // Where in a granule (rows of row_bytes) this lane's bytes of load i come from; past the head: nowhere.
+    template <bool V>
+    static __device__ __forceinline__ uint32_t from(int i, uint32_t lane, uint32_t row_bytes, uint32_t head_bytes) {
+        const uint32_t x = 64 * i + lane, slot = x / UNITS, turn = V ? turn_v(slot) : turn_k(slot);
+        const uint32_t unit = (x % UNITS + UNITS - turn) % UNITS;
+        return 16 * unit < head_bytes ? slot * row_bytes + 16 * unit : 0x80000000u;
+    }
+};
+
+// A sequence's slots of one KV head.
+struct PgList {
+    const uint32_t* table;
+    uint32_t end, shift, npages;
+    uint32_t row_bytes, head;  // bytes of a slot, and of the heads before this one
+    __device__ __forceinline__ uint32_t page(uint32_t slot) const {  // of a slot, or of the last one
+        return ((const __attribute__((address_space(4))) uint32_t*)table)[min(slot, end - 1) >> shift];
+    }
+    __device__ __forceinline__ bool bad(uint32_t slot, uint32_t page) const { return slot < end && page >= npages; }
+    // The granule from `slot` on (a multiple of 16), which lies in `page`.
+    __device__ __forceinline__ pg_u32x4 granule(const uint8_t* cache, uint32_t slot, uint32_t page) const {
+        const uint32_t n = slot < end && page < npages ? min(16u, end - slot) : 0;
+        const uint64_t at = (uint64_t)cache + (((uint64_t)page << shift) + (slot & ((1u << shift) - 1))) * row_bytes + head;
+        auto same = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
+        return pg_u32x4{same((uint32_t)at), same((uint32_t)(at >> 32) & 0xffffu),
+                        same(n ? n * row_bytes - head : 0u), 0x00020000u};
+    }
+};
+
+__device__ __forceinline__ PgList list_of(const PgParams& p, const PgItem& it, uint32_t kvh, uint32_t es) {
+    return PgList{p.pages + (size_t)(it.rows_seq & 255) * p.page_stride, it.len, p.page_shift, p.npages, p.nkv * p.hd * es, kvh * p.hd * es};
+}
+
+// Lane i of 16 gets the i'th f16 of each of four rows that the sixteen lanes' addresses name, four
+// lanes a row.
+__device__ __forceinline__ half4 read_transposed(const uint8_t* at) {
+    typedef int16_t s16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
+}
+
+// One f32 product of 16 x 16 x 4: lane l holds A[l % 16][l / 16], B[l / 16][l % 16], D[4 (l / 16) + i][l % 16].
+__device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+// Where result register i of lane group g of operand f lies in a head. f16: dims 16 f + 4 g + i. f32: the
+// operands of a segment of 64 dims (four; of a last one of 32, two) take every fourth (second) of them.
+template <typename KVT, int NB>
+__device__ __forceinline__ uint32_t dim_of(uint32_t f, uint32_t g, uint32_t i) {
+    if (sizeof(KVT) == 2) return 16 * f + 4 * g + i;
+    const uint32_t s = f / 4;
+    return 64 * s + (s < NB / 2 ? 4 : 2) * (4 * g + i) + f % 4;
+}
+
+__device__ __forceinline__ bool odd16(uint32_t pair) {  // either half an infinity or a NaN
+    return (pair & 0x7c00u) == 0x7c00u || (pair & 0x7c000000u) == 0x7c000000u;
+}
+__device__ __forceinline__ bool odd32(uint32_t x) { return (x & 0x7f800000u) == 0x7f800000u; }
+
+}  // namespace bchip

@@ -50,7 +50,8 @@ extern "C" {
 #endif
 
 /* BCHIP_Q4 and bchip_logprobs were added under version 6: a program that may meet an older library of
- * that version looks bchip_logprobs up before it uses either. */
+ * that version looks bchip_logprobs up before it uses either; and bchip_attention_paged before it uses
+ * that, bchip_rope_append_paged, bchip_copy_pages or bchip_beam_select. */
 #define BCHIP_ABI_VERSION 6
 
 enum bchip_type { BCHIP_F32 = 0, BCHIP_F16 = 1, BCHIP_Q4 = 2 }; /* T_F32 / T_F16 of kernels.h:14-15 */
@@ -260,6 +261,55 @@ int bchip_rope_append_attention_ragged(bchip_ctx* ctx, float* q, const float* k,
                                        const uint64_t* kv_offsets, uint32_t nseq, uint32_t nh, uint32_t nkv,
                                        uint32_t hd, uint32_t rope_dim, uint32_t neox, float scale, float* out);
 
+/* ---- A KV cache in pages: a pool of npages pages, K and V each [npages][page_slots][n_head_kv*head_dim]
+ * (BCHIP_F32 or BCHIP_F16), from which any number of conversations take pages as they grow (the
+ * reference keeps a contiguous cache a stream, engine.rs:25, 305-309). A call takes several
+ * sequences, each with any number of new rows (a piece of a prompt, a verify pass, one token, none):
+ *  - row_starts (host u32 [nseq + 1], from 0, not descending): sequence i's rows of q, k, v, out and
+ *    positions are row_starts[i] .. row_starts[i + 1] - 1; rows from row_starts[nseq] on (a padded
+ *    batch) are neither read nor written.
+ *  - seq_lens (host u32 [nseq]): its slots, of which its rows are the last.
+ *  - pages (device u32 [nseq][page_stride]): slot t of sequence i is slot t % page_slots of page
+ *    pages[i * page_stride + t / page_slots]. Entries past a sequence's last slot are not read.
+ *    A page number of npages or more is never followed: a row that goes there is not stored, and
+ *    rows that see such a slot come out NaN (K and V of other rows are untouched).
+ *    Pages may be shared between sequences for reading; a page that a call appends to belongs to
+ *    one sequence.
+ * page_slots is a power of two from 16 to 2^20; nseq <= 256; fewer than 2^24 rows and 2^31 query
+ * heads of rows; lists of at most 2^32 - 256 slots; slots of at most 2^20 elements and 65535 KV
+ * heads; head dims as bchip_attention. q, k, v, out, kc and vc are 16-byte aligned. Lengths are host
+ * values, so a captured call replays them as they were; what the page table, positions and data hold
+ * is read at every replay. */
+
+/* bchip_rope_append of every sequence's rows: q turns in place, k and v go to the rows' slots. Each
+ * row's bits are those of bchip_rope_append. */
+int bchip_rope_append_paged(bchip_ctx* ctx, float* q, const float* k, const float* v, void* kc, void* vc,
+                            uint32_t kv_type, const float* inv_freq, const uint32_t* positions,
+                            const uint32_t* row_starts, const uint32_t* seq_lens, const uint32_t* pages,
+                            uint32_t page_stride, uint32_t page_slots, uint32_t npages, uint32_t nseq, uint32_t nh,
+                            uint32_t nkv, uint32_t hd, uint32_t rope_dim, uint32_t neox);
+
+/* Causal attention of every sequence's rows over its pages: row r of n sees the slots up to
+ * seq_lens[i] - n + r. f16 caches: K and V are f16 MFMA operands as they are, q and the softmax weights
+ * two f16 each (22 bits), f32 accumulation; f32 caches: f32 products and sums. Results are within f32
+ * rounding of the formula over the stored values, for one row, a batch or a piece of a prompt alike; a
+ * row's last bits depend on the call it is in (lists are cut by the call's size), reruns give the same
+ * bits. An element of K or V that is not finite leaves the rows that see its slot unspecified and no
+ * other; what a page holds past a list's end is never used. Where scratch cannot be had (memory full, a
+ * call under graph capture that has not run before at its size) lists run uncut. */
+int bchip_attention_paged(bchip_ctx* ctx, const float* q, const void* kc, const void* vc, uint32_t kv_type, float* out,
+                          const uint32_t* row_starts, const uint32_t* seq_lens, const uint32_t* pages,
+                          uint32_t page_stride, uint32_t page_slots, uint32_t npages, uint32_t nseq, uint32_t nh,
+                          uint32_t nkv, uint32_t hd, float scale);
+
+/* Whole pages copied in every one of nbufs pool buffers (each layer's K and V): page dst[i] becomes
+ * page src[i], i < n, pages of page_elems elements (page_slots * n_head_kv * head_dim) of type. The step
+ * by which a conversation that shares pages with another gets its own (a fork's last page, beams that
+ * part). src and dst are host arrays of page numbers below npages; dst names no page twice and none
+ * that src names. bufs is a host array of device pointers; a page is a multiple of 16 bytes. */
+int bchip_copy_pages(bchip_ctx* ctx, void* const* bufs, uint32_t nbufs, uint32_t type, uint64_t page_elems,
+                     uint32_t npages, const uint32_t* src, const uint32_t* dst, uint32_t n);
+
 /* ---- The rest of a layer (Layers::forward, mod.rs:454-491): the GGUF block-format
  * product, RMSNorm and the elementwise ops. Weight types are ggml's numbers
  * (quant.rs:35-49): BCHIP_GGML_F32 0, F16 1, Q4_0 2, Q4_1 3, Q5_0 6, Q5_1 7, Q8_0 8,
@@ -337,6 +387,21 @@ int bchip_sample(bchip_ctx* ctx, const float* scores, uint32_t rows, uint32_t vo
 int bchip_logprobs(bchip_ctx* ctx, const float* scores, uint32_t rows, uint32_t vocab, float temperature,
                    const uint32_t* tokens, float* logprob, float* entropy, uint32_t top, uint32_t* top_ids,
                    float* top_logprobs);
+
+/* A step of beam search beside the sampler, for `batch` searches of `beams` beams each: of the beams x vocab
+ * continuations of search i, whose score is sums[i][b] plus the log probability of token t under the
+ * softmax of scores[i * beams + b] (device f32 [batch * beams][vocab]), the k best in descending order:
+ * best[i][j] (their scores), beam[i][j] and token[i][j] (device [batch][k]). sums (device f32
+ * [batch][beams]) are the log probabilities of the beams so far; -inf for a beam that is not there (a
+ * search's first step has one). Equal scores go to the lower beam, then the lower token; scores are
+ * formed in 64 bits from f32 exponentials, and rounded to f32. A row with a NaN, a score of +inf or
+ * nothing above -inf gives NaN scores, behind every number. beams and k <= 64, k <= beams * vocab,
+ * batch * beams <= 65535. A caller that ends beams at a token asks for 2 beams of k and keeps the beams that
+ * go on. Takes scratch of at most 70 bytes a row and unit of 8192 scores, and 8 k bytes a part of a row; fails
+ * with BCHIP_E_OOM where it cannot be had (memory full, a call under graph capture that has not run
+ * before at its size). */
+int bchip_beam_select(bchip_ctx* ctx, const float* scores, const float* sums, uint32_t batch, uint32_t beams,
+                      uint32_t vocab, uint32_t k, float* best, uint32_t* beam, uint32_t* token);
 
 /* Seeded N(0,1) draws into dst (n elements of type): splitmix64 (Steele, Lea and Flood
  * 2014) + Box-Muller (1958), the generator of the benchmark inputs; draw i of seed s is
