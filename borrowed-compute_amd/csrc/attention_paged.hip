@@ -75,7 +75,7 @@ __global__ __launch_bounds__(RT == 1 ? 512 : 256, 2) void attn_paged_tile16(cons
     const uint32_t ks = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const uint32_t m16 = lane & 15, g = lane >> 4;
     const uint32_t block = blockIdx.x / p.nkv;
-    const PgItem& it = p.items[item_of<false>(p, block)];
+    const PgItem it = item_with_arguments<false>(p, block);
     const PgBlock b = block_of<QT, SLOTS>(p, it, block);
     if (b.t0 >= b.t1) {  // nothing of these rows' lists
         if (threadIdx.x < QT) {
@@ -120,34 +120,39 @@ __global__ __launch_bounds__(RT == 1 ? 512 : 256, 2) void attn_paged_tile16(cons
     half8 qh[RT][NB], ql[RT][NB];
     float c[RT];
     {
-        float x[RT][NB][8];
+        f32x4 y[RT][NB][2];
 #pragma unroll
         for (int r = 0; r < RT; r++) {
             row[r] = row_of(p, it, b, (wave * RT + r) * 16 + m16);
 #pragma unroll
-            for (int j = 0; j < NB; j++) {
-                const uint32_t d = 32 * j + 8 * g;
-                f32x4 lo{0, 0, 0, 0}, hi{0, 0, 0, 0};
-                if (row[r].valid && d < p.hd) {
-                    lo = *(const f32x4*)(p.q + row[r].at + d);
-                    hi = *(const f32x4*)(p.q + row[r].at + d + 4);
-                }
+            for (int j = 0; j < NB; j++)  // (no branch around them)
 #pragma unroll
-                for (int e = 0; e < 8; e++) x[r][j][e] = e < 4 ? lo[e & 3] : hi[e & 3];
-            }
+                for (int e = 0; e < 2; e++) y[r][j][e] = *(const f32x4*)(p.q + row[r].at + (32 * j + 8 * g < p.hd ? 32 * j + 8 * g : 0) + 4 * e);
         }
+        // They are waited for here, beside the page: behind the tile's loads, which the compiler does not
+        // count, its wait for them would be one for those too.
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+            for (int j = 0; j < NB; j++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) asm volatile("" : "+v"(y[r][j][e]));
         fetch(b.t0, 0);
         look(b.t0 + 1);
 #pragma unroll
         for (int r = 0; r < RT; r++) {
-            float top = 0.0f, k;
+            float top = 0.0f, k, x[NB][8];
 #pragma unroll
-            for (int j = 0; j < NB; j++) top = q_top(x[r][j], top);
+            for (int j = 0; j < NB; j++) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[j][e] = row[r].valid && 32 * j + 8 * g < p.hd ? y[r][j][e >> 2][e & 3] : 0.0f;
+                top = q_top(x[j], top);
+            }
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
             q_scale(top, p.sc, k, c[r]);
 #pragma unroll
-            for (int j = 0; j < NB; j++) q_parts(x[r][j], k, qh[r][j], ql[r][j]);
+            for (int j = 0; j < NB; j++) q_parts(x[j], k, qh[r][j], ql[r][j]);
         }
     }
     uint32_t kat[NB], vat[NF];
@@ -340,7 +345,7 @@ __global__ __launch_bounds__(256, NB > 4 ? 1 : 2) void attn_paged_tile32(const P
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t m16 = lane & 15, g = lane >> 4;
     const uint32_t block = blockIdx.x / p.nkv;
-    const PgItem& it = p.items[item_of<false>(p, block)];
+    const PgItem it = item_with_arguments<false>(p, block);
     const PgBlock b = block_of<QT, SLOTS>(p, it, block);
     if (b.t0 >= b.t1) {
         if (threadIdx.x < QT) {
@@ -377,9 +382,14 @@ __global__ __launch_bounds__(256, NB > 4 ? 1 : 2) void attn_paged_tile32(const P
     const PgRow row = row_of(p, it, b, wave * 16 + m16);
     f32x4 q[NJ];
 #pragma unroll
-    for (int j = 0; j < NJ; j++) q[j] = row.valid && 16 * j + 4 * g < p.hd ? *(const f32x4*)(p.q + row.at + 16 * j + 4 * g) : f32x4{0, 0, 0, 0};
+    for (int j = 0; j < NJ; j++) q[j] = *(const f32x4*)(p.q + row.at + (16 * j + 4 * g < p.hd ? 16 * j + 4 * g : 0));
+#pragma unroll
+    for (int j = 0; j < NJ; j++) asm volatile("" : "+v"(q[j]));  // (as in attn_paged_tile16)
     fetch(b.t0, 0);
     look(b.t0 + 1);
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+        if (!row.valid || 16 * j + 4 * g >= p.hd) q[j] = f32x4{0, 0, 0, 0};
     uint32_t kat[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; j++) kat[j] = T::at(m16, 4 * j + g, T::turn_k(m16));
@@ -516,7 +526,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_paged_fold(const PgParams p) 
     __shared__ float sr[WAVES][64], sl[WAVES][64];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m16 = lane & 15, g = lane >> 4;
     const uint32_t f = blockIdx.z, kvh = blockIdx.y;
-    const PgItem& it = p.items[item_of<true>(p, blockIdx.x)];
+    const PgItem it = item_with_arguments<true>(p, blockIdx.x);
     const uint32_t slots = p.qt == 16 ? (sizeof(KVT) == 2 ? 32 : 16) : (sizeof(KVT) == 2 ? 64 : 32);  // of a tile
     const uint32_t rows = it.rows_seq >> 8, nq = rows * p.G, groups = ((nq - 1) / p.qt + 1) * (p.qt / 16);
     const uint32_t chunks = ((it.len - 1) / slots) / p.chunk + 1, group = blockIdx.x - it.fold0, n = 16 * group + m16;
@@ -583,6 +593,7 @@ void launch_fold(const PgParams& p, uint32_t groups, uint32_t most, hipStream_t 
     // A wave alone holds a few chunks' states at once; more chunks are shared out.
     const dim3 grid(groups, p.nkv, 2 * NB);
     if (most <= 8) hipLaunchKernelGGL((attn_paged_fold<KVT, NB, 1>), grid, dim3(64), 0, s, p);
+    else if (most <= 16) hipLaunchKernelGGL((attn_paged_fold<KVT, NB, 2>), grid, dim3(128), 0, s, p);
     else hipLaunchKernelGGL((attn_paged_fold<KVT, NB, 8>), grid, dim3(512), 0, s, p);
 }
 
@@ -649,7 +660,18 @@ hipError_t run_rows(PgParams& p, bool f16_cache, Workspace& ws, hipStream_t s) {
     p.qt = 16;
     // Lists that eight waves take in a few tiles each are not cut: no second launch.
     const bool brief = most <= 20;
-    p.chunk = brief ? WHOLE : std::max<uint32_t>(4, ceil_div(ceil_div(total * p.nkv, 512), 4) * 4);
+    p.chunk = WHOLE;
+    if (!brief) {
+        // Chunks of whole rounds of the waves, as short as leaves every workgroup a place at once.
+        constexpr uint32_t groups = 512;
+        p.chunk = std::max<uint32_t>(4, ceil_div(ceil_div(total * p.nkv, groups), 4) * 4);
+        auto blocks = [&] {
+            uint64_t n = 0;
+            for (uint32_t i = 0; i < p.nitems; i++) n += (p.items[i].len - 1) / slots / p.chunk + 1;
+            return n * p.nkv;
+        };
+        while (p.chunk < most && blocks() > groups) p.chunk += std::max(4u, p.chunk / 16 / 4 * 4);
+    }
     PgPlan plan = place(p, slots);
     if (plan.groups && !reserve(p, plan, ws)) {  // whole lists
         p.chunk = WHOLE;
@@ -666,30 +688,31 @@ hipError_t run_rows(PgParams& p, bool f16_cache, Workspace& ws, hipStream_t s) {
 hipError_t run_tiles(PgParams& p, bool f16_cache, Workspace& ws, hipStream_t s) {
     const uint32_t slots = pg_tile(f16_cache);
     std::sort(p.items, p.items + p.nitems, [](const PgItem& a, const PgItem& b) { return a.len > b.len; });
-    uint64_t big = 0;
-    for (uint32_t i = 0; i < p.nitems; i++) big += ceil_div((uint64_t)(p.items[i].rows_seq >> 8) * p.G, 128) * (uint64_t)p.nkv;
-    p.qt = f16_cache && p.hd <= 128 && big >= 352 ? 128 : 64;
-    uint64_t work = 0, units = 0, longest = 0;  // tiles of the query blocks, as many as there are, the longest list's
-    for (uint32_t i = 0; i < p.nitems; i++) {
-        const PgItem& it = p.items[i];
-        const uint64_t rows = it.rows_seq >> 8, n = ceil_div(rows * p.G, p.qt) * (uint64_t)p.nkv;
-        units += n;
-        work += n * (((uint64_t)it.len - rows / 2) / slots + 1);
-        longest = std::max<uint64_t>(longest, (it.len - 1) / slots + 1);
-    }
+    uint64_t few = 0, many = 0;  // query blocks of at most 64 rows, of more
+    for (uint32_t i = 0; i < p.nitems; i++) ((uint64_t)(p.items[i].rows_seq >> 8) * p.G <= 64 ? few : many)++;
+    p.qt = f16_cache && p.hd <= 128 && many >= few ? 128 : 64;
+    uint64_t longest = 0;  // list's tiles
+    for (uint32_t i = 0; i < p.nitems; i++) longest = std::max<uint64_t>(longest, (p.items[i].len - 1) / slots + 1);
     constexpr uint64_t CUS = 256;
-    const float tile = 0.6f + 0.006f * p.hd, launch = 2.0f + 0.0006f * p.hd * units, states = 64.0f * 8.0f / 5e6f * p.hd * units;
-    auto time = [&](uint64_t chunk, uint64_t n) {
-        return (std::max((float)work / CUS, (float)chunk) + (float)chunk * 0.25f) * tile + 7.0f + (n > 1 ? launch + states * n : 0.0f);
+    const float tile = f16_cache ? 0.2f + 0.011f * p.hd : 0.0133f * p.hd;
+    auto time = [&](uint64_t chunk) {
+        uint64_t work = 0, blocks = 0, cut = 0;
+        for (uint32_t i = 0; i < p.nitems; i++) {
+            const PgItem& it = p.items[i];
+            const uint64_t rows = it.rows_seq >> 8, n = ceil_div(rows * p.G, p.qt) * (uint64_t)p.nkv, tiles = ((uint64_t)it.len - rows / 2) / slots + 1;
+            const uint64_t chunks = (tiles - 1) / chunk + 1;
+            work += n * tiles;
+            blocks += n * chunks;
+            if (chunks > 1) cut += n * chunks;
+        }
+        return std::max((float)chunk, (float)ceil_div(blocks, CUS) * work / blocks) * tile + (cut ? 5.0f + (float)cut * p.qt * p.hd * 8 / 4.5e6f : 0.0f);
     };
     p.chunk = WHOLE;
-    float least = time(longest, 1);
+    float least = time(longest);
     for (uint64_t n = 2; n <= 64 && longest / n >= 2; n++) {
         const uint64_t chunk = ceil_div(longest, n);
-        if (time(chunk, n) < least) {
-            least = time(chunk, n);
-            p.chunk = (uint32_t)chunk;
-        }
+        const float t = time(chunk);
+        if (t < least) least = t, p.chunk = (uint32_t)chunk;
     }
     PgPlan plan = place(p, slots);
     if (plan.groups && !reserve(p, plan, ws)) {

@@ -41,8 +41,8 @@ __global__ __launch_bounds__(64 * WAVES, NB > 4 ? 1 : 2) void attn_paged_row(con
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t m16 = lane & 15, g = lane >> 4;
     const uint32_t block = (blockIdx.x / (8 * p.nkv)) * 8 + (blockIdx.x & 7), kvh = (blockIdx.x >> 3) % p.nkv;
+    const PgItem it = item_with_arguments<false>(p, block);
     if (block >= p.blocks) return;
-    const PgItem& it = p.items[item_of<false>(p, block)];
     const uint32_t rows = it.rows_seq >> 8, nq = rows * p.G, seen = it.len - rows + 1;  // slots every row sees
     const PgList list = list_of(p, it, kvh, T::ES);
     const uint32_t all = (it.len - 1) / SLOTS + 1, chunk = block - it.block0, nchunk = (all - 1) / p.chunk + 1;
@@ -78,17 +78,27 @@ __global__ __launch_bounds__(64 * WAVES, NB > 4 ? 1 : 2) void attn_paged_row(con
     const uint32_t vis = valid ? seen + r : list.end;  // slots this lane's row sees
     const size_t qrow = ((size_t)row * p.nh + head) * p.hd;
     f32x4 x[NJ][F16 ? 2 : 1];
+    auto dim = [&](int j) { return HD / NJ * j + HD / NJ / 4 * g; };
 #pragma unroll
-    for (int j = 0; j < NJ; j++) {
-        const uint32_t d = HD / NJ * j + HD / NJ / 4 * g;
+    for (int j = 0; j < NJ; j++)  // (no branch around them)
 #pragma unroll
-        for (int e = 0; e < (F16 ? 2 : 1); e++) x[j][e] = valid && d < p.hd ? *(const f32x4*)(p.q + qrow + d + 4 * e) : f32x4{0, 0, 0, 0};
-    }
+        for (int e = 0; e < (F16 ? 2 : 1); e++) x[j][e] = *(const f32x4*)(p.q + qrow + (dim(j) < p.hd ? dim(j) : 0) + 4 * e);
+    // They are waited for here, beside the pages: behind the tile's loads, which the compiler does not
+    // count, its wait for them would be one for those too.
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+#pragma unroll
+        for (int e = 0; e < (F16 ? 2 : 1); e++) asm volatile("" : "+v"(x[j][e]));
     fetch(p.kc, kfrom, kl, wave);
     fetch(p.vc, vfrom, vl, wave);
 #pragma unroll
     for (int h = 0; h < NG; h++) bad |= list.bad((first + wave) * SLOTS + 16 * h, page[h]) ? 1u << h : 0;
     look(wave + WAVES);
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+#pragma unroll
+        for (int e = 0; e < (F16 ? 2 : 1); e++)
+            if (!valid || dim(j) >= p.hd) x[j][e] = f32x4{0, 0, 0, 0};
     float c = 1.0f;
     const float keep = PK && m16 >= 8 ? 1.0f : 0.0f;
     half8 qa[F16 ? NB : 1], qb[F16 && !PK ? NB : 1];

@@ -1199,7 +1199,7 @@ int bchip_beam_select(bchip_ctx* c, const float* scores, const float* sums, uint
     CHECK(check_span(c, best, found * 4, "best"));
     CHECK(check_span(c, beam, found * 4, "beam"));
     CHECK(check_span(c, token, found * 4, "token"));
-    const size_t need = beam_scratch_bytes((uint32_t)rows, vocab, k);
+    const size_t need = beam_scratch_bytes((uint32_t)rows, vocab);
     if (!c->ws.reserve_vt_if(need)) return fail(BCHIP_E_OOM, "%zu bytes of scratch for beam search cannot be had", need);
     HIP_TRY(beam_launch(scores, sums, batch, beams, vocab, k, best, beam, token, c->ws.vt, c->stream), "beam_select");
     return BCHIP_OK;

@@ -207,8 +207,8 @@ hipError_t logprobs_launch(const float* scores, uint32_t rows, uint32_t vocab, f
                            float* logprob, float* entropy, uint32_t top, uint32_t* ids, float* tops, void* scratch,
                            hipStream_t s);
 
-// A step of beam search (beam.hip). scratch: beam_scratch_bytes(...) bytes.
-size_t beam_scratch_bytes(uint32_t rows, uint32_t vocab, uint32_t k);
+// A step of beam search (beam.hip). scratch: beam_scratch_bytes bytes.
+size_t beam_scratch_bytes(uint32_t rows, uint32_t vocab);
 hipError_t beam_launch(const float* scores, const float* sums, uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t k,
                        float* best, uint32_t* beam, uint32_t* token, void* scratch, hipStream_t s);
 

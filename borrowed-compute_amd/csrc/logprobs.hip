@@ -154,8 +154,7 @@ struct __attribute__((packed, aligned(4))) Float4Any {  // rows of an odd vocabu
     float x, y, z, w;
 };
 
-// BEAM: a row's parts leave their states (without A) and keys to k_beam_join, whatever their number.
-template <bool TOP, bool BEAM>
+template <bool TOP>
 __global__ __launch_bounds__(LP_THREADS, TOP ? 3 : 8) void k_logprobs(const LpParams p) {
     __shared__ uint64_t cand[4][TOP ? LP_SEG : 1], best[2][TOP ? LP_TOP : 1], pick[4];
     __shared__ LpState waves[LP_PARTS][4], whole;
@@ -200,7 +199,7 @@ __global__ __launch_bounds__(LP_THREADS, TOP ? 3 : 8) void k_logprobs(const LpPa
             const float x = (v[e] - m) * p.k, w = exp2_hw(x);
             st.l += x == 0.0f ? 0.0f : w;
             ones += x == 0.0f;
-            if constexpr (!BEAM) st.a = __builtin_fmaf(w, fmaxf(x, -1e4f), st.a);  // (0 for a score of -inf; a NaN stays one)
+            st.a = __builtin_fmaf(w, fmaxf(x, -1e4f), st.a);  // (0 for a score of -inf; a NaN stays one)
         }
         st.c += (float)ones;
         if (b + 1 == next || end) {  // of the unit
@@ -345,14 +344,14 @@ __global__ __launch_bounds__(LP_THREADS, TOP ? 3 : 8) void k_logprobs(const LpPa
                 x.l += y.l;
                 x.a += y.a;
             }
-            if (BEAM || p.parts > 1) p.states[(size_t)row * p.units + u0 + tid] = x;
+            if (p.parts > 1) p.states[(size_t)row * p.units + u0 + tid] = x;
         }
-        if (!BEAM && p.parts == 1) {
+        if (p.parts == 1) {
             x = lp_row(x, p.k);
             if (tid == 0) whole = x;
         }
     }
-    if (!BEAM && p.parts == 1) {
+    if (p.parts == 1) {
         __syncthreads();
         lp_finish(p, row, whole, best[which]);
         return;
@@ -412,108 +411,6 @@ __global__ __launch_bounds__(LP_THREADS) void k_logprobs_join(const LpParams p) 
     lp_finish(p, row, all, best);
 }
 
-// A step of beam search: of a search's beams x vocabulary continuations, whose scores are the beam's sum
-// plus the token's log probability, the k best. A search's workgroup brings its rows' states together,
-// log L in 64 bits, gives every row's best keys their scores in 64 bits (two rows' continuations may lie
-// nearer than an f32 tells apart), and ranks: 4096 keys at a time, of which those that reach the k'th
-// largest of the threads' maxima go into a pool with the best so far, and a key's rank is the number
-// of better ones. Equal scores go by beam, then by token; what is not a number comes last.
-constexpr uint32_t BEAM_MOST = 64;                 // beams of a search, and continuations asked for
-constexpr uint32_t BEAM_THREADS = 256, BEAM_EACH = 16;
-
-struct BeamKey {
-    uint64_t score;  // ascending with the score; 0: none, 1: not a number
-    uint64_t place;  // beam << 32 | token
-    __device__ __forceinline__ bool above(const BeamKey& o) const { return score != o.score ? score > o.score : place < o.place; }
-};
-
-struct BeamParams {
-    const float* sums;
-    float* best;
-    uint32_t* beam;
-    uint32_t* token;
-    const LpState* states;  // [row][units]
-    const uint64_t* keys;   // [row][parts][top]
-    uint32_t beams, k, top, units, parts;
-};
-
-__global__ __launch_bounds__(BEAM_THREADS) void k_beam_join(const BeamParams p) {
-    __shared__ double lse[BEAM_MOST];
-    __shared__ BeamKey pool[BEAM_THREADS * BEAM_EACH + BEAM_MOST], best[BEAM_MOST];
-    __shared__ uint64_t most[BEAM_THREADS], least;
-    __shared__ uint32_t count;
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const size_t row0 = (size_t)blockIdx.x * p.beams;
-    for (uint32_t b = wave; b < p.beams; b += BEAM_THREADS / 64) {
-        LpState s = lane < p.units ? p.states[(row0 + b) * p.units + lane] : LpState{-INFINITY, 0.0f, 0.0f, 0.0f};
-        const float M = wave_max(s.m);
-        double l = s.m == -INFINITY ? 0.0 : ((double)s.c + (double)s.l) * exp((double)s.m - (double)M);
-        if (s.l != s.l) l = s.l;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) l += __shfl_xor(l, d);
-        if (lane == 0) lse[b] = (double)M + log(l);
-    }
-    if (tid == 0) count = 0;
-    uint32_t kept = 0;
-    __syncthreads();
-    const uint32_t row_keys = p.parts * p.top, all = p.beams * row_keys;
-    for (uint32_t x0 = 0; x0 < all; x0 += BEAM_THREADS * BEAM_EACH) {
-        BeamKey mine[BEAM_EACH];
-        uint64_t top = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < BEAM_EACH; i++) {
-            const uint32_t x = x0 + i * BEAM_THREADS + tid;
-            mine[i] = BeamKey{0, 0};
-            if (x >= all) continue;
-            const uint32_t b = x / row_keys;
-            const uint64_t key = p.keys[(row0 + b) * row_keys + (x - b * row_keys)];
-            if (key == 0) continue;
-            const double v = (double)p.sums[row0 + b] + ((double)lp_score(key) - lse[b]);
-            const uint64_t bits = __double_as_longlong(v + 0.0);
-            mine[i] = BeamKey{v != v ? 1 : bits >> 63 ? ~bits : bits | 1ull << 63, (uint64_t)b << 32 | lp_index(key)};
-            top = max(top, mine[i].score);
-        }
-        // The k'th largest of the threads' maxima (the smallest that fewer than k are larger than): at least
-        // k keys reach it, if there are as many threads' with any.
-        most[tid] = top;
-        if (tid == 0) least = 0;
-        __syncthreads();
-        uint32_t larger = 0;
-        for (uint32_t i = 0; i < BEAM_THREADS; i++) larger += most[i] > top;
-        uint64_t low = larger < p.k ? ~top : 0;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) low = max(low, (uint64_t)__shfl_xor((unsigned long long)low, d));
-        if (lane == 0) atomicMax((unsigned long long*)&least, (unsigned long long)low);
-        __syncthreads();
-        const uint64_t worst = kept == p.k ? best[p.k - 1].score : 0, from = ~least > worst ? ~least : worst;
-#pragma unroll
-        for (uint32_t i = 0; i < BEAM_EACH; i++)
-            if (mine[i].score != 0 && mine[i].score >= from) pool[atomicAdd(&count, 1u)] = mine[i];
-        __syncthreads();
-        if (tid < kept) pool[count + tid] = best[tid];
-        __syncthreads();
-        const uint32_t n = count + kept;
-        for (uint32_t i = tid; i < n; i += BEAM_THREADS) {
-            const BeamKey x = pool[i];
-            uint32_t rank = 0;
-            for (uint32_t j = 0; j < n; j++) rank += pool[j].above(x);
-            if (rank < p.k) best[rank] = x;
-        }
-        __syncthreads();
-        if (tid == 0) count = 0;
-        kept = min(n, p.k);
-        __syncthreads();
-    }
-    if (tid < p.k) {
-        const BeamKey x = best[tid];
-        const uint64_t bits = x.score >> 63 ? x.score & ~(1ull << 63) : ~x.score;
-        const size_t at = (size_t)blockIdx.x * p.k + tid;
-        p.best[at] = x.score == 1 ? NAN : (float)__longlong_as_double(bits);
-        p.beam[at] = (uint32_t)(x.place >> 32);
-        p.token[at] = (uint32_t)x.place;
-    }
-}
-
 // Blocks a unit, units a row, and units a workgroup of `rows` rows.
 void lp_plan(uint32_t rows, uint32_t vocab, LpParams& p) {
     const uint32_t all = (vocab - 1) / LP_BLOCK + 1;
@@ -554,36 +451,10 @@ hipError_t logprobs_launch(const float* scores, uint32_t rows, uint32_t vocab, f
     p.k = (float)(1.4426950408889634 / (double)temperature);
     p.keys = (uint64_t*)scratch;
     p.states = (LpState*)((uint64_t*)scratch + (size_t)rows * p.parts * top);
-    hipLaunchKernelGGL((top ? k_logprobs<true, false> : k_logprobs<false, false>), dim3(p.parts, rows), dim3(LP_THREADS), 0, s, p);
+    hipLaunchKernelGGL(top ? k_logprobs<true> : k_logprobs<false>, dim3(p.parts, rows), dim3(LP_THREADS), 0, s, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.parts == 1) return e;
     hipLaunchKernelGGL(top ? k_logprobs_join<true> : k_logprobs_join<false>, dim3(rows), dim3(LP_THREADS), 0, s, p);
-    return hipGetLastError();
-}
-
-size_t beam_scratch_bytes(uint32_t rows, uint32_t vocab, uint32_t k) {
-    LpParams p{};
-    lp_plan(rows, vocab, p);
-    return (size_t)rows * (p.units * sizeof(LpState) + (size_t)p.parts * std::min(k, vocab) * sizeof(uint64_t));
-}
-
-hipError_t beam_launch(const float* scores, const float* sums, uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t k,
-                       float* best, uint32_t* beam, uint32_t* token, void* scratch, hipStream_t s) {
-    const uint32_t rows = batch * beams;
-    LpParams p{};
-    p.scores = scores;
-    p.vocab = vocab;
-    p.top = std::min(k, vocab);
-    lp_plan(rows, vocab, p);
-    p.inv_t = 1.0f;
-    p.k = LOG2E;
-    p.keys = (uint64_t*)scratch;
-    p.states = (LpState*)((uint64_t*)scratch + (size_t)rows * p.parts * p.top);
-    hipLaunchKernelGGL((k_logprobs<true, true>), dim3(p.parts, rows), dim3(LP_THREADS), 0, s, p);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    const BeamParams b{sums, best, beam, token, p.states, p.keys, beams, k, p.top, p.units, p.parts};
-    hipLaunchKernelGGL(k_beam_join, dim3(batch), dim3(BEAM_THREADS), 0, s, b);
     return hipGetLastError();
 }
 

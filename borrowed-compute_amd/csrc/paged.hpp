@@ -48,16 +48,23 @@ struct PgParams {
 // The last item whose first block (fold: group) is at most x.
 template <bool FOLD>
 __device__ __forceinline__ uint32_t item_of(const PgParams& p, uint32_t x) {
-    if (p.nitems == 1) return 0;
     const uint32_t lane = threadIdx.x & 63;
-    uint32_t n = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < PG_ITEMS; i += 64) {
-        if (i >= p.nitems) break;
-        const uint32_t k = min(lane + i, PG_ITEMS - 1);
-        n += __popcll(__ballot(lane + i < p.nitems && (FOLD ? p.items[k].fold0 : p.items[k].block0) <= x));
-    }
+    const uint32_t a = FOLD ? p.items[lane].fold0 : p.items[lane].block0, b = FOLD ? p.items[lane + 64].fold0 : p.items[lane + 64].block0;
+    const uint32_t n = __popcll(__ballot(lane < p.nitems && a <= x)) + __popcll(__ballot(lane + 64 < p.nitems && b <= x));
     return __builtin_amdgcn_readfirstlane(n - 1);
+}
+
+// A block's item. Every argument that a kernel's first loads need is read here, item 0 with them, in one
+// round trip: a branch that waits for one argument would else put the others' behind it (the empty asm
+// is their use).
+template <bool FOLD>
+__device__ __forceinline__ PgItem item_with_arguments(const PgParams& p, uint32_t x) {
+    PgItem it = p.items[0];
+    asm volatile("" ::"s"(p.q), "s"(p.kc), "s"(p.vc), "s"(p.out), "s"(p.part_o), "s"(p.part_ml), "s"(p.pages), "s"(p.page_stride),
+                 "s"(p.page_shift), "s"(p.npages), "s"(p.nh), "s"(p.nkv), "s"(p.hd), "s"(p.G), "s"(p.sc), "s"(p.chunk), "s"(p.qt),
+                 "s"(p.blocks), "s"(p.nitems), "s"(it.row0), "s"(it.len), "s"(it.rows_seq), "s"(it.block0), "s"(it.fold0));
+    if (p.nitems > 1) it = p.items[item_of<FOLD>(p, x)];
+    return it;
 }
 
 typedef uint32_t pg_u32x4 __attribute__((ext_vector_type(4)));

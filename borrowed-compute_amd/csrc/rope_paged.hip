@@ -140,7 +140,8 @@ __global__ __launch_bounds__(RP_THREADS) void k_rope_append_paged(const RopePage
     }
 }
 
-constexpr uint32_t CP_PAIRS = 256, CP_BUFS = 128, CP_THREADS = 256, CP_EACH = 4;
+constexpr uint32_t CP_PAIRS = 256, CP_BUFS = 128, CP_THREADS = 256;
+constexpr int CP_EACH = 4;
 
 struct CopyPages {
     uint8_t* bufs[CP_BUFS];
@@ -153,14 +154,14 @@ __global__ __launch_bounds__(CP_THREADS) void k_copy_pages(const CopyPages p) {
     uint8_t* buf = p.bufs[blockIdx.z];
     const uint8_t* from = buf + p.src[blockIdx.y] * p.bytes;
     uint8_t* to = buf + p.dst[blockIdx.y] * p.bytes;
-    uint4 x[CP_EACH] = {};
+    pg_u32x4 x[CP_EACH];
     const uint64_t at = 16 * ((uint64_t)blockIdx.x * CP_THREADS * CP_EACH + threadIdx.x);
 #pragma unroll
-    for (uint32_t i = 0; i < CP_EACH; i++)
-        if (at + 16 * CP_THREADS * i < p.bytes) x[i] = *(const uint4*)(from + at + 16 * CP_THREADS * i);
+    for (int i = 0; i < CP_EACH; i++)  // (past the page: its last piece, not stored)
+        x[i] = *(const pg_u32x4*)(from + (at + 16 * CP_THREADS * i < p.bytes ? at + 16 * CP_THREADS * i : p.bytes - 16));
 #pragma unroll
-    for (uint32_t i = 0; i < CP_EACH; i++)
-        if (at + 16 * CP_THREADS * i < p.bytes) *(uint4*)(to + at + 16 * CP_THREADS * i) = x[i];
+    for (int i = 0; i < CP_EACH; i++)
+        if (at + 16 * CP_THREADS * i < p.bytes) *(pg_u32x4*)(to + at + 16 * CP_THREADS * i) = x[i];
 }
 
 }  // namespace
