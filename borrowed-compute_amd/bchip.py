@@ -7,6 +7,7 @@ here, and loading fails loudly when the library is missing.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import os
 import re
@@ -309,11 +310,11 @@ class Ctx:
 
     def copy_pages(self, bufs, t, page_elems, npages, src, dst) -> None:
         """Page dst[i] becomes page src[i] in every buffer of a pool, pages of page_elems elements of type t."""
-        arr = (ctypes.c_void_p * len(bufs))(*[_ptr(b) for b in bufs])
+        arr = array.array("Q", [_ptr(b) or 0 for b in bufs])
         s, d = np.ascontiguousarray(src, np.uint32), np.ascontiguousarray(dst, np.uint32)
         if s.shape != d.shape or s.ndim != 1:
             raise ValueError(f"{s.shape} source pages for {d.shape} destinations")
-        check(lib().bchip_copy_pages(self.h, arr, len(bufs), t, page_elems, npages, s.ctypes.data, d.ctypes.data, len(s)))
+        check(lib().bchip_copy_pages(self.h, arr.buffer_info()[0], len(bufs), t, page_elems, npages, s.ctypes.data, d.ctypes.data, len(s)))
 
     def matmul(self, w, wtype, x, out, rows, cols, n) -> None:
         check(lib().bchip_matmul(self.h, _ptr(w), wtype, _ptr(x), _ptr(out), rows, cols, n))
@@ -412,6 +413,114 @@ class KvCache:
         for b in self.k + self.v:
             b.free()
         self.k, self.v, self.cap = [], [], 0
+
+
+class PagePool:
+    """A model's KV cache in pages on the device, for any number of conversations: per layer a K and a V
+    pool of npages x page_slots x kvd elements of kv_type (F32 or F16). A conversation is a number from
+    new() or fork(); it takes pages as it grows and gives them back with drop(). A fork shares its
+    parent's pages: whoever writes into a shared one first gets a copy (bchip_copy_pages, every layer
+    in one call). The host keeps the tables; a step's is uploaded with it."""
+
+    def __init__(self, ctx: "Ctx", n_layer: int, kvd: int, npages: int, page_slots: int = 16, kv_type: int = F16):
+        self.ctx, self.n_layer, self.kvd, self.kv_type = ctx, n_layer, kvd, kv_type
+        self.npages, self.page_slots = npages, page_slots
+        nbytes = nbytes_of(kv_type, npages * page_slots * kvd)
+        self.k = [Buf(ctx, nbytes) for _ in range(n_layer)]
+        self.v = [Buf(ctx, nbytes) for _ in range(n_layer)]
+        self.spare = list(range(npages - 1, -1, -1))  # the lowest first
+        self.users = [0] * npages                     # conversations that hold a page
+        self.pages: dict[int, list[int]] = {}
+        self.len: dict[int, int] = {}
+        self._next = 0
+        self._table: Buf | None = None
+
+    def new(self) -> int:
+        """A conversation without slots."""
+        self._next += 1
+        self.pages[self._next], self.len[self._next] = [], 0
+        return self._next
+
+    def fork(self, seq: int) -> int:
+        """A conversation with the slots of seq, its pages shared."""
+        to = self.new()
+        self.pages[to], self.len[to] = list(self.pages[seq]), self.len[seq]
+        for p in self.pages[to]:
+            self.users[p] += 1
+        return to
+
+    def drop(self, seq: int) -> None:
+        """The end of a conversation: its pages go back to the pool, but for those that others share."""
+        self.truncate(seq, 0)
+        del self.pages[seq], self.len[seq]
+
+    def truncate(self, seq: int, length: int) -> None:
+        """Keeps a conversation's first `length` slots (the rows of a verify pass that were accepted)."""
+        if length > self.len[seq]:
+            raise ValueError(f"conversation {seq} has {self.len[seq]} slots, not {length}")
+        held = self.pages[seq]
+        while len(held) > -(-length // self.page_slots):
+            p = held.pop()
+            self.users[p] -= 1
+            if self.users[p] == 0:
+                self.spare.append(p)
+        self.len[seq] = length
+
+    def extend(self, seqs, rows) -> None:
+        """Slots for rows[i] new rows of each conversation seqs[i] (each named once): pages that a
+        conversation lacks, and its own copy of a shared page that the rows go into. With too few
+        pages left nothing changes (MemoryError)."""
+        if len(set(seqs)) != len(seqs) or len(seqs) != len(rows):
+            raise ValueError("each conversation once, with a number of rows")
+        src, dst, plan, users, left = [], [], [], {}, len(self.spare)
+        for s, n in zip(seqs, rows):
+            held, length = self.pages[s], self.len[s]
+            last = length // self.page_slots  # the page of the first new row
+            own = None
+            if n > 0 and last < len(held):
+                have = users.get(held[last], self.users[held[last]])
+                if have > 1:
+                    own, users[held[last]] = last, have - 1
+            need = -(-(length + n) // self.page_slots) - len(held)
+            left -= need + (own is not None)
+            plan.append((s, own, need, length + n))
+        if left < 0:
+            raise MemoryError(f"{-left} pages too few for {sum(rows)} rows")
+        for s, own, need, length in plan:
+            held = self.pages[s]
+            if own is not None:
+                to = self._take()
+                src.append(held[own])
+                dst.append(to)
+                self.users[held[own]] -= 1
+                held[own] = to
+            held.extend(self._take() for _ in range(need))
+            self.len[s] = length
+        if src:
+            self.ctx.copy_pages(self.k + self.v, self.kv_type, self.page_slots * self.kvd, self.npages, src, dst)
+
+    def _take(self) -> int:
+        p = self.spare.pop()
+        self.users[p] = 1
+        return p
+
+    def table(self, seqs):
+        """The device page table of these conversations, and its pages a line."""
+        stride = max([len(self.pages[s]) for s in seqs] + [1])
+        t = np.full((len(seqs), stride), self.npages, np.uint32)
+        for line, s in zip(t, seqs):
+            line[:len(self.pages[s])] = self.pages[s]
+        if self._table is None or self._table.nbytes < t.nbytes:
+            if self._table is not None:
+                self._table.free()
+            self._table = Buf(self.ctx, max(2 * t.nbytes, 4096))
+        self.ctx.upload(t, self._table)
+        return self._table, stride
+
+    def free(self) -> None:
+        for b in self.k + self.v + ([self._table] if self._table is not None else []):
+            b.free()
+        self.k, self.v, self._table = [], [], None
 
 
 def _batch(row_starts, seq_lens):

@@ -248,7 +248,7 @@ __global__ __launch_bounds__(BM_JOIN) void k_beam_join(const BmParams p) {
             // threads' decides.)
             BmKey mine[BM_KEYS];
             const BmKey last = best[p.k - 1];
-            uint64_t from = floor;
+            uint64_t from = found >= p.k ? floor : 0;  // (fewer groups say nothing of the k'th continuation)
             top = 0;
             uint32_t more = 0;
 #pragma unroll

@@ -11,7 +11,10 @@ residual add,
 RMSNorm, gate and up products, SiLU-mul, the down product and the residual add. Weights
 stay in their ggml blocks (bchip_matmul). The cache is a bchip.KvCache (Gpu::reserve's
 growth, mod.rs:404-423); positions and the tree's visibility masks come from the caller's
-Shape (model.rs:405-443), as in the reference."""
+Shape (model.rs:405-443), as in the reference.
+
+GpuLayers.forward_paged takes the rows of several conversations at once instead, their caches pages
+of one bchip.PagePool, and GpuLayers.beams picks the continuations of beam searches."""
 from __future__ import annotations
 
 import contextlib
@@ -134,25 +137,16 @@ class GpuLayers:
         c, ctx = self.cfg, self.ctx
         rows = len(positions)
         cache.reserve(pos + rows, pos, c.context)
-        e, hd, nh, nkv = c.n_embd, c.head_dim, c.n_head, c.n_head_kv
-        qd, kvd = nh * hd, nkv * hd
+        hd, nh, nkv = c.head_dim, c.n_head, c.n_head_kv
         s = self._scratch(rows)
-        ctx.upload(np.ascontiguousarray(x, np.float32), s["x"])
-        ctx.upload(np.ascontiguousarray(positions, np.uint32), s["pos"])
         mb, seen = None, pos
         if masks is not None:
             seen, visible = masks
             ctx.upload(bchip.masks_words(visible), s["mask"])
             mb = s["mask"]
         scale = 1.0 / math.sqrt(hd)
-        for l, kc, vc in zip(self.layers, cache.k, cache.v):
-            ctx.rms_norm(s["x"], l["attn_norm"], s["n"], rows, e, c.eps)
-            self._matmul(l["wq"], s["n"], s["q"], rows)
-            self._matmul(l["wk"], s["n"], s["k"], rows)
-            self._matmul(l["wv"], s["n"], s["v"], rows)
-            for bias, out, dim in ((l["bq"], s["q"], qd), (l["bk"], s["k"], kvd), (l["bv"], s["v"], kvd)):
-                if bias is not None:
-                    ctx.bias_add(out, bias, rows * dim, dim)
+
+        def attend(kc, vc):
             if rows == 1 and masks is None:
                 # A one-token line step: the five commands as one launch (same bits).
                 ctx.rope_append_attention(s["q"], s["k"], s["v"], kc, vc, self.kv_type, self.freq, s["pos"], nh, nkv,
@@ -167,6 +161,56 @@ class GpuLayers:
                                 c.rope_dim, c.rope_neox, pos)
                 ctx.attention(s["q"], kc, vc, self.kv_type, s["att"], mb, masks is not None, rows, nh, nkv, hd, seen,
                               scale)
+
+        return self._layers(x, positions, cache, attend)
+
+    def new_pool(self, npages: int, page_slots: int = 16) -> bchip.PagePool:
+        """A pool of pages for this stage's caches (kv_type F32 or F16)."""
+        return bchip.PagePool(self.ctx, len(self.layers), self.cfg.n_head_kv * self.cfg.head_dim, npages, page_slots, self.kv_type)
+
+    def forward_paged(self, x: np.ndarray, seqs, rows, pool: bchip.PagePool) -> np.ndarray:
+        """The layers over new rows of several conversations in one pass: rows[i] hidden states of
+        conversation seqs[i] (a piece of a prompt, a token, none), in that order, appended to its pages
+        at its next slots; returns the updated states. Pages that a conversation lacks or shares are
+        taken first (PagePool.extend)."""
+        c, ctx = self.cfg, self.ctx
+        if len(x) != sum(rows):
+            raise ValueError(f"{len(x)} states for {sum(rows)} rows")
+        pool.extend(seqs, rows)
+        lens = [pool.len[s] for s in seqs]
+        positions = np.concatenate([np.arange(m - n, m) for n, m in zip(rows, lens)]) if len(x) else np.zeros(0)
+        starts = np.concatenate([[0], np.cumsum(rows)]).astype(np.uint32)
+        table, stride = pool.table(seqs)
+        s = self._scratch(max(len(x), 1))
+        hd, nh, nkv = c.head_dim, c.n_head, c.n_head_kv
+        batch = (starts, np.asarray(lens, np.uint32), table, stride, pool.page_slots, pool.npages, nh, nkv, hd)
+
+        def attend(kc, vc):
+            ctx.rope_append_paged(s["q"], s["k"], s["v"], kc, vc, pool.kv_type, self.freq, s["pos"], *batch, c.rope_dim, c.rope_neox)
+            ctx.attention_paged(s["q"], kc, vc, pool.kv_type, s["att"], *batch, 1.0 / math.sqrt(hd))
+
+        return self._layers(x, positions, pool, attend)
+
+    def _layers(self, x: np.ndarray, positions, cache, attend) -> np.ndarray:
+        """Every layer over the states x at `positions`; attend(kc, vc) turns the layer's q, k and v
+        rows, appends, and leaves the attention's output in the scratch."""
+        c, ctx = self.cfg, self.ctx
+        rows, e = len(positions), c.n_embd
+        qd, kvd = c.n_head * c.head_dim, c.n_head_kv * c.head_dim
+        if rows == 0:
+            return np.zeros((0, e), np.float32)
+        s = self._scratch(rows)
+        ctx.upload(np.ascontiguousarray(x, np.float32), s["x"])
+        ctx.upload(np.ascontiguousarray(positions, np.uint32), s["pos"])
+        for l, kc, vc in zip(self.layers, cache.k, cache.v):
+            ctx.rms_norm(s["x"], l["attn_norm"], s["n"], rows, e, c.eps)
+            self._matmul(l["wq"], s["n"], s["q"], rows)
+            self._matmul(l["wk"], s["n"], s["k"], rows)
+            self._matmul(l["wv"], s["n"], s["v"], rows)
+            for bias, out, dim in ((l["bq"], s["q"], qd), (l["bk"], s["k"], kvd), (l["bv"], s["v"], kvd)):
+                if bias is not None:
+                    ctx.bias_add(out, bias, rows * dim, dim)
+            attend(kc, vc)
             self._matmul(l["wo"], s["att"], s["o"], rows)
             ctx.add(s["x"], s["o"], rows * e)
             ctx.rms_norm(s["x"], l["ffn_norm"], s["n"], rows, e, c.eps)
@@ -256,6 +300,41 @@ class GpuLayers:
             got = self.ctx.read(vals, rows * (2 + top))
             best = self.ctx.read(ids, (rows, top), np.uint32)
         return (None if tokens is None else got[:rows]), got[rows:2 * rows], best, got[2 * rows:].reshape(rows, top)
+
+    def beams(self, x: np.ndarray, sums, k: int, upto: int | None = None):
+        """A step of beam search on the device: the logits head of x (a row for every beam, `sums`
+        [searches][beams] of them, the log probabilities of the beams so far, -inf for one that is not
+        there), then the k best continuations of each search (bchip_beam_select). Gives their scores, beams
+        and tokens [searches][k]; only these come back to the host. Searches are scored in pieces of at
+        most SCORE_BYTES (one search at least), with the same results."""
+        if self.head is None:
+            raise ValueError("this stage has no output head")
+        sums = np.ascontiguousarray(sums, np.float32)
+        n, beams = sums.shape
+        if len(x) != n * beams:
+            raise ValueError(f"{len(x)} states for {n} searches of {beams} beams")
+        norm, out, ty, vr, vc = self.head
+        upto = vr if upto is None else min(upto, vr)
+        if n == 0:
+            return np.zeros((0, k), np.float32), np.zeros((0, k), np.uint32), np.zeros((0, k), np.uint32)
+        s, ctx, bufs = self._scratch(len(x)), self.ctx, []
+        ctx.upload(np.ascontiguousarray(x, np.float32), s["x"])
+        ctx.rms_norm(s["x"], norm, s["n"], len(x), self.cfg.n_embd, self.cfg.eps)
+        count = max(1, min(-(-len(x) * upto * 4 // self.SCORE_BYTES), n // 2 if beams == 1 else n))
+        ends = [n * i // count for i in range(count + 1)]
+        try:
+            for words in (n * beams, n * k, n * k, n * k, max(b - a for a, b in zip(ends, ends[1:])) * beams * upto):
+                bufs.append(ctx.zeros(4 * words))
+            sb, best, beam, token, scores = bufs
+            ctx.upload(sums, sb)
+            for a, b in zip(ends, ends[1:]):
+                ctx.matmul(out, ty, s["n"].offset(a * beams * vc * 4), scores, upto, vc, (b - a) * beams)
+                at = [y.offset(4 * a * k) for y in (best, beam, token)]
+                ctx.beam_select(scores, sb.offset(4 * a * beams), b - a, beams, upto, k, *at)
+            return ctx.read(best, (n, k)), ctx.read(beam, (n, k), np.uint32), ctx.read(token, (n, k), np.uint32)
+        finally:
+            for y in bufs:
+                y.free()
 
     def free(self) -> None:
         for l in self.layers:

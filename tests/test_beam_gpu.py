@@ -72,7 +72,8 @@ def drawn(rng, n, beams, vocab):
 
 
 @pytest.mark.parametrize("n,beams,vocab,k", [(1, 1, 1, 1), (1, 1, 5, 5), (3, 2, 7, 14), (1, 4, 1000, 8), (5, 3, 8191, 6), (2, 4, 8193, 64), (1, 64, 500, 64),
-                                             (2, 8, 40000, 16), (1, 4, 151936, 8), (1, 2, 600000, 4), (40, 5, 3000, 10), (700, 4, 300, 8), (1, 64, 70000, 64)])
+                                             (2, 8, 40000, 16), (1, 4, 151936, 8), (1, 2, 600000, 4), (40, 5, 3000, 10), (700, 4, 300, 8), (1, 64, 70000, 64), (5, 1, 256, 6),
+                                             (6, 1, 1000, 20), (4, 1, 1025, 64), (2, 3, 2048, 33), (1, 1, 1048576, 64), (1, 5, 900000, 64)])
 def test_the_best_continuations(ctx, n, beams, vocab, k):
     rng = np.random.default_rng(vocab + k)
     check(ctx, *drawn(rng, n, beams, vocab), k)
