@@ -1,12 +1,13 @@
 // Attention over a cache in pages (paged.hpp) of many query rows a KV head: prompts, pieces of them,
 // verify passes; the fold of chunks, and the plan of a call.
 //
-// Mathematics and layout as in attention_paged_row.hip. A workgroup takes 64 or 128 query rows of one
+// Mathematics and layout as in paged_row.hpp. A workgroup takes 64 or 128 query rows of one
 // KV head and its waves share each tile of K and V, two of which are in LDS: the next one arrives
 // while this one is computed.
 #include "internal.hpp"
 #include "paged.hpp"
 #include "paged_launch.hpp"
+#include "paged_row.hpp"
 #include "parts.hpp"
 
 #include <algorithm>
@@ -24,10 +25,10 @@ struct PgBlock {
 };
 
 template <uint32_t QT, uint32_t SLOTS>
-__device__ __forceinline__ PgBlock block_of(const PgParams& p, const PgItem& it, uint32_t block) {
+__device__ __forceinline__ PgBlock block_of(const PgParams& p, const PgItem& it, uint32_t kvh, uint32_t block) {
     PgBlock b;
     const uint32_t rows = it.rows_seq >> 8, nq = rows * p.G, nqt = (nq - 1) / QT + 1, local = block - it.block0;
-    b.kvh = blockIdx.x % p.nkv;
+    b.kvh = kvh;
     const uint32_t qt = nqt - 1 - local % nqt, chunk = local / nqt;  // the longest lists first
     b.q0 = qt * QT;
     b.q1 = min(b.q0 + QT, nq);
@@ -35,12 +36,12 @@ __device__ __forceinline__ PgBlock block_of(const PgParams& p, const PgItem& it,
     b.h0 = b.q0 - b.r0 * p.G;
     b.seen = it.len - rows + b.r0 + 1;                // slots that every row here sees,
     b.end = it.len - rows + (b.q1 - 1) / p.G + 1;     // and the last one
-    b.nchunk = ((it.len - 1) / SLOTS) / p.chunk + 1;
+    b.nchunk = ((it.len - 1) / SLOTS) / p.tchunk + 1;
     const uint32_t all = (b.end - 1) / SLOTS + 1;
-    b.t0 = min(chunk * p.chunk, all);
-    b.t1 = min(b.t0 + p.chunk, all);
+    b.t0 = min(chunk * p.tchunk, all);
+    b.t1 = min(b.t0 + p.tchunk, all);
     b.next = b.nchunk;
-    b.unit = ((size_t)it.block0 * p.nkv + (size_t)b.kvh * nqt * b.nchunk + (size_t)qt * b.nchunk) * (QT / 16) + chunk;
+    b.unit = (size_t)p.blocks * p.nkv + ((size_t)it.block0 * p.nkv + (size_t)b.kvh * nqt * b.nchunk + (size_t)qt * b.nchunk) * (QT / 16) + chunk;
     return b;
 }
 
@@ -60,23 +61,28 @@ __device__ __forceinline__ PgRow row_of(const PgParams& p, const PgItem& it, con
 // Every wave's LDS writes and reads are done, its loads have arrived.
 __device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// Bytes of LDS of a workgroup: two tiles of K and V each.
+template <typename KVT, int NB>
+constexpr uint32_t PG_TILE_LDS = (sizeof(KVT) == 2 ? 16 : 8) * PgTile<KVT, NB>::GRANULE + 16;
+
 // f16 caches. RT 2: four waves of 32 query rows; RT 1: eight waves, four of them 16 query rows each over
 // half of a tile's slots and four the same rows over the other half.
+// Block `id` of the items of more than 16 query rows. lds: PG_TILE_LDS bytes, 16-byte aligned.
 template <int NB, int RT>
-__global__ __launch_bounds__(RT == 1 ? 512 : 256, 2) void attn_paged_tile16(const PgParams p) {
+__device__ __forceinline__ void tile16_block(const PgParams& p, uint32_t id, uint8_t* lds) {
     using T = PgTile<f16, NB>;
     constexpr int NF = 2 * NB, KS = RT == 1 ? 2 : 1;
     constexpr uint32_t QT = 64 * RT, SLOTS = 64;
-    __shared__ __attribute__((aligned(16))) uint8_t kt[2][4 * T::GRANULE];
-    __shared__ __attribute__((aligned(16))) uint8_t vt[2][4 * T::GRANULE];
-    __shared__ uint32_t odd_tile[2];  // 1 + the tile of each buffer whose V holds an infinity or a NaN
-    static_assert(KS == 1 || sizeof kt >= sizeof(f32x4) * 4 * NF * 64, "the second waves' states");
+    uint8_t(*kt)[4 * T::GRANULE] = (uint8_t(*)[4 * T::GRANULE])lds, (*vt)[4 * T::GRANULE] = (uint8_t(*)[4 * T::GRANULE])(lds + 8 * T::GRANULE);
+    uint32_t* odd_tile = (uint32_t*)(lds + 16 * T::GRANULE);  // 1 + the tile of each buffer whose V holds an infinity or a NaN
+    static_assert(KS == 1 || 8 * T::GRANULE >= sizeof(f32x4) * 4 * NF * 64, "the second waves' states");
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) & 3);
     const uint32_t ks = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const uint32_t m16 = lane & 15, g = lane >> 4;
-    const uint32_t block = blockIdx.x / p.nkv;
-    const PgItem it = item_with_arguments<false>(p, block);
-    const PgBlock b = block_of<QT, SLOTS>(p, it, block);
+    const uint32_t block = id / p.nkv;
+    uint32_t which;
+    const PgItem it = item_with_arguments<false>(p, false, block, which);
+    const PgBlock b = block_of<QT, SLOTS>(p, it, id % p.nkv, block);
     if (b.t0 >= b.t1) {  // nothing of these rows' lists
         if (threadIdx.x < QT) {
             const size_t u = b.unit + threadIdx.x / 16 * b.next;
@@ -293,8 +299,8 @@ __global__ __launch_bounds__(RT == 1 ? 512 : 256, 2) void attn_paged_tile16(cons
     }
 
     if constexpr (KS == 2) {  // the two halves of the slots
-        f32x4(*so)[NF][64] = (f32x4(*)[NF][64]) & kt;
-        float(*sr)[2][64] = (float(*)[2][64]) & vt;
+        f32x4(*so)[NF][64] = (f32x4(*)[NF][64])kt;
+        float(*sr)[2][64] = (float(*)[2][64])vt;
         __syncthreads();
         if (ks) {
             sr[wave][0][lane] = ref[0];
@@ -335,18 +341,18 @@ __global__ __launch_bounds__(RT == 1 ? 512 : 256, 2) void attn_paged_tile16(cons
 
 // f32 caches: four waves of 16 query rows, tiles of 32 slots.
 template <int NB>
-__global__ __launch_bounds__(256, NB > 4 ? 1 : 2) void attn_paged_tile32(const PgParams p) {
+__device__ __forceinline__ void tile32_block(const PgParams& p, uint32_t id, uint8_t* lds) {
     using T = PgTile<float, NB>;
     constexpr int NF = 2 * NB, NJ = 2 * NB, NS = NB / 2, TAIL = NB % 2;
     constexpr uint32_t QT = 64, SLOTS = 32;
-    __shared__ __attribute__((aligned(16))) uint8_t kt[2][2 * T::GRANULE];
-    __shared__ __attribute__((aligned(16))) uint8_t vt[2][2 * T::GRANULE];
-    __shared__ uint32_t odd_tile[2];
+    uint8_t(*kt)[2 * T::GRANULE] = (uint8_t(*)[2 * T::GRANULE])lds, (*vt)[2 * T::GRANULE] = (uint8_t(*)[2 * T::GRANULE])(lds + 4 * T::GRANULE);
+    uint32_t* odd_tile = (uint32_t*)(lds + 8 * T::GRANULE);
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t m16 = lane & 15, g = lane >> 4;
-    const uint32_t block = blockIdx.x / p.nkv;
-    const PgItem it = item_with_arguments<false>(p, block);
-    const PgBlock b = block_of<QT, SLOTS>(p, it, block);
+    const uint32_t block = id / p.nkv;
+    uint32_t which;
+    const PgItem it = item_with_arguments<false>(p, false, block, which);
+    const PgBlock b = block_of<QT, SLOTS>(p, it, id % p.nkv, block);
     if (b.t0 >= b.t1) {
         if (threadIdx.x < QT) {
             const size_t u = b.unit + threadIdx.x / 16 * b.next;
@@ -516,6 +522,37 @@ __global__ __launch_bounds__(256, NB > 4 ? 1 : 2) void attn_paged_tile32(const P
         }
 }
 
+template <int NB, int RT>
+__global__ __launch_bounds__(RT == 1 ? 512 : 256, 2) void attn_paged_tile16(const PgParams p) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[PG_TILE_LDS<f16, NB>];
+    tile16_block<NB, RT>(p, blockIdx.x, lds);
+}
+template <int NB>
+__global__ __launch_bounds__(256, NB > 4 ? 1 : 2) void attn_paged_tile32(const PgParams p) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[PG_TILE_LDS<float, NB>];
+    tile32_block<NB>(p, blockIdx.x, lds);
+}
+
+// A batch of both kinds in one launch: the second kind's blocks first, which take longest and are bound by the
+// matrix cores, the first kind's beside and behind them, bound by memory. MIXED: where those start (a
+// multiple of 8: their place among the XCDs).
+__host__ __device__ __forceinline__ uint32_t mixed_rows(const PgParams& p) { return (p.tblocks * p.nkv + 7) / 8 * 8; }
+
+template <int NB, bool PK>
+__global__ __launch_bounds__(256, 2) void attn_paged_mixed16(const PgParams p) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[std::max(PG_TILE_LDS<f16, NB>, PG_ROW_LDS<f16, NB, 4>)];
+    const uint32_t rows = mixed_rows(p);
+    if (blockIdx.x >= rows) row_block<f16, NB, PK, 4>(p, blockIdx.x - rows, lds);
+    else if (blockIdx.x < p.tblocks * p.nkv) tile16_block<NB, 2>(p, blockIdx.x, lds);
+}
+template <int NB>
+__global__ __launch_bounds__(256, NB > 4 ? 1 : 2) void attn_paged_mixed32(const PgParams p) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[std::max(PG_TILE_LDS<float, NB>, PG_ROW_LDS<float, NB, 4>)];
+    const uint32_t rows = mixed_rows(p);
+    if (blockIdx.x >= rows) row_block<float, NB, false, 4>(p, blockIdx.x - rows, lds);
+    else if (blockIdx.x < p.tblocks * p.nkv) tile32_block<NB>(p, blockIdx.x, lds);
+}
+
 // The chunks of 16 query rows of a list brought together, one operand's columns a workgroup, each wave a
 // share of the chunks; states lie as their waves held them. A chunk without a weight left its columns
 // unwritten.
@@ -526,12 +563,14 @@ __global__ __launch_bounds__(64 * WAVES) void attn_paged_fold(const PgParams p) 
     __shared__ float sr[WAVES][64], sl[WAVES][64];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m16 = lane & 15, g = lane >> 4;
     const uint32_t f = blockIdx.z, kvh = blockIdx.y;
-    const PgItem it = item_with_arguments<true>(p, blockIdx.x);
-    const uint32_t slots = p.qt == 16 ? (sizeof(KVT) == 2 ? 32 : 16) : (sizeof(KVT) == 2 ? 64 : 32);  // of a tile
-    const uint32_t rows = it.rows_seq >> 8, nq = rows * p.G, groups = ((nq - 1) / p.qt + 1) * (p.qt / 16);
-    const uint32_t chunks = ((it.len - 1) / slots) / p.chunk + 1, group = blockIdx.x - it.fold0, n = 16 * group + m16;
+    uint32_t which;
+    const PgItem it = item_with_arguments<true>(p, false, blockIdx.x, which);
+    const bool row = which < p.nrow;
+    const uint32_t slots = (row ? 16 : 32) * (sizeof(KVT) == 2 ? 2 : 1), qt = row ? 16 : p.qt;  // of a tile, of a block
+    const uint32_t rows = it.rows_seq >> 8, nq = rows * p.G, groups = ((nq - 1) / qt + 1) * (qt / 16);
+    const uint32_t chunks = ((it.len - 1) / slots) / (row ? p.chunk : p.tchunk) + 1, group = blockIdx.x - it.fold0, n = 16 * group + m16;
     const bool valid = n < nq;
-    const size_t u0 = (size_t)it.block0 * p.nkv * (p.qt / 16) + ((size_t)kvh * groups + group) * chunks;
+    const size_t u0 = (row ? 0 : (size_t)p.blocks * p.nkv) + (size_t)it.block0 * p.nkv * (qt / 16) + ((size_t)kvh * groups + group) * chunks;
     const float2* ml = (const float2*)p.part_ml + u0 * 16 + m16;
     const f32x4* at = (const f32x4*)p.part_o + (u0 * NF + f) * 64 + lane;
     f32x4 a = {0, 0, 0, 0};
@@ -590,16 +629,18 @@ __global__ __launch_bounds__(64 * WAVES) void attn_paged_fold(const PgParams p) 
 
 template <typename KVT, int NB>
 void launch_fold(const PgParams& p, uint32_t groups, uint32_t most, hipStream_t s) {
-    // A wave alone holds a few chunks' states at once; more chunks are shared out.
+    // A wave alone holds eight chunks' states at once; more chunks are shared out, among few waves where there
+    // are many groups (two prompts' pieces beside ten steps: 30 us by eight waves, as their longest list
+    // would have it, 14 by two).
     const dim3 grid(groups, p.nkv, 2 * NB);
     if (most <= 8) hipLaunchKernelGGL((attn_paged_fold<KVT, NB, 1>), grid, dim3(64), 0, s, p);
-    else if (most <= 16) hipLaunchKernelGGL((attn_paged_fold<KVT, NB, 2>), grid, dim3(128), 0, s, p);
+    else if (most <= 16 || groups >= 64) hipLaunchKernelGGL((attn_paged_fold<KVT, NB, 2>), grid, dim3(128), 0, s, p);
     else hipLaunchKernelGGL((attn_paged_fold<KVT, NB, 8>), grid, dim3(512), 0, s, p);
 }
 
 template <int NB>
 void launch_tile16(const PgParams& p, hipStream_t s) {
-    const dim3 grid(p.blocks * p.nkv);
+    const dim3 grid(p.tblocks * p.nkv);
     if constexpr (NB <= 4) {
         if (p.qt == 128) {
             hipLaunchKernelGGL((attn_paged_tile16<NB, 2>), grid, dim3(256), 0, s, p);
@@ -610,31 +651,42 @@ void launch_tile16(const PgParams& p, hipStream_t s) {
 }
 template <int NB>
 void launch_tile32(const PgParams& p, hipStream_t s) {
-    hipLaunchKernelGGL((attn_paged_tile32<NB>), dim3(p.blocks * p.nkv), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((attn_paged_tile32<NB>), dim3(p.tblocks * p.nkv), dim3(256), 0, s, p);
+}
+template <int NB>
+void launch_mixed(const PgParams& p, bool f16_cache, hipStream_t s) {
+    const dim3 grid(mixed_rows(p) + (p.blocks + 7) / 8 * 8 * p.nkv);
+    if (!f16_cache) {
+        hipLaunchKernelGGL((attn_paged_mixed32<NB>), grid, dim3(256), 0, s, p);
+    } else if constexpr (NB <= 4) {
+        if (pg_few(p)) hipLaunchKernelGGL((attn_paged_mixed16<NB, true>), grid, dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((attn_paged_mixed16<NB, false>), grid, dim3(256), 0, s, p);
+    }
 }
 
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
-// What a launch over p's items (block rows p.qt, tiles of `slots` slots) takes in chunks of p.chunk
-// tiles: their places, the states, and the groups of the fold (which gives its own places to items
-// whose lists are whole, none of them).
+// What a launch over p's items in chunks of p.chunk and p.tchunk tiles takes: the blocks' places, the
+// states, and the groups of the fold (items whose lists are whole have none).
 struct PgPlan {
     uint64_t states = 0;  // groups of 16 query rows
     uint32_t groups = 0, most = 1;
 };
-PgPlan place(PgParams& p, uint32_t slots) {
+PgPlan place(PgParams& p, bool f16_cache) {
     PgPlan plan;
-    p.blocks = 0;
+    p.blocks = p.tblocks = 0;
     for (uint32_t i = 0; i < p.nitems; i++) {
         PgItem& it = p.items[i];
-        const uint32_t nq = (it.rows_seq >> 8) * p.G, nqt = ceil_div(nq, p.qt), chunks = (it.len - 1) / slots / p.chunk + 1;
-        it.block0 = p.blocks;
+        const bool row = i < p.nrow;
+        const uint32_t nq = (it.rows_seq >> 8) * p.G, chunks = (it.len - 1) / (row ? pg_row_tile(f16_cache) : pg_tile(f16_cache)) / (row ? p.chunk : p.tchunk) + 1;
+        uint32_t& blocks = row ? p.blocks : p.tblocks;
+        it.block0 = blocks;
         it.fold0 = plan.groups;
-        p.blocks += nqt * chunks;
+        blocks += (row ? 1 : ceil_div(nq, p.qt)) * chunks;
         if (chunks > 1) plan.groups += ceil_div(nq, 16);
         plan.most = std::max(plan.most, chunks);
     }
-    plan.states = (uint64_t)p.blocks * p.nkv * (p.qt / 16);
+    plan.states = ((uint64_t)p.blocks + (uint64_t)p.tblocks * (p.qt / 16)) * p.nkv;
     return plan;
 }
 
@@ -648,56 +700,47 @@ bool reserve(PgParams& p, const PgPlan& plan, Workspace& ws) {
 
 constexpr uint32_t WHOLE = 0x40000000u;  // tiles: no list has as many
 
-// Items of at most 16 query rows.
-hipError_t run_rows(PgParams& p, bool f16_cache, Workspace& ws, hipStream_t s) {
+// Items of at most 16 query rows: the chunks. Whether they are brief: lists that eight waves take in a few
+// tiles each are not cut (no second launch).
+bool cut_rows(PgParams& p, bool f16_cache) {
     const uint32_t slots = pg_row_tile(f16_cache);
     uint64_t total = 0, most = 0;
-    for (uint32_t i = 0; i < p.nitems; i++) {
+    for (uint32_t i = 0; i < p.nrow; i++) {
         const uint64_t tiles = (p.items[i].len - 1) / slots + 1;
         total += tiles;
         most = std::max(most, tiles);
     }
-    p.qt = 16;
-    // Lists that eight waves take in a few tiles each are not cut: no second launch.
-    const bool brief = most <= 20;
     p.chunk = WHOLE;
-    if (!brief) {
-        // Chunks of whole rounds of the waves, as short as leaves every workgroup a place at once.
-        constexpr uint32_t groups = 512;
-        p.chunk = std::max<uint32_t>(4, ceil_div(ceil_div(total * p.nkv, groups), 4) * 4);
-        auto blocks = [&] {
-            uint64_t n = 0;
-            for (uint32_t i = 0; i < p.nitems; i++) n += (p.items[i].len - 1) / slots / p.chunk + 1;
-            return n * p.nkv;
-        };
-        while (p.chunk < most && blocks() > groups) p.chunk += std::max(4u, p.chunk / 16 / 4 * 4);
-    }
-    PgPlan plan = place(p, slots);
-    if (plan.groups && !reserve(p, plan, ws)) {  // whole lists
-        p.chunk = WHOLE;
-        plan = place(p, slots);
-    }
-    paged_rows_launch(p, f16_cache, brief, s);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || !plan.groups) return e;
-    paged_fold_launch(p, f16_cache, plan.groups, plan.most, s);
-    return hipGetLastError();
+    if (most <= 20) return true;
+    // Chunks of whole rounds of the waves, as short as leaves every workgroup a place at once; beside blocks of
+    // the second kind, which fill the CUs, a quarter of as many (ten steps beside two prompts' pieces of
+    // 28 x 4 heads of 128: 83 us, 95 with as many).
+    const uint32_t groups = p.nrow < p.nitems ? 128 : 512;
+    p.chunk = std::max<uint32_t>(4, ceil_div(ceil_div(total * p.nkv, groups), 4) * 4);
+    auto blocks = [&] {
+        uint64_t n = 0;
+        for (uint32_t i = 0; i < p.nrow; i++) n += (p.items[i].len - 1) / slots / p.chunk + 1;
+        return n * p.nkv;
+    };
+    while (p.chunk < most && blocks() > groups) p.chunk += std::max(4u, p.chunk / 16 / 4 * 4);
+    return false;
 }
 
-// Items of more.
-hipError_t run_tiles(PgParams& p, bool f16_cache, Workspace& ws, hipStream_t s) {
+// Items of more: query rows a block, and the chunks.
+void cut_tiles(PgParams& p, bool f16_cache) {
     const uint32_t slots = pg_tile(f16_cache);
-    std::sort(p.items, p.items + p.nitems, [](const PgItem& a, const PgItem& b) { return a.len > b.len; });
-    uint64_t few = 0, many = 0;  // query blocks of at most 64 rows, of more
-    for (uint32_t i = 0; i < p.nitems; i++) ((uint64_t)(p.items[i].rows_seq >> 8) * p.G <= 64 ? few : many)++;
+    std::sort(p.items + p.nrow, p.items + p.nitems, [](const PgItem& a, const PgItem& b) { return a.len > b.len; });
+    uint64_t few = 0, many = 0, longest = 0;  // query blocks of at most 64 rows, of more; a list's tiles
+    for (uint32_t i = p.nrow; i < p.nitems; i++) {
+        ((uint64_t)(p.items[i].rows_seq >> 8) * p.G <= 64 ? few : many)++;
+        longest = std::max<uint64_t>(longest, (p.items[i].len - 1) / slots + 1);
+    }
     p.qt = f16_cache && p.hd <= 128 && many >= few ? 128 : 64;
-    uint64_t longest = 0;  // list's tiles
-    for (uint32_t i = 0; i < p.nitems; i++) longest = std::max<uint64_t>(longest, (p.items[i].len - 1) / slots + 1);
     constexpr uint64_t CUS = 256;
     const float tile = f16_cache ? 0.2f + 0.011f * p.hd : 0.0133f * p.hd;
     auto time = [&](uint64_t chunk) {
         uint64_t work = 0, blocks = 0, cut = 0;
-        for (uint32_t i = 0; i < p.nitems; i++) {
+        for (uint32_t i = p.nrow; i < p.nitems; i++) {
             const PgItem& it = p.items[i];
             const uint64_t rows = it.rows_seq >> 8, n = ceil_div(rows * p.G, p.qt) * (uint64_t)p.nkv, tiles = ((uint64_t)it.len - rows / 2) / slots + 1;
             const uint64_t chunks = (tiles - 1) / chunk + 1;
@@ -707,19 +750,35 @@ hipError_t run_tiles(PgParams& p, bool f16_cache, Workspace& ws, hipStream_t s) 
         }
         return std::max((float)chunk, (float)ceil_div(blocks, CUS) * work / blocks) * tile + (cut ? 5.0f + (float)cut * p.qt * p.hd * 8 / 4.5e6f : 0.0f);
     };
-    p.chunk = WHOLE;
+    p.tchunk = WHOLE;
+    uint64_t blocks = 0;
+    for (uint32_t i = p.nrow; i < p.nitems; i++) blocks += ceil_div((uint64_t)(p.items[i].rows_seq >> 8) * p.G, p.qt) * (uint64_t)p.nkv;
+    if (blocks >= 4 * CUS) return;  // (every CU has several: nothing to be had)
     float least = time(longest);
     for (uint64_t n = 2; n <= 64 && longest / n >= 2; n++) {
         const uint64_t chunk = ceil_div(longest, n);
         const float t = time(chunk);
-        if (t < least) least = t, p.chunk = (uint32_t)chunk;
+        if (t < least) least = t, p.tchunk = (uint32_t)chunk;
     }
-    PgPlan plan = place(p, slots);
-    if (plan.groups && !reserve(p, plan, ws)) {
-        p.chunk = WHOLE;
-        plan = place(p, slots);
+}
+
+hipError_t run(PgParams& p, bool f16_cache, Workspace& ws, hipStream_t s) {
+    p.qt = 64;
+    p.chunk = p.tchunk = WHOLE;
+    const bool rows = p.nrow > 0, tiles = p.nrow < p.nitems;
+    if (tiles) cut_tiles(p, f16_cache);
+    const bool brief = rows && cut_rows(p, f16_cache);
+    PgPlan plan = place(p, f16_cache);
+    if (plan.groups && !reserve(p, plan, ws)) {  // whole lists
+        p.chunk = p.tchunk = WHOLE;
+        plan = place(p, f16_cache);
     }
-    paged_tiles_launch(p, f16_cache, s);
+    if (rows && tiles && (!f16_cache || p.qt == 128)) {
+        paged_mixed_launch(p, f16_cache, s);
+    } else {
+        if (rows) paged_rows_launch(p, f16_cache, brief, s);
+        if (tiles) paged_tiles_launch(p, f16_cache, s);
+    }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !plan.groups) return e;
     paged_fold_launch(p, f16_cache, plan.groups, plan.most, s);
@@ -732,6 +791,12 @@ void paged_tiles_launch(const PgParams& p, bool f16_cache, hipStream_t s) {
 #define PG_TILE(NB) (f16_cache ? launch_tile16<NB>(p, s) : launch_tile32<NB>(p, s))
     PG_BY_DIM(p.hd, PG_TILE)
 #undef PG_TILE
+}
+
+void paged_mixed_launch(const PgParams& p, bool f16_cache, hipStream_t s) {
+#define PG_MIXED(NB) launch_mixed<NB>(p, f16_cache, s)
+    PG_BY_DIM(p.hd, PG_MIXED)
+#undef PG_MIXED
 }
 
 void paged_fold_launch(const PgParams& p, bool f16_cache, uint32_t groups, uint32_t most, hipStream_t s) {
@@ -756,19 +821,24 @@ hipError_t paged_attention(const PagedCall& a, Workspace& ws, hipStream_t s) {
     base.hd = a.hd;
     base.G = a.nh / a.nkv;
     base.sc = a.scale * LOG2E;
-    for (int many = 0; many < 2; many++) {
+    // Sequences with rows, the first kind first, as many as a launch takes at a time.
+    uint32_t next = 0;
+    while (next < a.pages.nseq) {
         PgParams p = base;
-        for (uint32_t i = 0; i <= a.pages.nseq; i++) {
-            if (p.nitems == PG_ITEMS || (i == a.pages.nseq && p.nitems)) {
-                const hipError_t e = many ? run_tiles(p, f16_cache, ws, s) : run_rows(p, f16_cache, ws, s);
-                if (e != hipSuccess) return e;
-                p.nitems = 0;
+        uint32_t end = next, n = 0;
+        for (; end < a.pages.nseq && n < PG_ITEMS; end++) n += a.pages.starts[end + 1] > a.pages.starts[end];
+        for (int many = 0; many < 2; many++) {
+            if (many) p.nrow = p.nitems;
+            for (uint32_t i = next; i < end; i++) {
+                const uint32_t rows = a.pages.starts[i + 1] - a.pages.starts[i];
+                if (rows == 0 || ((uint64_t)rows * base.G > 16) != (many == 1)) continue;
+                p.items[p.nitems++] = PgItem{a.pages.starts[i], a.pages.lens[i], rows << 8 | i, 0, 0};
             }
-            if (i == a.pages.nseq) break;
-            const uint32_t rows = a.pages.starts[i + 1] - a.pages.starts[i];
-            if (rows == 0 || ((uint64_t)rows * base.G > 16) != (many == 1)) continue;
-            p.items[p.nitems++] = PgItem{a.pages.starts[i], a.pages.lens[i], rows << 8 | i, 0, 0};
         }
+        next = end;
+        if (p.nitems == 0) continue;
+        const hipError_t e = run(p, f16_cache, ws, s);
+        if (e != hipSuccess) return e;
     }
     return hipSuccess;
 }

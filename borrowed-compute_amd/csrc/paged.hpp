@@ -19,14 +19,16 @@
 namespace bchip {
 
 // A sequence's new rows (q and out rows row0 ..) over its `len` slots, which end with theirs: row r sees
-// the slots below len - rows + r + 1. block0: the first of its blocks of the launch; fold0: of its
-// groups of 16 query rows in the fold's.
+// the slots below len - rows + r + 1. block0: the first of its blocks of its kind in the launch; fold0: of
+// its groups of 16 query rows in the fold's.
 struct PgItem {
     uint32_t row0, len, rows_seq, block0, fold0;  // rows << 8 | sequence (its line of the table)
 };
 
 constexpr uint32_t PG_ITEMS = 128;  // of a launch: two a lane
 
+// Items are of two kinds: the first nrow have at most 16 query rows (attn_paged_row's), the others more
+// (attn_paged_tile16's or 32's).
 struct PgParams {
     const float* q;
     const uint8_t* kc;
@@ -37,33 +39,37 @@ struct PgParams {
     const uint32_t* pages;
     uint32_t page_stride, page_shift, npages;
     uint32_t nh, nkv, hd, G;
-    float sc;        // scale * log2(e)
-    uint32_t chunk;  // tiles a chunk
-    uint32_t qt;     // query rows a block
-    uint32_t blocks; // blocks of the launch / KV heads
-    uint32_t nitems;
+    float sc;                 // scale * log2(e)
+    uint32_t chunk, tchunk;   // tiles a chunk, of either kind
+    uint32_t blocks, tblocks; // blocks / KV heads
+    uint32_t qt;              // query rows a block of the second kind, whose states lie behind the first's
+    uint32_t nrow, nitems;
     PgItem items[PG_ITEMS];
 };
 
-// The last item whose first block (fold: group) is at most x.
+// The last of items lo .. hi - 1 whose first block (fold: group) is at most x.
 template <bool FOLD>
-__device__ __forceinline__ uint32_t item_of(const PgParams& p, uint32_t x) {
+__device__ __forceinline__ uint32_t item_of(const PgParams& p, uint32_t lo, uint32_t hi, uint32_t x) {
     const uint32_t lane = threadIdx.x & 63;
     const uint32_t a = FOLD ? p.items[lane].fold0 : p.items[lane].block0, b = FOLD ? p.items[lane + 64].fold0 : p.items[lane + 64].block0;
-    const uint32_t n = __popcll(__ballot(lane < p.nitems && a <= x)) + __popcll(__ballot(lane + 64 < p.nitems && b <= x));
-    return __builtin_amdgcn_readfirstlane(n - 1);
+    const uint32_t n = __popcll(__ballot(lane >= lo && lane < hi && a <= x)) + __popcll(__ballot(lane + 64 >= lo && lane + 64 < hi && b <= x));
+    return __builtin_amdgcn_readfirstlane(lo + n - 1);
 }
 
-// A block's item. Every argument that a kernel's first loads need is read here, item 0 with them, in one
-// round trip: a branch that waits for one argument would else put the others' behind it (the empty asm
-// is their use).
+// A block's item and its number. Every argument that a kernel's first loads need is read here, item 0 with
+// them, in one round trip: a branch that waits for one argument would else put the others' behind it (the
+// empty asm is their use).
 template <bool FOLD>
-__device__ __forceinline__ PgItem item_with_arguments(const PgParams& p, uint32_t x) {
+__device__ __forceinline__ PgItem item_with_arguments(const PgParams& p, bool rows, uint32_t x, uint32_t& which) {
     PgItem it = p.items[0];
     asm volatile("" ::"s"(p.q), "s"(p.kc), "s"(p.vc), "s"(p.out), "s"(p.part_o), "s"(p.part_ml), "s"(p.pages), "s"(p.page_stride),
-                 "s"(p.page_shift), "s"(p.npages), "s"(p.nh), "s"(p.nkv), "s"(p.hd), "s"(p.G), "s"(p.sc), "s"(p.chunk), "s"(p.qt),
-                 "s"(p.blocks), "s"(p.nitems), "s"(it.row0), "s"(it.len), "s"(it.rows_seq), "s"(it.block0), "s"(it.fold0));
-    if (p.nitems > 1) it = p.items[item_of<FOLD>(p, x)];
+                 "s"(p.page_shift), "s"(p.npages), "s"(p.nh), "s"(p.nkv), "s"(p.hd), "s"(p.G), "s"(p.sc), "s"(p.chunk), "s"(p.tchunk), "s"(p.qt),
+                 "s"(p.blocks), "s"(p.nrow), "s"(p.nitems), "s"(it.row0), "s"(it.len), "s"(it.rows_seq), "s"(it.block0), "s"(it.fold0));
+    which = 0;
+    if (p.nitems > 1) {
+        which = item_of<FOLD>(p, FOLD || rows ? 0 : p.nrow, !FOLD && rows ? p.nrow : p.nitems, x);
+        it = p.items[which];
+    }
     return it;
 }
 

@@ -229,3 +229,59 @@ def test_a_page_past_the_pool_gives_nan_and_nothing_else(ctx, rows, n, kv_type):
             sees = (n - rows + np.arange(at.stop - at.start) >= 16 * at_page) if i == 0 else np.zeros(1, bool)
             assert np.isnan(got[at][sees]).all()
             assert (np.abs(got[at] - want) <= most)[~sees].all()
+
+
+@pytest.mark.parametrize("kv_type", [bchip.F16, bchip.F32])
+def test_pages_past_4_gb(ctx, kv_type):
+    """A pool of 4.5 GB a buffer whose sequences' pages lie around and past 2^32 bytes: append, attention and
+    copies as over a small pool."""
+    nh, nkv, hd, es = 16, 8, 128, 2 if kv_type == bchip.F16 else 4
+    page_bytes = 16 * nkv * hd * es
+    npages = int(4.5 * 2 ** 30) // page_bytes
+    edge = 2 ** 32 // page_bytes
+    rng = np.random.default_rng(18)
+    b = Batch(rng, [1, 40], [70, 100], nkv, hd, kv_type)
+    high = np.concatenate([[edge - 1, edge, npages - 1, 3], edge + 1 + np.arange(b.npages - 4)]).astype(np.uint32)  # a page's place in the large pool
+    big = [ctx.zeros(npages * page_bytes) for _ in range(2)]
+    for pool, buf in zip((b.k, b.v), big):
+        for page, at in zip(pool, high):
+            ctx.upload(page, buf, int(at) * page_bytes)
+    table = np.where(b.table < b.npages, high[np.minimum(b.table, b.npages - 1)], 0xFFFFFFFF).astype(np.uint32)
+    q = rng.standard_normal((b.total, nh, hd)).astype(np.float32)
+    kn, vn = (rng.standard_normal((b.total, nkv, hd)).astype(np.float32) for _ in range(2))
+    positions = np.concatenate([np.arange(m - n, m) for n, m in zip(b.rows, b.lens)]).astype(np.uint32)
+    inv = ctx.upload(np.ones(hd // 2, np.float32))
+    outs = []
+    for (kc, vc), tab, pages in ((big, table, npages), ([ctx.upload(b.k), ctx.upload(b.v)], b.table, b.npages)):
+        qb, kb, vb, pb, tb, ob = (ctx.upload(x) for x in (q, kn, vn, positions, tab, np.zeros_like(q)))
+        ctx.rope_append_paged(qb, kb, vb, kc, vc, kv_type, inv, pb, b.starts, b.lens, tb, b.stride, 16, pages, nh, nkv, hd, hd, True)
+        ctx.attention_paged(qb, kc, vc, kv_type, ob, b.starts, b.lens, tb, b.stride, 16, pages, nh, nkv, hd, 0.1)
+        last = int(tab[1, 6])
+        free = 1 if pages == npages else [p for p in range(b.npages) if p not in b.table][0]
+        ctx.copy_pages([kc, vc], kv_type, 16 * nkv * hd, pages, [last], [free])
+        bits = np.uint16 if es == 2 else np.uint32
+        outs.append([ctx.read(ob, q.size, np.uint32)] + [ctx.read(x, 16 * nkv * hd, bits, at * page_bytes) for x in (kc, vc) for at in (last, free)])
+    for x, y in zip(*outs):
+        np.testing.assert_array_equal(x, y)
+    assert np.isfinite(outs[0][0].view(np.float32)).all()
+    for buf in big:
+        buf.free()
+
+
+def test_two_contexts_at_once(ctx):
+    """Calls queued on two contexts beside each other, each with scratch of its own."""
+    rng = np.random.default_rng(19)
+    with bchip.Ctx(0) as other:
+        work = []
+        for c, (rows, lens) in ((ctx, ([1, 1, 30], [9000, 4000, 700])), (other, ([1, 64], [12000, 3000]))):
+            b = Batch(rng, rows, lens, 4, 128, bchip.F16)
+            q = rng.standard_normal((b.total, 16, 128)).astype(np.float32)
+            want = call(c, b, q, 16, 0.1)
+            kb, vb, qb, ob = (c.upload(x) for x in (b.k, b.v, q, np.zeros_like(q)))
+            starts, ln, table, *rest = b.args(c)
+            work.append((c, lambda c=c, a=(qb, kb, vb, bchip.F16, ob, starts, ln, table, *rest, 16, 4, 128, 0.1): c.attention_paged(*a), ob, want))
+        for _ in range(10):
+            for _, go, _, _ in work:
+                go()
+        for c, _, ob, want in work:
+            np.testing.assert_array_equal(c.read(ob, want.shape).view(np.uint32), want.view(np.uint32))

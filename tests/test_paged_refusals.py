@@ -42,8 +42,16 @@ for t in (bchip.F16, bchip.F32):
     assert len(launches()) == 1 and "k_rope_append_paged" in launches()[0][0] and launches()[0][1][0] == 21, launches()
     clear()
     a.attend()
-    names = [n for n, _ in launches()]
-    assert sum("attn_paged_row" in n for n in names) == 1 and sum("attn_paged_tile" in n for n in names) == 1, names
+    assert len(launches()) == 1 and "attn_paged_mixed" in launches()[0][0], launches()  # both kinds of rows at once
+    for rows, name in ((1, "attn_paged_row"), (20, "attn_paged_tile")):
+        a = Args(t=t, starts=[0, rows], lens=[40])
+        clear()
+        a.attend()
+        assert len(launches()) == 1 and name in launches()[0][0], launches()
+    a = Args(t=t, hd=256, rope_dim=256)  # f16 heads past 128: a launch a kind
+    clear()
+    a.attend()
+    assert len(launches()) == (2 if t == bchip.F16 else 1), launches()
 """)
 
 
