@@ -149,12 +149,14 @@ __device__ __forceinline__ uint64_t bm_reach(uint64_t top, uint32_t k, uint32_t*
     high = max(high, (uint32_t)__shfl_xor((int)high, 2));
     if ((threadIdx.x & 3) == 0) highs[threadIdx.x / 4] = high;
     __syncthreads();
-    uint32_t larger = 0;
+    uint32_t larger = 0;  // (a quarter of them each, for the four's largest)
 #pragma unroll 8
-    for (uint32_t i = 0; i < BM_JOIN / 4; i += 4) {
-        const uint4 x = *(const uint4*)&highs[i];
+    for (uint32_t i = 0; i < BM_JOIN / 16; i += 4) {
+        const uint4 x = *(const uint4*)&highs[4 * i + 4 * (threadIdx.x & 3)];
         larger += (uint32_t)(x.x > high) + (uint32_t)(x.y > high) + (uint32_t)(x.z > high) + (uint32_t)(x.w > high);
     }
+    larger += (uint32_t)__shfl_xor((int)larger, 1);
+    larger += (uint32_t)__shfl_xor((int)larger, 2);
     uint32_t low = larger < k ? high : ~0u;
 #pragma unroll
     for (int d = 4; d < 64; d *= 2) low = min(low, (uint32_t)__shfl_xor((int)low, d));
