@@ -423,6 +423,10 @@ class PagePool:
     in one call). The host keeps the tables; a step's is uploaded with it."""
 
     def __init__(self, ctx: "Ctx", n_layer: int, kvd: int, npages: int, page_slots: int = 16, kv_type: int = F16):
+        if kv_type not in (F32, F16):
+            raise ValueError(f"a pool of type {kv_type} (F32 or F16)")
+        if npages < 1 or not 16 <= page_slots <= 1 << 20 or page_slots & (page_slots - 1):
+            raise ValueError(f"{npages} pages of {page_slots} slots (a power of two from 16 to 2^20)")
         self.ctx, self.n_layer, self.kvd, self.kv_type = ctx, n_layer, kvd, kv_type
         self.npages, self.page_slots = npages, page_slots
         nbytes = nbytes_of(kv_type, npages * page_slots * kvd)
@@ -456,7 +460,7 @@ class PagePool:
 
     def truncate(self, seq: int, length: int) -> None:
         """Keeps a conversation's first `length` slots (the rows of a verify pass that were accepted)."""
-        if length > self.len[seq]:
+        if not 0 <= length <= self.len[seq]:
             raise ValueError(f"conversation {seq} has {self.len[seq]} slots, not {length}")
         held = self.pages[seq]
         while len(held) > -(-length // self.page_slots):
@@ -470,7 +474,7 @@ class PagePool:
         """Slots for rows[i] new rows of each conversation seqs[i] (each named once): pages that a
         conversation lacks, and its own copy of a shared page that the rows go into. With too few
         pages left nothing changes (MemoryError)."""
-        if len(set(seqs)) != len(seqs) or len(seqs) != len(rows):
+        if len(set(seqs)) != len(seqs) or len(seqs) != len(rows) or any(n < 0 for n in rows):
             raise ValueError("each conversation once, with a number of rows")
         src, dst, plan, users, left = [], [], [], {}, len(self.spare)
         for s, n in zip(seqs, rows):

@@ -172,16 +172,21 @@ class GpuLayers:
         """The layers over new rows of several conversations in one pass: rows[i] hidden states of
         conversation seqs[i] (a piece of a prompt, a token, none), in that order, appended to its pages
         at its next slots; returns the updated states. Pages that a conversation lacks or shares are
-        taken first (PagePool.extend)."""
+        taken first (PagePool.extend). At most 256 conversations a pass; a refused pass leaves the pool as
+        it was."""
         c, ctx = self.cfg, self.ctx
         if len(x) != sum(rows):
             raise ValueError(f"{len(x)} states for {sum(rows)} rows")
+        if len(seqs) > 256:
+            raise ValueError(f"{len(seqs)} conversations (at most 256 a pass)")
+        if (pool.ctx, pool.n_layer, pool.kvd, pool.kv_type) != (ctx, len(self.layers), c.n_head_kv * c.head_dim, self.kv_type):
+            raise ValueError("the pool is another stage's")
+        s = self._scratch(max(len(x), 1))
         pool.extend(seqs, rows)
         lens = [pool.len[s] for s in seqs]
         positions = np.concatenate([np.arange(m - n, m) for n, m in zip(rows, lens)]) if len(x) else np.zeros(0)
         starts = np.concatenate([[0], np.cumsum(rows)]).astype(np.uint32)
         table, stride = pool.table(seqs)
-        s = self._scratch(max(len(x), 1))
         hd, nh, nkv = c.head_dim, c.n_head, c.n_head_kv
         batch = (starts, np.asarray(lens, np.uint32), table, stride, pool.page_slots, pool.npages, nh, nkv, hd)
 

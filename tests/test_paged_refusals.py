@@ -277,3 +277,74 @@ for call in (lambda: p.extend([a, a], [1, 1]), lambda: p.extend([a], [1, 2]), la
 p.extend([a, f], [12, 13 + 16])
 check()
 """)
+
+
+STAGE = POOL + """
+import layers as L
+m = L.Matrix(0, bytes(4 * 64 * 64), 64, 64)
+one = dict(attn_norm=np.ones(64), ffn_norm=np.ones(64), **{k: m for k in ("wq", "wk", "wv", "wo", "gate", "up", "down")})
+cfg = L.Config(n_embd=64, n_layer=2, n_head=2, n_head_kv=2, head_dim=32, rope_dim=32)
+def raises(what, call):
+    try:
+        call()
+    except what as e:
+        return str(e)
+    raise AssertionError("taken")
+"""
+
+
+def test_a_refused_pass_takes_no_pages(fake):
+    """What forward_paged refuses, and a pass without memory for its rows, leave the pool as it was."""
+    host_side.run(fake, STAGE + """
+g = L.GpuLayers(c, cfg, [one, one], None, bchip.F16)
+many = [p.new() for _ in range(257)]
+def untouched():
+    assert len(p.spare) == 10 and not any(p.len.values()), p.len
+x = lambda n: np.zeros((n, 64), np.float32)
+assert "257" in raises(ValueError, lambda: g.forward_paged(x(1), many, [1] + [0] * 256, p)); untouched()
+raises(ValueError, lambda: g.forward_paged(x(2), many[:1], [1], p)); untouched()
+raises(ValueError, lambda: g.forward_paged(x(1), many[:2], [2, -1], p)); untouched()
+raises(ValueError, lambda: g.forward_paged(x(1), many[:1], [1, 0], p)); untouched()
+fake.fake_budget(1 << 10)
+raises(bchip.BchipError, lambda: g.forward_paged(x(40), many[:1], [40], p)); untouched()
+fake.fake_budget((1 << 64) - 1)
+g.forward_paged(x(40), many[:256], [40] + [0] * 255, p)
+assert p.len[many[0]] == 40 and len(p.spare) == 7
+""")
+
+
+def test_pools_of_another_stage(fake):
+    """A stage takes pools of its own layers, elements and context."""
+    host_side.run(fake, STAGE + """
+x = np.zeros((1, 64), np.float32)
+for n, t in ((1, bchip.F16), (3, bchip.F16), (2, bchip.F32)):
+    g = L.GpuLayers(c, cfg, [one] * n, None, t)
+    s = p.new()
+    raises(ValueError, lambda: g.forward_paged(x, [s], [1], p))
+    assert p.len[s] == 0
+g = L.GpuLayers(c, cfg, [one] * 2, None, bchip.F16)
+small = bchip.PagePool(c, 2, 32, 10)
+s = small.new()
+raises(ValueError, lambda: g.forward_paged(x, [s], [1], small))
+with bchip.Ctx(0) as other:
+    theirs = bchip.PagePool(other, 2, 64, 10)
+    s = theirs.new()
+    raises(ValueError, lambda: g.forward_paged(x, [s], [1], theirs))
+    theirs.free()
+""")
+
+
+def test_pools_that_are_refused(fake):
+    host_side.run(fake, STAGE + """
+raises(ValueError, lambda: bchip.PagePool(c, 2, 64, 10, 16, bchip.Q4))
+for slots in (0, 8, 24, 1 << 21):
+    raises(ValueError, lambda: bchip.PagePool(c, 2, 64, 10, slots))
+raises(ValueError, lambda: bchip.PagePool(c, 2, 64, 0))
+raises(ValueError, lambda: L.GpuLayers(c, cfg, [one], None, bchip.Q4).new_pool(10))
+s = p.new()
+p.extend([s], [20])
+for call in (lambda: p.truncate(s, -1), lambda: p.extend([s], [-1])):
+    raises(ValueError, call)
+    assert p.len[s] == 20
+    check()
+""")
