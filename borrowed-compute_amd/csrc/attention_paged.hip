@@ -10,6 +10,8 @@
 #include "paged_row.hpp"
 #include "parts.hpp"
 
+#include <math.h>
+
 #include <algorithm>
 #include <vector>
 
@@ -61,9 +63,11 @@ __device__ __forceinline__ PgRow row_of(const PgParams& p, const PgItem& it, con
 // Every wave's LDS writes and reads are done, its loads have arrived.
 __device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// Bytes of LDS of a workgroup: two tiles of K and V each.
+// Bytes of LDS of a workgroup: two tiles of K and V each (f32 in parts: half as much again).
 template <typename KVT, int NB>
 constexpr uint32_t PG_TILE_LDS = (sizeof(KVT) == 2 ? 16 : 8) * PgTile<KVT, NB>::GRANULE + 16;
+template <int NB>
+constexpr uint32_t PG_TILE3_LDS = 12 * PgTile<float, NB>::GRANULE + 16;
 
 // f16 caches. RT 2: four waves of 32 query rows; RT 1: eight waves, four of them 16 query rows each over
 // half of a tile's slots and four the same rows over the other half.
@@ -339,7 +343,9 @@ __device__ __forceinline__ void tile16_block(const PgParams& p, uint32_t id, uin
     }
 }
 
-// f32 caches: four waves of 16 query rows, tiles of 32 slots.
+// f32 caches, on the f32 matrix cores: four waves of 16 query rows, tiles of 32 slots. For few query rows (verify
+// passes of 6 rows before 5000 slots: 32 us, by tile3_block's parts in four waves 37), and for heads past 128
+// dims, whose parts leave no room for a second wave (8 x 4 heads of 256, 777 rows: 84 us, 88).
 template <int NB>
 __device__ __forceinline__ void tile32_block(const PgParams& p, uint32_t id, uint8_t* lds) {
     using T = PgTile<float, NB>;
@@ -522,6 +528,279 @@ __device__ __forceinline__ void tile32_block(const PgParams& p, uint32_t id, uin
         }
 }
 
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// Two numbers as three bf16 each, which add up to them: the first cut off after eight bits (so the largest
+// stay finite), the second rounded, the third what is left.
+__device__ __forceinline__ void split3(float a, float b, uint32_t& h, uint32_t& m, uint32_t& l) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+    h = __builtin_amdgcn_perm(y, x, 0x07060302);
+    a -= __uint_as_float(x & 0xffff0000u);
+    b -= __uint_as_float(y & 0xffff0000u);
+    m = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+    a -= __uint_as_float(m << 16);
+    b -= __uint_as_float(m & 0xffff0000u);
+    l = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+}
+__device__ __forceinline__ void split3(const float (&x)[8], bf16x8 (&to)[3]) {
+    pg_u32x4 w[3];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t h, m, l;
+        split3(x[2 * i], x[2 * i + 1], h, m, l);
+        w[0][i] = h, w[1][i] = m, w[2][i] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 3; i++) to[i] = __builtin_bit_cast(bf16x8, w[i]);
+}
+__device__ __forceinline__ f32x4 mfma_bf16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// f32 caches, many query rows: K, V, q and the weights are three bf16 each (24 bits, f32's range), and of their
+// nine products the six down to 2^-16 of the first are formed: what is left out is under 2^-22 of a
+// product, and the six take 3/8 of the time of one on the f32 matrix cores. Eight waves of 16 query rows, tiles
+// of 32 slots, which come through registers: each is cut into its parts, into LDS, while the one before is
+// computed, its successor's on their way. Bound by the matrix cores: 2048 rows before 6000 slots, 32 x 8
+// heads of 128, take 1.22 ms, 194 TFLOP/s of the formula (1.85 ms on the f32 cores, in tile32_block); 777
+// rows before 300 79 us (127). Four waves of 32 query rows read half as much LDS, but alone on their SIMD
+// hide less: 88 us where these take 77.
+template <int NB>
+__device__ __forceinline__ void tile3_block(const PgParams& p, uint32_t id, uint8_t* lds) {
+    using P = PgTile<f16, NB>;  // of a part
+    constexpr int NF = 2 * NB;
+    constexpr uint32_t QT = 128, SLOTS = 32, PIECES = NB;  // a wave's loads, half a granule
+    constexpr uint32_t KV = 6 * P::GRANULE, STAGE = 2 * KV;        // [K, V][granule][part]
+    uint32_t* odd_tile = (uint32_t*)(lds + 2 * STAGE);        // 1 + the tile of each stage whose V holds an infinity or a NaN
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t m16 = lane & 15, g = lane >> 4;
+    const uint32_t block = id / p.nkv;
+    uint32_t which;
+    const PgItem it = item_with_arguments<false>(p, false, block, which);
+    const PgBlock b = block_of<QT, SLOTS>(p, it, id % p.nkv, block);
+    if (b.t0 >= b.t1) {
+        if (threadIdx.x < QT) {
+            const size_t u = b.unit + threadIdx.x / 16 * b.next;
+            *(float2*)(p.part_ml + 2 * (u * 16 + (threadIdx.x & 15))) = float2{-INFINITY, 0.0f};
+        }
+        return;
+    }
+    PgList list = list_of(p, it, b.kvh, 4);
+    list.end = b.end;
+
+    // Four waves bring a tile's two granules of K, half a granule each, four V's.
+    const uint32_t half = wave & 1, isv = (wave >> 1) & 1;
+    const uint8_t* cache = isv ? p.vc : p.kc;
+    uint32_t from[PIECES], to[PIECES], page;
+#pragma unroll
+    for (uint32_t i = 0; i < PIECES; i++) {
+        const uint32_t x = 64 * (i + (wave >> 2) * PIECES) + lane, slot = x / (8 * NB), four = x % (8 * NB);
+        from[i] = 4 * four < p.hd ? slot * list.row_bytes + 16 * four : 0x80000000u;
+        to[i] = isv * KV + half * 3 * P::GRANULE + P::at(slot, four / 2, isv ? P::turn_v(slot) : P::turn_k(slot)) + 8 * (four & 1);
+    }
+    auto look = [&](uint32_t t) { page = list.page(t * SLOTS + 16 * half); };
+    pg_u32x4 in[PIECES];  // the next tile's,
+    bool bad;             // whose page is past the pool
+    auto source = [&](uint32_t t) { return list.buffer(cache, t < b.t1 ? t * SLOTS + 16 * half : list.end, page); };
+    auto load = [&](__amdgpu_buffer_rsrc_t r, uint32_t i) { in[i] = __builtin_amdgcn_raw_buffer_load_b128(r, from[i], 0, 0); };
+    auto put = [&](uint32_t i, uint8_t* stage) {
+        u32x2 h, m, l;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            uint32_t x, y, z;
+            split3(__uint_as_float(in[i][2 * e]), __uint_as_float(in[i][2 * e + 1]), x, y, z);
+            h[e] = x, m[e] = y, l[e] = z;
+        }
+        *(u32x2*)(stage + to[i]) = h;
+        *(u32x2*)(stage + to[i] + P::GRANULE) = m;
+        *(u32x2*)(stage + to[i] + 2 * P::GRANULE) = l;
+    };
+    // Whether a tile is one that some row sees a part of; its V is looked through for what is not finite.
+    auto mixed = [&](uint32_t t) { return t * SLOTS + SLOTS > b.seen && b.seen < b.end; };
+    auto watch = [&](uint32_t t, uint32_t stage) {
+        if (!isv || t >= b.t1 || !mixed(t)) return;
+        bool odd = false;
+#pragma unroll
+        for (uint32_t i = 0; i < PIECES; i++) odd = odd || odd32(in[i].x) || odd32(in[i].y) || odd32(in[i].z) || odd32(in[i].w);
+        if (odd) odd_tile[stage] = t + 1;
+    };
+    // (A page past the pool: the rows that see its slots are NaN.)
+    auto spoil = [&] {
+        if (bad)
+#pragma unroll
+            for (uint32_t i = 0; i < PIECES; i++) in[i] = pg_u32x4{0x7fc00000u, 0x7fc00000u, 0x7fc00000u, 0x7fc00000u};
+    };
+    auto bad_page = [&](uint32_t t) { return !isv && t < b.t1 && list.bad(t * SLOTS + 16 * half, page); };
+    look(b.t0);
+    if (threadIdx.x < 2) odd_tile[threadIdx.x] = 0;
+
+    const PgRow row = row_of(p, it, b, wave * 16 + m16);
+    bf16x8 q[NB][3];
+    {
+        f32x4 y[NB][2];
+#pragma unroll
+        for (int j = 0; j < NB; j++)  // (no branch around them)
+#pragma unroll
+            for (int e = 0; e < 2; e++) y[j][e] = *(const f32x4*)(p.q + row.at + (32 * j + 8 * g < p.hd ? 32 * j + 8 * g : 0) + 4 * e);
+        {
+            const __amdgpu_buffer_rsrc_t r = source(b.t0);
+#pragma unroll
+            for (uint32_t i = 0; i < PIECES; i++) load(r, i);
+        }
+        bad = bad_page(b.t0);
+        look(b.t0 + 1);
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = row.valid && 32 * j + 8 * g < p.hd ? y[j][e >> 2][e & 3] * p.sc : 0.0f;
+            split3(x, q[j]);
+        }
+    }
+    uint32_t kat[NB], vat[NF];
+#pragma unroll
+    for (int j = 0; j < NB; j++) kat[j] = P::at(m16, 4 * j + g, P::turn_k(m16));
+    {
+        const uint32_t slot = 4 * g + (m16 >> 2);
+#pragma unroll
+        for (int f = 0; f < NF; f++) vat[f] = KV + P::at(slot, 2 * f + ((m16 >> 1) & 1), P::turn_v(slot)) + 8 * (m16 & 1);
+    }
+    f32x4 o[NF];
+#pragma unroll
+    for (int f = 0; f < NF; f++) o[f] = f32x4{0, 0, 0, 0};
+    float ref = -INFINITY, l = 0.0f;
+    auto barrier = [] {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    };
+    barrier();  // (odd_tile)
+    watch(b.t0, 0);
+    spoil();
+    {
+        const __amdgpu_buffer_rsrc_t r = source(b.t0 + 1);
+#pragma unroll
+        for (uint32_t i = 0; i < PIECES; i++) {
+            put(i, lds);
+            load(r, i);
+        }
+        bad = bad_page(b.t0 + 1);
+        look(b.t0 + 2);
+    }
+    for (uint32_t t = b.t0; t < b.t1; t++) {
+        const uint32_t stage = (t - b.t0) & 1, next = 1 - stage, ts = t * SLOTS;
+        uint8_t* at = lds + stage * STAGE;
+        const bool edge = ts + SLOTS > b.seen;
+        barrier();
+        if (mixed(t) && odd_tile[stage] == t + 1) {
+            // (As in attn_paged_tile16.)
+#pragma unroll 1
+            for (uint32_t i = 0; i < SLOTS; i++)
+#pragma unroll
+                for (int f = 0; f < NF; f++) {
+                    const half4 v = *(const half4*)(at + KV + (i >> 4) * 3 * P::GRANULE + P::at(i & 15, 2 * f + (g >> 1), P::turn_v(i & 15)) + 8 * (g & 1));
+                    if (ts + i < row.vis)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if ((__builtin_bit_cast(uint16_t, v[e]) & 0x7f80u) == 0x7f80u) o[f][e] = NAN;
+                }
+            barrier();
+            for (uint32_t x = threadIdx.x; x < 2 * 64 * NF; x += 512) {
+                uint8_t* v = at + KV + x / (64 * NF) * 3 * P::GRANULE + x % (64 * NF) * 8;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if ((((const uint16_t*)v)[e] & 0x7f80u) == 0x7f80u)
+#pragma unroll
+                        for (int z = 0; z < 3; z++) ((uint16_t*)(v + z * P::GRANULE))[e] = 0;
+            }
+            barrier();
+        }
+        f32x4 s[2] = {}, s2[2] = {};
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+            bf16x8 k[2][3];
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int z = 0; z < 3; z++) k[h][z] = *(const bf16x8*)(at + (3 * h + z) * P::GRANULE + kat[j]);
+            // (Four sums in turn, so that no MFMA waits for the one before.)
+#pragma unroll
+            for (int z = 0; z < 6; z++) {
+                constexpr int KP[6] = {2, 1, 0, 1, 0, 0}, QP[6] = {0, 1, 2, 0, 1, 0};
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    f32x4& sum = z % 2 ? s[h] : s2[h];
+                    sum = mfma_bf16(k[h][KP[z]], q[j][QP[z]], sum);
+                }
+            }
+        }
+        bf16x8 w[3];
+        s[0] += s2[0];
+        s[1] += s2[1];
+        if (edge)
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (ts + 16 * (e >> 2) + 4 * g + (e & 3) >= row.vis) s[e >> 2][e & 3] = -INFINITY;
+        float f;
+        if (raise(s, 1.0f, ref, f)) {
+            l *= f;
+#pragma unroll
+            for (int k = 0; k < NF; k++) o[k] *= f;
+        }
+        {
+            const float base = ref == -INFINITY ? 0.0f : ref;
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                x[e] = exp2_hw(s[e >> 2][e & 3] - base);
+                l += x[e];
+            }
+            split3(x, w);
+        }
+        const __amdgpu_buffer_rsrc_t after = source(t + 2);
+        watch(t + 1, next);
+        spoil();
+#pragma unroll
+        for (int f = 0; f < NF; f += 2) {
+            bf16x8 v[2][3];
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int z = 0; z < 3; z++) {
+                    const half4 x = read_transposed(at + z * P::GRANULE + vat[f + e]), y = read_transposed(at + (3 + z) * P::GRANULE + vat[f + e]);
+                    v[e][z] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+#pragma unroll
+            for (int z = 0; z < 6; z++) {
+                constexpr int VP[6] = {2, 1, 0, 1, 0, 0}, WP[6] = {0, 1, 2, 0, 1, 0};
+#pragma unroll
+                for (int e = 0; e < 2; e++) o[f + e] = mfma_bf16(v[e][VP[z]], w[WP[z]], o[f + e]);
+            }
+            put(f / 2, lds + next * STAGE);  // (the next tile's parts, a share beside each operand)
+            load(after, f / 2);
+        }
+        bad = bad_page(t + 2);
+        look(t + 3);
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (!row.valid) return;
+    if (b.nchunk > 1) {
+        const size_t u = b.unit + wave * b.next;
+        f32x4* part = (f32x4*)p.part_o + u * NF * 64 + lane;
+#pragma unroll
+        for (int f = 0; f < NF; f++) part[64 * f] = o[f];
+        if (g == 0) *(float2*)(p.part_ml + 2 * (u * 16 + m16)) = float2{ref, l};
+        return;
+    }
+    const float k = 1.0f / l;
+#pragma unroll
+    for (int f = 0; f < NF; f++) {
+        const uint32_t d = 16 * f + 4 * g;
+        if (d < p.hd) *(f32x4*)(p.out + row.at + d) = o[f] * k;
+    }
+}
+
 template <int NB, int RT>
 __global__ __launch_bounds__(RT == 1 ? 512 : 256, 2) void attn_paged_tile16(const PgParams p) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[PG_TILE_LDS<f16, NB>];
@@ -532,18 +811,24 @@ __global__ __launch_bounds__(256, NB > 4 ? 1 : 2) void attn_paged_tile32(const P
     __shared__ __attribute__((aligned(16))) uint8_t lds[PG_TILE_LDS<float, NB>];
     tile32_block<NB>(p, blockIdx.x, lds);
 }
+template <int NB>
+__global__ __launch_bounds__(512, 2) void attn_paged_tile3(const PgParams p) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[PG_TILE3_LDS<NB>];
+    tile3_block<NB>(p, blockIdx.x, lds);
+}
 
 // A batch of both kinds in one launch: the second kind's blocks first, which take longest and are bound by the
 // matrix cores, the first kind's beside and behind them, bound by memory. MIXED: where those start (a
 // multiple of 8: their place among the XCDs).
 __host__ __device__ __forceinline__ uint32_t mixed_rows(const PgParams& p) { return (p.tblocks * p.nkv + 7) / 8 * 8; }
 
-template <int NB, bool PK>
-__global__ __launch_bounds__(256, 2) void attn_paged_mixed16(const PgParams p) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[std::max(PG_TILE_LDS<f16, NB>, PG_ROW_LDS<f16, NB, 4>)];
+template <int NB, int RT, bool PK>
+__global__ __launch_bounds__(RT == 1 ? 512 : 256, 2) void attn_paged_mixed16(const PgParams p) {
+    constexpr int WAVES = RT == 1 ? 8 : 4;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[std::max(PG_TILE_LDS<f16, NB>, PG_ROW_LDS<f16, NB, WAVES>)];
     const uint32_t rows = mixed_rows(p);
-    if (blockIdx.x >= rows) row_block<f16, NB, PK, 4>(p, blockIdx.x - rows, lds);
-    else if (blockIdx.x < p.tblocks * p.nkv) tile16_block<NB, 2>(p, blockIdx.x, lds);
+    if (blockIdx.x >= rows) row_block<f16, NB, PK, WAVES>(p, blockIdx.x - rows, lds);
+    else if (blockIdx.x < p.tblocks * p.nkv) tile16_block<NB, RT>(p, blockIdx.x, lds);
 }
 template <int NB>
 __global__ __launch_bounds__(256, NB > 4 ? 1 : 2) void attn_paged_mixed32(const PgParams p) {
@@ -551,6 +836,13 @@ __global__ __launch_bounds__(256, NB > 4 ? 1 : 2) void attn_paged_mixed32(const 
     const uint32_t rows = mixed_rows(p);
     if (blockIdx.x >= rows) row_block<float, NB, false, 4>(p, blockIdx.x - rows, lds);
     else if (blockIdx.x < p.tblocks * p.nkv) tile32_block<NB>(p, blockIdx.x, lds);
+}
+template <int NB>
+__global__ __launch_bounds__(512, 2) void attn_paged_mixed3(const PgParams p) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[std::max(PG_TILE3_LDS<NB>, PG_ROW_LDS<float, NB, 8>)];
+    const uint32_t rows = mixed_rows(p);
+    if (blockIdx.x >= rows) row_block<float, NB, false, 8>(p, blockIdx.x - rows, lds);
+    else if (blockIdx.x < p.tblocks * p.nkv) tile3_block<NB>(p, blockIdx.x, lds);
 }
 
 // The chunks of 16 query rows of a list brought together, one operand's columns a workgroup, each wave a
@@ -622,7 +914,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_paged_fold(const PgParams p) 
     float* dst = p.out + ((size_t)(it.row0 + r) * p.nh + kvh * p.G + n - r * p.G) * p.hd;
 #pragma unroll
     for (uint32_t i = 0; i < 4; i++) {
-        const uint32_t d = dim_of<KVT, NB>(f, g, i);
+        const uint32_t d = qt == 128 ? 16 * f + 4 * g + i : dim_of<KVT, NB>(f, g, i);  // (f16: the same)
         if (d < p.hd) dst[d] = a[i] * k;
     }
 }
@@ -651,16 +943,28 @@ void launch_tile16(const PgParams& p, hipStream_t s) {
 }
 template <int NB>
 void launch_tile32(const PgParams& p, hipStream_t s) {
-    hipLaunchKernelGGL((attn_paged_tile32<NB>), dim3(p.tblocks * p.nkv), dim3(256), 0, s, p);
+    const dim3 grid(p.tblocks * p.nkv);
+    if constexpr (NB <= 4) {
+        if (p.qt == 128) {
+            hipLaunchKernelGGL((attn_paged_tile3<NB>), grid, dim3(512), 0, s, p);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((attn_paged_tile32<NB>), grid, dim3(256), 0, s, p);
 }
 template <int NB>
 void launch_mixed(const PgParams& p, bool f16_cache, hipStream_t s) {
     const dim3 grid(mixed_rows(p) + (p.blocks + 7) / 8 * 8 * p.nkv);
-    if (!f16_cache) {
+    if constexpr (NB <= 4) {
+        const bool few = pg_few(p);
+        if (!f16_cache && p.qt == 128) hipLaunchKernelGGL((attn_paged_mixed3<NB>), grid, dim3(512), 0, s, p);
+        else if (!f16_cache) hipLaunchKernelGGL((attn_paged_mixed32<NB>), grid, dim3(256), 0, s, p);
+        else if (p.qt == 128 && few) hipLaunchKernelGGL((attn_paged_mixed16<NB, 2, true>), grid, dim3(256), 0, s, p);
+        else if (p.qt == 128) hipLaunchKernelGGL((attn_paged_mixed16<NB, 2, false>), grid, dim3(256), 0, s, p);
+        else if (few) hipLaunchKernelGGL((attn_paged_mixed16<NB, 1, true>), grid, dim3(512), 0, s, p);
+        else hipLaunchKernelGGL((attn_paged_mixed16<NB, 1, false>), grid, dim3(512), 0, s, p);
+    } else {
         hipLaunchKernelGGL((attn_paged_mixed32<NB>), grid, dim3(256), 0, s, p);
-    } else if constexpr (NB <= 4) {
-        if (pg_few(p)) hipLaunchKernelGGL((attn_paged_mixed16<NB, true>), grid, dim3(256), 0, s, p);
-        else hipLaunchKernelGGL((attn_paged_mixed16<NB, false>), grid, dim3(256), 0, s, p);
     }
 }
 
@@ -712,10 +1016,11 @@ bool cut_rows(PgParams& p, bool f16_cache) {
     }
     p.chunk = WHOLE;
     if (most <= 20) return true;
-    // Chunks of whole rounds of the waves, as short as leaves every workgroup a place at once; beside blocks of
-    // the second kind, which fill the CUs, a quarter of as many (ten steps beside two prompts' pieces of
-    // 28 x 4 heads of 128: 83 us, 95 with as many).
-    const uint32_t groups = p.nrow < p.nitems ? 128 : 512;
+    // Chunks of whole rounds of the waves, as short as leaves every workgroup a place at once, 512; beside blocks
+    // of the second kind what those leave, 128 to 256 (two prompts' pieces and ten steps, 28 x 4 heads of
+    // 128: 80 us by 128, 95 by 512; verify passes of 1 to 6 rows before 5000 slots, 64 x 8 heads: 24.8 by
+    // 256, 25.9 by 128, 26.7 by 512).
+    const uint32_t groups = p.nrow == p.nitems ? 512 : std::min(256u, std::max(128u, 512 - std::min(512u, p.tblocks * p.nkv)));
     p.chunk = std::max<uint32_t>(4, ceil_div(ceil_div(total * p.nkv, groups), 4) * 4);
     auto blocks = [&] {
         uint64_t n = 0;
@@ -730,35 +1035,68 @@ bool cut_rows(PgParams& p, bool f16_cache) {
 void cut_tiles(PgParams& p, bool f16_cache) {
     const uint32_t slots = pg_tile(f16_cache);
     std::sort(p.items + p.nrow, p.items + p.nitems, [](const PgItem& a, const PgItem& b) { return a.len > b.len; });
-    uint64_t few = 0, many = 0, longest = 0;  // query blocks of at most 64 rows, of more; a list's tiles
+    uint32_t few = 0, many = 0, longest = 0;  // query blocks of at most 64 rows, of more; a list's tiles
     for (uint32_t i = p.nrow; i < p.nitems; i++) {
         ((uint64_t)(p.items[i].rows_seq >> 8) * p.G <= 64 ? few : many)++;
-        longest = std::max<uint64_t>(longest, (p.items[i].len - 1) / slots + 1);
+        longest = std::max(longest, (p.items[i].len - 1) / slots + 1);
     }
-    p.qt = f16_cache && p.hd <= 128 && many >= few ? 128 : 64;
-    constexpr uint64_t CUS = 256;
-    const float tile = f16_cache ? 0.2f + 0.011f * p.hd : 0.0133f * p.hd;
-    auto time = [&](uint64_t chunk) {
-        uint64_t work = 0, blocks = 0, cut = 0;
-        for (uint32_t i = p.nrow; i < p.nitems; i++) {
-            const PgItem& it = p.items[i];
-            const uint64_t rows = it.rows_seq >> 8, n = ceil_div(rows * p.G, p.qt) * (uint64_t)p.nkv, tiles = ((uint64_t)it.len - rows / 2) / slots + 1;
-            const uint64_t chunks = (tiles - 1) / chunk + 1;
-            work += n * tiles;
-            blocks += n * chunks;
-            if (chunks > 1) cut += n * chunks;
-        }
-        return std::max((float)chunk, (float)ceil_div(blocks, CUS) * work / blocks) * tile + (cut ? 5.0f + (float)cut * p.qt * p.hd * 8 / 4.5e6f : 0.0f);
-    };
+    p.qt = p.hd <= 128 && many >= few ? 128 : 64;
+    // The chunks. What a launch in chunks of n tiles takes is counted out: a KV head's share of the CUs takes its
+    // blocks in their order, each the place that is free first, one or two a CU as LDS has it. A block's start
+    // (arguments, pages, q, the first tile) takes START us, a tile PAIRED us beside another block and ALONE
+    // of that without one; the fold 8 us and its states' bytes. (Within 5% of what launches in any chunks were
+    // measured to take: 600 rows before 2000 slots, 32 x 8 heads of 128 in f16, 62 to 104 us; the pieces
+    // of two prompts 77 to 115; 777 rows in f32 75 to 96. The chunks that it picks: 63, 78 and 76.)
+    constexpr uint32_t CUS = 256, TIMES = 512, NONE = 0xffff;
+    constexpr float START = 6.5f, ALONE = 0.7f;
+    const bool whole_cu = !f16_cache && p.qt == 128 && p.hd > 96;
+    const float paired = f16_cache ? (p.qt == 128 ? 0.36f + 0.02f * p.hd : 0.25f + 0.014f * p.hd) : p.qt == 128 ? (whole_cu ? 0.0195f : 0.039f) * p.hd : 0.027f * p.hd;
     p.tchunk = WHOLE;
-    uint64_t blocks = 0;
-    for (uint32_t i = p.nrow; i < p.nitems; i++) blocks += ceil_div((uint64_t)(p.items[i].rows_seq >> 8) * p.G, p.qt) * (uint64_t)p.nkv;
-    if (blocks >= 4 * CUS) return;  // (every CU has several: nothing to be had)
+    uint32_t tiles[4 * CUS], units = 0;  // of a KV head's query blocks
+    uint64_t sum = 0;
+    for (uint32_t i = p.nrow; i < p.nitems; i++) {
+        const PgItem& it = p.items[i];
+        const uint32_t rows = it.rows_seq >> 8, nqt = ceil_div(rows * p.G, p.qt);
+        if ((uint64_t)(units + nqt) * p.nkv >= 4 * CUS) return;  // (every CU has several: nothing to be had)
+        for (uint32_t qt = nqt; qt-- > 0; sum += tiles[units++]) tiles[units] = (it.len - rows + std::min(((qt + 1) * p.qt - 1) / p.G, rows - 1)) / slots + 1;
+    }
+    const uint32_t cus = std::max(1u, CUS / p.nkv), places = whole_cu ? cus : 2 * cus;
+    const float evenly = (START * units + (float)sum * paired) / places, unit = (START + longest * paired + evenly) / (TIMES / 2);  // of the count
+    const float start = START / unit + 0.5f, each = paired / unit, state = (float)p.nkv * p.qt * p.hd * 8 / 8e6f;
+    auto time = [&](uint32_t chunk) {
+        uint16_t first[TIMES], next[2 * CUS], ends[2 * CUS] = {};  // places that are free at a time, one after another
+        std::fill(first, first + TIMES, NONE);
+        for (uint32_t x = 0; x < places; x++) next[x] = x + 1 < places ? x + 1 : NONE;
+        first[0] = 0;
+        uint32_t now = 0, cut = 0, at = 0;
+        for (uint32_t i = p.nrow; i < p.nitems; i++) {
+            const uint32_t nqt = ceil_div((p.items[i].rows_seq >> 8) * p.G, p.qt), chunks = (tiles[at] - 1) / chunk + 1;
+            if (chunks > 1) cut += nqt * chunks;
+            for (uint32_t c = 0; c < chunks; c++)
+                for (uint32_t x = at; x < at + nqt && tiles[x] > c * chunk; x++) {
+                    while (first[now] == NONE) now++;
+                    const uint32_t place = first[now];
+                    first[now] = next[place];
+                    const uint32_t to = std::min(now + (uint32_t)(start + std::min(chunk, tiles[x] - c * chunk) * each), TIMES - 1);
+                    ends[place] = (uint16_t)to;
+                    next[place] = first[to];
+                    first[to] = (uint16_t)place;
+                }
+            at += nqt;
+        }
+        float last = 0.0f;
+        for (uint32_t x = 0; x < cus; x++) {
+            const float a = ends[x], b = whole_cu ? a : ends[x + cus];
+            last = std::max(last, std::min(a, b) + fabsf(a - b) * ALONE);
+        }
+        return last * unit + (cut ? 8.0f + cut * state : 0.0f);
+    };
     float least = time(longest);
-    for (uint64_t n = 2; n <= 64 && longest / n >= 2; n++) {
-        const uint64_t chunk = ceil_div(longest, n);
+    for (uint32_t chunk = longest; chunk > 2;) {
+        chunk = std::min(chunk - 1, chunk * 27 / 32);
+        if (units * ceil_div(longest, chunk) * p.nkv > 8 * CUS || 0.7f * evenly + 8.0f + (float)sum / chunk * state > least) break;
         const float t = time(chunk);
-        if (t < least) least = t, p.tchunk = (uint32_t)chunk;
+        if (t < least) least = t, p.tchunk = chunk;
     }
 }
 
@@ -767,13 +1105,14 @@ hipError_t run(PgParams& p, bool f16_cache, Workspace& ws, hipStream_t s) {
     p.chunk = p.tchunk = WHOLE;
     const bool rows = p.nrow > 0, tiles = p.nrow < p.nitems;
     if (tiles) cut_tiles(p, f16_cache);
+    PgPlan plan = place(p, f16_cache);  // (the second kind's, beside which the first's are cut)
     const bool brief = rows && cut_rows(p, f16_cache);
-    PgPlan plan = place(p, f16_cache);
+    if (rows) plan = place(p, f16_cache);
     if (plan.groups && !reserve(p, plan, ws)) {  // whole lists
         p.chunk = p.tchunk = WHOLE;
         plan = place(p, f16_cache);
     }
-    if (rows && tiles && (!f16_cache || p.qt == 128)) {
+    if (rows && tiles && (!f16_cache || p.hd <= 128)) {
         paged_mixed_launch(p, f16_cache, s);
     } else {
         if (rows) paged_rows_launch(p, f16_cache, brief, s);

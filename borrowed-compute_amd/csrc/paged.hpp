@@ -119,13 +119,23 @@ struct PgList {
         return ((const __attribute__((address_space(4))) uint32_t*)table)[min(slot, end - 1) >> shift];
     }
     __device__ __forceinline__ bool bad(uint32_t slot, uint32_t page) const { return slot < end && page >= npages; }
-    // The granule from `slot` on (a multiple of 16), which lies in `page`.
-    __device__ __forceinline__ pg_u32x4 granule(const uint8_t* cache, uint32_t slot, uint32_t page) const {
+    // The granule from `slot` on (a multiple of 16), which lies in `page`: where it starts, its bytes.
+    __device__ __forceinline__ uint64_t place(const uint8_t* cache, uint32_t slot, uint32_t page) const {
+        return (uint64_t)cache + (((uint64_t)page << shift) + (slot & ((1u << shift) - 1))) * row_bytes + head;
+    }
+    __device__ __forceinline__ uint32_t size(uint32_t slot, uint32_t page) const {
         const uint32_t n = slot < end && page < npages ? min(16u, end - slot) : 0;
-        const uint64_t at = (uint64_t)cache + (((uint64_t)page << shift) + (slot & ((1u << shift) - 1))) * row_bytes + head;
-        auto same = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
-        return pg_u32x4{same((uint32_t)at), same((uint32_t)(at >> 32) & 0xffffu),
-                        same(n ? n * row_bytes - head : 0u), 0x00020000u};
+        return n ? n * row_bytes - head : 0u;
+    }
+    static __device__ __forceinline__ uint32_t same(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+    __device__ __forceinline__ pg_u32x4 granule(const uint8_t* cache, uint32_t slot, uint32_t page) const {
+        const uint64_t at = place(cache, slot, page);
+        return pg_u32x4{same((uint32_t)at), same((uint32_t)(at >> 32) & 0xffffu), same(size(slot, page)), 0x00020000u};
+    }
+    // The same for loads into registers.
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const uint8_t* cache, uint32_t slot, uint32_t page) const {
+        const uint64_t at = place(cache, slot, page);
+        return __builtin_amdgcn_make_buffer_rsrc((void*)((uint64_t)same((uint32_t)(at >> 32)) << 32 | same((uint32_t)at)), 0, (int)same(size(slot, page)), 0x00020000);
     }
 };
 

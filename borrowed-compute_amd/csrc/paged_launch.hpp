@@ -16,10 +16,10 @@ constexpr uint32_t pg_row_tile(bool f16_cache) { return f16_cache ? 32 : 16; }
 // brief: lists of few tiles, by eight waves each (heads past 128 dims: four).
 void paged_rows_launch(const PgParams& p, bool f16_cache, bool brief, hipStream_t s);
 
-// Tiles of 64 slots (f16) or 32 (f32); p.qt query rows a block: 128 or 64 (f16), 64 (f32).
+// Tiles of 64 slots (f16) or 32 (f32); p.qt query rows a block: 128 (heads of up to 128 dims) or 64.
 constexpr uint32_t pg_tile(bool f16_cache) { return f16_cache ? 64 : 32; }
 void paged_tiles_launch(const PgParams& p, bool f16_cache, hipStream_t s);
-// Both kinds in one launch: f16 caches with p.qt 128, f32 caches.
+// Both kinds in one launch: f32 caches, and f16 heads of up to 128 dims.
 void paged_mixed_launch(const PgParams& p, bool f16_cache, hipStream_t s);
 // The chunks of the items that have more than one (`most` at most), groups of 16 query rows of them.
 void paged_fold_launch(const PgParams& p, bool f16_cache, uint32_t groups, uint32_t most, hipStream_t s);

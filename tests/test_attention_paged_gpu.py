@@ -285,3 +285,17 @@ def test_two_contexts_at_once(ctx):
                 go()
         for c, _, ob, want in work:
             np.testing.assert_array_equal(c.read(ob, want.shape).view(np.uint32), want.view(np.uint32))
+
+
+@pytest.mark.parametrize("rows", [1, 6, 40, 200])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_f32_values_of_any_size(ctx, rows, hd):
+    """An f32 cache keeps f32's range: dims of K and of V, and slots of V, 2^60 apart, as near as others."""
+    rng = np.random.default_rng(20 + rows)
+    b = Batch(rng, [rows, 1], [rows + 300, 50], 2, hd, bchip.F32)
+    size = 2.0 ** rng.integers(-30, 31, hd)
+    b.k *= size.astype(np.float32)
+    b.v *= (2.0 ** rng.integers(-30, 31, hd)).astype(np.float32)
+    b.v *= (2.0 ** rng.integers(-30, 31, (b.npages, 16, 1, 1))).astype(np.float32)
+    q = (rng.standard_normal((b.total, 4, hd)) / size).astype(np.float32)
+    check(ctx, b, q, 4, hd ** -0.5)
