@@ -845,35 +845,38 @@ __global__ __launch_bounds__(512, 2) void attn_paged_mixed3(const PgParams p) {
     else if (blockIdx.x < p.tblocks * p.nkv) tile3_block<NB>(p, blockIdx.x, lds);
 }
 
-// The chunks of 16 query rows of a list brought together, one operand's columns a workgroup, each wave a
-// share of the chunks; states lie as their waves held them. A chunk without a weight left its columns
-// unwritten.
+// The chunks of 16 query rows of a list brought together, those that some of the rows see. An operand's columns are
+// a wave's (WAVES 1: a workgroup takes fold_share operands), or its chunks' a share for each of WAVES waves;
+// states lie as their waves held them. A chunk without a weight left its columns unwritten.
+constexpr uint32_t fold_share(int nf) { return nf <= 8 ? nf : nf / 2; }
+
 template <typename KVT, int NB, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void attn_paged_fold(const PgParams p) {
+__global__ __launch_bounds__(64 * (WAVES == 1 ? fold_share(2 * NB) : WAVES)) void attn_paged_fold(const PgParams p) {
     constexpr int NF = 2 * NB, AHEAD = 8;
     __shared__ f32x4 sum[WAVES][64];
     __shared__ float sr[WAVES][64], sl[WAVES][64];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m16 = lane & 15, g = lane >> 4;
-    const uint32_t f = blockIdx.z, kvh = blockIdx.y;
+    const uint32_t lane = threadIdx.x & 63, at_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m16 = lane & 15, g = lane >> 4;
+    const uint32_t wave = WAVES == 1 ? 0 : at_wave, f = WAVES == 1 ? blockIdx.z * fold_share(NF) + at_wave : blockIdx.z, kvh = blockIdx.y;
     uint32_t which;
     const PgItem it = item_with_arguments<true>(p, false, blockIdx.x, which);
     const bool row = which < p.nrow;
     const uint32_t slots = (row ? 16 : 32) * (sizeof(KVT) == 2 ? 2 : 1), qt = row ? 16 : p.qt;  // of a tile, of a block
     const uint32_t rows = it.rows_seq >> 8, nq = rows * p.G, groups = ((nq - 1) / qt + 1) * (qt / 16);
-    const uint32_t chunks = ((it.len - 1) / slots) / (row ? p.chunk : p.tchunk) + 1, group = blockIdx.x - it.fold0, n = 16 * group + m16;
+    const uint32_t chunk = row ? p.chunk : p.tchunk, chunks = ((it.len - 1) / slots) / chunk + 1, group = blockIdx.x - it.fold0, n = 16 * group + m16;
+    const uint32_t seen = ((it.len - rows + min(16 * group + 15, nq - 1) / p.G) / slots) / chunk + 1;
     const bool valid = n < nq;
     const size_t u0 = (row ? 0 : (size_t)p.blocks * p.nkv) + (size_t)it.block0 * p.nkv * (qt / 16) + ((size_t)kvh * groups + group) * chunks;
     const float2* ml = (const float2*)p.part_ml + u0 * 16 + m16;
     const f32x4* at = (const f32x4*)p.part_o + (u0 * NF + f) * 64 + lane;
     f32x4 a = {0, 0, 0, 0};
     float R = -INFINITY, L = 0.0f;
-    for (uint32_t c0 = wave; c0 < chunks; c0 += AHEAD * WAVES) {
+    for (uint32_t c0 = wave; c0 < seen; c0 += AHEAD * WAVES) {
         float2 s[AHEAD];
         f32x4 x[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
             const uint32_t c = c0 + i * WAVES;
-            const bool there = valid && c < chunks;
+            const bool there = valid && c < seen;
             s[i] = there ? ml[(size_t)c * 16] : float2{-INFINITY, 0.0f};
             x[i] = there ? at[(size_t)c * NF * 64] : f32x4{0, 0, 0, 0};
         }
@@ -912,20 +915,27 @@ __global__ __launch_bounds__(64 * WAVES) void attn_paged_fold(const PgParams p) 
     const float k = 1.0f / L;
     const uint32_t r = n / p.G;
     float* dst = p.out + ((size_t)(it.row0 + r) * p.nh + kvh * p.G + n - r * p.G) * p.hd;
+    if (sizeof(KVT) == 2 || qt == 128) {
+        const uint32_t d = 16 * f + 4 * g;
+        if (d < p.hd) *(f32x4*)(dst + d) = a * k;
+    } else {
 #pragma unroll
-    for (uint32_t i = 0; i < 4; i++) {
-        const uint32_t d = qt == 128 ? 16 * f + 4 * g + i : dim_of<KVT, NB>(f, g, i);  // (f16: the same)
-        if (d < p.hd) dst[d] = a[i] * k;
+        for (uint32_t i = 0; i < 4; i++) {
+            const uint32_t d = dim_of<KVT, NB>(f, g, i);
+            if (d < p.hd) dst[d] = a[i] * k;
+        }
     }
 }
 
 template <typename KVT, int NB>
 void launch_fold(const PgParams& p, uint32_t groups, uint32_t most, hipStream_t s) {
     // A wave alone holds eight chunks' states at once; more chunks are shared out, among few waves where there
-    // are many groups (two prompts' pieces beside ten steps: 30 us by eight waves, as their longest list
-    // would have it, 14 by two).
+    // are many groups (two prompts' pieces beside ten steps, whose longest list is in 17 chunks: 30 us by eight
+    // waves, 14 by two). 25 MB of states of such pieces and their results take 9 us, of which stores of 4
+    // bytes had cost 3.
     const dim3 grid(groups, p.nkv, 2 * NB);
-    if (most <= 8) hipLaunchKernelGGL((attn_paged_fold<KVT, NB, 1>), grid, dim3(64), 0, s, p);
+    constexpr uint32_t share = fold_share(2 * NB);
+    if (most <= 8) hipLaunchKernelGGL((attn_paged_fold<KVT, NB, 1>), dim3(groups, p.nkv, 2 * NB / share), dim3(64 * share), 0, s, p);
     else if (most <= 16 || groups >= 64) hipLaunchKernelGGL((attn_paged_fold<KVT, NB, 2>), grid, dim3(128), 0, s, p);
     else hipLaunchKernelGGL((attn_paged_fold<KVT, NB, 8>), grid, dim3(512), 0, s, p);
 }

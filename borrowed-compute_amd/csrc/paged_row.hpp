@@ -369,6 +369,8 @@ __device__ __forceinline__ void row_block(const PgParams& p, uint32_t id, uint8_
         v *= inv;
         if (nchunk > 1) {
             *(f32x4*)(p.part_o + ((unit * NF + f) * 64 + lane) * 4) = v;
+        } else if constexpr (F16) {
+            if (16 * f + 4 * g < p.hd) *(f32x4*)(p.out + qrow + 16 * f + 4 * g) = v;
         } else {
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++) {
