@@ -70,7 +70,10 @@ template <int NB>
 constexpr uint32_t PG_TILE3_LDS = 12 * PgTile<float, NB>::GRANULE + 16;
 
 // f16 caches. RT 2: four waves of 32 query rows; RT 1: eight waves, four of them 16 query rows each over
-// half of a tile's slots and four the same rows over the other half.
+// half of a tile's slots and four the same rows over the other half. Bound by the matrix cores where rows are
+// many: 2048 before 8192 slots, 32 x 8 heads of 128, take 526 us, 1176 TFLOP/s with both parts of q and
+// of the weights (a large library product in f16 reaches 1132); 600 before 2000 63 us, of which the
+// last blocks and the fold's 8.8 us are a third.
 // Block `id` of the items of more than 16 query rows. lds: PG_TILE_LDS bytes, 16-byte aligned.
 template <int NB, int RT>
 __device__ __forceinline__ void tile16_block(const PgParams& p, uint32_t id, uint8_t* lds) {
@@ -563,7 +566,7 @@ __device__ __forceinline__ f32x4 mfma_bf16(bf16x8 a, bf16x8 b, f32x4 c) { return
 // of 32 slots, which come through registers: each is cut into its parts, into LDS, while the one before is
 // computed, its successor's on their way. Bound by the matrix cores: 2048 rows before 6000 slots, 32 x 8
 // heads of 128, take 1.22 ms, 194 TFLOP/s of the formula (1.85 ms on the f32 cores, in tile32_block); 777
-// rows before 300 79 us (127). Four waves of 32 query rows read half as much LDS, but alone on their SIMD
+// rows before 300 77 us (127). Four waves of 32 query rows read half as much LDS, but alone on their SIMD
 // hide less: 88 us where these take 77.
 template <int NB>
 __device__ __forceinline__ void tile3_block(const PgParams& p, uint32_t id, uint8_t* lds) {
@@ -930,8 +933,8 @@ __global__ __launch_bounds__(64 * (WAVES == 1 ? fold_share(2 * NB) : WAVES)) voi
 template <typename KVT, int NB>
 void launch_fold(const PgParams& p, uint32_t groups, uint32_t most, hipStream_t s) {
     // A wave alone holds eight chunks' states at once; more chunks are shared out, among few waves where there
-    // are many groups (two prompts' pieces beside ten steps, whose longest list is in 17 chunks: 30 us by eight
-    // waves, 14 by two). 25 MB of states of such pieces and their results take 9 us, of which stores of 4
+    // are many groups (two prompts' pieces beside ten steps: 30 us by eight waves, as their longest list would have
+    // it, 14 by two). 25 MB of states of such pieces and their results take 9 us, of which stores of 4
     // bytes had cost 3.
     const dim3 grid(groups, p.nkv, 2 * NB);
     constexpr uint32_t share = fold_share(2 * NB);

@@ -12,8 +12,13 @@
 // is a continuation, so what does not reach the k'th of them is not among the k best: only the k groups
 // that do (and their equals) are read again. Of their continuations, 4096 at a time, those that reach it too
 // go into a pool with the best so far, and a key's rank in it is the number of better ones. Nothing here
-// can overflow, whatever the scores: equal ones (a mask) only take more rounds. (The candidates taken from each part as it is read, as k_logprobs has it, cost
-// the scan twice its time at 16 best and 100 times at 64.)
+// can overflow, whatever the scores: equal ones (a mask) only take more rounds. (The candidates taken from
+// each part as it is read, as k_logprobs has it, cost the scan twice its time at 16 best and 100 times
+// at 64.)
+//
+// The scan is bound by its read: 128 rows of 128256 scores 12.5 us, 5.3 TB/s. The join is one chain of a
+// workgroup a search: 11 us beside it, 9.5 for a search of 4 beams of 151936; 64 best take 16 us more
+// than the best alone.
 #include "common.hpp"
 #include "internal.hpp"
 
