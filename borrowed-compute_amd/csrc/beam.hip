@@ -8,16 +8,17 @@
 //
 // k_beam_scan: one pass over the scores, which keeps of a row the sum and the largest score of every group
 // of 256, nothing else: a wave takes a part of a row alone, 1024 scores a step, the next step's on their
-// way. k_beam_join: a search's workgroup looks at its rows' groups, 4096 at a time. Every group's largest
+// way. k_beam_join: a search's workgroup looks at its rows' groups, 16384 at a time. Every group's largest
 // is a continuation, so what does not reach the k'th of them is not among the k best: only the k groups
-// that do (and their equals) are read again. Of their continuations, 4096 at a time, those that reach it too
-// go into a pool with the best so far, and a key's rank in it is the number of better ones. Nothing here
-// can overflow, whatever the scores: equal ones (a mask) only take more rounds. (The candidates taken from
+// that do (and their equals) are read again. Of their continuations, 16384 at a time, those that reach it too
+// go into a pool with the best so far, and a key's rank in it is the number of better ones. The pool holds
+// 4096: where more reach, whatever the scores (a mask's equal ones), a quarter as many are taken at a
+// time. (Always a quarter: 70 us for 6 searches of 16 beams and their 64 best, 36 so. The candidates taken from
 // each part as it is read, as k_logprobs has it, cost the scan twice its time at 16 best and 100 times
 // at 64.)
 //
 // The scan is bound by its read: 128 rows of 128256 scores 12.5 us, 5.3 TB/s. The join is one chain of a
-// workgroup a search: 11 us beside it, 9.5 for a search of 4 beams of 151936; 64 best take 16 us more
+// workgroup a search: 11 us beside it, 9.5 for a search of 4 beams of 151936; 64 best take 10 us more
 // than the best alone.
 #include "common.hpp"
 #include "internal.hpp"
@@ -25,6 +26,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace bchip {
 
@@ -178,12 +180,16 @@ __global__ __launch_bounds__(BM_JOIN) void k_beam_join(const BmParams p) {
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const size_t row0 = (size_t)blockIdx.x * p.beams;
     const uint32_t all = p.beams * p.groups;
-    float high[BM_KEYS];
-    auto load = [&](uint32_t g0) {  // (no branch around the loads: all on their way at once)
+    constexpr int WIDE = 4 * BM_KEYS;
+    float high[WIDE];
+    auto load = [&](uint32_t g0, bool wide) {  // (no branch around either's loads: all on their way at once)
 #pragma unroll
         for (int i = 0; i < BM_KEYS; i++) high[i] = p.highs[row0 * p.groups + min(g0 + BM_JOIN * i + tid, all - 1)];
+        if (wide)
+#pragma unroll
+            for (int i = BM_KEYS; i < WIDE; i++) high[i] = p.highs[row0 * p.groups + min(g0 + BM_JOIN * i + tid, all - 1)];
     };
-    load(0);
+    load(0, all > BM_ROUND);
     for (uint32_t b = wave; b < p.beams; b += BM_JOIN / 64) {
         const float2* states = p.states + (row0 + b) * p.parts;
         const float2 none = {-INFINITY, 0.0f}, x = lane < p.parts ? states[lane] : none, y = lane + 64 < p.parts ? states[lane + 64] : none;
@@ -201,76 +207,113 @@ __global__ __launch_bounds__(BM_JOIN) void k_beam_join(const BmParams p) {
         floor = ~0ull;
     }
     uint32_t kept = 0;
+    const float per = 1.0f / p.groups;
     __syncthreads();
-    for (uint32_t g0 = 0; g0 < all; g0 += BM_ROUND) {
-        // This round's groups: those that reach the k'th largest of the threads' go into the pool, those of them
-        // that fewer than k are larger than on the list.
-        uint64_t order[BM_KEYS], top = 0;
-        uint32_t place[BM_KEYS];
+    // Groups from g0 on, N a thread: those that reach the k'th largest of the threads' go into the pool, those of
+    // them that fewer than k are larger than on the list. False where the pool has no room for all.
+    auto look = [&](uint32_t g0, auto each) {
+        constexpr int N = decltype(each)::value;
+        uint64_t order[N], top = 0;
+        uint32_t place[N], more = 0;
 #pragma unroll
-        for (int i = 0; i < BM_KEYS; i++) {
-            const uint32_t g = min(g0 + BM_JOIN * i + tid, all - 1), b = g / p.groups;
+        for (int i = 0; i < N; i++) {
+            const uint32_t g = min(g0 + BM_JOIN * i + tid, all - 1);
+            uint32_t b = (uint32_t)((float)g * per);  // g / p.groups, or one beside it
+            b -= b * p.groups > g;
+            b += (b + 1) * p.groups <= g;
             order[i] = g0 + BM_JOIN * i + tid < all ? bm_order(base[b] + (double)high[i]) : 0;
             place[i] = b << 25 | (g - b * p.groups);
             top = top > order[i] ? top : order[i];
         }
-        if (g0 + BM_ROUND < all) load(g0 + BM_ROUND);
-        {
-            const uint64_t reach = bm_reach(top, p.k, highs, &least), worst = kept == p.k ? best[p.k - 1].score : 0, from = reach > worst ? reach : worst;
+        const uint64_t reach = bm_reach(top, p.k, highs, &least), worst = kept == p.k ? best[p.k - 1].score : 0, from = reach > worst ? reach : worst;
 #pragma unroll
-            for (int i = 0; i < BM_KEYS; i++)
-                if (order[i] != 0 && order[i] >= from) pool[atomicAdd(&count, 1u)] = BmKey{order[i], place[i]};
+        for (int i = 0; i < N; i++) {
+            if (order[i] < from) order[i] = 0;
+            more += order[i] != 0;
         }
+        if (N > BM_KEYS && __syncthreads_count(more > BM_KEYS)) {
+            if (tid == 0) least = ~0u;
+            __syncthreads();
+            return false;
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (order[i] != 0) pool[atomicAdd(&count, 1u)] = BmKey{order[i], place[i]};
         __syncthreads();
-        {
-            const uint32_t n = count;
-            for (uint32_t i = tid; i < n; i += BM_JOIN) {
-                const uint64_t x = pool[i].score;
-                uint32_t larger = 0;
+        const uint32_t n = count;
+        for (uint32_t i = tid; i < n; i += BM_JOIN) {
+            const uint64_t x = pool[i].score;
+            uint32_t larger = 0;
 #pragma unroll 8
-                for (uint32_t j = 0; j < n; j++) larger += pool[j].score > x;
-                if (larger < p.k) {
-                    list[atomicAdd(&listed, 1u)] = (uint32_t)pool[i].place;
-                    atomicMin((unsigned long long*)&floor, (unsigned long long)x);
-                }
+            for (uint32_t j = 0; j < n; j++) larger += pool[j].score > x;
+            if (larger < p.k) {
+                list[atomicAdd(&listed, 1u)] = (uint32_t)pool[i].place;
+                atomicMin((unsigned long long*)&floor, (unsigned long long)x);
             }
         }
         __syncthreads();
+        return true;
+    };
+    uint32_t narrow = 0;  // rounds of BM_ROUND to come in place of one of four times as many
+    for (uint32_t g0 = 0; g0 < all;) {
+        const bool wide = narrow == 0 && all - g0 > BM_ROUND;
+        if (g0 > 0) load(g0, wide);
+        if (wide) {
+            if (!look(g0, std::integral_constant<int, WIDE>())) {
+                narrow = WIDE / BM_KEYS;
+                continue;
+            }
+        } else {
+            look(g0, std::integral_constant<int, BM_KEYS>());
+            narrow -= narrow > 0;
+        }
+        g0 += wide ? WIDE * BM_JOIN : BM_ROUND;
         const uint32_t found = listed;
         if (tid == 0) {
             count = 0;
             least = ~0u;
         }
-        for (uint32_t l0 = 0; l0 < found; l0 += BM_ROUND / 256) {
-            // Their continuations, sixteen groups at a time.
-            float v[BM_KEYS];
-#pragma unroll
-            for (int i = 0; i < BM_KEYS; i++) {
+        // Their continuations, those of 4 N groups from l0 on: N a thread. What reaches the k'th of the groups (with
+        // fewer of them nothing is known of the k'th continuation) and the best so far goes into the pool. Where
+        // the pool has no room for all: false, if N is more than BM_KEYS; else the k'th largest of the threads'
+        // decides too (good tokens that lie side by side).
+        auto take = [&](uint32_t l0, auto each) {
+            constexpr int N = decltype(each)::value;
+            const uint64_t from = found >= p.k ? floor : 0;
+            float v[N];
+            auto of = [&](int i, uint32_t& b) {  // the token
                 const uint32_t x = list[min(l0 + BM_JOIN / 256 * i + tid / 256, found - 1)], in = x & 0x1ffffffu;
-                const uint64_t t = (uint64_t)(in / BM_GROUPS) * BM_STEP + 256 * (wave & 3) + 64 * (in % BM_GROUPS) + lane;
-                v[i] = p.scores[(row0 + (x >> 25)) * p.vocab + (t < p.vocab ? t : p.vocab - 1)];
+                b = x >> 25;
+                return (uint64_t)(in / BM_GROUPS) * BM_STEP + 256 * (wave & 3) + 64 * (in % BM_GROUPS) + lane;
+            };
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                uint32_t b;
+                const uint64_t t = of(i, b);
+                v[i] = p.scores[(row0 + b) * p.vocab + (t < p.vocab ? t : p.vocab - 1)];
             }
             __syncthreads();  // (count)
-            // (Many may reach the groups' k'th, where good tokens lie side by side: then the k'th largest of the
-            // threads' decides.)
-            BmKey mine[BM_KEYS];
+            BmKey mine[N];
             const BmKey last = best[p.k - 1];
-            uint64_t from = found >= p.k ? floor : 0;  // (fewer groups say nothing of the k'th continuation)
-            top = 0;
+            uint64_t top = 0, reach = 0;
             uint32_t more = 0;
 #pragma unroll
-            for (int i = 0; i < BM_KEYS; i++) {
-                const uint32_t x = list[min(l0 + BM_JOIN / 256 * i + tid / 256, found - 1)], in = x & 0x1ffffffu, b = x >> 25;
-                const uint64_t t = (uint64_t)(in / BM_GROUPS) * BM_STEP + 256 * (wave & 3) + 64 * (in % BM_GROUPS) + lane;
+            for (int i = 0; i < N; i++) {
+                uint32_t b;
+                const uint64_t t = of(i, b);
                 mine[i] = BmKey{l0 + BM_JOIN / 256 * i + tid / 256 < found && t < p.vocab ? bm_order(base[b] + (double)v[i]) : 0, (uint64_t)b << 32 | t};
                 if (mine[i].score < from || (kept == p.k && !mine[i].above(last))) mine[i].score = 0;
                 top = top > mine[i].score ? top : mine[i].score;
                 more += mine[i].score != 0;
             }
-            if (__syncthreads_count(more > 2)) from = bm_reach(top, p.k, highs, &least);
+            if (N > BM_KEYS) {
+                if (__syncthreads_count(more > BM_KEYS)) return false;
+            } else if (__syncthreads_count(more > 2)) {
+                reach = bm_reach(top, p.k, highs, &least);
+            }
 #pragma unroll
-            for (int i = 0; i < BM_KEYS; i++)
-                if (mine[i].score != 0 && mine[i].score >= from) pool[atomicAdd(&count, 1u)] = mine[i];
+            for (int i = 0; i < N; i++)
+                if (mine[i].score != 0 && mine[i].score >= reach) pool[atomicAdd(&count, 1u)] = mine[i];
             __syncthreads();
             if (tid < kept) pool[count + tid] = best[tid];
             __syncthreads();
@@ -288,7 +331,11 @@ __global__ __launch_bounds__(BM_JOIN) void k_beam_join(const BmParams p) {
                 least = ~0u;
             }
             kept = min(n, p.k);
-        }
+            return true;
+        };
+        constexpr uint32_t ROUND = BM_ROUND / 256;  // groups
+        if (found <= 2 * ROUND || found > 4 * ROUND || !take(0, std::integral_constant<int, WIDE>()))
+            for (uint32_t l0 = 0; l0 < found; l0 += ROUND) take(l0, std::integral_constant<int, BM_KEYS>());
         __syncthreads();
         if (tid == 0) {
             listed = count = 0;

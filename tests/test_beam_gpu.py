@@ -139,3 +139,33 @@ def test_reruns(ctx):
     a, b = select(ctx, scores, sums, 16), select(ctx, scores, sums, 16)
     for x, y in zip(a, b):
         np.testing.assert_array_equal(x.view(np.uint32), y.view(np.uint32))
+
+
+@pytest.mark.parametrize("beams,vocab", [(8, 200000), (30, 151936)])
+@pytest.mark.parametrize("form", ["equal", "slope", "plateau", "masked"])
+def test_many_groups_at_once(ctx, beams, vocab, form):
+    """Searches of more groups than one round holds a thread's few of: scores all equal (first beams, first tokens),
+    falling slowly along the vocabulary (the best side by side), a few levels, and all but one token masked."""
+    rng = np.random.default_rng(vocab)
+    sums = np.zeros((1, beams), np.float32)
+    if form == "equal":
+        scores = np.zeros((beams, vocab), np.float32)
+    elif form == "slope":
+        scores = np.tile(np.linspace(8, -8, vocab).astype(np.float32), (beams, 1))
+        sums[0] = -0.001 * np.arange(beams)
+    elif form == "plateau":
+        scores = rng.integers(0, 3, (beams, vocab)).astype(np.float32)
+        sums[0] = -np.arange(beams)
+    else:
+        scores = np.full((beams, vocab), -np.inf, np.float32)
+        scores[np.arange(beams), rng.integers(0, vocab, beams)] = 1.0
+        sums[0] = -rng.random(beams)
+    for k in (1, 33, 64):
+        check(ctx, scores, sums, k)
+        if form in ("equal", "masked"):
+            best, beam, token = select(ctx, scores, sums, k)
+            got = list(zip(beam[0].tolist(), token[0].tolist()))
+            if form == "equal":
+                assert got == [(0, t) for t in range(k)]
+            else:
+                assert got[:beams] == [(b, int(scores[b].argmax())) for b in np.argsort(-sums[0])][:k]
