@@ -274,9 +274,9 @@ __global__ __launch_bounds__(BM_JOIN) void k_beam_join(const BmParams p) {
             least = ~0u;
         }
         // Their continuations, those of 4 N groups from l0 on: N a thread. What reaches the k'th of the groups (with
-        // fewer of them nothing is known of the k'th continuation) and the best so far goes into the pool. Where
-        // the pool has no room for all: false, if N is more than BM_KEYS; else the k'th largest of the threads'
-        // decides too (good tokens that lie side by side).
+        // fewer of them nothing is known of the k'th continuation) and the best so far goes into the pool; of
+        // many (good tokens that lie side by side) what reaches the k'th largest of the threads'. False where
+        // the pool has no room for all.
         auto take = [&](uint32_t l0, auto each) {
             constexpr int N = decltype(each)::value;
             const uint64_t from = found >= p.k ? floor : 0;
@@ -295,7 +295,7 @@ __global__ __launch_bounds__(BM_JOIN) void k_beam_join(const BmParams p) {
             __syncthreads();  // (count)
             BmKey mine[N];
             const BmKey last = best[p.k - 1];
-            uint64_t top = 0, reach = 0;
+            uint64_t top = 0;
             uint32_t more = 0;
 #pragma unroll
             for (int i = 0; i < N; i++) {
@@ -306,14 +306,23 @@ __global__ __launch_bounds__(BM_JOIN) void k_beam_join(const BmParams p) {
                 top = top > mine[i].score ? top : mine[i].score;
                 more += mine[i].score != 0;
             }
-            if (N > BM_KEYS) {
-                if (__syncthreads_count(more > BM_KEYS)) return false;
-            } else if (__syncthreads_count(more > 2)) {
-                reach = bm_reach(top, p.k, highs, &least);
+            if (__syncthreads_count(more > 2)) {
+                const uint64_t reach = bm_reach(top, p.k, highs, &least);
+                more = 0;
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    if (mine[i].score < reach) mine[i].score = 0;
+                    more += mine[i].score != 0;
+                }
+                if (N > BM_KEYS && __syncthreads_count(more > BM_KEYS)) {
+                    if (tid == 0) least = ~0u;
+                    __syncthreads();
+                    return false;
+                }
             }
 #pragma unroll
             for (int i = 0; i < N; i++)
-                if (mine[i].score != 0 && mine[i].score >= reach) pool[atomicAdd(&count, 1u)] = mine[i];
+                if (mine[i].score != 0) pool[atomicAdd(&count, 1u)] = mine[i];
             __syncthreads();
             if (tid < kept) pool[count + tid] = best[tid];
             __syncthreads();
