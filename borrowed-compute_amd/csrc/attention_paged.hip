@@ -11,6 +11,7 @@
 #include "parts.hpp"
 
 #include <math.h>
+#include <stdlib.h>
 
 #include <algorithm>
 #include <vector>
@@ -1044,47 +1045,50 @@ bool cut_rows(PgParams& p, bool f16_cache) {
     return false;
 }
 
-// Items of more: query rows a block, and the chunks.
-void cut_tiles(PgParams& p, bool f16_cache) {
-    const uint32_t slots = pg_tile(f16_cache);
-    std::sort(p.items + p.nrow, p.items + p.nitems, [](const PgItem& a, const PgItem& b) { return a.len > b.len; });
-    uint32_t few = 0, many = 0, longest = 0;  // query blocks of at most 64 rows, of more; a list's tiles
-    for (uint32_t i = p.nrow; i < p.nitems; i++) {
-        ((uint64_t)(p.items[i].rows_seq >> 8) * p.G <= 64 ? few : many)++;
-        longest = std::max(longest, (p.items[i].len - 1) / slots + 1);
-    }
-    p.qt = p.hd <= 128 && many >= few ? 128 : 64;
-    // The chunks. What a launch in chunks of n tiles takes is counted out: a KV head's share of the CUs takes its
-    // blocks in their order, each the place that is free first, one or two a CU as LDS has it. A block's start
-    // (arguments, pages, q, the first tile) takes START us, a tile PAIRED us beside another block and ALONE
-    // of that without one; the fold 8 us and its states' bytes. (Within 5% of what launches in any chunks were
-    // measured to take: 600 rows before 2000 slots, 32 x 8 heads of 128 in f16, 62 to 104 us; the pieces
-    // of two prompts 77 to 115; 777 rows in f32 75 to 96. The chunks that it picks: 63, 78 and 76.)
+// What a launch over the items of more in blocks of qt query rows takes, and in which chunks. It is counted out: a
+// KV head's share of the CUs takes its blocks in their order, each the place that is free first, one or two a
+// CU as LDS has it. A block's start (arguments, pages, q, the first tile) takes START us, a tile `paired` us
+// beside another block and `alone` of that without one; the fold FOLD us and its states' bytes. (Within 5%
+// of what launches in any chunks were measured to take: 600 rows before 2000 slots, 32 x 8 heads of 128 in
+// f16, 62 to 104 us; the pieces of two prompts 77 to 115; 777 rows in f32 75 to 96. The chunks that it picks:
+// 63, 78 and 76.)
+struct PgCut {
+    float us;
+    uint32_t chunk;
+};
+PgCut cut(const PgParams& p, bool f16_cache, uint32_t qt, uint32_t longest, float limit) {
     constexpr uint32_t CUS = 256, TIMES = 512, NONE = 0xffff;
-    constexpr float START = 6.5f, ALONE = 0.7f;
-    const bool whole_cu = !f16_cache && p.qt == 128 && p.hd > 96;
-    const float paired = f16_cache ? (p.qt == 128 ? 0.36f + 0.02f * p.hd : 0.25f + 0.014f * p.hd) : p.qt == 128 ? (whole_cu ? 0.0195f : 0.039f) * p.hd : 0.027f * p.hd;
-    p.tchunk = WHOLE;
+    constexpr float START = 6.5f, FOLD = 5.5f;
+    const uint32_t slots = pg_tile(f16_cache);
+    const bool whole_cu = !f16_cache && qt == 128 && p.hd > 96;
+    const float paired = f16_cache ? (qt == 128 ? 0.36f + 0.02f * p.hd : 0.28f + 0.015f * p.hd) : qt == 128 ? (whole_cu ? 0.0195f : 0.039f) * p.hd : 0.027f * p.hd;
+    const float alone = f16_cache ? (qt == 128 ? 0.8f : 0.65f) : 0.7f;
     uint32_t tiles[4 * CUS], units = 0;  // of a KV head's query blocks
-    uint64_t sum = 0;
+    uint64_t sum = 0, all = 0;
     for (uint32_t i = p.nrow; i < p.nitems; i++) {
         const PgItem& it = p.items[i];
-        const uint32_t rows = it.rows_seq >> 8, nqt = ceil_div(rows * p.G, p.qt);
-        if ((uint64_t)(units + nqt) * p.nkv >= 4 * CUS) return;  // (every CU has several: nothing to be had)
-        for (uint32_t qt = nqt; qt-- > 0; sum += tiles[units++]) tiles[units] = (it.len - rows + std::min(((qt + 1) * p.qt - 1) / p.G, rows - 1)) / slots + 1;
+        const uint32_t rows = it.rows_seq >> 8, nqt = ceil_div(rows * p.G, qt);
+        all += (uint64_t)nqt * ((it.len - rows / 2 - 1) / slots + 1);
+        if ((uint64_t)(units + nqt) * p.nkv >= 4 * CUS) units = 4 * CUS;
+        if (units == 4 * CUS) continue;
+        for (uint32_t x = nqt; x-- > 0; sum += tiles[units++]) tiles[units] = (it.len - rows + std::min(((x + 1) * qt - 1) / p.G, rows - 1)) / slots + 1;
     }
     const uint32_t cus = std::max(1u, CUS / p.nkv), places = whole_cu ? cus : 2 * cus;
+    if (units == 4 * CUS) return {(float)all * paired / places + START, WHOLE};  // (every CU has several: nothing to be had)
     const float evenly = (START * units + (float)sum * paired) / places, unit = (START + longest * paired + evenly) / (TIMES / 2);  // of the count
-    const float start = START / unit + 0.5f, each = paired / unit, state = (float)p.nkv * p.qt * p.hd * 8 / 8e6f;
+    if (0.7f * evenly > limit) return {limit, WHOLE};
+    const float start = START / unit + 0.5f, each = paired / unit, state = (float)p.nkv * qt * p.hd * 8 / 6.4e6f;
     auto time = [&](uint32_t chunk) {
-        uint16_t first[TIMES], next[2 * CUS], ends[2 * CUS] = {};  // places that are free at a time, one after another
+        uint16_t first[TIMES], next[2 * CUS], ends[2 * CUS];  // places that are free at a time, one after another
         std::fill(first, first + TIMES, NONE);
-        for (uint32_t x = 0; x < places; x++) next[x] = x + 1 < places ? x + 1 : NONE;
+        std::fill(ends, ends + places, 0);
+        for (uint32_t x = 0; x < places; x++) next[x] = (uint16_t)(x + 1);
+        next[places - 1] = NONE;
         first[0] = 0;
-        uint32_t now = 0, cut = 0, at = 0;
+        uint32_t now = 0, states = 0, at = 0;
         for (uint32_t i = p.nrow; i < p.nitems; i++) {
-            const uint32_t nqt = ceil_div((p.items[i].rows_seq >> 8) * p.G, p.qt), chunks = (tiles[at] - 1) / chunk + 1;
-            if (chunks > 1) cut += nqt * chunks;
+            const uint32_t nqt = ceil_div((p.items[i].rows_seq >> 8) * p.G, qt), chunks = (tiles[at] - 1) / chunk + 1;
+            if (chunks > 1) states += nqt * chunks;
             for (uint32_t c = 0; c < chunks; c++)
                 for (uint32_t x = at; x < at + nqt && tiles[x] > c * chunk; x++) {
                     while (first[now] == NONE) now++;
@@ -1099,18 +1103,41 @@ void cut_tiles(PgParams& p, bool f16_cache) {
         }
         float last = 0.0f;
         for (uint32_t x = 0; x < cus; x++) {
-            const float a = ends[x], b = whole_cu ? a : ends[x + cus];
-            last = std::max(last, std::min(a, b) + fabsf(a - b) * ALONE);
+            const int a = ends[x], b = whole_cu ? a : ends[x + cus];
+            last = std::max(last, std::min(a, b) + (float)std::abs(a - b) * alone);
         }
-        return last * unit + (cut ? 8.0f + cut * state : 0.0f);
+        return last * unit + (states ? FOLD + states * state : 0.0f);
     };
-    float least = time(longest);
+    PgCut best = {time(longest), WHOLE};
     for (uint32_t chunk = longest; chunk > 2;) {
         chunk = std::min(chunk - 1, chunk * 27 / 32);
-        if (units * ceil_div(longest, chunk) * p.nkv > 8 * CUS || 0.7f * evenly + 8.0f + (float)sum / chunk * state > least) break;
+        const uint32_t many = units * ceil_div(longest, chunk);  // (the count itself takes the host's time)
+        if (many > 320 || many * p.nkv > 8 * CUS || 0.7f * evenly + FOLD + (float)sum / chunk * state > best.us) break;
         const float t = time(chunk);
-        if (t < least) least = t, p.tchunk = chunk;
+        if (t < best.us) best = {t, chunk};
     }
+    return best;
+}
+
+// Items of more: query rows a block, and the chunks. Where most items have more than 64 query rows blocks of 128,
+// whose tiles are read half as often; f16 heads in blocks of 64 where those end sooner, there being few blocks
+// (494 rows, 32 x 8 heads of 128: 18 us, 27 by 128; before 1500 slots, 28 x 4 heads: 45, 48; 600 before
+// 2000, 32 x 8: 78, 63).
+void cut_tiles(PgParams& p, bool f16_cache) {
+    const uint32_t slots = pg_tile(f16_cache);
+    std::sort(p.items + p.nrow, p.items + p.nitems, [](const PgItem& a, const PgItem& b) { return a.len > b.len; });
+    uint32_t few = 0, many = 0, longest = 0;  // items of at most 64 query rows, of more; a list's tiles
+    for (uint32_t i = p.nrow; i < p.nitems; i++) {
+        ((uint64_t)(p.items[i].rows_seq >> 8) * p.G <= 64 ? few : many)++;
+        longest = std::max(longest, (p.items[i].len - 1) / slots + 1);
+    }
+    p.qt = p.hd <= 128 && many >= few ? 128 : 64;
+    PgCut best = cut(p, f16_cache, p.qt, longest, INFINITY);
+    if (f16_cache && p.qt == 128) {
+        const PgCut other = cut(p, f16_cache, 64, longest, best.us);
+        if (other.us < best.us) best = other, p.qt = 64;
+    }
+    p.tchunk = best.chunk;
 }
 
 hipError_t run(PgParams& p, bool f16_cache, Workspace& ws, hipStream_t s) {
