@@ -1018,6 +1018,13 @@ bool reserve(PgParams& p, const PgPlan& plan, Workspace& ws) {
 
 constexpr uint32_t WHOLE = 0x40000000u;  // tiles: no list has as many
 
+// K and V of the items of at most 16 query rows.
+uint64_t row_bytes(const PgParams& p, bool f16_cache) {
+    uint64_t slots = 0;
+    for (uint32_t i = 0; i < p.nrow; i++) slots += p.items[i].len;
+    return slots * p.nkv * p.hd * (f16_cache ? 4 : 8);
+}
+
 // Items of at most 16 query rows: the chunks. Whether they are brief: lists that eight waves take in a few
 // tiles each are not cut (no second launch).
 bool cut_rows(PgParams& p, bool f16_cache) {
@@ -1031,10 +1038,10 @@ bool cut_rows(PgParams& p, bool f16_cache) {
     p.chunk = WHOLE;
     if (most <= 20) return true;
     // Chunks of whole rounds of the waves, as short as leaves every workgroup a place at once, 512; beside blocks
-    // of the second kind what those leave, 128 to 256 (two prompts' pieces and ten steps, 28 x 4 heads of
-    // 128: 80 us by 128, 95 by 512; verify passes of 1 to 6 rows before 5000 slots, 64 x 8 heads: 24.8 by
-    // 256, 25.9 by 128, 26.7 by 512).
-    const uint32_t groups = p.nrow == p.nitems ? 512 : std::min(256u, std::max(128u, 512 - std::min(512u, p.tblocks * p.nkv)));
+    // of the second kind, which take most places, one for every 200 KB, 192 to 512 (29 steps of up to 6000 slots
+    // beside a piece of a prompt, 28 x 4 heads of 128: 64 us by 512, 87 by 128; two pieces and ten steps 78 by
+    // 192, 82 by 512; verify passes of 1 to 6 rows before 5000 slots, 64 x 8 heads: 24.6, 27.0).
+    const uint32_t groups = p.nrow == p.nitems ? 512 : (uint32_t)std::min<uint64_t>(512, std::max<uint64_t>(192, row_bytes(p, f16_cache) / 200000));
     p.chunk = std::max<uint32_t>(4, ceil_div(ceil_div(total * p.nkv, groups), 4) * 4);
     auto blocks = [&] {
         uint64_t n = 0;
@@ -1133,7 +1140,9 @@ void cut_tiles(PgParams& p, bool f16_cache) {
     }
     p.qt = p.hd <= 128 && many >= few ? 128 : 64;
     PgCut best = cut(p, f16_cache, p.qt, longest, INFINITY);
-    if (f16_cache && p.qt == 128) {
+    // (Beside longer work of the first kind, at 5 MB a us, blocks of 128 leave it more of LDS: 40 steps of up to 3000
+    // slots and 100 rows, 32 x 8 heads of 128, 73 us, 79 by 64.)
+    if (f16_cache && p.qt == 128 && row_bytes(p, f16_cache) / 5e6f < best.us) {
         const PgCut other = cut(p, f16_cache, 64, longest, best.us);
         if (other.us < best.us) best = other, p.qt = 64;
     }
@@ -1145,9 +1154,8 @@ hipError_t run(PgParams& p, bool f16_cache, Workspace& ws, hipStream_t s) {
     p.chunk = p.tchunk = WHOLE;
     const bool rows = p.nrow > 0, tiles = p.nrow < p.nitems;
     if (tiles) cut_tiles(p, f16_cache);
-    PgPlan plan = place(p, f16_cache);  // (the second kind's, beside which the first's are cut)
     const bool brief = rows && cut_rows(p, f16_cache);
-    if (rows) plan = place(p, f16_cache);
+    PgPlan plan = place(p, f16_cache);
     if (plan.groups && !reserve(p, plan, ws)) {  // whole lists
         p.chunk = p.tchunk = WHOLE;
         plan = place(p, f16_cache);
