@@ -299,3 +299,18 @@ def test_f32_values_of_any_size(ctx, rows, hd):
     b.v *= (2.0 ** rng.integers(-30, 31, (b.npages, 16, 1, 1))).astype(np.float32)
     q = (rng.standard_normal((b.total, 4, hd)) / size).astype(np.float32)
     check(ctx, b, q, 4, hd ** -0.5)
+
+
+@pytest.mark.parametrize("kv_type", [bchip.F16, bchip.F32])
+@pytest.mark.parametrize("shape", [(16, 4, 128), (14, 2, 64)])
+@pytest.mark.parametrize("rows,lens", [([1] * 40 + [100], [2000] * 40 + [100]), ([1, 1, 2, 200], [3000, 900, 1500, 200]),
+                                       ([3, 3, 200, 90], [3000, 800, 200, 400]), ([1, 1, 1, 20, 12], [2500] * 5), ([600], [1500]),
+                                       ([3, 60, 60, 60], [4000, 60, 60, 90]), ([300, 1], [300, 6000])])
+def test_batches_that_are_cut_in_different_ways(ctx, rows, lens, shape, kv_type):
+    """Many long steps beside a piece of a prompt, few beside a large one, prompts alone, from their start and
+    before many slots: blocks of 64 and of 128 query rows, steps of 8 query rows and of 16, whole lists and chunks."""
+    nh, nkv, hd = shape
+    rng = np.random.default_rng(len(rows) * hd)
+    b = Batch(rng, rows, lens, nkv, hd, kv_type, pad=2)
+    q = (2 * rng.standard_normal((b.total, nh, hd))).astype(np.float32)
+    check(ctx, b, q, nh, hd ** -0.5)
