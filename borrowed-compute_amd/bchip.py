@@ -297,15 +297,15 @@ class Ctx:
         row_starts[i + 1] - 1 and the last of its seq_lens[i] slots; pages: device u32 [nseq][page_stride]."""
         starts, lens = _batch(row_starts, seq_lens)
         check(lib().bchip_rope_append_paged(self.h, _ptr(q), _ptr(k), _ptr(v), _ptr(kc), _ptr(vc), kv_type, _ptr(inv_freq),
-                                            _ptr(positions), starts.ctypes.data, lens.ctypes.data, _ptr(pages), page_stride,
+                                            _ptr(positions), _host(starts), _host(lens), _ptr(pages), page_stride,
                                             page_slots, npages, len(lens), nh, nkv, hd, rope_dim, int(neox)))
 
     def attention_paged(self, q, kc, vc, kv_type, out, row_starts, seq_lens, pages, page_stride, page_slots, npages, nh, nkv,
                         hd, scale) -> None:
         """Attention of several sequences' new rows over a cache in pages (arguments as rope_append_paged)."""
         starts, lens = _batch(row_starts, seq_lens)
-        check(lib().bchip_attention_paged(self.h, _ptr(q), _ptr(kc), _ptr(vc), kv_type, _ptr(out), starts.ctypes.data,
-                                          lens.ctypes.data, _ptr(pages), page_stride, page_slots, npages, len(lens), nh, nkv,
+        check(lib().bchip_attention_paged(self.h, _ptr(q), _ptr(kc), _ptr(vc), kv_type, _ptr(out), _host(starts),
+                                          _host(lens), _ptr(pages), page_stride, page_slots, npages, len(lens), nh, nkv,
                                           hd, scale))
 
     def copy_pages(self, bufs, t, page_elems, npages, src, dst) -> None:
@@ -314,7 +314,7 @@ class Ctx:
         s, d = np.ascontiguousarray(src, np.uint32), np.ascontiguousarray(dst, np.uint32)
         if s.shape != d.shape or s.ndim != 1:
             raise ValueError(f"{s.shape} source pages for {d.shape} destinations")
-        check(lib().bchip_copy_pages(self.h, arr.buffer_info()[0], len(bufs), t, page_elems, npages, s.ctypes.data, d.ctypes.data, len(s)))
+        check(lib().bchip_copy_pages(self.h, arr.buffer_info()[0], len(bufs), t, page_elems, npages, _host(s), _host(d), len(s)))
 
     def matmul(self, w, wtype, x, out, rows, cols, n) -> None:
         check(lib().bchip_matmul(self.h, _ptr(w), wtype, _ptr(x), _ptr(out), rows, cols, n))
@@ -533,6 +533,14 @@ def _batch(row_starts, seq_lens):
     if len(starts) != len(lens) + 1:
         raise ValueError(f"{len(starts)} row starts for {len(lens)} sequences (one more is needed)")
     return starts, lens
+
+
+_Here = ctypes.c_char * 0
+
+
+def _host(a):
+    """Where a host array lies, for the length of a call (.ctypes takes four times as long)."""
+    return _Here.from_buffer(a) if a.flags.writeable else a.ctypes.data
 
 
 def _ptr(x):
