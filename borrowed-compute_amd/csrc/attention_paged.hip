@@ -119,12 +119,12 @@ __device__ __forceinline__ void tile16_block(const PgParams& p, uint32_t id, uin
         } else if (k) {
             const pg_u32x4 r = list.granule(p.kc, slot, page);
 #pragma unroll
-            for (int i = 0; i < T::LOADS; i++) load_lds(r, kfrom[i], kl + at + 1024 * i);
+            for (int i = 0; i < T::LOADS; i++) load_lds(r, kfrom[i], kl + at, 1024 * i);
         }
         if (v) {
             const pg_u32x4 r = list.granule(p.vc, slot, page);
 #pragma unroll
-            for (int i = 0; i < T::LOADS; i++) load_lds(r, KS == 1 ? vfrom[KS == 1 ? i : 0] : kfrom[i], vl + at + 1024 * i);
+            for (int i = 0; i < T::LOADS; i++) load_lds(r, KS == 1 ? vfrom[KS == 1 ? i : 0] : kfrom[i], vl + at, 1024 * i);
         }
     };
     look(b.t0);
@@ -390,7 +390,7 @@ __device__ __forceinline__ void tile32_block(const PgParams& p, uint32_t id, uin
             const pg_u32x4 r = list.granule(wave < 2 ? p.kc : p.vc, slot, page);
             const uint32_t to = (wave < 2 ? kl : vl) + at;
 #pragma unroll
-            for (int i = 0; i < T::LOADS; i++) load_lds(r, from[i], to + 1024 * i);
+            for (int i = 0; i < T::LOADS; i++) load_lds(r, from[i], to, 1024 * i);
         }
     };
     look(b.t0);

@@ -72,7 +72,7 @@ __device__ __forceinline__ void row_block(const PgParams& p, uint32_t id, uint8_
         for (int h = 0; h < NG; h++) {
             const pg_u32x4 r = list.granule(cache, t < tiles ? (first + t) * SLOTS + 16 * h : list.end, page[h]);
 #pragma unroll
-            for (int i = 0; i < T::LOADS; i++) load_lds(r, from[i], to + h * T::GRANULE + 1024 * i);
+            for (int i = 0; i < T::LOADS; i++) load_lds(r, from[i], to, h * T::GRANULE + 1024 * i);
         }
     };
     look(wave);
