@@ -72,7 +72,7 @@ constexpr uint32_t PG_TILE3_LDS = 12 * PgTile<float, NB>::GRANULE + 16;
 
 // f16 caches. RT 2: four waves of 32 query rows; RT 1: eight waves, four of them 16 query rows each over
 // half of a tile's slots and four the same rows over the other half. Bound by the matrix cores where rows are
-// many: 2048 before 8192 slots, 32 x 8 heads of 128, take 526 us, 1176 TFLOP/s with both parts of q and
+// many: 2048 before 8192 slots, 32 x 8 heads of 128, take 516 us, 1200 TFLOP/s with both parts of q and
 // of the weights (a large library product in f16 reaches 1132); 600 before 2000 63 us, of which the
 // last blocks and the fold's 8.8 us are a third.
 // Block `id` of the items of more than 16 query rows. lds: PG_TILE_LDS bytes, 16-byte aligned.

@@ -19,7 +19,7 @@
 // the KV heads of one chunk.
 //
 // Bound by the bytes of K and V: 16 steps at up to 24001 slots, 32 x 8 heads of 128 in f16, take 137 us and
-// the fold 4.8 (5.07 TB/s together; a large copy reaches 5.15), 16 at up to 8000 in f32 98 us (4.9). A list of
+// the fold 4.8 (5.07 TB/s together; a large copy reaches 5.15), 16 at up to 8000 in f32 95 us (5.05). A list of
 // 400 slots takes 6.5 us, the latency of arguments, page number, first tile and the states' way through LDS.
 #pragma once
 

@@ -28,7 +28,10 @@ def call(ctx, b, q, nh, scale, out=None):
 
 
 def expect(b, q, nh, scale, only=None):
-    """Per sequence: rows' results, and how far an f32-grade one may lie."""
+    """Per sequence: rows' results, and how far an f32-grade one may lie. (The bound's terms hold for f32 caches too. By
+    f32 products: hd of them, each sum's rounding 2^-24. In three bf16 parts: what is left out of a product, twice
+    2^-7 2^-16 of it, is 2^-22, as with two f16; the first parts' sums round 16 times an MFMA, hd / 32 of
+    them, and the five others', 5 hd / 2 times, at 2^-7 of that: less than hd in all.)"""
     for i, (n, m) in enumerate(zip(b.rows, b.lens)):
         if n == 0 or (only is not None and i not in only):
             continue
