@@ -199,11 +199,15 @@ __device__ __forceinline__ void tile16_block(const PgParams& p, uint32_t id, uin
         if (edge && b.seen < b.end) {
             // Some row does not see all of the tile: an infinity or a NaN in V, which a weight of 0
             // would not silence, reaches the rows that see its slot and is 0 from then on.
-            constexpr int EACH = 4 * T::GRANULE / (16 * 256 * KS);
+            // (The threads' last round may reach past the tile: heads of 32 and 96 dims by eight waves.)
+            constexpr uint32_t BYTES = 4 * T::GRANULE, ROUND = 16 * 256 * KS;
+            constexpr bool WHOLE_ROUNDS = BYTES % ROUND == 0;
             bool odd = false;
 #pragma unroll
-            for (int i = 0; i < EACH; i++) {
-                const pg_u32x4 w = *(const pg_u32x4*)(vb + 16 * (threadIdx.x + 256 * KS * i));
+            for (uint32_t from = 0; from < BYTES; from += ROUND) {
+                const uint32_t x = from + 16 * threadIdx.x;
+                if (!WHOLE_ROUNDS && x >= BYTES) break;
+                const pg_u32x4 w = *(const pg_u32x4*)(vb + x);
                 odd = odd || odd16(w.x) || odd16(w.y) || odd16(w.z) || odd16(w.w);
             }
             if (odd) odd_tile[buf] = t + 1;
@@ -225,8 +229,8 @@ __device__ __forceinline__ void tile16_block(const PgParams& p, uint32_t id, uin
                 __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
                 __builtin_amdgcn_s_barrier();
                 __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-                for (int i = 0; i < EACH; i++) {
-                    pg_u32x4* at = (pg_u32x4*)(vb + 16 * (threadIdx.x + 256 * KS * i));
+                for (uint32_t x = 16 * threadIdx.x; x < BYTES; x += ROUND) {
+                    pg_u32x4* at = (pg_u32x4*)(vb + x);
                     pg_u32x4 w = *at;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
@@ -425,6 +429,7 @@ __device__ __forceinline__ void tile32_block(const PgParams& p, uint32_t id, uin
         const bool edge = ts + SLOTS > b.seen;
         if (edge && b.seen < b.end) {  // (as in attn_paged_tile16)
             constexpr int EACH = 2 * T::GRANULE / (16 * 256);
+            static_assert(EACH * 16 * 256 == 2 * T::GRANULE, "a share for every thread");
             bool odd = false;
 #pragma unroll
             for (int i = 0; i < EACH; i++) {
