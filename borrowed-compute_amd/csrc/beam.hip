@@ -221,8 +221,10 @@ __global__ __launch_bounds__(BM_JOIN) void k_beam_join(const BmParams p) {
             uint32_t b = (uint32_t)((float)g * per);  // g / p.groups, or one beside it
             b -= b * p.groups > g;
             b += (b + 1) * p.groups <= g;
-            order[i] = g0 + BM_JOIN * i + tid < all ? bm_order(base[b] + (double)high[i]) : 0;
-            place[i] = b << 25 | (g - b * p.groups);
+            // (A row's last groups may lie past its end, and are none of it: their -inf would stand above a NaN.)
+            const uint32_t in = g - b * p.groups, first = in / BM_GROUPS * BM_STEP + 64 * (in % BM_GROUPS);
+            order[i] = g0 + BM_JOIN * i + tid < all && first < p.vocab ? bm_order(base[b] + (double)high[i]) : 0;
+            place[i] = b << 25 | in;
             top = top > order[i] ? top : order[i];
         }
         const uint64_t reach = bm_reach(top, p.k, highs, &least), worst = kept == p.k ? best[p.k - 1].score : 0, from = reach > worst ? reach : worst;
