@@ -81,9 +81,12 @@ typedef __attribute__((address_space(3))) int16_t __attribute__((ext_vector_type
 // unrolled (sums made outside would each hold a scalar register, and there are not as many). A vector memory
 // instruction may read a scalar that a vector one wrote (a spilled descriptor's v_readlane) five wait states
 // later, and M0 one; the compiler counts neither for an asm block. The sum is one, s_nop 3 the other four.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // (M0 is one of its reserved registers: named so that it keeps no offset of its own there)
 __device__ __forceinline__ void load_lds(pg_u32x4 from, uint32_t offset, uint32_t to, uint32_t plus) {
-    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(from), "s"(to), "i"(plus) : "memory", "scc");
+    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(from), "s"(to), "i"(plus) : "memory", "m0", "scc");
 }
+#pragma clang diagnostic pop
 // Until at most N of this wave's loads are on their way.
 template <int N>
 __device__ __forceinline__ void wait_loads() {

@@ -7,10 +7,11 @@ so a load written in one has to bring its own."""
 import glob
 import os
 import re
+import subprocess
 
 import pytest
 
-from test_build_guard import BUILD, _disassemble, _objects
+from test_build_guard import BUILD, ROOT, _disassemble, _objects
 
 STATES = 5
 SDST_SECOND = re.compile(r"v_(add|sub|subrev|addc|subb|subbrev)_co|v_div_scale|v_mad_[ui]64")
@@ -115,3 +116,32 @@ def test_descriptors_are_waited_for(obj, tmp_path):
         found = short(function)
         assert not found, f"{name}: {len(found)} too early, e.g. {found[0]}"
     assert loads or obj == "bchip.o"
+
+
+OFFSETS = """
+#include "paged.hpp"
+namespace bchip {
+__global__ void probe(pg_u32x4 from, const uint8_t* at, uint32_t n, float* out) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[4096];
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, (int)n, 0x00020000);
+    pg_lds* to = (pg_lds*)lds + 2048;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, to, 4, 4 * threadIdx.x, 0, 0, 0);
+    load_lds(from, 16 * threadIdx.x, (uint32_t)(uintptr_t)(pg_lds*)lds, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, to, 4, 4 * threadIdx.x, 4096, 0, 0);
+    __syncthreads();
+    out[threadIdx.x] = ((float*)lds)[threadIdx.x];
+}
+}
+"""
+
+
+def test_the_compiler_sets_its_own_offsets_again(tmp_path):
+    """Loads into LDS take their place from M0: one that the compiler makes behind load_lds, which sets it, does not
+    find its own there any more. (Compiled, not run.)"""
+    source, listing = tmp_path / "probe.hip", tmp_path / "probe.s"
+    source.write_text(OFFSETS)
+    subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "--cuda-device-only", "-S", "-O3", "-std=c++17", "-w", "-Xclang", "-target-feature",
+                    "-Xclang", "-packed-fp32-ops", f"-I{ROOT}/include", f"-I{ROOT}/borrowed-compute_amd/csrc", str(source), "-o", str(listing)],
+                   check=True, capture_output=True)
+    steps = re.findall(r"^\s+(s_\w+ m0|buffer_load_\w+).*", listing.read_text(), re.M)
+    assert [x.split("_")[0] for x in steps] == ["s", "buffer"] * 3, steps
