@@ -172,8 +172,8 @@ class GpuLayers:
         """The layers over new rows of several conversations in one pass: rows[i] hidden states of
         conversation seqs[i] (a piece of a prompt, a token, none), in that order, appended to its pages
         at its next slots; returns the updated states. Pages that a conversation lacks or shares are
-        taken first (PagePool.extend). At most 256 conversations a pass; a refused pass leaves the pool as
-        it was."""
+        taken first (PagePool.extend). At most 256 conversations a pass. A pass that raises leaves every
+        conversation the slots it had (its own copy of a page that it shared may stay)."""
         c, ctx = self.cfg, self.ctx
         if len(x) != sum(rows):
             raise ValueError(f"{len(x)} states for {sum(rows)} rows")
@@ -183,18 +183,23 @@ class GpuLayers:
             raise ValueError("the pool is another stage's")
         s = self._scratch(max(len(x), 1))
         pool.extend(seqs, rows)
-        lens = [pool.len[s] for s in seqs]
-        positions = np.concatenate([np.arange(m - n, m) for n, m in zip(rows, lens)]) if len(x) else np.zeros(0)
-        starts = np.concatenate([[0], np.cumsum(rows)]).astype(np.uint32)
-        table, stride = pool.table(seqs)
-        hd, nh, nkv = c.head_dim, c.n_head, c.n_head_kv
-        batch = (starts, np.asarray(lens, np.uint32), table, stride, pool.page_slots, pool.npages, nh, nkv, hd)
+        try:
+            lens = [pool.len[s] for s in seqs]
+            positions = np.concatenate([np.arange(m - n, m) for n, m in zip(rows, lens)]) if len(x) else np.zeros(0)
+            starts = np.concatenate([[0], np.cumsum(rows)]).astype(np.uint32)
+            table, stride = pool.table(seqs)
+            hd, nh, nkv = c.head_dim, c.n_head, c.n_head_kv
+            batch = (starts, np.asarray(lens, np.uint32), table, stride, pool.page_slots, pool.npages, nh, nkv, hd)
 
-        def attend(kc, vc):
-            ctx.rope_append_paged(s["q"], s["k"], s["v"], kc, vc, pool.kv_type, self.freq, s["pos"], *batch, c.rope_dim, c.rope_neox)
-            ctx.attention_paged(s["q"], kc, vc, pool.kv_type, s["att"], *batch, 1.0 / math.sqrt(hd))
+            def attend(kc, vc):
+                ctx.rope_append_paged(s["q"], s["k"], s["v"], kc, vc, pool.kv_type, self.freq, s["pos"], *batch, c.rope_dim, c.rope_neox)
+                ctx.attention_paged(s["q"], kc, vc, pool.kv_type, s["att"], *batch, 1.0 / math.sqrt(hd))
 
-        return self._layers(x, positions, pool, attend)
+            return self._layers(x, positions, pool, attend)
+        except BaseException:
+            for q, n in reversed(list(zip(seqs, rows))):
+                pool.truncate(q, pool.len[q] - n)
+            raise
 
     def _layers(self, x: np.ndarray, positions, cache, attend) -> np.ndarray:
         """Every layer over the states x at `positions`; attend(kc, vc) turns the layer's q, k and v

@@ -1,0 +1,88 @@
+"""A pool of pages after a call that failed, on the CPU (host_side.py): conversations keep the slots they had, and the
+next call is as if the failed one had not been."""
+import pytest
+
+import host_side
+from test_paged_refusals import POOL, STAGE
+
+
+@pytest.fixture(scope="module")
+def fake(tmp_path_factory):
+    return host_side.build(tmp_path_factory.mktemp("fake"))
+
+
+STATE = """
+def state():
+    return dict(p.len), {s: list(x) for s, x in p.pages.items()}, list(p.spare), list(p.users)
+x = lambda n: np.zeros((n, 64), np.float32)
+def no_table(*a):
+    raise bchip.BchipError(bchip.E_OOM, "no memory for a table")
+"""
+
+
+def test_a_pass_that_is_refused_after_its_pages_were_taken(fake):
+    """No memory for the table; heads that the library refuses; states of another width; an error in a layer behind
+    the first, whose rows are appended by then."""
+    host_side.run(fake, STAGE + STATE + """
+g = L.GpuLayers(c, cfg, [one, one], None, bchip.F16)
+a, b, e = p.new(), p.new(), p.new()
+g.forward_paged(x(25), [a, b], [20, 5], p)
+was, real = state(), p.table
+def again():  # the same pass, as if nothing had been
+    g.forward_paged(x(24), [b, a, e], [20, 3, 1], p)
+    check()
+    assert p.len == {a: 23, b: 25, e: 1}
+    for s, n in ((a, 20), (b, 5), (e, 0)):
+        p.truncate(s, n)
+    check()
+run = lambda: g.forward_paged(x(24), [b, a, e], [20, 3, 1], p)
+p.table = no_table
+assert "table" in raises(bchip.BchipError, run)
+assert state() == was
+p.table = real
+again()
+was = state()
+g.cfg.n_head = 17 * cfg.n_head_kv
+g.scratch_rows = 0
+assert "group" in raises(bchip.BchipError, run)
+g.cfg.n_head = 2
+assert state() == was
+again()
+was = state()
+wide = np.zeros((24, 640), np.float32)
+raises(bchip.BchipError, lambda: g.forward_paged(wide, [b, a, e], [20, 3, 1], p))
+assert state() == was
+again()
+was, real, calls = state(), c.attention_paged, []
+def second(*args):
+    calls.append(1)
+    if len(calls) == 2:
+        raise KeyboardInterrupt
+    return real(*args)
+c.attention_paged = second
+raises(KeyboardInterrupt, run)
+c.attention_paged = real
+assert state() == was
+again()
+""")
+
+
+def test_a_refused_pass_of_forks(fake):
+    """A conversation's own copy of a page that it shared may stay; its slots, and the others', are as they were."""
+    host_side.run(fake, STAGE + STATE + """
+g = L.GpuLayers(c, cfg, [one, one], None, bchip.F16)
+a = p.new()
+g.forward_paged(x(20), [a], [20], p)
+f, h = p.fork(a), p.fork(a)
+lens, real = dict(p.len), p.table
+p.table = no_table
+raises(bchip.BchipError, lambda: g.forward_paged(x(32), [f, a], [2, 30], p))
+p.table = real
+assert p.len == lens
+check()
+assert p.pages[h][0] == p.pages[f][0] == p.pages[a][0]
+spare = len(p.spare)
+g.forward_paged(x(32), [f, a], [2, 30], p)
+check()
+assert p.len == {a: 50, f: 22, h: 20} and spare - len(p.spare) == 2  # (a's two; the copies are there already)
+""")
