@@ -473,10 +473,10 @@ class PagePool:
     def extend(self, seqs, rows) -> None:
         """Slots for rows[i] new rows of each conversation seqs[i] (each named once): pages that a
         conversation lacks, and its own copy of a shared page that the rows go into. With too few
-        pages left nothing changes (MemoryError)."""
+        pages left (MemoryError), or where the copies fail, nothing changes."""
         if len(set(seqs)) != len(seqs) or len(seqs) != len(rows) or any(n < 0 for n in rows):
             raise ValueError("each conversation once, with a number of rows")
-        src, dst, plan, users, left = [], [], [], {}, len(self.spare)
+        src, plan, users, taken = [], [], {}, 0
         for s, n in zip(seqs, rows):
             held, length = self.pages[s], self.len[s]
             last = length // self.page_slots  # the page of the first new row
@@ -485,23 +485,22 @@ class PagePool:
                 have = users.get(held[last], self.users[held[last]])
                 if have > 1:
                     own, users[held[last]] = last, have - 1
+                    src.append(held[last])
             need = -(-(length + n) // self.page_slots) - len(held)
-            left -= need + (own is not None)
+            taken += need + (own is not None)
             plan.append((s, own, need, length + n))
-        if left < 0:
-            raise MemoryError(f"{-left} pages too few for {sum(rows)} rows")
-        for s, own, need, length in plan:
-            held = self.pages[s]
-            if own is not None:
-                to = self._take()
-                src.append(held[own])
-                dst.append(to)
-                self.users[held[own]] -= 1
-                held[own] = to
-            held.extend(self._take() for _ in range(need))
-            self.len[s] = length
+        if taken > len(self.spare):
+            raise MemoryError(f"{taken - len(self.spare)} pages too few for {sum(rows)} rows")
         if src:
+            dst = self.spare[-len(src):][::-1]  # (as they will be taken, the copies first)
             self.ctx.copy_pages(self.k + self.v, self.kv_type, self.page_slots * self.kvd, self.npages, src, dst)
+        for s, own, _, _ in plan:
+            if own is not None:
+                self.users[self.pages[s][own]] -= 1
+                self.pages[s][own] = self._take()
+        for s, _, need, length in plan:
+            self.pages[s].extend(self._take() for _ in range(need))
+            self.len[s] = length
 
     def _take(self) -> int:
         p = self.spare.pop()

@@ -86,3 +86,29 @@ g.forward_paged(x(32), [f, a], [2, 30], p)
 check()
 assert p.len == {a: 50, f: 22, h: 20} and spare - len(p.spare) == 2  # (a's two; the copies are there already)
 """)
+
+
+def test_copies_that_fail(fake):
+    """A page that was to be copied stays shared, and its conversation's."""
+    host_side.run(fake, STAGE + STATE + """
+g = L.GpuLayers(c, cfg, [one, one], None, bchip.F16)
+a = p.new()
+p.extend([a], [20])
+f, h = p.fork(a), p.fork(a)
+was, real = state(), c.copy_pages
+def refused_copy(*args):
+    assert state() == was  # the tables name no page that was not copied
+    raise bchip.BchipError(bchip.E_HIP, "a copy")
+c.copy_pages = refused_copy
+raises(bchip.BchipError, lambda: p.extend([f, a], [2, 30]))
+assert state() == was
+raises(bchip.BchipError, lambda: g.forward_paged(x(32), [f, a], [2, 30], p))
+assert state() == was
+seen = []
+c.copy_pages = lambda bufs, t, n, pages, src, dst: (seen.append((list(src), list(dst))), real(bufs, t, n, pages, src, dst))
+p.extend([f, a], [2, 30])
+check()
+assert p.len == {a: 50, f: 22, h: 20}
+(src, dst), = seen
+assert src == [p.pages[h][1]] * 2 and dst == [p.pages[f][1], p.pages[a][1]], (src, dst)
+""")
