@@ -514,8 +514,9 @@ class PagePool:
         for line, s in zip(t, seqs):
             line[:len(self.pages[s])] = self.pages[s]
         if self._table is None or self._table.nbytes < t.nbytes:
-            if self._table is not None:
-                self._table.free()
+            old, self._table = self._table, None
+            if old is not None:
+                old.free()
             self._table = Buf(self.ctx, max(2 * t.nbytes, 4096))
         self.ctx.upload(t, self._table)
         return self._table, stride

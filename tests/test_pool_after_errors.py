@@ -112,3 +112,23 @@ assert p.len == {a: 50, f: 22, h: 20}
 (src, dst), = seen
 assert src == [p.pages[h][1]] * 2 and dst == [p.pages[f][1], p.pages[a][1]], (src, dst)
 """)
+
+
+def test_a_table_that_found_no_memory(fake):
+    """The pool goes on with tables that there is memory for, and frees each buffer once."""
+    host_side.run(fake, STAGE + STATE + """
+a = p.new()
+p.extend([a], [40])
+first, _ = p.table([a])
+for size in (first.nbytes, 64):  # a larger one is refused: then one of the first's size, and a small one
+    raises(bchip.BchipError, lambda: (fake.fake_budget(64), p.table([a] * 3000)))
+    fake.fake_budget((1 << 64) - 1)
+    seqs = [a] * (size // 12)
+    buf, stride = p.table(seqs)
+    assert buf.ptr and buf.nbytes >= 12 * len(seqs) and stride == 3
+    got = c.read(buf, (len(seqs), 3), np.uint32)
+    assert (got == p.pages[a]).all()
+was = fake.fake_live_count()
+p.free()
+assert was - fake.fake_live_count() == 5  # two layers' K and V, the table
+""")
