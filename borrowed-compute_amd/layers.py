@@ -119,13 +119,22 @@ class GpuLayers:
         if rows > self.scratch_rows:
             c = self.cfg
             qd, kvd = c.n_head * c.head_dim, c.n_head_kv * c.head_dim
-            for b in self.scratch.values():
-                b.free()
+            self._free_scratch()
             sizes = {"x": c.n_embd, "n": c.n_embd, "q": qd, "k": kvd, "v": kvd, "att": qd, "o": c.n_embd,
                      "gate": self.ff, "up": self.ff, "pos": 1, "mask": 2}
-            self.scratch = {k: self.ctx.zeros(max(rows * w, 1) * 4) for k, w in sizes.items()}
+            try:
+                for k, w in sizes.items():
+                    self.scratch[k] = self.ctx.zeros(max(rows * w, 1) * 4)
+            except BaseException:
+                self._free_scratch()
+                raise
             self.scratch_rows = rows
         return self.scratch
+
+    def _free_scratch(self) -> None:
+        for b in self.scratch.values():
+            b.free()
+        self.scratch, self.scratch_rows = {}, 0
 
     def _matmul(self, w, x, out, rows: int, nrows: int | None = None) -> None:
         buf, ty, wr, wc = w
@@ -357,6 +366,4 @@ class GpuLayers:
             self.head[0].free()
             self.head[1].free()
         self.freq.free()
-        for b in self.scratch.values():
-            b.free()
-        self.scratch, self.scratch_rows = {}, 0
+        self._free_scratch()

@@ -132,3 +132,31 @@ was = fake.fake_live_count()
 p.free()
 assert was - fake.fake_live_count() == 5  # two layers' K and V, the table
 """)
+
+
+def test_a_stage_that_found_no_memory_for_its_rows(fake):
+    """It goes on with passes that there is memory for, and keeps no buffer of the refused one."""
+    host_side.run(fake, STAGE + STATE + """
+g = L.GpuLayers(c, cfg, [one, one], None, bchip.F16)
+a = p.new()
+g.forward_paged(x(4), [a], [4], p)
+kept = fake.fake_live_count()
+zeros, had = c.zeros, []
+def some(nbytes):
+    if len(had) == fit:
+        raise bchip.BchipError(bchip.E_OOM, "no more")
+    had.append(nbytes)
+    return zeros(nbytes)
+for fit in (0, 1, 5):  # buffers that there is memory for
+    c.zeros = some
+    had.clear()
+    raises(bchip.BchipError, lambda: g.forward_paged(x(100), [a], [100], p))
+    assert len(had) == fit
+    c.zeros = zeros
+    assert p.len[a] == 4
+    assert fake.fake_live_count() <= kept
+    g.forward_paged(x(4), [a], [4], p)
+    p.truncate(a, 4)
+    assert fake.fake_live_count() == kept
+g.forward_paged(x(100), [a], [100], p)
+""")
