@@ -429,15 +429,22 @@ class PagePool:
             raise ValueError(f"{npages} pages of {page_slots} slots (a power of two from 16 to 2^20)")
         self.ctx, self.n_layer, self.kvd, self.kv_type = ctx, n_layer, kvd, kv_type
         self.npages, self.page_slots = npages, page_slots
+        self.k: list[Buf] = []
+        self.v: list[Buf] = []
+        self._table: Buf | None = None
         nbytes = nbytes_of(kv_type, npages * page_slots * kvd)
-        self.k = [Buf(ctx, nbytes) for _ in range(n_layer)]
-        self.v = [Buf(ctx, nbytes) for _ in range(n_layer)]
+        try:
+            for bufs in (self.k, self.v):
+                for _ in range(n_layer):
+                    bufs.append(Buf(ctx, nbytes))
+        except BaseException:
+            self.free()
+            raise
         self.spare = list(range(npages - 1, -1, -1))  # the lowest first
         self.users = [0] * npages                     # conversations that hold a page
         self.pages: dict[int, list[int]] = {}
         self.len: dict[int, int] = {}
         self._next = 0
-        self._table: Buf | None = None
 
     def new(self) -> int:
         """A conversation without slots."""

@@ -160,3 +160,32 @@ for fit in (0, 1, 5):  # buffers that there is memory for
     assert fake.fake_live_count() == kept
 g.forward_paged(x(100), [a], [100], p)
 """)
+
+
+def test_a_pool_that_finds_no_memory_keeps_none(fake):
+    """A pool is asked for again with fewer pages: what the refused one had got is free by then."""
+    host_side.run(fake, """
+Buf, had = bchip.Buf, []
+class Some(Buf):
+    def __init__(self, ctx, nbytes):
+        if len(had) == fit:
+            raise bchip.BchipError(bchip.E_OOM, "no more")
+        had.append(nbytes)
+        super().__init__(ctx, nbytes)
+was = fake.fake_live_count()
+for fit in (0, 1, 3, 7):  # of four layers' K and V
+    bchip.Buf = Some
+    had.clear()
+    try:
+        bchip.PagePool(c, 4, 64, 10)
+    except bchip.BchipError as e:
+        assert e.code == bchip.E_OOM
+    else:
+        raise AssertionError("there was room")
+    assert len(had) == fit and fake.fake_live_count() == was, fit
+    bchip.Buf = Buf
+p = bchip.PagePool(c, 4, 64, 10)
+assert fake.fake_live_count() == was + 8
+p.free()
+assert fake.fake_live_count() == was
+""")
