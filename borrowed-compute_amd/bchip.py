@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import array
 import ctypes
+import operator
 import os
 import re
 
@@ -467,6 +468,7 @@ class PagePool:
 
     def truncate(self, seq: int, length: int) -> None:
         """Keeps a conversation's first `length` slots (the rows of a verify pass that were accepted)."""
+        length = operator.index(length)
         if not 0 <= length <= self.len[seq]:
             raise ValueError(f"conversation {seq} has {self.len[seq]} slots, not {length}")
         held = self.pages[seq]
@@ -481,6 +483,7 @@ class PagePool:
         """Slots for rows[i] new rows of each conversation seqs[i] (each named once): pages that a
         conversation lacks, and its own copy of a shared page that the rows go into. With too few
         pages left (MemoryError), or where the copies fail, nothing changes."""
+        rows = [operator.index(n) for n in rows]
         if len(set(seqs)) != len(seqs) or len(seqs) != len(rows) or any(n < 0 for n in rows):
             raise ValueError("each conversation once, with a number of rows")
         src, plan, users, taken = [], [], {}, 0

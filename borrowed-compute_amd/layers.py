@@ -21,6 +21,7 @@ import contextlib
 import ctypes
 import ctypes.util
 import math
+import operator
 from dataclasses import dataclass
 
 import numpy as np
@@ -183,7 +184,7 @@ class GpuLayers:
         at its next slots; returns the updated states. Pages that a conversation lacks or shares are
         taken first (PagePool.extend). At most 256 conversations a pass. A pass that raises leaves every
         conversation the slots it had (its own copy of a page that it shared may stay)."""
-        c, ctx = self.cfg, self.ctx
+        c, ctx, rows = self.cfg, self.ctx, [operator.index(n) for n in rows]
         if len(x) != sum(rows):
             raise ValueError(f"{len(x)} states for {sum(rows)} rows")
         if len(seqs) > 256:

@@ -189,3 +189,31 @@ assert fake.fake_live_count() == was + 8
 p.free()
 assert fake.fake_live_count() == was
 """)
+
+
+@pytest.mark.parametrize("kind", ["uint8", "uint32", "uint64", "int32"])
+def test_numbers_of_numpys_types(fake, kind):
+    """Rows and lengths as arrays hold them (a device's accepted lengths are u32): as Python's numbers."""
+    host_side.run(fake, STAGE + STATE + f"kind = np.{kind}" + """
+g = L.GpuLayers(c, cfg, [one, one], None, bchip.F16)
+a, b = p.new(), p.new()
+p.extend([a, b], np.array([20, 33], kind))
+check()
+assert p.len == {a: 20, b: 33}
+p.truncate(b, kind(16))
+check()
+assert len(p.pages[b]) == 1
+p.truncate(a, np.array([3], kind)[0])
+check()
+g.forward_paged(x(30), np.array([b, a], kind), np.array([1, 29], kind), p)
+check()
+assert p.len == {a: 32, b: 17}
+was, real = state(), p.table
+p.table = no_table
+raises(bchip.BchipError, lambda: g.forward_paged(x(30), [b, a], np.array([1, 29], kind), p))
+p.table = real
+assert state() == was
+assert all(type(n) is int for n in p.len.values())
+p.extend([a], [20])
+check()
+""")
