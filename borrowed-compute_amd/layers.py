@@ -326,7 +326,7 @@ class GpuLayers:
         [searches][beams] of them, the log probabilities of the beams so far, -inf for one that is not
         there), then the k best continuations of each search (bchip_beam_select). Gives their scores, beams
         and tokens [searches][k]; only these come back to the host. Searches are scored in pieces of at
-        most SCORE_BYTES (one search at least), with the same results."""
+        most SCORE_BYTES (one search at least) and the rows that a selection takes, with the same results."""
         if self.head is None:
             raise ValueError("this stage has no output head")
         sums = np.ascontiguousarray(sums, np.float32)
@@ -341,6 +341,7 @@ class GpuLayers:
         ctx.upload(np.ascontiguousarray(x, np.float32), s["x"])
         ctx.rms_norm(s["x"], norm, s["n"], len(x), self.cfg.n_embd, self.cfg.eps)
         count = max(1, min(-(-len(x) * upto * 4 // self.SCORE_BYTES), n // 2 if beams == 1 else n))
+        count = max(count, -(-n // max(1, 65535 // max(1, beams))))
         ends = [n * i // count for i in range(count + 1)]
         try:
             for words in (n * beams, n * k, n * k, n * k, max(b - a for a, b in zip(ends, ends[1:])) * beams * upto):
