@@ -399,8 +399,8 @@ int bchip_logprobs(bchip_ctx* ctx, const float* scores, uint32_t rows, uint32_t 
  * formed in 64 bits from f32 exponentials, and rounded to f32. A row with a NaN, a score of +inf or
  * nothing above -inf gives NaN scores, behind every number. beams and k <= 64, k <= beams * vocab,
  * batch * beams <= 65535. A caller that ends beams at a token asks for 2 beams of k and keeps the beams that
- * go on. Takes scratch of a 64th of the scores' bytes and 1 KB a row; fails with BCHIP_E_OOM where it
- * cannot be had (memory full, a call under graph capture that has not run before at its size). */
+ * go on. Takes scratch of a 256th of the scores' bytes (of rows rounded up to 1024 scores) and at most
+ * 1 KB a row beside; fails with BCHIP_E_OOM where it cannot be had (memory full, a call under graph capture that has not run before at its size). */
 int bchip_beam_select(bchip_ctx* ctx, const float* scores, const float* sums, uint32_t batch, uint32_t beams,
                       uint32_t vocab, uint32_t k, float* best, uint32_t* beam, uint32_t* token);
 

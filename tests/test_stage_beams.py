@@ -61,3 +61,18 @@ for x, sums in ((5, np.zeros((2, 3))), (6, np.zeros(6))):
         raise AssertionError("taken")
 assert pieces(0, 3) == []
 """)
+
+
+def test_scratch_of_a_selection(fake):
+    """As include/bchip.h has it: a 256th of the bytes of rows of whole 1024 scores, and up to 1 KB a row."""
+    host_side.run(fake, """
+big = c.zeros(64 << 20).ptr
+for n, beams, vocab in ((1, 1, 1), (1, 4, 1024), (1, 4, 1025), (3, 5, 151), (2, 8, 128256), (1, 16, 600000), (2000, 4, 900)):
+    with bchip.Ctx(0) as fresh:
+        clear()
+        fresh.beam_select(big, big, n, beams, vocab, 1, big, big, big)
+        taken = sum(size for _, size, _ in mallocs())
+    rows = n * beams
+    groups = rows * -(-vocab // 1024) * 1024 * 4 // 256
+    assert groups < taken <= groups + 1024 * rows, (n, beams, vocab, taken)
+""")
