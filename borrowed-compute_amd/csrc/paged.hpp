@@ -75,7 +75,6 @@ __device__ __forceinline__ PgItem item_with_arguments(const PgParams& p, bool ro
 
 typedef uint32_t pg_u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) uint8_t pg_lds;
-typedef __attribute__((address_space(3))) int16_t __attribute__((ext_vector_type(4))) pg_s16x4_lds;
 
 // 64 lanes' 16 bytes at their offsets to LDS, one after another from `to` + `plus`, a constant once its loop is
 // unrolled (sums made outside would each hold a scalar register, and there are not as many). A vector memory
