@@ -72,8 +72,8 @@ constexpr uint32_t PG_TILE3_LDS = 12 * PgTile<float, NB>::GRANULE + 16;
 
 // f16 caches. RT 2: four waves of 32 query rows; RT 1: eight waves, four of them 16 query rows each over
 // half of a tile's slots and four the same rows over the other half. Bound by the matrix cores where rows are
-// many: 2048 before 8192 slots, 32 x 8 heads of 128, take 516 us, 1200 TFLOP/s with both parts of q and
-// of the weights (a large library product in f16 reaches 1132); 600 before 2000 63 us, of which the
+// many: 2048 before 8192 slots, 32 x 8 heads of 128, take 509 to 527 us by card, 1174 to 1214 TFLOP/s with both
+// parts of q and of the weights (a large library product in f16 reaches 1132); 600 before 2000 63 us, of which the
 // last blocks and the fold's 8.8 us are a third.
 // Block `id` of the items of more than 16 query rows. lds: PG_TILE_LDS bytes, 16-byte aligned.
 template <int NB, int RT>
@@ -1132,7 +1132,8 @@ PgCut cut(const PgParams& p, bool f16_cache, uint32_t qt, uint32_t longest, floa
 }
 
 // Items of more: query rows a block, and the chunks. Where most items have more than 64 query rows blocks of 128,
-// whose tiles are read half as often; f16 heads in blocks of 64 where those end sooner, there being few blocks
+// whose tiles are read half as often (and f32 heads of up to 128 dims run in bf16 parts, the few smaller items among
+// them too); f16 heads in blocks of 64 where those end sooner, there being few blocks
 // (494 rows, 32 x 8 heads of 128: 18 us, 27 by 128; before 1500 slots, 28 x 4 heads: 45, 48; 600 before
 // 2000, 32 x 8: 78, 63).
 void cut_tiles(PgParams& p, bool f16_cache) {

@@ -4,7 +4,8 @@
 // Mathematics. log p_i = x_i - m - log L with m the row's largest score and L = sum e^(x_i - m). Within a
 // row the order is the scores' own, so a row's k best tokens by score are all that the search can
 // take from it; between rows the sums and log L decide, in 64 bits (two rows' continuations may lie nearer
-// than an f32 tells apart).
+// than an f32 tells apart). The terms of L and a lane's sum of them are f32: by at most
+// 2^-17 they move all of a row's continuations alike; from lane to lane and part to part L is a tree and 64 bits.
 //
 // k_beam_scan: one pass over the scores, which keeps of a row the sum and the largest score of every group
 // of 256, nothing else: a wave takes a part of a row alone, 1024 scores a step, the next step's on their

@@ -291,8 +291,9 @@ int bchip_rope_append_paged(bchip_ctx* ctx, float* q, const float* k, const floa
 
 /* Causal attention of every sequence's rows over its pages: row r of n sees the slots up to
  * seq_lens[i] - n + r. f16 caches: K and V are f16 MFMA operands as they are, q and the softmax weights
- * two f16 each (22 bits), f32 accumulation; f32 caches: f32 products, or for many rows three bf16 a value
- * (24 bits) less what is under 2^-22 of a product, f32 sums. Results are within f32 rounding of the
+ * two f16 each (22 bits), f32 accumulation; f32 caches: f32 products, or, for rows past 16 query rows a KV head in
+ * calls where most such sequences have more than 64, three bf16 a value (24 bits) less what is under 2^-22 of a
+ * product, f32 sums. Results are within f32 rounding of the
  * formula over the stored values, for one row, a batch or a piece of a prompt alike
  * (f16 elements below 2^-14, f16's smallest normal number, count as if they were that large: the
  * matrix cores keep 24 bits from there); a row's last bits depend on the call it is in (lists are cut
