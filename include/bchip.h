@@ -291,15 +291,15 @@ int bchip_rope_append_paged(bchip_ctx* ctx, float* q, const float* k, const floa
 
 /* Causal attention of every sequence's rows over its pages: row r of n sees the slots up to
  * seq_lens[i] - n + r. f16 caches: K and V are f16 MFMA operands as they are, q and the softmax weights
- * two f16 each (22 bits), f32 accumulation; f32 caches: f32 products, or, for rows past 16 query rows a KV head in
- * calls where most such sequences have more than 64, three bf16 a value (24 bits) less what is under 2^-22 of a
- * product, f32 sums. Results are within f32 rounding of the
- * formula over the stored values, for one row, a batch or a piece of a prompt alike
- * (f16 elements below 2^-14, f16's smallest normal number, count as if they were that large: the
- * matrix cores keep 24 bits from there); a row's last bits depend on the call it is in (lists are cut
- * by the call's size), reruns give the same bits. An element of K or V that is not finite leaves the rows that see its slot unspecified and no
- * other; what a page holds past a list's end is never used. Where scratch cannot be had (memory full, a
- * call under graph capture that has not run before at its size) lists run uncut. */
+ * two f16 each (22 bits), f32 accumulation; f32 caches: f32 products, or, for rows past 16 query rows a
+ * KV head in calls where most such sequences have more than 64, three bf16 a value (24 bits) less what is
+ * under 2^-22 of a product, f32 sums. Results are within f32 rounding of the formula over the stored
+ * values, for one row, a batch or a piece of a prompt alike (f16 elements below 2^-14, f16's smallest
+ * normal number, count as if they were that large: the matrix cores keep 24 bits from there); a row's last
+ * bits depend on the call it is in (lists are cut by the call's size), reruns give the same bits. An
+ * element of K or V that is not finite leaves the rows that see its slot unspecified and no other; what a
+ * page holds past a list's end is never used. Where scratch cannot be had (memory full, a call under graph
+ * capture that has not run before at its size) lists run uncut. */
 int bchip_attention_paged(bchip_ctx* ctx, const float* q, const void* kc, const void* vc, uint32_t kv_type, float* out,
                           const uint32_t* row_starts, const uint32_t* seq_lens, const uint32_t* pages,
                           uint32_t page_stride, uint32_t page_slots, uint32_t npages, uint32_t nseq, uint32_t nh,
@@ -401,7 +401,8 @@ int bchip_logprobs(bchip_ctx* ctx, const float* scores, uint32_t rows, uint32_t 
  * nothing above -inf gives NaN scores, behind every number. beams and k <= 64, k <= beams * vocab,
  * batch * beams <= 65535. A caller that ends beams at a token asks for 2 beams of k and keeps the beams that
  * go on. Takes scratch of a 256th of the scores' bytes (of rows rounded up to 1024 scores) and at most
- * 1 KB a row beside; fails with BCHIP_E_OOM where it cannot be had (memory full, a call under graph capture that has not run before at its size). */
+ * 1 KB a row beside; fails with BCHIP_E_OOM where it cannot be had (memory full, a call under graph
+ * capture that has not run before at its size). */
 int bchip_beam_select(bchip_ctx* ctx, const float* scores, const float* sums, uint32_t batch, uint32_t beams,
                       uint32_t vocab, uint32_t k, float* best, uint32_t* beam, uint32_t* token);
 
